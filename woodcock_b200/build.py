@@ -2,8 +2,8 @@
 
     python -m woodcock_b200.build [--verbose]
 
-One nvcc invocation over woodcock_b200/csrc/runtime.cu (which includes the kernel
-headers). The CUDA runtime is linked statically; the library exports only the
+One nvcc invocation per woodcock_b200/csrc/*.cu (which include the kernel headers), side by
+side, and one that links them. The CUDA runtime is linked statically; the library exports only the
 C ABI of include/woodcock_b200.h.
 """
 
@@ -14,6 +14,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -48,20 +50,26 @@ def build(verbose: bool = False, force: bool = False, ptxas_info: bool = False) 
         return LIB
     LIB_DIR.mkdir(exist_ok=True)
     tmp = LIB.with_suffix(".so.tmp")
-    cmd = [nvcc(), *ARCH, "-lineinfo", "-O3", "-std=c++17", "--use_fast_math=false",
-           "-Xcompiler", "-fPIC,-fvisibility=hidden", "-shared", "-cudart", "static",
-           "-I", str(REPO / "include"), str(CSRC / "runtime.cu"), "-o", str(tmp)]
-    cmd = [c for c in cmd if c != "--use_fast_math=false"]
+    base = [nvcc(), *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC,-fvisibility=hidden",
+            "-I", str(REPO / "include")]
     if ptxas_info:
-        cmd.insert(1, "-Xptxas=-v")
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        sys.stderr.write(r.stdout + r.stderr)
-        raise RuntimeError("nvcc failed building libwoodcock_b200.so")
-    if verbose or ptxas_info:
-        sys.stderr.write(r.stderr)
+        base.insert(1, "-Xptxas=-v")
+
+    def run(cmd: list[str]) -> None:
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            sys.stderr.write(r.stdout + r.stderr)
+            raise RuntimeError("nvcc failed building libwoodcock_b200.so")
+        if verbose or ptxas_info:
+            sys.stderr.write(r.stderr)
+
+    with tempfile.TemporaryDirectory(dir=LIB_DIR) as work:
+        units = [(cu, Path(work) / (cu.stem + ".o")) for cu in sorted(CSRC.glob("*.cu"))]
+        with ThreadPoolExecutor(len(units)) as pool:
+            list(pool.map(lambda u: run([*base, "-c", str(u[0]), "-o", str(u[1])]), units))
+        run([*base, "-shared", "-cudart", "static", *(str(o) for _, o in units), "-o", str(tmp)])
     tmp.replace(LIB)
     return LIB
 
