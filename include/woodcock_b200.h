@@ -362,6 +362,98 @@ WC_API wc_status wc_batch_read_kv(wc_batch* b, int r, int layer, int n, void* k_
 WC_API wc_status wc_gemm_bf16(wc_ctx* ctx, const void* A, const void* B, float* C, int M, int N, int K,
                               const float* residual);
 
+/* ------------------------------------------------------------------ paged KV cache
+ * Operators over keys and values in pages (no counterpart in the reference, whose cache is one
+ * contiguous arena per request, include/woodcock/cache.h:9-28): what a server needs to run requests
+ * of unequal length, and requests with a common prompt, in one batch. The caller owns every buffer.
+ *  - Pages: [pages][kv_heads][page_size][head_dim] (with any strides, rows contiguous); key j of
+ *    request b is row j % page_size of page page_table[b][j / page_size].
+ *  - kv_lens[b] counts request b's keys, its new rows included; its new rows are rows
+ *    q_offsets[b] .. q_offsets[b + 1] of q, k, v and out (q_offsets NULL: rows / requests each) and
+ *    hold its last keys. Rows behind q_offsets[requests] are neither read nor written.
+ *  - Lengths, offsets and tables are device memory, so a captured graph may be replayed on new ones.
+ *    A table entry outside the pool, a length beyond the table and offsets out of range are never
+ *    followed: the keys count as absent, append drops the row, and the device error word is raised
+ *    (wc_ctx_synchronize returns WC_ERR_DEVICE once the stream's work is done).
+ *  - head_dim 64 or 128; page_size a power of two from 16 to 256; pages of WC_F32 or WC_BF16;
+ *    16-byte aligned pointers and strides.
+ *  - `stream`: the cudaStream_t to enqueue on (NULL: the context's; cudaStreamLegacy for the
+ *    default stream). Nothing is allocated and no state is kept between calls. */
+typedef struct {
+  void *k, *v;
+  int64_t k_stride[4], v_stride[4]; /* layer, page, head, row; in elements */
+  int dtype, pages, page_size, kv_heads, head_dim, layers;
+} wc_pages;
+
+typedef struct {
+  const int* page_table; /* [requests][table_cols], rows table_stride ints apart */
+  int64_t table_stride;
+  int table_cols, requests;
+  const int* kv_lens;
+  const int* q_offsets; /* [requests + 1] or NULL */
+  int rows;             /* rows of q */
+  int heads;
+} wc_paged_batch;
+
+typedef struct {
+  wc_pages pages;
+  wc_paged_batch batch;
+  const void *q, *k, *v;            /* [rows][heads or kv_heads][head_dim] of src_dtype */
+  int64_t q_stride[2], k_stride[2], v_stride[2]; /* row, head; in elements */
+  const int* positions;             /* [rows] or NULL: a row's place among its request's keys */
+  const float *q_norm, *k_norm;     /* gains [head_dim] or NULL: no normalisation */
+  void* q_out;                      /* [rows][heads][head_dim] of the pages' dtype */
+  double base;
+  float eps;
+  int src_dtype, layer;
+} wc_paged_append_args;
+/* RMSNorm of each head's q and k (where gains are given), rotate-half rotation at `positions` (angles in
+ * 64 bits, so far positions keep theirs), k and v written to the rows' page slots, q to q_out. Two
+ * rows of a call must not share a slot. */
+WC_API wc_status wc_paged_append(wc_ctx* ctx, void* stream, const wc_paged_append_args* args);
+
+typedef struct {
+  wc_pages pages;
+  wc_paged_batch batch;
+  const void* q; /* [rows][heads][head_dim] of the pages' dtype */
+  int64_t q_stride[2];
+  const int64_t* tree_mask; /* [rows] or NULL: bit i set: the row sees its request's new row i (at most
+                               64 new rows a request); NULL: row i sees new rows 0 .. i */
+  const int* prefix_table;  /* [groups][prefix_cols], rows prefix_stride ints apart */
+  int64_t prefix_stride;
+  const int* prefix_lens;   /* [groups] */
+  const int* group_offsets; /* [groups + 1]: the requests of each group */
+  int groups, prefix_cols;  /* groups 0: no shared prefixes */
+  void* out;                /* [rows][heads][head_dim] of the pages' dtype */
+  void* workspace;          /* 256-byte aligned; used by this call alone until its work is done */
+  uint64_t workspace_bytes;
+  float scale;
+  int layer;
+} wc_paged_attention_args;
+/* out = softmax(scale q K^T + mask) V for every row: over all keys of the group's prefix, the request's
+ * keys before its new rows, and the new rows that the mask shows. A row that sees nothing gives 0.
+ * Sums and softmax statistics are fp32; bf16 pages: weights rounded to bf16 for the second product. */
+WC_API wc_status wc_paged_attention(wc_ctx* ctx, void* stream, const wc_paged_attention_args* args);
+/* Bytes of workspace that wc_paged_attention needs for these arguments (buffers are not looked at). */
+WC_API wc_status wc_paged_attention_workspace(wc_ctx* ctx, const wc_paged_attention_args* args, uint64_t* bytes);
+
+typedef struct {
+  wc_pages pages;
+  const int* page_table;
+  int64_t table_stride;
+  int table_cols, requests;
+  const int* starts; /* [requests]: keys committed before the verified rows */
+  const int* keep;   /* [requests][max_keep], rows keep_stride ints apart; strictly increasing from >= 0 */
+  int64_t keep_stride;
+  const int* n_keep; /* [requests], at most max_keep */
+  int* lens_out;     /* [requests]: starts + n_keep */
+  int max_keep;      /* at most 64 */
+} wc_paged_compact_args;
+/* Key starts[b] + keep[b][i] -> starts[b] + i in every layer (wc_kv_compact over pages). A request with a
+ * bad list keeps its rows and length `starts`, and raises the device error word. Requests must not
+ * share the pages that their moved rows lie in. */
+WC_API wc_status wc_paged_compact(wc_ctx* ctx, void* stream, const wc_paged_compact_args* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -135,6 +135,10 @@ SIGNATURES = {
     "wc_batch_lens": (S, [P, C.c_int, P]),
     "wc_batch_read_kv": (S, [P, C.c_int, C.c_int, C.c_int, P, P]),
     "wc_gemm_bf16": (S, [P, P, P, P, C.c_int, C.c_int, C.c_int, P]),
+    "wc_paged_append": (S, [P, P, P]),
+    "wc_paged_attention": (S, [P, P, P]),
+    "wc_paged_attention_workspace": (S, [P, P, C.POINTER(C.c_uint64)]),
+    "wc_paged_compact": (S, [P, P, P]),
     "wc_decoder_save_state": (S, [P]),
     "wc_decoder_restore_state": (S, [P]),
     "wc_decoder_round_logits": (S, [P, C.c_int, P, P, I32P, C.POINTER(C.c_uint64)]),

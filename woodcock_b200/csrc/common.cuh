@@ -21,6 +21,7 @@ enum DeviceError : int {
   kErrTree = 16,          // malformed tree (parent >= child)
   kErrTimeout = 32,       // a bounded wait (mbarrier / pipeline) expired
   kErrSample = 64,        // a sampled draw found no token with positive probability
+  kErrPage = 128,         // a page table entry outside the pool
 };
 
 __device__ __forceinline__ void raise_error(int* err, int bit) {

@@ -1,0 +1,368 @@
+// The paged-cache entry points of include/woodcock_b200.h: argument checks, workspace layout and
+// launches of the kernels in paged.cuh.
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "host.h"
+#include "paged.cuh"
+
+using namespace wc;
+
+namespace {
+
+// Work goes to the caller's stream, which may belong to another device than the current one.
+struct DeviceScope {
+  int before = -1;
+  explicit DeviceScope(int device) {
+    int cur = 0;
+    CUDA_TRY(cudaGetDevice(&cur));
+    if (cur != device) {
+      CUDA_TRY(cudaSetDevice(device));
+      before = cur;
+    }
+  }
+  ~DeviceScope() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
+
+void need(bool ok, const char* what) {
+  if (!ok) fail(WC_ERR_INVALID, what);
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+int log2i(int n) {
+  int l = 0;
+  while ((1 << l) < n) ++l;
+  return l;
+}
+
+void check_pages(const wc_pages& g) {
+  need(g.k && g.v, "paged: null pages");
+  need(g.dtype == WC_F32 || g.dtype == WC_BF16, "paged: pages must be fp32 or bf16");
+  if (g.head_dim != 64 && g.head_dim != 128) fail(WC_ERR_UNSUPPORTED, "paged: head_dim must be 64 or 128");
+  if (g.page_size < 16 || g.page_size > 256 || (g.page_size & (g.page_size - 1)))
+    fail(WC_ERR_UNSUPPORTED, "paged: page_size must be a power of two from 16 to 256");
+  need(g.pages > 0 && g.kv_heads > 0 && g.layers > 0, "paged: empty pool");
+  need(aligned16(g.k) && aligned16(g.v), "paged: pages must be 16-byte aligned");
+  const int unit = g.dtype == WC_BF16 ? 8 : 4;
+  for (int i = 0; i < 4; ++i) {
+    need(g.k_stride[i] % unit == 0 && g.v_stride[i] % unit == 0, "paged: page strides must be multiples of 16 bytes");
+    need(g.k_stride[i] >= 0 && g.v_stride[i] >= 0, "paged: negative page stride");
+  }
+}
+
+void check_table(const int* table, long long stride, int cols, int page_size, const char* what) {
+  need(cols >= 0 && (table || cols == 0) && stride >= cols && stride < (1ll << 31), what);
+  need((long long)cols * page_size < (1ll << 30), "paged: a table of 2^30 keys or more");
+}
+
+PagePool pool(const wc_pages& g, const void* base, const int64_t* st, int layer) {
+  PagePool r;
+  r.ptr = static_cast<char*>(const_cast<void*>(base)) + st[0] * layer * (g.dtype == WC_BF16 ? 2 : 4);
+  r.page = st[1];
+  r.head = st[2];
+  r.row = st[3];
+  return r;
+}
+
+void check_batch(const wc_pages& g, const wc_paged_batch& b) {
+  need(b.requests > 0 && b.rows >= 0 && b.heads > 0, "paged: bad batch sizes");
+  need(b.heads % g.kv_heads == 0, "paged: heads must be a multiple of kv_heads");
+  need(b.kv_lens != nullptr, "paged: null kv_lens");
+  need(b.q_offsets || b.rows % b.requests == 0, "paged: rows must be a multiple of requests without q_offsets");
+  need((long long)b.rows * b.heads < (1ll << 30) && b.requests < (1 << 24), "paged: batch too large");
+  check_table(b.page_table, b.table_stride, b.table_cols, g.page_size, "paged: bad page table");
+}
+
+void check_rows(const void* p, const int64_t* st, int dtype, const char* what) {
+  const int unit = dtype == WC_BF16 ? 8 : 4;
+  need(p != nullptr, what);
+  need(aligned16(p) && st[0] % unit == 0 && st[1] % unit == 0 && st[0] >= 0 && st[1] >= 0, what);
+}
+
+cudaStream_t stream_of(wc_ctx* ctx, void* s) { return s ? static_cast<cudaStream_t>(s) : ctx->stream; }
+
+template <typename S, typename P, int D>
+void launch_append(wc_ctx* ctx, cudaStream_t st, const PagedAppendParams& p) {
+  launch_on(ctx, st, "paged_append", paged_append_kernel<S, P, D>, dim3(p.T), dim3(PA_THREADS), 0, true, 1, p);
+}
+
+template <typename S, typename P>
+void launch_append(wc_ctx* ctx, cudaStream_t st, const PagedAppendParams& p, int D) {
+  if (D == 64) launch_append<S, P, 64>(ctx, st, p);
+  else launch_append<S, P, 128>(ctx, st, p);
+}
+
+}  // namespace
+
+extern "C" wc_status wc_paged_append(wc_ctx* ctx, void* stream, const wc_paged_append_args* a) {
+  if (!ctx || !a) return WC_ERR_INVALID;
+  return guard(ctx, [&] {
+    const wc_pages& g = a->pages;
+    const wc_paged_batch& b = a->batch;
+    check_pages(g);
+    check_batch(g, b);
+    need(a->layer >= 0 && a->layer < g.layers, "paged_append: layer out of range");
+    need(a->src_dtype == WC_F32 || a->src_dtype == WC_BF16, "paged_append: rows must be fp32 or bf16");
+    if (b.rows == 0) return;
+    check_rows(a->q, a->q_stride, a->src_dtype, "paged_append: q must be 16-byte aligned, rows contiguous");
+    check_rows(a->k, a->k_stride, a->src_dtype, "paged_append: k must be 16-byte aligned, rows contiguous");
+    check_rows(a->v, a->v_stride, a->src_dtype, "paged_append: v must be 16-byte aligned, rows contiguous");
+    need(a->q_out && aligned16(a->q_out), "paged_append: q_out must be 16-byte aligned");
+    need(!a->q_norm || aligned16(a->q_norm), "paged_append: q_norm must be 16-byte aligned");
+    need(!a->k_norm || aligned16(a->k_norm), "paged_append: k_norm must be 16-byte aligned");
+    need(a->base > 0 && std::isfinite(a->base), "paged_append: base must be positive");
+    need(a->eps >= 0 && std::isfinite(a->eps), "paged_append: eps must not be negative");
+    DeviceScope scope(ctx->device);
+    PagedAppendParams p;
+    std::memset(&p, 0, sizeof(p));
+    p.q = a->q;
+    p.k = a->k;
+    p.v = a->v;
+    p.q_row = a->q_stride[0];
+    p.q_head = a->q_stride[1];
+    p.k_row = a->k_stride[0];
+    p.k_head = a->k_stride[1];
+    p.v_row = a->v_stride[0];
+    p.v_head = a->v_stride[1];
+    p.q_norm = a->q_norm;
+    p.k_norm = a->k_norm;
+    p.eps = a->eps;
+    p.q_out = a->q_out;
+    p.K = pool(g, g.k, g.k_stride, a->layer);
+    p.V = pool(g, g.v, g.v_stride, a->layer);
+    p.pages = g.pages;
+    p.page_log2 = log2i(g.page_size);
+    p.table = b.page_table;
+    p.table_ld = int(b.table_stride);
+    p.table_cols = b.table_cols;
+    p.lens = b.kv_lens;
+    p.offsets = b.q_offsets;
+    p.positions = a->positions;
+    p.T = b.rows;
+    p.B = b.requests;
+    p.H = b.heads;
+    p.Hk = g.kv_heads;
+    p.err = ctx->d_err;
+    for (int i = 0; i < g.head_dim / 2; ++i) p.freq[i] = std::pow(a->base, -2.0 * i / g.head_dim);
+    const cudaStream_t st = stream_of(ctx, stream);
+    const bool sb = a->src_dtype == WC_BF16, pb = g.dtype == WC_BF16;
+    if (sb && pb) launch_append<uint16_t, uint16_t>(ctx, st, p, g.head_dim);
+    else if (sb) launch_append<uint16_t, float>(ctx, st, p, g.head_dim);
+    else if (pb) launch_append<float, uint16_t>(ctx, st, p, g.head_dim);
+    else launch_append<float, float>(ctx, st, p, g.head_dim);
+  });
+}
+
+extern "C" wc_status wc_paged_compact(wc_ctx* ctx, void* stream, const wc_paged_compact_args* a) {
+  if (!ctx || !a) return WC_ERR_INVALID;
+  return guard(ctx, [&] {
+    const wc_pages& g = a->pages;
+    check_pages(g);
+    check_table(a->page_table, a->table_stride, a->table_cols, g.page_size, "paged_compact: bad page table");
+    need(a->requests > 0 && a->starts && a->keep && a->n_keep && a->lens_out, "paged_compact: null argument");
+    need(a->max_keep > 0 && a->keep_stride >= a->max_keep && a->keep_stride < (1ll << 31), "paged_compact: bad keep list");
+    if (a->max_keep > PC_MAXKEEP) fail(WC_ERR_UNSUPPORTED, "paged_compact: keep list longer than 64");
+    if (g.layers > 65535) fail(WC_ERR_UNSUPPORTED, "paged_compact: more than 65535 layers");
+    DeviceScope scope(ctx->device);
+    PagedCompactParams p;
+    std::memset(&p, 0, sizeof(p));
+    p.K = pool(g, g.k, g.k_stride, 0);
+    p.V = pool(g, g.v, g.v_stride, 0);
+    p.k_layer = g.k_stride[0];
+    p.v_layer = g.v_stride[0];
+    p.pages = g.pages;
+    p.page_log2 = log2i(g.page_size);
+    p.Hk = g.kv_heads;
+    p.esize_log2 = g.dtype == WC_BF16 ? 1 : 2;
+    p.row_chunks = (g.head_dim << p.esize_log2) / 16;
+    p.table = a->page_table;
+    p.table_ld = int(a->table_stride);
+    p.table_cols = a->table_cols;
+    p.starts = a->starts;
+    p.keep = a->keep;
+    p.keep_ld = int(a->keep_stride);
+    p.max_keep = a->max_keep;
+    p.n_keep = a->n_keep;
+    p.lens_out = a->lens_out;
+    p.err = ctx->d_err;
+    launch_on(ctx, stream_of(ctx, stream), "paged_compact", paged_compact_kernel, dim3(a->requests, g.layers),
+              dim3(PC_THREADS), 0, true, 1, p);
+  });
+}
+
+// ============================================================================ attention
+
+namespace {
+
+enum Variant { kSimt };
+
+struct Launch {
+  Variant variant;
+  int M, blocks, min_per;
+};
+
+// One launch: its row tile, blocks and the least key tiles a block takes on.
+Launch plan_launch(const wc_ctx* ctx, const wc_pages& g) {
+  Launch l;
+  l.variant = kSimt;
+  l.M = PS_M;
+  l.blocks = ctx->num_sms * 2;
+  l.min_per = 1;
+  return l;
+}
+
+struct Layout {
+  Launch own, prefix;
+  size_t part_o[2], part_ml[2], desc[2], whole_o[2], whole_ml[2], bytes;
+};
+
+size_t take(size_t& at, size_t bytes) {
+  const size_t here = at;
+  at += (bytes + 255) / 256 * 256;
+  return here;
+}
+
+Layout layout(const wc_ctx* ctx, const wc_paged_attention_args& a) {
+  const wc_pages& g = a.pages;
+  const wc_paged_batch& b = a.batch;
+  const int rep = b.heads / g.kv_heads;
+  Layout l;
+  std::memset(&l, 0, sizeof(l));
+  l.own = plan_launch(ctx, g);
+  l.prefix = plan_launch(ctx, g);
+  size_t at = 0;
+  for (int kind = 0; kind < (a.groups ? 2 : 1); ++kind) {
+    const Launch& x = kind ? l.prefix : l.own;
+    const size_t slots = size_t(x.blocks) * 2 * x.M;
+    const size_t items = size_t((long long)b.rows * rep / x.M) + (kind ? a.groups : b.requests) + 2;
+    l.part_o[kind] = take(at, slots * g.head_dim * sizeof(float));
+    l.part_ml[kind] = take(at, slots * sizeof(float2));
+    l.desc[kind] = take(at, items * g.kv_heads * sizeof(int2));
+    if (a.groups) {
+      l.whole_o[kind] = take(at, size_t(b.rows) * b.heads * g.head_dim * sizeof(float));
+      l.whole_ml[kind] = take(at, size_t(b.rows) * b.heads * sizeof(float2));
+    }
+  }
+  l.bytes = at;
+  return l;
+}
+
+void check_attention(const wc_paged_attention_args& a) {
+  check_pages(a.pages);
+  check_batch(a.pages, a.batch);
+  need(a.layer >= 0 && a.layer < a.pages.layers, "paged_attention: layer out of range");
+  need(a.groups >= 0 && a.groups < (1 << 24), "paged_attention: bad group count");
+  need(std::isfinite(a.scale) && a.scale > 0, "paged_attention: scale must be positive");
+}
+
+template <typename S, int D>
+void launch_simt(wc_ctx* ctx, cudaStream_t st, const PagedAttnParams& p, int kinds, const Launch& l) {
+  static bool ready[64] = {};
+  static std::mutex mu;
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (ctx->device >= 64 || !ready[ctx->device]) {
+      CUDA_TRY(cudaFuncSetAttribute(paged_simt_kernel<S, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    int(paged_simt_smem<D>())));
+      if (ctx->device < 64) ready[ctx->device] = true;
+    }
+  }
+  launch_on(ctx, st, "paged_simt", paged_simt_kernel<S, D>, dim3(l.blocks), dim3(PS_THREADS), paged_simt_smem<D>(),
+            true, 1, p, kinds, l.min_per);
+}
+
+template <typename S, int D>
+void attend(wc_ctx* ctx, cudaStream_t st, PagedAttnParams p, const Layout& l, char* ws) {
+  PagedCombineParams c;
+  std::memset(&c, 0, sizeof(c));
+  for (int kind = p.G ? 1 : 0; kind >= 0; --kind) {
+    const Launch& x = kind ? l.prefix : l.own;
+    p.part_o = reinterpret_cast<float*>(ws + l.part_o[kind]);
+    p.part_ml = reinterpret_cast<float2*>(ws + l.part_ml[kind]);
+    launch_simt<S, D>(ctx, st, p, kind ? kPrefixRows : kOwnRows, x);
+    c.part_o[kind] = p.part_o;
+    c.part_ml[kind] = p.part_ml;
+    c.M[kind] = x.M;
+    c.blocks[kind] = x.blocks;
+  }
+  c.a = p;
+  launch_on(ctx, st, "paged_combine", paged_combine_kernel<S, D>, dim3(p.T), dim3(PJ_THREADS), 0, true, 1, c);
+}
+
+}  // namespace
+
+extern "C" wc_status wc_paged_attention_workspace(wc_ctx* ctx, const wc_paged_attention_args* a, uint64_t* bytes) {
+  if (!ctx || !a || !bytes) return WC_ERR_INVALID;
+  return guard(ctx, [&] {
+    check_attention(*a);
+    *bytes = layout(ctx, *a).bytes;
+  });
+}
+
+extern "C" wc_status wc_paged_attention(wc_ctx* ctx, void* stream, const wc_paged_attention_args* a) {
+  if (!ctx || !a) return WC_ERR_INVALID;
+  return guard(ctx, [&] {
+    check_attention(*a);
+    const wc_pages& g = a->pages;
+    const wc_paged_batch& b = a->batch;
+    if (b.rows == 0) return;
+    check_rows(a->q, a->q_stride, g.dtype, "paged_attention: q must be 16-byte aligned, rows contiguous");
+    need(a->out && aligned16(a->out), "paged_attention: out must be 16-byte aligned");
+    if (a->groups) {
+      check_table(a->prefix_table, a->prefix_stride, a->prefix_cols, g.page_size, "paged_attention: bad prefix table");
+      need(a->prefix_lens && a->group_offsets, "paged_attention: null prefix_lens or group_offsets");
+    }
+    const Layout l = layout(ctx, *a);
+    if (!a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 256 || a->workspace_bytes < l.bytes)
+      fail(WC_ERR_CAPACITY, "paged_attention: workspace missing, misaligned or too small");
+    DeviceScope scope(ctx->device);
+    char* ws = static_cast<char*>(a->workspace);
+    PagedAttnParams p;
+    std::memset(&p, 0, sizeof(p));
+    p.q = a->q;
+    p.q_row = a->q_stride[0];
+    p.q_head = a->q_stride[1];
+    p.K = pool(g, g.k, g.k_stride, a->layer);
+    p.V = pool(g, g.v, g.v_stride, a->layer);
+    p.pages = g.pages;
+    p.page_log2 = log2i(g.page_size);
+    p.table = b.page_table;
+    p.table_ld = int(b.table_stride);
+    p.table_cols = b.table_cols;
+    p.lens = b.kv_lens;
+    p.offsets = b.q_offsets;
+    p.tree = reinterpret_cast<const long long*>(a->tree_mask);
+    p.prefix_table = a->prefix_table;
+    p.prefix_ld = int(a->prefix_stride);
+    p.prefix_cols = a->prefix_cols;
+    p.prefix_lens = a->prefix_lens;
+    p.groups = a->group_offsets;
+    p.T = b.rows;
+    p.B = b.requests;
+    p.G = a->groups;
+    p.H = b.heads;
+    p.Hk = g.kv_heads;
+    p.rep = b.heads / g.kv_heads;
+    p.scale_log2 = a->scale * kLog2e;
+    p.out = a->out;
+    p.desc_own = reinterpret_cast<int2*>(ws + l.desc[0]);
+    p.desc_prefix = reinterpret_cast<int2*>(ws + l.desc[1]);
+    for (int i = 0; i < 2; ++i) {
+      p.whole_o[i] = reinterpret_cast<float*>(ws + l.whole_o[i]);
+      p.whole_ml[i] = reinterpret_cast<float2*>(ws + l.whole_ml[i]);
+    }
+    p.err = ctx->d_err;
+    const cudaStream_t st = stream_of(ctx, stream);
+    if (g.dtype == WC_BF16) {
+      if (g.head_dim == 64) attend<uint16_t, 64>(ctx, st, p, l, ws);
+      else attend<uint16_t, 128>(ctx, st, p, l, ws);
+    } else {
+      if (g.head_dim == 64) attend<float, 64>(ctx, st, p, l, ws);
+      else attend<float, 128>(ctx, st, p, l, ws);
+    }
+  });
+}

@@ -1,0 +1,711 @@
+// Operators over a paged KV cache: append with rotation, ragged attention (causal or tree-masked),
+// attention under shared prefixes, compaction. Pages are [pages][kv_heads][page_size][head_dim],
+// any strides with contiguous rows; a request's key j lives in page table[b][j / page_size], row
+// j % page_size. The device checks every page number and length it reads before it uses them.
+#pragma once
+
+#include "common.cuh"
+
+namespace wc {
+
+constexpr int kPagedMaxHeadDim = 128;
+
+// One pool (K or V) and its strides in elements; rows are contiguous.
+struct PagePool {
+  void* ptr;
+  long long page, head, row;
+};
+
+// ---------------------------------------------------------------------------- append
+// y = x rsqrt(mean x^2 + eps) w per head (q and k, when gains are given), the rotation
+// (a, b) -> (a cos - b sin, b cos + a sin) of the halves' pairs at theta_i = position * base^(-2i/D),
+// then q to a dense tensor and k, v to the row's page slot.
+struct PagedAppendParams {
+  const void *q, *k, *v;
+  long long q_row, q_head, k_row, k_head, v_row, v_head;  // strides in elements
+  const float *q_norm, *k_norm;
+  float eps;
+  void* q_out;  // [T][H][D]
+  PagePool K, V;
+  int pages, page_log2;
+  const int* table;
+  int table_ld, table_cols;
+  const int* lens;       // keys per request, the new rows included
+  const int* offsets;    // [B + 1] first row of each request, or null: T / B rows each
+  const int* positions;  // [T] or null: the row's slot
+  int T, B, H, Hk;
+  int* err;
+  double freq[kPagedMaxHeadDim / 2];  // base^(-2i/D)
+};
+
+// Eight consecutive elements as fp32.
+__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+__device__ __forceinline__ void load8(const uint16_t* p, float (&x)[8]) {
+  const uint4 a = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ void store8(uint16_t* p, const float (&x)[8]) {
+  *reinterpret_cast<uint4*>(p) =
+      make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+}
+
+// Which request row t belongs to: the number of requests that end at or before it (block-collective;
+// B when the row lies behind the last request).
+__device__ __forceinline__ int request_of_row(const int* offsets, int t, int T, int B) {
+  if (!offsets) return t / (T / B);
+  int n = 0;
+  for (int b0 = 0; b0 < B; b0 += int(blockDim.x)) {
+    const int b = b0 + int(threadIdx.x);
+    n += __syncthreads_count(b < B && offsets[b + 1] <= t);
+  }
+  return n;
+}
+
+constexpr int PA_THREADS = 128;
+
+// One block per row; D / 16 lanes share a head, eight pairs each.
+template <typename S, typename P, int D>
+__global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_constant__ PagedAppendParams p) {
+  constexpr int LPH = D / 16, HPB = PA_THREADS / LPH;  // lanes per head, heads per step
+  __shared__ __align__(16) float cs[2][D / 2];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int t = blockIdx.x;
+  const int b = request_of_row(p.offsets, t, p.T, p.B);
+  if (b >= p.B) return;  // a row behind the last request
+  const int row0 = p.offsets ? p.offsets[b] : b * (p.T / p.B);
+  const int n = p.offsets ? p.offsets[b + 1] - row0 : p.T / p.B;
+  const int slot = p.lens[b] - n + (t - row0);
+  const int pi = slot >> p.page_log2;
+  int page = -1;
+  if (slot >= 0 && t >= row0 && pi < p.table_cols) page = p.table[(long long)b * p.table_ld + pi];
+  if (page < 0 || page >= p.pages) {
+    if (threadIdx.x == 0) raise_error(p.err, page < 0 && (slot < 0 || pi >= p.table_cols) ? kErrCapacity : kErrPage);
+    page = -1;  // k and v are not written
+  }
+  const int pos = p.positions ? p.positions[t] : slot;
+  if (threadIdx.x < D / 2) {
+    // The angle in 64 bits: at position 10^6 a 32-bit product would be off by 0.06. Reduced to
+    // [-pi, pi] before it is rounded, so the cosine is within 2^-22 of the exact one.
+    constexpr double kTwoPi = 6.283185307179586476925287;
+    const double a = double(pos) * p.freq[threadIdx.x];
+    const float r = float(a - kTwoPi * rint(a * (1.0 / kTwoPi)));
+    float s, c;
+    sincosf(r, &s, &c);
+    cs[0][threadIdx.x] = c;
+    cs[1][threadIdx.x] = s;
+  }
+  __syncthreads();
+  const int sub = threadIdx.x % LPH;  // pairs [8 sub, 8 sub + 8)
+  float c8[8], s8[8];
+  load8(cs[0] + 8 * sub, c8);
+  load8(cs[1] + 8 * sub, s8);
+  const int r = slot & ((1 << p.page_log2) - 1);
+  const int nh = p.H + 2 * p.Hk;
+  for (int h0 = 0; h0 < nh; h0 += HPB) {
+    const int h = h0 + int(threadIdx.x) / LPH;
+    const bool live = h < nh;
+    const bool isq = h < p.H, isk = !isq && h < p.H + p.Hk;
+    float a[8] = {}, c[8] = {};
+    if (live) {
+      const S* x = isq ? static_cast<const S*>(p.q) + t * p.q_row + h * p.q_head
+                       : (isk ? static_cast<const S*>(p.k) + t * p.k_row + (h - p.H) * p.k_head
+                              : static_cast<const S*>(p.v) + t * p.v_row + (h - p.H - p.Hk) * p.v_head);
+      load8(x + 8 * sub, a);
+      load8(x + D / 2 + 8 * sub, c);
+    }
+    const float* w = isq ? p.q_norm : (isk ? p.k_norm : nullptr);
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + c[i] * c[i];
+#pragma unroll
+    for (int o = 1; o < LPH; o *= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (!live) continue;
+    if (w) {
+      const float inv = 1.f / sqrtf(ss / float(D) + p.eps);
+      float wa[8], wc8[8];
+      load8(w + 8 * sub, wa);
+      load8(w + D / 2 + 8 * sub, wc8);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        a[i] *= inv * wa[i];
+        c[i] *= inv * wc8[i];
+      }
+    }
+    if (isq || isk) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x0 = a[i] * c8[i] - c[i] * s8[i], x1 = c[i] * c8[i] + a[i] * s8[i];
+        a[i] = x0;
+        c[i] = x1;
+      }
+    }
+    P* dst;
+    if (isq) {
+      dst = static_cast<P*>(p.q_out) + ((long long)t * p.H + h) * D;
+    } else {
+      if (page < 0) continue;
+      const PagePool& pool = isk ? p.K : p.V;
+      dst = static_cast<P*>(pool.ptr) + page * pool.page + (isk ? h - p.H : h - p.H - p.Hk) * pool.head + r * pool.row;
+    }
+    store8(dst + 8 * sub, a);
+    store8(dst + D / 2 + 8 * sub, c);
+  }
+}
+
+// ---------------------------------------------------------------------------- compaction
+// Rows start + keep[i] -> start + i of every layer, new length start + n_keep. keep is strictly
+// increasing from keep[0] >= 0 (checked), so keep[i] >= i: each thread moves one 16-byte column
+// chunk of all rows in order, up to eight rows read before they are written, and a row is read
+// before any later step overwrites it.
+constexpr int PC_THREADS = 256;
+constexpr int PC_MAXKEEP = 64;
+
+struct PagedCompactParams {
+  PagePool K, V;
+  long long k_layer, v_layer;  // layer strides in elements
+  int pages, page_log2, Hk, row_chunks;  // 16-byte pieces of a row
+  int esize_log2;
+  const int* table;
+  int table_ld, table_cols;
+  const int* starts;
+  const int* keep;  // [B][keep_ld]
+  int keep_ld, max_keep;
+  const int* n_keep;
+  int* lens_out;
+  int* err;
+};
+
+__global__ void __launch_bounds__(PC_THREADS) paged_compact_kernel(const __grid_constant__ PagedCompactParams p) {
+  __shared__ int s_src[PC_MAXKEEP], s_dst[PC_MAXKEEP], s_sr[PC_MAXKEEP], s_dr[PC_MAXKEEP];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int b = blockIdx.x, layer = blockIdx.y;
+  const int start = p.starts[b], nk = p.n_keep[b];
+  const int mask = (1 << p.page_log2) - 1;
+  bool bad = nk < 0 || nk > p.max_keep || start < 0;
+  if (!bad && int(threadIdx.x) < nk) {
+    const int i = threadIdx.x;
+    const int* keep = p.keep + (long long)b * p.keep_ld;
+    const int k = keep[i];
+    const long long from = (long long)start + k;
+    bad = k < 0 || (i > 0 && k <= keep[i - 1]) || (from >> p.page_log2) >= p.table_cols;
+    if (!bad) {
+      const int to = start + i;
+      const int ps = p.table[(long long)b * p.table_ld + int(from >> p.page_log2)];
+      const int pd = p.table[(long long)b * p.table_ld + (to >> p.page_log2)];
+      bad = ps < 0 || ps >= p.pages || pd < 0 || pd >= p.pages;
+      s_src[i] = ps;
+      s_sr[i] = int(from) & mask;
+      s_dst[i] = pd;
+      s_dr[i] = to & mask;
+    }
+  }
+  if (__syncthreads_or(bad)) {
+    if (threadIdx.x == 0) raise_error(p.err, kErrTree);
+    if (layer == 0 && threadIdx.x == 0) p.lens_out[b] = start;
+    return;
+  }
+  if (layer == 0 && threadIdx.x == 0) p.lens_out[b] = start + nk;
+  const int units = 2 * p.Hk * p.row_chunks;
+  for (int u = threadIdx.x; u < units; u += PC_THREADS) {
+    const int chunk = u % p.row_chunks, hv = u / p.row_chunks, head = hv >> 1;
+    const PagePool& pool = (hv & 1) ? p.V : p.K;
+    char* base = static_cast<char*>(pool.ptr) +
+                 ((((hv & 1) ? p.v_layer : p.k_layer) * layer + head * pool.head) << p.esize_log2) + chunk * 16;
+    for (int i0 = 0; i0 < nk; i0 += 8) {
+      uint4 x[8];
+      const int m = min(8, nk - i0);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < m)
+          x[j] = *reinterpret_cast<const uint4*>(
+              base + ((s_src[i0 + j] * pool.page + s_sr[i0 + j] * pool.row) << p.esize_log2));
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < m && (s_src[i0 + j] != s_dst[i0 + j] || s_sr[i0 + j] != s_dr[i0 + j]))
+          *reinterpret_cast<uint4*>(base + ((s_dst[i0 + j] * pool.page + s_dr[i0 + j] * pool.row) << p.esize_log2)) = x[j];
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------- attention: the work
+// o = softmax(scale q K^T) V for every query row, over the keys it sees. A segment is a set of rows
+// that share keys: a request's rows and its own pages, or a group's rows and the group's prefix
+// pages (seen whole). Query rows of a segment and KV head are numbered rho = token * rep + j (the
+// rep query heads of one KV head), cut into tiles of M rows; keys into tiles of KT. An item is
+// (segment, KV head, row tile); its key tiles, in one line over all items, are cut into equal
+// ranges, one per block, so blocks carry equal work whatever the lengths. An item that crosses a
+// cut leaves partial states (running maximum in log2 units, sum, unnormalised output), joined in
+// block order by the combine kernel: no atomics, the same result every time.
+enum PagedKinds : int { kOwnRows = 1, kPrefixRows = 2 };
+
+struct PagedAttnParams {
+  const void* q;
+  long long q_row, q_head;
+  PagePool K, V;
+  int pages, page_log2;
+  const int* table;
+  int table_ld, table_cols;
+  const int* lens;
+  const int* offsets;           // [B + 1] or null: T / B rows each
+  const long long* tree;        // [T] visible new rows as bits, or null: causal
+  const int* prefix_table;
+  int prefix_ld, prefix_cols;
+  const int* prefix_lens;
+  const int* groups;            // [G + 1] first request of each group
+  int T, B, G, H, Hk, rep;
+  float scale_log2;             // scale * log2(e)
+  void* out;                    // [T][H][D]
+  // workspace
+  float* part_o;                // [blocks][2][M][D]
+  float2* part_ml;              // [blocks][2][M]
+  int2* desc_own;               // per item: {first block, number of blocks}
+  int2* desc_prefix;
+  float* whole_o[2];            // with prefixes: items of one block, [T][H][D] (own, prefix)
+  float2* whole_ml[2];          // [T][H]
+  int* err;
+};
+
+struct PagedSeg {
+  int prefix, idx;   // group or request
+  int tok0, n, klen; // rows and keys
+};
+
+__device__ __forceinline__ int paged_row0(const PagedAttnParams& p, int b) {
+  return p.offsets ? min(max(p.offsets[b], 0), p.T) : b * (p.T / p.B);
+}
+
+__device__ __forceinline__ PagedSeg paged_seg(const PagedAttnParams& p, int kinds, int s) {
+  PagedSeg g;
+  const int ng = (kinds & kPrefixRows) ? p.G : 0;
+  g.prefix = s < ng;
+  g.idx = g.prefix ? s : s - ng;
+  int cap;
+  if (g.prefix) {
+    const int r0 = min(max(p.groups[s], 0), p.B), r1 = min(max(p.groups[s + 1], r0), p.B);
+    g.tok0 = paged_row0(p, r0);
+    g.n = max(0, paged_row0(p, r1) - g.tok0);
+    g.klen = p.prefix_lens[s];
+    cap = p.prefix_cols << p.page_log2;
+  } else {
+    g.tok0 = paged_row0(p, g.idx);
+    g.n = max(0, paged_row0(p, g.idx + 1) - g.tok0);
+    g.klen = p.lens[g.idx];
+    cap = p.table_cols << p.page_log2;
+    if (p.tree && g.n > 64) raise_error(p.err, kErrRows);
+  }
+  if (g.klen < 0 || g.klen > cap) raise_error(p.err, kErrCapacity);
+  g.klen = min(max(g.klen, 0), cap);
+  return g;
+}
+
+// Key tiles of one row tile: at least one, so that rows without keys are answered too.
+template <int M, int KT>
+__device__ __forceinline__ int paged_item_tiles(const PagedAttnParams& p, const PagedSeg& g, int qt) {
+  int seen = g.klen;
+  if (!g.prefix && !p.tree) {
+    const int last = min(g.n - 1, ((qt + 1) * M - 1) / p.rep);
+    seen = min(max(g.klen - g.n + last + 1, 0), g.klen);
+  }
+  return max(1, (seen + KT - 1) / KT);
+}
+
+template <int M, int KT>
+__device__ __forceinline__ long long paged_head_tiles(const PagedAttnParams& p, const PagedSeg& g) {
+  const int qts = (g.n * p.rep + M - 1) / M;
+  if (g.prefix || p.tree) return (long long)qts * paged_item_tiles<M, KT>(p, g, 0);
+  long long n = 0;
+  for (int qt = 0; qt < qts; ++qt) n += paged_item_tiles<M, KT>(p, g, qt);
+  return n;
+}
+
+// One block's walk over its range of key tiles, item by item.
+template <int M, int KT>
+struct PagedWalk {
+  PagedSeg g;
+  int head, qt, qts;    // the item
+  int kt0, kt1, ktn;    // this block's key tiles [kt0, kt1) of the item's ktn
+  int first, count;     // the blocks that share the item
+  int seg, nseg;
+  long long pos, end;   // tiles of the line: the item's first one here, the block's end
+  int per;
+
+  // Block-collective; `sh` holds kWalkShared words. False: the block has no work.
+  __device__ bool begin(const PagedAttnParams& p, int kinds, int min_per, long long* sh) {
+    nseg = ((kinds & kPrefixRows) ? p.G : 0) + ((kinds & kOwnRows) ? p.B : 0);
+    const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, nw = (nt + 31) >> 5;
+    long long total = 0;
+    pos = 0;
+    for (int pass = 0; pass < 2; ++pass) {
+      if (pass) {
+        per = int(max((long long)min_per, (total + gridDim.x - 1) / gridDim.x));
+        pos = (long long)blockIdx.x * per;
+        end = min(pos + per, total);
+        if (pos >= end) return false;
+      }
+      long long base = 0;
+      for (int s0 = 0; s0 < nseg; s0 += nt) {
+        const int s = s0 + tid;
+        long long w = 0;
+        if (s < nseg) w = paged_head_tiles<M, KT>(p, paged_seg(p, kinds, s)) * p.Hk;
+        long long x = w;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+          const long long y = __shfl_up_sync(0xffffffffu, x, o);
+          if (lane >= o) x += y;
+        }
+        if (lane == 31) sh[warp] = x;
+        __syncthreads();
+        long long before = base, all = 0;
+        for (int i = 0; i < nw; ++i) {
+          if (i < warp) before += sh[i];
+          all += sh[i];
+        }
+        const long long a = before + x - w;  // the segment's first tile
+        if (pass && a <= pos && pos < a + w) {
+          sh[32] = s;
+          sh[33] = pos - a;
+        }
+        base += all;
+        __syncthreads();
+      }
+      total = base;
+    }
+    seg = int(sh[32]);
+    long long off = sh[33];
+    g = paged_seg(p, kinds, seg);
+    qts = (g.n * p.rep + M - 1) / M;
+    const long long ph = paged_head_tiles<M, KT>(p, g);
+    head = int(off / ph);
+    off -= head * ph;
+    qt = 0;
+    while (off >= (ktn = paged_item_tiles<M, KT>(p, g, qt))) {
+      off -= ktn;
+      ++qt;
+    }
+    place(int(off));
+    return true;
+  }
+  __device__ void place(int off) {
+    kt0 = off;
+    kt1 = int(min((long long)ktn, off + (end - pos)));
+    first = int((pos - off) / per);
+    count = int((pos - off + ktn - 1) / per) - first + 1;
+  }
+  __device__ bool next(const PagedAttnParams& p, int kinds) {
+    pos += kt1 - kt0;
+    if (pos >= end) return false;
+    if (++qt == qts) {
+      qt = 0;
+      if (++head == p.Hk) {
+        head = 0;
+        do {
+          g = paged_seg(p, kinds, ++seg);
+        } while (g.n == 0);
+        qts = (g.n * p.rep + M - 1) / M;
+      }
+    }
+    ktn = paged_item_tiles<M, KT>(p, g, qt);
+    place(0);
+    return true;
+  }
+  // Number of the item among those of its kind and head: distinct, below T rep / M + segments + 1.
+  __device__ int item(const PagedAttnParams& p) const {
+    return int((long long)g.tok0 * p.rep / M) + g.idx + qt;
+  }
+  // Where this block's share of a divided item goes: slot 0 when the item began in an earlier block.
+  __device__ int slot() const { return kt0 > 0 ? 0 : 1; }
+};
+constexpr int kWalkShared = 34;
+
+// What one query row sees: keys below `lim`, and with a tree the new rows in `bits`.
+struct PagedRow {
+  bool valid;
+  int tok, h;  // row and query head
+  int lim;
+  int base, klen;
+  unsigned long long bits;
+  __device__ bool sees(int key) const {
+    if (key < lim) return true;
+    const int i = key - base;
+    return key < klen && unsigned(i) < 64u && ((bits >> i) & 1ull);
+  }
+};
+
+__device__ __forceinline__ PagedRow paged_row(const PagedAttnParams& p, const PagedSeg& g, int head, int rho) {
+  PagedRow r;
+  r.valid = rho < g.n * p.rep;
+  const int i = r.valid ? rho / p.rep : 0;
+  r.tok = g.tok0 + i;
+  r.h = head * p.rep + (r.valid ? rho - i * p.rep : 0);
+  r.klen = g.klen;
+  r.base = g.klen - g.n;
+  r.bits = 0ull;
+  if (g.prefix) {
+    r.lim = g.klen;
+  } else if (p.tree) {
+    r.lim = r.base;
+    if (r.valid) r.bits = (unsigned long long)p.tree[r.tok];
+  } else {
+    r.lim = min(r.base + i + 1, g.klen);
+  }
+  if (!r.valid) r.lim = 0;
+  return r;
+}
+
+// Page of a segment's key, or -1 (an entry outside the pool raises the error bit).
+__device__ __forceinline__ int paged_page(const PagedAttnParams& p, const PagedSeg& g, int pi) {
+  if (pi >= (g.prefix ? p.prefix_cols : p.table_cols)) return -1;
+  const int page = g.prefix ? p.prefix_table[(long long)g.idx * p.prefix_ld + pi]
+                            : p.table[(long long)g.idx * p.table_ld + pi];
+  if (page < 0 || page >= p.pages) {
+    raise_error(p.err, kErrPage);
+    return -1;
+  }
+  return page;
+}
+
+__device__ __forceinline__ void store4(float* p, const float (&x)[4]) {
+  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+}
+__device__ __forceinline__ void store4(uint16_t* p, const float (&x)[4]) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+}
+
+// ---------------------------------------------------------------------------- attention on the CUDA cores
+// 16 query rows x 64 keys per tile, 8 warps: scores with one key and four rows per thread, the
+// softmax of two rows per warp, then the same warp's rows of P V with four columns per thread.
+constexpr int PS_THREADS = 256, PS_M = 16, PS_KT = 64;
+
+template <int D>
+constexpr size_t paged_simt_smem() {
+  return sizeof(float) * (size_t(2) * PS_KT * (D + 4) + PS_M * D + PS_M * (PS_KT + 4)) + 8 * kWalkShared;
+}
+
+template <typename S, int D>
+__global__ void __launch_bounds__(PS_THREADS)
+    paged_simt_kernel(const __grid_constant__ PagedAttnParams p, int kinds, int min_per) {
+  constexpr int M = PS_M, KT = PS_KT, LD = D + 4, LS = KT + 4;
+  constexpr int RPT = D / 64;  // rows per thread of P V: two (D 128), one (D 64)
+  extern __shared__ __align__(16) float ps_smem[];
+  float* ks = ps_smem;
+  float* vs = ks + KT * LD;
+  float* qs = vs + KT * LD;
+  float* ss = qs + M * D;
+  long long* sh = reinterpret_cast<long long*>(ss + M * LS);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_launch_dependents();
+  pdl_wait();
+  PagedWalk<M, KT> w;
+  if (!w.begin(p, kinds, min_per, sh)) return;
+  do {
+    __syncthreads();
+    for (int c = tid; c < M * (D / 8); c += PS_THREADS) {
+      const int m = c / (D / 8), col = (c % (D / 8)) * 8;
+      const PagedRow r = paged_row(p, w.g, w.head, w.qt * M + m);
+      float x[8] = {};
+      if (r.valid) load8(static_cast<const S*>(p.q) + r.tok * p.q_row + r.h * p.q_head + col, x);
+      store8(qs + m * D + col, x);
+    }
+    const int sk = tid & 63, sr = (tid >> 6) * 4;
+    PagedRow rows[2];  // the warp's rows
+#pragma unroll
+    for (int i = 0; i < 2; ++i) rows[i] = paged_row(p, w.g, w.head, w.qt * M + 2 * warp + i);
+    float m2[2] = {-INFINITY, -INFINITY}, l2[2] = {0.f, 0.f};
+    float o[RPT][4] = {};
+    const int col = (lane % (D / 4)) * 4, prow = 2 * warp + (D == 64 ? lane / 16 : 0);
+    for (int kt = w.kt0; kt < w.kt1; ++kt) {
+      __syncthreads();
+      for (int c = tid; c < KT * (D / 8); c += PS_THREADS) {
+        const int kr = c / (D / 8), cc = (c % (D / 8)) * 8, key = kt * KT + kr;
+        float x[8] = {}, y[8] = {};
+        const int page = key < w.g.klen ? paged_page(p, w.g, key >> p.page_log2) : -1;
+        if (page >= 0) {
+          const int r = key & ((1 << p.page_log2) - 1);
+          load8(static_cast<const S*>(p.K.ptr) + page * p.K.page + w.head * p.K.head + r * p.K.row + cc, x);
+          load8(static_cast<const S*>(p.V.ptr) + page * p.V.page + w.head * p.V.head + r * p.V.row + cc, y);
+        }
+        store8(ks + kr * LD + cc, x);
+        store8(vs + kr * LD + cc, y);
+      }
+      __syncthreads();
+      float s[4] = {};
+#pragma unroll 8
+      for (int d = 0; d < D; d += 4) {
+        const float4 k4 = *reinterpret_cast<const float4*>(ks + sk * LD + d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float4 q4 = *reinterpret_cast<const float4*>(qs + (sr + i) * D + d);
+          s[i] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, s[i]))));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ss[(sr + i) * LS + sk] = s[i];
+      __syncthreads();
+      float alpha[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float z[2], mx = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          z[h] = ss[(2 * warp + i) * LS + lane + 32 * h] * p.scale_log2;
+          if (!rows[i].sees(kt * KT + lane + 32 * h)) z[h] = -INFINITY;
+          mx = fmaxf(mx, z[h]);
+        }
+        mx = fmaxf(warp_max(mx), m2[i]);
+        const float mg = mx == -INFINITY ? 0.f : mx;
+        alpha[i] = exp2f(m2[i] - mg);
+        const float e0 = exp2f(z[0] - mg), e1 = exp2f(z[1] - mg);
+        l2[i] = l2[i] * alpha[i] + warp_sum(e0 + e1);
+        m2[i] = mx;
+        ss[(2 * warp + i) * LS + lane] = e0;
+        ss[(2 * warp + i) * LS + lane + 32] = e1;
+      }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < RPT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][e] *= D == 64 ? (lane < 16 ? alpha[0] : alpha[1]) : alpha[i];
+      // a key of weight zero adds nothing, whatever its value holds
+      for (int k = 0; k < KT; ++k) {
+        const float4 v = *reinterpret_cast<const float4*>(vs + k * LD + col);
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) {
+          const float e = ss[(prow + i) * LS + k];
+          if (e != 0.f) {
+            o[i][0] = fmaf(e, v.x, o[i][0]);
+            o[i][1] = fmaf(e, v.y, o[i][1]);
+            o[i][2] = fmaf(e, v.z, o[i][2]);
+            o[i][3] = fmaf(e, v.w, o[i][3]);
+          }
+        }
+      }
+    }
+    if (w.kt0 == 0 && tid == 0)
+      (w.g.prefix ? p.desc_prefix : p.desc_own)[w.item(p) * p.Hk + w.head] = make_int2(w.first, w.count);
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+      const int ri = D == 64 ? lane / 16 : i;
+      const PagedRow& r = rows[ri];
+      if (!r.valid) continue;
+      const float m = ri ? m2[1] : m2[0], l = ri ? l2[1] : l2[0];
+      if (w.count == 1 && p.G == 0) {
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = o[i][e] * inv;
+        store4(static_cast<S*>(p.out) + ((long long)r.tok * p.H + r.h) * D + col, y);
+      } else {
+        float* po;
+        float2* pm;
+        if (w.count == 1) {
+          const long long at = (long long)r.tok * p.H + r.h;
+          po = p.whole_o[w.g.prefix] + at * D;
+          pm = p.whole_ml[w.g.prefix] + at;
+        } else {
+          const long long at = ((long long)blockIdx.x * 2 + w.slot()) * M + prow + i;
+          po = p.part_o + at * D;
+          pm = p.part_ml + at;
+        }
+        store4(po + col, o[i]);
+        if (col == 0) *pm = make_float2(m, l);
+      }
+    }
+  } while (w.next(p, kinds));
+}
+
+// ---------------------------------------------------------------------------- joining
+// One block per row, one warp per query head: the states of the row's prefix and own items, each
+// whole or in parts, joined in order: with M = max m_i, o = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i.
+struct PagedCombineParams {
+  PagedAttnParams a;
+  const float* part_o[2];    // own, prefix
+  const float2* part_ml[2];
+  int M[2];
+  int blocks[2];  // blocks of the launch that wrote them
+};
+
+constexpr int PJ_THREADS = 256;
+
+template <typename S, int D>
+__global__ void __launch_bounds__(PJ_THREADS) paged_combine_kernel(const __grid_constant__ PagedCombineParams c) {
+  const PagedAttnParams& p = c.a;
+  constexpr int E = D / 32;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b = request_of_row(p.offsets, t, p.T, p.B);
+  if (b >= p.B) return;
+  int grp = -1;
+  if (p.G > 0) {
+    int n = 0;
+    for (int g0 = 0; g0 < p.G; g0 += PJ_THREADS) {
+      const int g = g0 + int(threadIdx.x);
+      n += __syncthreads_count(g < p.G && p.groups[g + 1] <= b);
+    }
+    if (n < p.G && p.groups[n] <= b) grp = n;
+  }
+  for (int h = warp; h < p.H; h += PJ_THREADS / 32) {
+    float M = -INFINITY, L = 0.f, o[E] = {};
+    bool write = p.G > 0;
+    for (int kind = 1; kind >= 0; --kind) {
+      if (kind && grp < 0) continue;
+      const int tok0 = paged_row0(p, kind ? min(max(p.groups[grp], 0), p.B) : b);
+      const int rho = (t - tok0) * p.rep + h % p.rep;
+      if (rho < 0) continue;  // offsets that do not increase
+      const int m = c.M[kind], qt = rho / m;
+      const int item = int((long long)tok0 * p.rep / m) + (kind ? grp : b) + qt;
+      const int2 d = (kind ? p.desc_prefix : p.desc_own)[item * p.Hk + h / p.rep];
+      if (d.x < 0 || d.y < 1 || d.y > c.blocks[kind] || d.x > c.blocks[kind] - d.y) continue;  // never written
+      if (d.y > 1) write = true;
+      if (!write) continue;
+      for (int i = 0; i < d.y; ++i) {
+        const float* po;
+        float2 ml;
+        if (d.y == 1) {
+          const long long at = (long long)t * p.H + h;
+          po = p.whole_o[kind] + at * D;
+          ml = p.whole_ml[kind][at];
+        } else {
+          const long long at = ((long long)(d.x + i) * 2 + (i == 0 ? 1 : 0)) * m + (rho - qt * m);
+          po = c.part_o[kind] + at * D;
+          ml = c.part_ml[kind][at];
+        }
+        const float mn = fmaxf(M, ml.x), mg = mn == -INFINITY ? 0.f : mn;
+        const float wa = exp2f(M - mg), wb = exp2f(ml.x - mg);
+        L = L * wa + ml.y * wb;
+        M = mn;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = o[e] * wa + po[lane * E + e] * wb;
+      }
+    }
+    if (!write) continue;
+    const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+    S* dst = static_cast<S*>(p.out) + ((long long)t * p.H + h) * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if constexpr (sizeof(S) == 2) dst[e] = f32_to_bf16_bits(o[e] * inv);
+      else dst[e] = o[e] * inv;
+    }
+  }
+}
+
+}  // namespace wc

@@ -10,6 +10,10 @@ import torch
 
 from ._lib import WC_BF16, WC_F32, lib
 from .context import Context, device_ints, ptr
+from .paged import paged_append, paged_attention, paged_compact, shared_prefix_attention
+
+__all__ = ["Weight", "argmax", "attention", "linear", "paged_append", "paged_attention", "paged_compact", "rmsnorm",
+           "rope", "shared_prefix_attention", "silu_mul", "softmax"]
 
 
 class Weight:
