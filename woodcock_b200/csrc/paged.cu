@@ -48,7 +48,9 @@ void check_pages(const wc_pages& g) {
   need(g.pages > 0 && g.kv_heads > 0 && g.layers > 0, "paged: empty pool");
   need(aligned16(g.k) && aligned16(g.v), "paged: pages must be 16-byte aligned");
   const int unit = g.dtype == WC_BF16 ? 8 : 4;
+  const int sizes[4] = {g.layers, g.pages, g.kv_heads, g.page_size};
   for (int i = 0; i < 4; ++i) {
+    if (sizes[i] == 1) continue;  // never stepped over
     need(g.k_stride[i] % unit == 0 && g.v_stride[i] % unit == 0, "paged: page strides must be multiples of 16 bytes");
     need(g.k_stride[i] >= 0 && g.v_stride[i] >= 0, "paged: negative page stride");
   }
@@ -198,20 +200,27 @@ extern "C" wc_status wc_paged_compact(wc_ctx* ctx, void* stream, const wc_paged_
 
 namespace {
 
-enum Variant { kSimt };
+enum Variant { kSimt, kFew16, kFew32 };
 
 struct Launch {
   Variant variant;
   int M, blocks, min_per;
 };
 
-// One launch: its row tile, blocks and the least key tiles a block takes on.
-Launch plan_launch(const wc_ctx* ctx, const wc_pages& g) {
+// One launch: its row tile, blocks and the least key tiles a block takes on. `rows`: query rows per
+// segment and KV head, on average.
+Launch plan_launch(const wc_ctx* ctx, const wc_pages& g, long long rows) {
   Launch l;
-  l.variant = kSimt;
-  l.M = PS_M;
-  l.blocks = ctx->num_sms * 2;
   l.min_per = 1;
+  if (g.dtype == WC_F32) {
+    l.variant = kSimt;
+    l.M = PS_M;
+    l.blocks = ctx->num_sms * 2;
+  } else {
+    l.variant = rows <= 16 ? kFew16 : kFew32;
+    l.M = rows <= 16 ? 16 : 32;
+    l.blocks = ctx->num_sms;
+  }
   return l;
 }
 
@@ -232,8 +241,9 @@ Layout layout(const wc_ctx* ctx, const wc_paged_attention_args& a) {
   const int rep = b.heads / g.kv_heads;
   Layout l;
   std::memset(&l, 0, sizeof(l));
-  l.own = plan_launch(ctx, g);
-  l.prefix = plan_launch(ctx, g);
+  const long long rows = (long long)b.rows * rep;
+  l.own = plan_launch(ctx, g, (rows + b.requests - 1) / b.requests);
+  l.prefix = plan_launch(ctx, g, a.groups ? (rows + a.groups - 1) / a.groups : 0);
   size_t at = 0;
   for (int kind = 0; kind < (a.groups ? 2 : 1); ++kind) {
     const Launch& x = kind ? l.prefix : l.own;
@@ -259,31 +269,67 @@ void check_attention(const wc_paged_attention_args& a) {
   need(std::isfinite(a.scale) && a.scale > 0, "paged_attention: scale must be positive");
 }
 
-template <typename S, int D>
-void launch_simt(wc_ctx* ctx, cudaStream_t st, const PagedAttnParams& p, int kinds, const Launch& l) {
-  static bool ready[64] = {};
+// Dynamic shared memory above 48 KB is opted into once per kernel and device.
+template <typename K>
+void opt_in(const wc_ctx* ctx, K kernel, size_t bytes) {
   static std::mutex mu;
-  {
-    std::lock_guard<std::mutex> lock(mu);
-    if (ctx->device >= 64 || !ready[ctx->device]) {
-      CUDA_TRY(cudaFuncSetAttribute(paged_simt_kernel<S, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    int(paged_simt_smem<D>())));
-      if (ctx->device < 64) ready[ctx->device] = true;
-    }
-  }
-  launch_on(ctx, st, "paged_simt", paged_simt_kernel<S, D>, dim3(l.blocks), dim3(PS_THREADS), paged_simt_smem<D>(),
-            true, 1, p, kinds, l.min_per);
+  static std::map<std::pair<int, const void*>, bool> done;
+  std::lock_guard<std::mutex> lock(mu);
+  bool& d = done[{ctx->device, reinterpret_cast<const void*>(kernel)}];
+  if (d) return;
+  CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
+  d = true;
+}
+
+// K or V pages as a 4-D tensor (dim, row, head, page); a copy takes `rows` rows of one page and half
+// a row of head_dim 128 (128 bytes, the swizzle's width).
+CUtensorMap page_map(const wc_pages& g, const PagePool& pool, int rows) {
+  CUtensorMap m;
+  const cuuint64_t dims[4] = {cuuint64_t(g.head_dim), cuuint64_t(g.page_size), cuuint64_t(g.kv_heads),
+                              cuuint64_t(g.pages)};
+  const long long st[3] = {pool.row, g.kv_heads > 1 ? pool.head : 64, g.pages > 1 ? pool.page : 64};
+  const cuuint64_t strides[3] = {cuuint64_t(st[0]) * 2, cuuint64_t(st[1]) * 2, cuuint64_t(st[2]) * 2};
+  const cuuint32_t box[4] = {64, cuuint32_t(std::min(rows, g.page_size)), 1, 1};
+  const cuuint32_t es[4] = {1, 1, 1, 1};
+  const CUresult r = encode_tiled()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, pool.ptr, dims, strides, box, es,
+                                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) fail(WC_ERR_INVALID, "paged: the pages' strides cannot be described to the copy engine");
+  return m;
+}
+
+template <int D, int RG>
+void launch_few(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, const PagedAttnParams& p, int kinds, const Launch& l) {
+  const size_t smem = PfLayout<D>::bytes();
+  static_assert(PfLayout<D>::bytes() <= kSmemOptinBytes, "shared memory");
+  opt_in(ctx, paged_few_kernel<D, RG>, smem);
+  launch_on(ctx, st, "paged_few", paged_few_kernel<D, RG>, dim3(l.blocks), dim3(PF_THREADS), smem, true, 1,
+            page_map(g, p.K, PF_KT), page_map(g, p.V, PF_KT), p, kinds, l.min_per);
 }
 
 template <typename S, int D>
-void attend(wc_ctx* ctx, cudaStream_t st, PagedAttnParams p, const Layout& l, char* ws) {
+void launch_attention(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, const PagedAttnParams& p, int kinds,
+                      const Launch& l) {
+  if constexpr (sizeof(S) == 4) {
+    opt_in(ctx, paged_simt_kernel<S, D>, paged_simt_smem<D>());
+    launch_on(ctx, st, "paged_simt", paged_simt_kernel<S, D>, dim3(l.blocks), dim3(PS_THREADS), paged_simt_smem<D>(),
+              true, 1, p, kinds, l.min_per);
+  } else if (l.variant == kFew16) {
+    launch_few<D, 1>(ctx, st, g, p, kinds, l);
+  } else {
+    launch_few<D, 2>(ctx, st, g, p, kinds, l);
+  }
+}
+
+template <typename S, int D>
+void attend(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, PagedAttnParams p, const Layout& l, char* ws) {
   PagedCombineParams c;
   std::memset(&c, 0, sizeof(c));
   for (int kind = p.G ? 1 : 0; kind >= 0; --kind) {
     const Launch& x = kind ? l.prefix : l.own;
     p.part_o = reinterpret_cast<float*>(ws + l.part_o[kind]);
     p.part_ml = reinterpret_cast<float2*>(ws + l.part_ml[kind]);
-    launch_simt<S, D>(ctx, st, p, kind ? kPrefixRows : kOwnRows, x);
+    launch_attention<S, D>(ctx, st, g, p, kind ? kPrefixRows : kOwnRows, x);
     c.part_o[kind] = p.part_o;
     c.part_ml[kind] = p.part_ml;
     c.M[kind] = x.M;
@@ -358,11 +404,11 @@ extern "C" wc_status wc_paged_attention(wc_ctx* ctx, void* stream, const wc_page
     p.err = ctx->d_err;
     const cudaStream_t st = stream_of(ctx, stream);
     if (g.dtype == WC_BF16) {
-      if (g.head_dim == 64) attend<uint16_t, 64>(ctx, st, p, l, ws);
-      else attend<uint16_t, 128>(ctx, st, p, l, ws);
+      if (g.head_dim == 64) attend<uint16_t, 64>(ctx, st, g, p, l, ws);
+      else attend<uint16_t, 128>(ctx, st, g, p, l, ws);
     } else {
-      if (g.head_dim == 64) attend<float, 64>(ctx, st, p, l, ws);
-      else attend<float, 128>(ctx, st, p, l, ws);
+      if (g.head_dim == 64) attend<float, 64>(ctx, st, g, p, l, ws);
+      else attend<float, 128>(ctx, st, g, p, l, ws);
     }
   });
 }

@@ -5,6 +5,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace wc {
 
@@ -632,6 +633,376 @@ __global__ void __launch_bounds__(PS_THREADS)
   } while (w.next(p, kinds));
 }
 
+// ---------------------------------------------------------------------------- few rows: streamed pages
+// Decoding steps and short chains: at most 32 rows against each key, so the pages' bytes bound the
+// time. One producer warp streams 64-key tiles of K and V (TMA, 128-byte swizzle, a page's rows per
+// copy) through a ring that fills most of shared memory; eight consumer warps cut every tile into
+// 16-key slices, so that a tile is held only for a quarter of its arithmetic and no two warps wait
+// for one another before the item's end: each keeps its own running maximum, sum and 16 x D output
+// (mma m16n8k16), joined in shared memory once per item. With 16 rows the tiles alternate between
+// two sets of four warps, with 32 rows each slice has a warp per 16 rows.
+constexpr int PF_CONSUMERS = 8;
+constexpr int PF_THREADS = 32 * (PF_CONSUMERS + 1);
+constexpr int PF_KT = 64;
+
+template <int D>
+struct PfLayout {
+  static constexpr int kTile = PF_KT * D * 2;          // K or V of one tile
+  static constexpr int kStage = 2 * kTile;
+  static constexpr int kJoin = 4 * 16 * D * 4;         // four 16-row partial outputs
+  static constexpr int kTail = 8 * kWalkShared + 256 + 8 * 16 * 8 + 32 * 8;
+  // An even number: a stage then always belongs to the same set of warps, whose waits see each of its
+  // phases. (With an odd ring a set would meet a stage every other use, and a wait by parity would take
+  // the use before last, which another set reads, for its own.)
+  static constexpr int kStages = (int(kSmemOptinBytes) - 1024 - kJoin - kTail) / kStage & ~1;
+  static constexpr size_t bytes() { return 1024 + size_t(kStages) * kStage + kJoin + kTail; }
+};
+
+// Waits give up after a bound; then `dead` lets the block's other waits pass, so that it ends.
+__device__ __forceinline__ void paged_wait(uint64_t* bar, uint32_t parity, volatile int* dead, int* err) {
+  if (*dead) return;
+  if (!mbar_wait(bar, parity)) {
+    *dead = 1;
+    raise_error(err, kErrTimeout);
+  }
+}
+
+// The page numbers of a segment, 32 at a time over the warp's lanes and 32 more on their way.
+struct PageWindow {
+  int base, cur, nxt, npages, cols;
+  const int* row;
+  __device__ int fetch(const PagedAttnParams& p, int i) const {
+    if (i >= npages || i >= cols) return p.pages;  // behind the last key: the copy fills zeros
+    const int page = row[i];
+    if (page < 0 || page >= p.pages) {
+      raise_error(p.err, kErrPage);
+      return p.pages;
+    }
+    return page;
+  }
+  __device__ void start(const PagedAttnParams& p, const PagedSeg& g, int first, int lane) {
+    row = g.prefix ? p.prefix_table + (long long)g.idx * p.prefix_ld : p.table + (long long)g.idx * p.table_ld;
+    cols = g.prefix ? p.prefix_cols : p.table_cols;
+    npages = (g.klen + (1 << p.page_log2) - 1) >> p.page_log2;
+    base = first;
+    cur = fetch(p, base + lane);
+    nxt = fetch(p, base + 32 + lane);
+  }
+  // Warp-collective: page of index i (not before the last call's window) for each lane.
+  __device__ void seek(const PagedAttnParams& p, int first, int lane) {
+    if (first >= base + 32) {
+      base += 32;
+      cur = nxt;
+      nxt = fetch(p, base + 32 + lane);
+    }
+  }
+};
+
+template <int D, int RG>
+__global__ void __launch_bounds__(PF_THREADS, 1)
+    paged_few_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                     const __grid_constant__ PagedAttnParams p, int kinds, int min_per) {
+  using L = PfLayout<D>;
+  constexpr int M = 16 * RG, KT = PF_KT, NST = L::kStages, NK = D / 16, ND = D / 8;
+  constexpr int kWarpsPerTile = RG == 1 ? 4 : 8;
+  extern __shared__ unsigned char pf_raw[];
+  unsigned char* sm = pf_raw + ((1024u - (smem_addr(pf_raw) & 1023u)) & 1023u);
+  float* join = reinterpret_cast<float*>(sm + size_t(NST) * L::kStage);
+  unsigned char* tail = reinterpret_cast<unsigned char*>(join) + L::kJoin;
+  long long* sh = reinterpret_cast<long long*>(tail);
+  uint64_t* full = reinterpret_cast<uint64_t*>(tail + 8 * kWalkShared);
+  uint64_t* empty = full + NST;
+  volatile int* dead = reinterpret_cast<volatile int*>(tail + 8 * kWalkShared + 248);
+  float2* wml = reinterpret_cast<float2*>(tail + 8 * kWalkShared + 256);  // [8 warps][16 rows]
+  float2* rml = wml + 8 * 16;                                            // [M]
+  static_assert(16 * NST <= 248, "barriers");
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int s = 0; s < NST; ++s) {
+      mbar_init(full + s, 1);
+      mbar_init(empty + s, kWarpsPerTile);
+    }
+    mbar_fence_init();
+    *dead = 0;
+  }
+  pdl_launch_dependents();
+  pdl_wait();
+  PagedWalk<M, KT> w;
+  __syncthreads();
+  if (!w.begin(p, kinds, min_per, sh)) return;
+
+  if (warp == PF_CONSUMERS) {  // ---- producer
+    const int psize = 1 << p.page_log2;
+    const int box = min(psize, KT), parts = KT / box;  // copies of one half row block per tile
+    constexpr int HALVES = D / 64;
+    const int part = lane / (2 * HALVES), half = (lane >> 1) % HALVES;
+    const bool isv = lane & 1, issue = part < parts;
+    int cnt = 0;
+    do {
+      PageWindow win;
+      win.start(p, w.g, (w.kt0 * KT) >> p.page_log2, lane);
+      for (int kt = w.kt0; kt < w.kt1; ++kt, ++cnt) {
+        const int s = cnt % NST;
+        const int first = (kt * KT) >> p.page_log2;
+        win.seek(p, first, lane);
+        const int page = __shfl_sync(0xffffffffu, win.cur, (first - win.base + part) & 31);
+        if (lane == 0) {
+          if (cnt >= NST) paged_wait(empty + s, ((cnt / NST) - 1) & 1, dead, p.err);
+          if (!*dead) mbar_arrive_expect_tx(full + s, L::kStage);
+        }
+        __syncwarp();
+        if (*dead) break;
+        if (issue)
+          tma_load_4d(sm + size_t(s) * L::kStage + (isv ? L::kTile : 0) + half * (KT * 128) + part * box * 128,
+                      isv ? &tv : &tk, half * 64, (kt * KT) & (psize - 1), w.head, page, full + s);
+        __syncwarp();
+      }
+    } while (!*dead && w.next(p, kinds));
+    // shared memory must outlive the copies
+    if (lane == 0)
+      for (int q = max(0, cnt - NST); q < cnt; ++q)
+        if (!mbar_wait(full + q % NST, (q / NST) & 1)) raise_error(p.err, kErrTimeout);
+    return;
+  }
+
+  // ---- consumers
+  const int g = lane >> 2, t = lane & 3;
+  const int rg = RG == 1 ? 0 : (warp & 1);
+  const int slice = RG == 1 ? (warp & 3) : (warp >> 1);
+  const float sl2 = p.scale_log2;
+  int cnt = 0;
+  do {
+    const PagedRow ra = paged_row(p, w.g, w.head, w.qt * M + rg * 16 + g);
+    const PagedRow rb = paged_row(p, w.g, w.head, w.qt * M + rg * 16 + g + 8);
+    uint32_t qa[NK][4];
+    {
+      const uint16_t* qp0 = static_cast<const uint16_t*>(p.q) + ra.tok * p.q_row + ra.h * p.q_head + 2 * t;
+      const uint16_t* qp1 = static_cast<const uint16_t*>(p.q) + rb.tok * p.q_row + rb.h * p.q_head + 2 * t;
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk) {
+        qa[kk][0] = ra.valid ? *reinterpret_cast<const uint32_t*>(qp0 + kk * 16) : 0u;
+        qa[kk][1] = rb.valid ? *reinterpret_cast<const uint32_t*>(qp1 + kk * 16) : 0u;
+        qa[kk][2] = ra.valid ? *reinterpret_cast<const uint32_t*>(qp0 + kk * 16 + 8) : 0u;
+        qa[kk][3] = rb.valid ? *reinterpret_cast<const uint32_t*>(qp1 + kk * 16 + 8) : 0u;
+      }
+    }
+    // rows that pad the tile count as seeing everything: their results go nowhere
+    const int lim0 = ra.valid ? ra.lim : 0x7fffffff, lim1 = rb.valid ? rb.lim : 0x7fffffff;
+    const int lim = min(lim0, lim1);
+    float o[ND][4];
+#pragma unroll
+    for (int j = 0; j < ND; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+    for (int kt = w.kt0; kt < w.kt1; ++kt, ++cnt) {
+      if (RG == 1 && (cnt & 1) != (warp >> 2)) continue;
+      const int s = cnt % NST;
+      paged_wait(full + s, (cnt / NST) & 1, dead, p.err);
+      const unsigned char* kb = sm + size_t(s) * L::kStage + slice * 16 * 128;  // the slice's first key
+      const unsigned char* vb = kb + L::kTile;
+      // ---- S = Q K^T, 16 keys: the dims in two chains of each n-tile
+      float sc[2][4], sx[2][4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[j][e] = sx[j][e] = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t b[4];
+          const int chunk = (i & 1) * 4 + (lane >> 3);
+          ldsm_x4(b, kb + (i >> 1) * (KT * 128) + (j * 8 + (lane & 7)) * 128 + ((chunk ^ (lane & 7)) << 4));
+          mma_bf16_16816r(sc[j], qa[2 * i], b[0], b[1]);
+          mma_bf16_16816r(sx[j], qa[2 * i + 1], b[2], b[3]);
+        }
+      }
+      // ---- visibility, scale, running maximum
+      const int key0 = kt * KT + slice * 16;
+      const bool masked = key0 + 16 > lim;
+      float tm[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float v = (sc[j][e] + sx[j][e]) * sl2;
+          if (masked) {
+            const int key = key0 + j * 8 + 2 * t + (e & 1);
+            if ((e & 2) ? (rb.valid && !rb.sees(key)) : (ra.valid && !ra.sees(key))) v = -INFINITY;
+          }
+          sc[j][e] = v;
+          tm[e >> 1] = fmaxf(tm[e >> 1], v);
+        }
+      float alpha[2], mg[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        tm[h] = fmaxf(tm[h], __shfl_xor_sync(0xffffffffu, tm[h], 1));
+        tm[h] = fmaxf(tm[h], __shfl_xor_sync(0xffffffffu, tm[h], 2));
+        const float mn = fmaxf(m[h], tm[h]);
+        mg[h] = mn == -INFINITY ? 0.f : mn;
+        alpha[h] = ex2_approx(m[h] - mg[h]);
+        m[h] = mn;
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[j][e] = ex2_approx(sc[j][e] - mg[e >> 1]);
+      l[0] = l[0] * alpha[0] + (sc[0][0] + sc[0][1]) + (sc[1][0] + sc[1][1]);
+      l[1] = l[1] * alpha[1] + (sc[0][2] + sc[0][3]) + (sc[1][2] + sc[1][3]);
+      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+        for (int j = 0; j < ND; ++j) {
+          o[j][0] *= alpha[0];
+          o[j][1] *= alpha[0];
+          o[j][2] *= alpha[1];
+          o[j][3] *= alpha[1];
+        }
+      }
+      // A masked place may hold anything: where the slice's values are not all finite, the product
+      // is summed without the keys of weight zero (0 x NaN would reach every row).
+      bool clean = true;
+      if (__any_sync(0xffffffffu, masked)) {
+        const unsigned char* vr = vb + (lane & 15) * 128 + (lane >> 4) * 64;
+        uint32_t worst = 0;
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const uint4 x = *reinterpret_cast<const uint4*>(vr + h * (KT * 128) + c * 16);
+            const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              worst = max(worst, xs[q] & 0x7f800000u);
+              worst = max(worst, (xs[q] << 16) & 0x7f800000u);
+            }
+          }
+        clean = !__any_sync(0xffffffffu, worst == 0x7f800000u);
+      }
+      if (clean) {
+        // ---- O += P V; the weights are rounded to bf16, as the values are: relative 2^-9 each, the
+        // size of the output's own rounding
+        const uint32_t a[4] = {pack_bf16(sc[0][0], sc[0][1]), pack_bf16(sc[0][2], sc[0][3]),
+                               pack_bf16(sc[1][0], sc[1][1]), pack_bf16(sc[1][2], sc[1][3])};
+#pragma unroll
+        for (int dj = 0; dj < ND; dj += 2) {
+          uint32_t b[4];
+          const int key = lane & 15, chunk = dj + (lane >> 4);
+          ldsm_x4_trans(b, vb + (chunk >> 3) * (KT * 128) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4));
+          mma_bf16_16816r(o[dj], a, b[0], b[1]);
+          mma_bf16_16816r(o[dj + 1], a, b[2], b[3]);
+        }
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < 16; ++c) {
+          const int from = (lane & ~3) | ((c & 7) >> 1);
+          const float x0 = c < 8 ? ((c & 1) ? sc[0][1] : sc[0][0]) : ((c & 1) ? sc[1][1] : sc[1][0]);
+          const float x1 = c < 8 ? ((c & 1) ? sc[0][3] : sc[0][2]) : ((c & 1) ? sc[1][3] : sc[1][2]);
+          const float p0 = __shfl_sync(0xffffffffu, x0, from), p1 = __shfl_sync(0xffffffffu, x1, from);
+#pragma unroll
+          for (int dj = 0; dj < ND; ++dj) {
+            const uint32_t v = *reinterpret_cast<const uint32_t*>(vb + (dj >> 3) * (KT * 128) + c * 128 +
+                                                                  (((dj & 7) ^ (c & 7)) << 4) + 4 * t);
+            const float v0 = __uint_as_float(v << 16), v1 = __uint_as_float(v & 0xffff0000u);
+            if (p0 != 0.f) {
+              o[dj][0] = fmaf(p0, v0, o[dj][0]);
+              o[dj][1] = fmaf(p0, v1, o[dj][1]);
+            }
+            if (p1 != 0.f) {
+              o[dj][2] = fmaf(p1, v0, o[dj][2]);
+              o[dj][3] = fmaf(p1, v1, o[dj][3]);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty + s);
+    }
+
+    // ---- the warps' states of this item joined: rows' maxima and sums, then the outputs in two steps
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+      if (t == 0) wml[warp * 16 + g + 8 * h] = make_float2(m[h], l[h]);
+    }
+    named_sync(1, 32 * PF_CONSUMERS);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int q = 0; q < PF_CONSUMERS; q += RG) mx = fmaxf(mx, wml[(q + rg) * 16 + g + 8 * h].x);
+      const float mgx = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+      for (int q = 0; q < PF_CONSUMERS; q += RG) {
+        const float2 x = wml[(q + rg) * 16 + g + 8 * h];
+        sum += x.y * ex2_approx(x.x - mgx);
+      }
+      const float f = ex2_approx(m[h] - mgx);
+#pragma unroll
+      for (int j = 0; j < ND; ++j) {
+        o[j][2 * h] *= f;
+        o[j][2 * h + 1] *= f;
+      }
+      if (warp < RG && t == 0) rml[rg * 16 + g + 8 * h] = make_float2(mx, sum);
+    }
+    float* mine = join + (warp & 3) * 16 * D;
+    auto at = [&](int row, int col) { return row * D + (col ^ ((row & 3) << 3)); };  // spreads rows over the banks
+    if (warp >= 4) {
+#pragma unroll
+      for (int j = 0; j < ND; ++j) {
+        *reinterpret_cast<float2*>(mine + at(g, j * 8 + 2 * t)) = make_float2(o[j][0], o[j][1]);
+        *reinterpret_cast<float2*>(mine + at(g + 8, j * 8 + 2 * t)) = make_float2(o[j][2], o[j][3]);
+      }
+    }
+    named_sync(1, 32 * PF_CONSUMERS);
+    if (warp < 4) {
+#pragma unroll
+      for (int j = 0; j < ND; ++j) {
+        float2* x0 = reinterpret_cast<float2*>(mine + at(g, j * 8 + 2 * t));
+        float2* x1 = reinterpret_cast<float2*>(mine + at(g + 8, j * 8 + 2 * t));
+        *x0 = make_float2(x0->x + o[j][0], x0->y + o[j][1]);
+        *x1 = make_float2(x1->x + o[j][2], x1->y + o[j][3]);
+      }
+    }
+    named_sync(1, 32 * PF_CONSUMERS);
+    if (w.kt0 == 0 && tid == 0)
+      (w.g.prefix ? p.desc_prefix : p.desc_own)[w.item(p) * p.Hk + w.head] = make_int2(w.first, w.count);
+    for (int c = tid; c < M * (D / 4); c += 32 * PF_CONSUMERS) {
+      const int row = c / (D / 4), col = (c % (D / 4)) * 4;
+      const int rho = w.qt * M + row;
+      if (rho >= w.g.n * p.rep) continue;
+      float y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int q = 0; q < 4; q += RG) {
+        const float4 x = *reinterpret_cast<const float4*>(join + (q + row / 16) * 16 * D + at(row % 16, col));
+        y[0] += x.x;
+        y[1] += x.y;
+        y[2] += x.z;
+        y[3] += x.w;
+      }
+      const float2 ml = rml[row];
+      const int i = rho / p.rep;
+      const long long to = (long long)(w.g.tok0 + i) * p.H + w.head * p.rep + (rho - i * p.rep);
+      if (w.count == 1 && p.G == 0) {
+        const float inv = ml.y > 0.f ? 1.f / ml.y : (ml.y == 0.f ? 0.f : ml.y);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] *= inv;
+        store4(static_cast<uint16_t*>(p.out) + to * D + col, y);
+      } else if (w.count == 1) {
+        store4(p.whole_o[w.g.prefix] + to * D + col, y);
+        if (col == 0) p.whole_ml[w.g.prefix][to] = ml;
+      } else {
+        const long long pt = ((long long)blockIdx.x * 2 + w.slot()) * M + row;
+        store4(p.part_o + pt * D + col, y);
+        if (col == 0) p.part_ml[pt] = ml;
+      }
+    }
+    named_sync(1, 32 * PF_CONSUMERS);  // the joining space is free for the next item
+  } while (w.next(p, kinds));
+}
+
 // ---------------------------------------------------------------------------- joining
 // One block per row, one warp per query head: the states of the row's prefix and own items, each
 // whole or in parts, joined in order: with M = max m_i, o = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i.
@@ -677,24 +1048,37 @@ __global__ void __launch_bounds__(PJ_THREADS) paged_combine_kernel(const __grid_
       if (d.x < 0 || d.y < 1 || d.y > c.blocks[kind] || d.x > c.blocks[kind] - d.y) continue;  // never written
       if (d.y > 1) write = true;
       if (!write) continue;
-      for (int i = 0; i < d.y; ++i) {
-        const float* po;
-        float2 ml;
-        if (d.y == 1) {
-          const long long at = (long long)t * p.H + h;
-          po = p.whole_o[kind] + at * D;
-          ml = p.whole_ml[kind][at];
-        } else {
-          const long long at = ((long long)(d.x + i) * 2 + (i == 0 ? 1 : 0)) * m + (rho - qt * m);
-          po = c.part_o[kind] + at * D;
-          ml = c.part_ml[kind][at];
-        }
-        const float mn = fmaxf(M, ml.x), mg = mn == -INFINITY ? 0.f : mn;
-        const float wa = exp2f(M - mg), wb = exp2f(ml.x - mg);
-        L = L * wa + ml.y * wb;
-        M = mn;
+      const float2* pm;
+      const float* po;
+      long long step;  // rows from one part to the next (the first part is its block's second slot)
+      if (d.y == 1) {
+        const long long at = (long long)t * p.H + h;
+        pm = p.whole_ml[kind] + at;
+        po = p.whole_o[kind] + at * D;
+        step = 0;
+      } else {
+        const long long at = ((long long)d.x * 2 + 1) * m + (rho - qt * m);
+        pm = c.part_ml[kind] + at;
+        po = c.part_o[kind] + at * D;
+        step = 2 * m;
+      }
+      auto row_of = [&](int i) { return i ? i * step - m : 0ll; };
+      float mk = M;
+      for (int i = lane; i < d.y; i += 32) mk = fmaxf(mk, pm[row_of(i)].x);
+      mk = warp_max(mk);
+      const float mg = mk == -INFINITY ? 0.f : mk, wa = exp2f(M - mg);
+      L *= wa;
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = o[e] * wa + po[lane * E + e] * wb;
+      for (int e = 0; e < E; ++e) o[e] *= wa;
+      M = mk;
+#pragma unroll 4
+      for (int i = 0; i < d.y; ++i) {
+        const long long r = row_of(i);
+        const float2 ml = pm[r];
+        const float wb = exp2f(ml.x - mg);
+        L += ml.y * wb;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] += po[r * D + lane * E + e] * wb;
       }
     }
     if (!write) continue;
