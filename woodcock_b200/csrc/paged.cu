@@ -200,7 +200,7 @@ extern "C" wc_status wc_paged_compact(wc_ctx* ctx, void* stream, const wc_paged_
 
 namespace {
 
-enum Variant { kSimt, kFew16, kFew32 };
+enum Variant { kSimt, kFew16, kFew32, kMany128, kMany256 };
 
 struct Launch {
   Variant variant;
@@ -217,8 +217,8 @@ Launch plan_launch(const wc_ctx* ctx, const wc_pages& g, long long rows) {
     l.M = PS_M;
     l.blocks = ctx->num_sms * 2;
   } else {
-    l.variant = rows <= 16 ? kFew16 : kFew32;
-    l.M = rows <= 16 ? 16 : 32;
+    l.variant = rows <= 16 ? kFew16 : rows <= 32 ? kFew32 : rows <= 128 ? kMany128 : kMany256;
+    l.M = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 128 ? 128 : 256;
     l.blocks = ctx->num_sms;
   }
   return l;
@@ -251,7 +251,7 @@ Layout layout(const wc_ctx* ctx, const wc_paged_attention_args& a) {
     const size_t items = size_t((long long)b.rows * rep / x.M) + (kind ? a.groups : b.requests) + 2;
     l.part_o[kind] = take(at, slots * g.head_dim * sizeof(float));
     l.part_ml[kind] = take(at, slots * sizeof(float2));
-    l.desc[kind] = take(at, items * g.kv_heads * sizeof(int2));
+    l.desc[kind] = take(at, items * g.kv_heads * sizeof(int4));
     if (a.groups) {
       l.whole_o[kind] = take(at, size_t(b.rows) * b.heads * g.head_dim * sizeof(float));
       l.whole_ml[kind] = take(at, size_t(b.rows) * b.heads * sizeof(float2));
@@ -307,6 +307,15 @@ void launch_few(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, const PagedAttn
             page_map(g, p.K, PF_KT), page_map(g, p.V, PF_KT), p, kinds, l.min_per);
 }
 
+template <int D, bool kTwo>
+void launch_many(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, const PagedAttnParams& p, int kinds, const Launch& l) {
+  const size_t smem = PmLayout<D, kTwo>::bytes();
+  static_assert(PmLayout<D, kTwo>::bytes() <= kSmemOptinBytes, "shared memory");
+  opt_in(ctx, paged_many_kernel<D, kTwo>, smem);
+  launch_on(ctx, st, "paged_many", paged_many_kernel<D, kTwo>, dim3(l.blocks), dim3(PM_THREADS), smem, true, 1,
+            page_map(g, p.K, PM_KT), page_map(g, p.V, PM_KT), p, kinds, l.min_per);
+}
+
 template <typename S, int D>
 void launch_attention(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, const PagedAttnParams& p, int kinds,
                       const Launch& l) {
@@ -316,8 +325,12 @@ void launch_attention(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, const Pag
               true, 1, p, kinds, l.min_per);
   } else if (l.variant == kFew16) {
     launch_few<D, 1>(ctx, st, g, p, kinds, l);
-  } else {
+  } else if (l.variant == kFew32) {
     launch_few<D, 2>(ctx, st, g, p, kinds, l);
+  } else if (l.variant == kMany128) {
+    launch_many<D, false>(ctx, st, g, p, kinds, l);
+  } else {
+    launch_many<D, true>(ctx, st, g, p, kinds, l);
   }
 }
 
@@ -395,8 +408,8 @@ extern "C" wc_status wc_paged_attention(wc_ctx* ctx, void* stream, const wc_page
     p.rep = b.heads / g.kv_heads;
     p.scale_log2 = a->scale * kLog2e;
     p.out = a->out;
-    p.desc_own = reinterpret_cast<int2*>(ws + l.desc[0]);
-    p.desc_prefix = reinterpret_cast<int2*>(ws + l.desc[1]);
+    p.desc_own = reinterpret_cast<int4*>(ws + l.desc[0]);
+    p.desc_prefix = reinterpret_cast<int4*>(ws + l.desc[1]);
     for (int i = 0; i < 2; ++i) {
       p.whole_o[i] = reinterpret_cast<float*>(ws + l.whole_o[i]);
       p.whole_ml[i] = reinterpret_cast<float2*>(ws + l.whole_ml[i]);

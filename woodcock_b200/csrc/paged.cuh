@@ -278,8 +278,8 @@ struct PagedAttnParams {
   // workspace
   float* part_o;                // [blocks][2][M][D]
   float2* part_ml;              // [blocks][2][M]
-  int2* desc_own;               // per item: {first block, number of blocks}
-  int2* desc_prefix;
+  int4* desc_own;               // per item: {first block, number of blocks, redo rows 0-127, redo rows 128-255}
+  int4* desc_prefix;
   float* whole_o[2];            // with prefixes: items of one block, [T][H][D] (own, prefix)
   float2* whole_ml[2];          // [T][H]
   int* err;
@@ -601,7 +601,7 @@ __global__ void __launch_bounds__(PS_THREADS)
       }
     }
     if (w.kt0 == 0 && tid == 0)
-      (w.g.prefix ? p.desc_prefix : p.desc_own)[w.item(p) * p.Hk + w.head] = make_int2(w.first, w.count);
+      (w.g.prefix ? p.desc_prefix : p.desc_own)[w.item(p) * p.Hk + w.head] = make_int4(w.first, w.count, 0, 0);
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
       const int ri = D == 64 ? lane / 16 : i;
@@ -968,7 +968,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     }
     named_sync(1, 32 * PF_CONSUMERS);
     if (w.kt0 == 0 && tid == 0)
-      (w.g.prefix ? p.desc_prefix : p.desc_own)[w.item(p) * p.Hk + w.head] = make_int2(w.first, w.count);
+      (w.g.prefix ? p.desc_prefix : p.desc_own)[w.item(p) * p.Hk + w.head] = make_int4(w.first, w.count, 0, 0);
     for (int c = tid; c < M * (D / 4); c += 32 * PF_CONSUMERS) {
       const int row = c / (D / 4), col = (c % (D / 4)) * 4;
       const int rho = w.qt * M + row;
@@ -1003,6 +1003,488 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   } while (w.next(p, kinds));
 }
 
+// ---------------------------------------------------------------------------- many rows: tensor memory
+// Prompts, draft trees and shared prefixes: tiles of 128 rows x 128 keys, both products on tcgen05.
+// Warp 0 streams K and V tiles (TMA), warp 1 issues the products, two groups of four warps each own
+// a slot of tensor memory: scores S (128 columns; the weights P overwrite them as bf16) and output O
+// (head_dim columns), one row per thread. While one slot's warps take the softmax of their scores,
+// the tensor core works for the other slot. The slots are two row tiles that share every K and V tile
+// (kTwo: an item has 256 rows), or alternate key tiles of one row tile, joined at the item's end
+// (128 rows). A row's output is rescaled only when its running maximum grows by more than 2^8: P is
+// then at most 2^8 instead of 1, and the final division by the sum takes the same factor out.
+constexpr int PM_THREADS = 320;
+constexpr int PM_KT = 128;
+
+template <int D, bool kTwo>
+struct PmLayout {
+  static constexpr int kTile = PM_KT * D * 2;  // a K or V tile
+  static constexpr int kQ = (kTwo ? 2 : 1) * 128 * D * 2;
+  static constexpr int kTail = 8 * kWalkShared + 512 + (kTwo ? 0 : 2 * 128 * 8);
+  static constexpr int kStages = (int(kSmemOptinBytes) - 1024 - kQ - kTail) / kTile > 12
+                                     ? 12
+                                     : (int(kSmemOptinBytes) - 1024 - kQ - kTail) / kTile;
+  static constexpr size_t bytes() { return 1024 + size_t(kQ) + size_t(kStages) * kTile + kTail; }
+};
+
+// Bits of the 32 keys from k0 on that a row sees.
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u); }
+__device__ __forceinline__ uint32_t seen_bits(const PagedRow& r, int k0) {
+  uint32_t w = low_bits(r.lim - k0);
+  if (r.bits) {
+    const int sh = k0 - r.base;
+    const uint32_t x = sh >= 64 ? 0u : (sh >= 0 ? uint32_t(r.bits >> sh) : (sh > -32 ? uint32_t(r.bits << -sh) : 0u));
+    w |= x & low_bits(r.klen - k0);
+  }
+  return w;
+}
+
+template <int D, bool kTwo>
+__global__ void __launch_bounds__(PM_THREADS, 1)
+    paged_many_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                      const __grid_constant__ PagedAttnParams p, int kinds, int min_per) {
+  using L = PmLayout<D, kTwo>;
+  constexpr int M = kTwo ? 256 : 128, KT = PM_KT, NST = L::kStages, HALVES = D / 64;
+  constexpr uint32_t kColO = 256;
+  extern __shared__ unsigned char pm_raw[];
+  unsigned char* sm = pm_raw + ((1024u - (smem_addr(pm_raw) & 1023u)) & 1023u);
+  unsigned char* qs = sm;                    // [slot][half][128 rows][128 B], swizzled
+  unsigned char* ring = sm + L::kQ;          // [stage][half][128 keys][128 B]
+  unsigned char* tail = ring + size_t(NST) * L::kTile;
+  long long* sh = reinterpret_cast<long long*>(tail);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(tail + 8 * kWalkShared);
+  uint64_t* kv_full = bars;                  // [12]
+  uint64_t* kv_empty = bars + 12;            // [12]
+  uint64_t* q_full = bars + 24;              // [2]: the slot's queries are in shared memory
+  uint64_t* s_full = bars + 26;              // [2]: scores complete (and every product issued before)
+  uint64_t* p_full = bars + 28;              // [2]: weights written, output rescaled
+  uint64_t* o_full = bars + 30;              // [2]: the item's output complete
+  uint64_t* o_empty = bars + 32;             // [2]: and read
+  uint64_t* drain = bars + 34;
+  volatile int* dead = reinterpret_cast<volatile int*>(bars + 36);
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + 37);
+  volatile int* redo = reinterpret_cast<volatile int*>(bars + 38);  // [2]: number of the item to be redone
+  float2* xml = reinterpret_cast<float2*>(tail + 8 * kWalkShared + 512);  // [slot][row]: the slots' states
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int s = 0; s < NST; ++s) {
+      mbar_init(kv_full + s, 1);
+      mbar_init(kv_empty + s, 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(q_full + s, 4);
+      mbar_init(s_full + s, 1);
+      mbar_init(p_full + s, 4);
+      mbar_init(o_full + s, 1);
+      mbar_init(o_empty + s, kTwo ? 4 : 8);
+    }
+    mbar_init(drain, 1);
+    mbar_fence_init();
+    *dead = 0;
+    redo[0] = redo[1] = -1;
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_addr(tslot)),
+                 "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+  pdl_launch_dependents();
+  pdl_wait();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tslot;
+  PagedWalk<M, KT> w;
+  const bool work = w.begin(p, kinds, min_per, sh);
+
+  if (!work) {
+    // nothing to do
+  } else if (warp == 0) {  // ---- K and V tiles, in the order that the products take them
+    const int psize = 1 << p.page_log2;
+    const int box = min(psize, KT), parts = KT / box;
+    const int part = lane / HALVES, half = lane % HALVES;
+    int cnt = 0;
+    auto load = [&](PageWindow& win, const CUtensorMap* map, int kt) {
+      const int s = cnt % NST;
+      const int first = (kt * KT) >> p.page_log2;
+      win.seek(p, first, lane);
+      const int page = __shfl_sync(0xffffffffu, win.cur, (first - win.base + part) & 31);
+      if (lane == 0) {
+        if (cnt >= NST) paged_wait(kv_empty + s, ((cnt / NST) - 1) & 1, dead, p.err);
+        if (!*dead) mbar_arrive_expect_tx(kv_full + s, L::kTile);
+      }
+      __syncwarp();
+      if (*dead) return;
+      if (part < parts)
+        tma_load_4d(ring + size_t(s) * L::kTile + half * (KT * 128) + part * box * 128, map, half * 64,
+                    (kt * KT) & (psize - 1), w.head, page, kv_full + s);
+      __syncwarp();
+      ++cnt;
+    };
+    do {
+      PageWindow wk, wv;
+      wk.start(p, w.g, (w.kt0 * KT) >> p.page_log2, lane);
+      wv = wk;
+      constexpr int kAhead = kTwo ? 1 : 2;  // K tiles that are taken before the first V tile
+      for (int i = 0; i < kAhead && w.kt0 + i < w.kt1; ++i) load(wk, &tk, w.kt0 + i);
+      for (int kt = w.kt0; kt < w.kt1 && !*dead; ++kt) {
+        load(wv, &tv, kt);
+        if (kt + kAhead < w.kt1) load(wk, &tk, kt + kAhead);
+      }
+    } while (!*dead && w.next(p, kinds));
+    if (lane == 0)
+      for (int q = max(0, cnt - NST); q < cnt; ++q)
+        if (!mbar_wait(kv_full + q % NST, (q / NST) & 1)) raise_error(p.err, kErrTimeout);
+  } else if (warp == 1) {  // ---- products
+    if (lane == 0) {
+      constexpr uint32_t id_s = umma_idesc_bf16_m128(KT, 0), id_o = umma_idesc_bf16_m128(D, 1);
+      int cnt = 0;                                        // ring position of the next tile taken
+      int items[2] = {0, 0}, np[2] = {0, 0};              // per slot: items, weights waited for
+      auto stage = [&]() {
+        const int s = cnt % NST;
+        paged_wait(kv_full + s, (cnt / NST) & 1, dead, p.err);
+        ++cnt;
+        return s;
+      };
+      auto scores = [&](int slot, int qslot, int s) {
+        tc_fence_after();
+        const uint32_t a = smem_addr(qs + qslot * 128 * D * 2), b = smem_addr(ring + size_t(s) * L::kTile);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_bf16(tmem + slot * 128, umma_desc_sw128(a + (kk / 4) * (128 * 128) + (kk % 4) * 32),
+                    umma_desc_sw128(b + (kk / 4) * (KT * 128) + (kk % 4) * 32), id_s, kk != 0);
+        umma_commit(s_full + slot);
+      };
+      auto output = [&](int slot, int s, bool first) {
+        paged_wait(p_full + slot, np[slot] & 1, dead, p.err);
+        ++np[slot];
+        if (first && items[slot] > 0) paged_wait(o_empty + slot, (items[slot] - 1) & 1, dead, p.err);
+        tc_fence_after();
+        const uint32_t b = smem_addr(ring + size_t(s) * L::kTile);
+#pragma unroll
+        for (int kk = 0; kk < KT / 16; ++kk)
+          umma_bf16_ta(tmem + kColO + slot * D, tmem + slot * 128 + kk * 8,
+                       umma_desc_sw128_mn(b + kk * 16 * 128, KT * 128), id_o, !first || kk != 0);
+      };
+      int nitem = 0;
+      do {
+        const int nt = w.kt1 - w.kt0;
+        if constexpr (kTwo) {
+          const bool two = w.g.n * p.rep - w.qt * M > 128;
+          int ks = stage();
+          paged_wait(q_full, nitem & 1, dead, p.err);
+          scores(0, 0, ks);
+          if (two) {
+            paged_wait(q_full + 1, items[1] & 1, dead, p.err);
+            scores(1, 1, ks);
+          }
+          umma_commit(kv_empty + ks);
+          for (int t = 0; t < nt && !*dead; ++t) {
+            const int vs = stage();
+            const bool more = t + 1 < nt;
+            output(0, vs, t == 0);
+            if (!two) umma_commit(kv_empty + vs);
+            if (more) {
+              ks = stage();
+              scores(0, 0, ks);
+            } else {
+              umma_commit(o_full);
+            }
+            if (two) {
+              output(1, vs, t == 0);
+              umma_commit(kv_empty + vs);
+              if (more) scores(1, 1, ks);
+              else umma_commit(o_full + 1);
+            }
+            if (more) umma_commit(kv_empty + ks);
+          }
+          ++items[0];
+          if (two) ++items[1];
+        } else {
+          int ks[2];
+          ks[0] = stage();
+          paged_wait(q_full, nitem & 1, dead, p.err);
+          scores(0, 0, ks[0]);
+          umma_commit(kv_empty + ks[0]);
+          if (nt > 1) {
+            ks[1] = stage();
+            scores(1, 0, ks[1]);
+            umma_commit(kv_empty + ks[1]);
+          }
+          for (int t = 0; t < nt && !*dead; ++t) {
+            const int vs = stage(), slot = t & 1;
+            output(slot, vs, t < 2);
+            umma_commit(kv_empty + vs);
+            if (t + 2 < nt) {
+              const int k2 = stage();
+              scores(slot, 0, k2);
+              umma_commit(kv_empty + k2);
+            } else {
+              umma_commit(o_full + slot);
+            }
+          }
+          ++items[0];
+          if (nt > 1) ++items[1];
+        }
+        ++nitem;
+      } while (!*dead && w.next(p, kinds));
+      umma_commit(drain);  // tensor memory is given back only when nothing writes it any more
+      if (!mbar_wait(drain, 0)) raise_error(p.err, kErrTimeout);
+    }
+    __syncwarp();
+  } else {  // ---- softmax: thread = row of its slot
+    const int slot = (warp - 2) >> 2, qd = warp & 3, r128 = qd * 32 + lane;
+    const uint32_t lanes = tmem + (uint32_t(qd * 32) << 16);
+    const uint32_t ts = lanes + slot * 128, to = lanes + kColO + slot * D;
+    const float sl2 = p.scale_log2;
+    int ns = 0, no[2] = {0, 0};  // scores and outputs waited for
+    int vcnt = 0;                // ring position of the item's first K tile
+    int nitem = 0;
+
+    // this thread's query row, 16 bytes at a time, into the slot's swizzled tile
+    auto load_q = [&](const PagedWalk<M, KT>& x) {
+      const int rho = x.qt * M + (kTwo ? slot * 128 : 0) + r128;
+      const PagedRow r = paged_row(p, x.g, x.head, rho);
+      const uint16_t* src = static_cast<const uint16_t*>(p.q) + r.tok * p.q_row + r.h * p.q_head;
+      unsigned char* dst = qs + (kTwo ? slot : 0) * (128 * D * 2) + r128 * 128;
+      uint4 v[8];
+#pragma unroll
+      for (int h = 0; h < HALVES; ++h) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          v[c] = r.valid ? *reinterpret_cast<const uint4*>(src + h * 64 + c * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          *reinterpret_cast<uint4*>(dst + h * (128 * 128) + ((c ^ (r128 & 7)) << 4)) = v[c];
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full + (kTwo ? slot : 0));
+    };
+    // whether an item's rows reach the second slot's tile; only then are its queries loaded and waited for
+    auto both = [&](const PagedWalk<M, KT>& x) { return x.g.n * p.rep - x.qt * M > 128; };
+    if (slot == 0 || (kTwo && both(w))) load_q(w);
+    bool more;
+    do {
+      const int nt = w.kt1 - w.kt0;
+      const bool two = kTwo ? both(w) : nt > 1;
+      const bool active = slot == 0 || two;
+      const PagedRow r = paged_row(p, w.g, w.head, w.qt * M + (kTwo ? slot * 128 : 0) + r128);
+      const int lim = r.valid ? r.lim : 0x7fffffff;  // rows that pad the tile see everything, for nobody
+      // keys that every row of the slot's tile sees
+      const int edge = min(w.g.klen, w.g.prefix ? w.g.klen
+                                                : w.g.klen - w.g.n + (p.tree ? 0 : (w.qt * M + (kTwo ? slot * 128 : 0)) / p.rep + 1));
+      float m = -INFINITY, l = 0.f;
+      PagedWalk<M, KT> nx = w;
+      more = nx.next(p, kinds);
+      const bool load_next = more && (!kTwo || slot == 0 || both(nx));
+      const int step = kTwo ? 1 : 2;
+      for (int t = kTwo ? 0 : slot; t < nt && active; t += step) {
+        paged_wait(s_full + slot, ns & 1, dead, p.err);
+        ++ns;
+        tc_fence_after();
+        // the item's queries have been used for the last time: the next item's take their place
+        if (load_next && t + 1 == nt) load_q(nx);
+        uint32_t s0[64], s1[64];
+        tmem_ld64(ts, s0);
+        tmem_ld64(ts + 64, s1);
+        const int key0 = (w.kt0 + t) * KT;
+        const bool masked = key0 + KT > lim;
+        if (masked && r.valid) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t see = seen_bits(r, key0 + 32 * q);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              uint32_t& x = q < 2 ? s0[(q & 1) * 32 + j] : s1[(q & 1) * 32 + j];
+              if (!((see >> j) & 1u)) x = 0xff800000u;
+            }
+          }
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < 64; j += 2) {
+          mx[0] = fmaxf(mx[0], __uint_as_float(s0[j]));
+          mx[1] = fmaxf(mx[1], __uint_as_float(s0[j + 1]));
+          mx[2] = fmaxf(mx[2], __uint_as_float(s1[j]));
+          mx[3] = fmaxf(mx[3], __uint_as_float(s1[j + 1]));
+        }
+        const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
+        const bool first = t < step;
+        if (first) {
+          m = mt;
+        } else if (__any_sync(0xffffffffu, mt > m + 8.f)) {
+          const float mn = mt > m + 8.f ? mt : m;
+          const float f = m == mn ? 1.f : ex2_approx(m - mn);
+          m = mn;
+          l *= f;
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t v[32];
+            tmem_ld32(to + c, v);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * f);
+            tmem_st32(to + c, v);
+          }
+        }
+        const float mg = m == -INFINITY ? 0.f : m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float a = ex2_approx(fmaf(__uint_as_float(q ? s1[2 * j] : s0[2 * j]), sl2, -mg));
+            const float b = ex2_approx(fmaf(__uint_as_float(q ? s1[2 * j + 1] : s0[2 * j + 1]), sl2, -mg));
+            sum[(j & 1) * 2] += a;
+            sum[(j & 1) * 2 + 1] += b;
+            pk[j] = pack_bf16(a, b);  // weights rounded to bf16, as the values are (2^-9 of each)
+          }
+          tmem_st32(ts + q * 32, pk);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        // Values in masked places may be anything, and 0 x NaN would reach every row. Behind the last
+        // key they are cleared; between keys (a later row, another branch) they mark the tile's rows
+        // for the joining kernel, which sums such rows over the seen keys alone.
+        if (key0 + KT > edge) {
+          const int vpos = vcnt + (kTwo ? 2 * t + 1 : min(2 * t + 2, nt + t));
+          const int vs = vpos % NST;
+          paged_wait(kv_full + vs, (vpos / NST) & 1, dead, p.err);
+          unsigned char* vrow = ring + size_t(vs) * L::kTile + r128 * 128;
+          if (key0 + r128 >= w.g.klen) {
+            if (slot == 0 || !kTwo) {  // slot 1 of a shared tile multiplies after slot 0
+#pragma unroll
+              for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                  *reinterpret_cast<uint4*>(vrow + h * (KT * 128) + c * 16) = make_uint4(0, 0, 0, 0);
+            }
+          } else {
+            uint32_t worst = 0;
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+              for (int c = 0; c < 8; ++c) {
+                const uint4 x = *reinterpret_cast<const uint4*>(vrow + h * (KT * 128) + c * 16);
+                const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  worst = max(worst, xs[e] & 0x7f800000u);
+                  worst = max(worst, (xs[e] << 16) & 0x7f800000u);
+                }
+              }
+            if (worst == 0x7f800000u) redo[slot] = nitem;
+          }
+          fence_proxy_async_smem();
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + slot);
+      }
+      if (kTwo && !active && load_next) load_q(nx);
+      vcnt += 2 * nt;
+      // ---- the item's result
+      float f0 = 1.f, f1 = 0.f;
+      if constexpr (!kTwo) {  // the slots' states joined; each group of warps takes half of the columns
+        xml[slot * 128 + r128] = make_float2(m, l);
+        named_sync(1, 256);
+        const float2 a = xml[r128], b = xml[128 + r128];
+        m = fmaxf(a.x, b.x);
+        const float mg = m == -INFINITY ? 0.f : m;
+        f0 = ex2_approx(a.x - mg);
+        f1 = ex2_approx(b.x - mg);
+        l = a.y * f0 + b.y * f1;
+        named_sync(1, 256);
+        paged_wait(o_full, no[0] & 1, dead, p.err);
+        ++no[0];
+        if (two) {
+          paged_wait(o_full + 1, no[1] & 1, dead, p.err);
+          ++no[1];
+        }
+      } else if (active) {
+        paged_wait(o_full + slot, no[0] & 1, dead, p.err);
+        ++no[0];
+      }
+      // every warp of the slot raised its mark before the product that o_full reports
+      const bool again = kTwo ? active && redo[slot] == nitem : redo[0] == nitem || redo[1] == nitem;
+      if (w.kt0 == 0 && qd == 0 && lane == 0) {
+        int4* d = (w.g.prefix ? p.desc_prefix : p.desc_own) + w.item(p) * p.Hk + w.head;
+        if (slot == 0) {
+          *reinterpret_cast<int2*>(d) = make_int2(w.first, w.count);
+          d->z = again;
+        } else if (kTwo) {
+          d->w = again;
+        }
+      }
+      if (again) m = __int_as_float(0x7fc00000);  // a state that the joining kernel does not take
+      if (active || !kTwo) {
+        tc_fence_after();
+        const bool direct = w.count == 1 && p.G == 0;
+        const float inv = direct ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;
+        const long long at = (long long)r.tok * p.H + r.h;
+        const long long pt = ((long long)blockIdx.x * 2 + w.slot()) * M + (kTwo ? slot * 128 : 0) + r128;
+        float* po = w.count == 1 ? p.whole_o[w.g.prefix] + at * D : p.part_o + pt * D;
+        const int c0 = kTwo ? 0 : slot * (D / 2), c1 = kTwo ? D : c0 + D / 2;
+#pragma unroll 1
+        for (int c = c0; c < c1; c += 32) {
+          uint32_t v[32];
+          tmem_ld32(lanes + kColO + (kTwo ? slot * D : 0) + c, v);
+          float y[32];
+          if constexpr (kTwo) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) y[j] = __uint_as_float(v[j]) * inv;
+          } else {
+            const float g0 = f0 * inv, g1 = f1 * inv;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) y[j] = __uint_as_float(v[j]) * g0;
+            if (two) {
+              tmem_ld32(lanes + kColO + D + c, v);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) y[j] = fmaf(__uint_as_float(v[j]), g1, y[j]);
+            }
+          }
+          if (r.valid) {
+            if (direct) {
+              uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at * D + c);
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                dst[j] = make_uint4(pack_bf16(y[8 * j], y[8 * j + 1]), pack_bf16(y[8 * j + 2], y[8 * j + 3]),
+                                    pack_bf16(y[8 * j + 4], y[8 * j + 5]), pack_bf16(y[8 * j + 6], y[8 * j + 7]));
+            } else {
+              float4* dst = reinterpret_cast<float4*>(po + c);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) dst[j] = make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (kTwo) {
+            mbar_arrive(o_empty + slot);
+          } else {
+            mbar_arrive(o_empty);
+            if (two) mbar_arrive(o_empty + 1);
+          }
+        }
+        if (r.valid && !direct && (kTwo || slot == 0)) {
+          if (w.count == 1) p.whole_ml[w.g.prefix][at] = make_float2(m, l);
+          else p.part_ml[pt] = make_float2(m, l);
+        }
+      }
+      w = nx;
+      ++nitem;
+    } while (more);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
 // ---------------------------------------------------------------------------- joining
 // One block per row, one warp per query head: the states of the row's prefix and own items, each
 // whole or in parts, joined in order: with M = max m_i, o = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i.
@@ -1015,6 +1497,41 @@ struct PagedCombineParams {
 };
 
 constexpr int PJ_THREADS = 256;
+
+// A row's state over a segment, key by key and without the keys that it does not see: the slow way
+// for rows beside a value that is not finite.
+template <typename S, int D>
+__device__ __noinline__ void paged_redo_row(const PagedAttnParams& p, int kind, int seg, int t, int h, int lane,
+                                            float& M, float& L, float (&o)[D / 32]) {
+  constexpr int E = D / 32;
+  const PagedSeg g = paged_seg(p, kind, seg);
+  const PagedRow r = paged_row(p, g, h / p.rep, (t - g.tok0) * p.rep + h % p.rep);
+  if (!r.valid) return;
+  auto get = [](const S* x) { return sizeof(S) == 2 ? bf16_bits_to_f32(uint16_t(*x)) : float(*x); };
+  float q[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) q[e] = get(static_cast<const S*>(p.q) + t * p.q_row + h * p.q_head + lane * E + e);
+  for (int key = 0; key < g.klen; ++key) {
+    if (!r.sees(key)) continue;
+    const int page = paged_page(p, g, key >> p.page_log2), pr = key & ((1 << p.page_log2) - 1);
+    float k[E] = {}, v[E] = {}, z = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (page >= 0) {
+        k[e] = get(static_cast<const S*>(p.K.ptr) + page * p.K.page + (h / p.rep) * p.K.head + pr * p.K.row + lane * E + e);
+        v[e] = get(static_cast<const S*>(p.V.ptr) + page * p.V.page + (h / p.rep) * p.V.head + pr * p.V.row + lane * E + e);
+      }
+      z = fmaf(q[e], k[e], z);
+    }
+    z = warp_sum(z) * p.scale_log2;
+    const float mn = fmaxf(M, z), mg = mn == -INFINITY ? 0.f : mn;
+    const float wa = exp2f(M - mg), wb = exp2f(z - mg);
+    M = mn;
+    L = L * wa + wb;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = o[e] * wa + wb * v[e];
+  }
+}
 
 template <typename S, int D>
 __global__ void __launch_bounds__(PJ_THREADS) paged_combine_kernel(const __grid_constant__ PagedCombineParams c) {
@@ -1036,7 +1553,7 @@ __global__ void __launch_bounds__(PJ_THREADS) paged_combine_kernel(const __grid_
   }
   for (int h = warp; h < p.H; h += PJ_THREADS / 32) {
     float M = -INFINITY, L = 0.f, o[E] = {};
-    bool write = p.G > 0;
+    bool write = p.G > 0, redo = false;
     for (int kind = 1; kind >= 0; --kind) {
       if (kind && grp < 0) continue;
       const int tok0 = paged_row0(p, kind ? min(max(p.groups[grp], 0), p.B) : b);
@@ -1044,10 +1561,13 @@ __global__ void __launch_bounds__(PJ_THREADS) paged_combine_kernel(const __grid_
       if (rho < 0) continue;  // offsets that do not increase
       const int m = c.M[kind], qt = rho / m;
       const int item = int((long long)tok0 * p.rep / m) + (kind ? grp : b) + qt;
-      const int2 d = (kind ? p.desc_prefix : p.desc_own)[item * p.Hk + h / p.rep];
+      const int4 d = (kind ? p.desc_prefix : p.desc_own)[item * p.Hk + h / p.rep];
       if (d.x < 0 || d.y < 1 || d.y > c.blocks[kind] || d.x > c.blocks[kind] - d.y) continue;  // never written
       if (d.y > 1) write = true;
-      if (!write) continue;
+      if (!write) {
+        redo = (rho - qt * m < 128 ? d.z : d.w) == 1;
+        continue;
+      }
       const float2* pm;
       const float* po;
       long long step;  // rows from one part to the next (the first part is its block's second slot)
@@ -1064,7 +1584,13 @@ __global__ void __launch_bounds__(PJ_THREADS) paged_combine_kernel(const __grid_
       }
       auto row_of = [&](int i) { return i ? i * step - m : 0ll; };
       float mk = M;
-      for (int i = lane; i < d.y; i += 32) mk = fmaxf(mk, pm[row_of(i)].x);
+      bool bad = false;
+      for (int i = lane; i < d.y; i += 32) {
+        const float x = pm[row_of(i)].x;
+        mk = fmaxf(mk, x);
+        bad |= x != x;
+      }
+      redo |= __any_sync(0xffffffffu, bad) != 0;
       mk = warp_max(mk);
       const float mg = mk == -INFINITY ? 0.f : mk, wa = exp2f(M - mg);
       L *= wa;
@@ -1080,6 +1606,15 @@ __global__ void __launch_bounds__(PJ_THREADS) paged_combine_kernel(const __grid_
 #pragma unroll
         for (int e = 0; e < E; ++e) o[e] += po[r * D + lane * E + e] * wb;
       }
+    }
+    if (redo) {
+      L = 0.f;
+      M = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = 0.f;
+      if (grp >= 0) paged_redo_row<S, D>(p, kPrefixRows, grp, t, h, lane, M, L, o);
+      paged_redo_row<S, D>(p, kOwnRows, b, t, h, lane, M, L, o);
+      write = true;
     }
     if (!write) continue;
     const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);

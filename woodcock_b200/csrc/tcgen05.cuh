@@ -58,4 +58,63 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// MN-major operand written by TMA with the 128-byte swizzle: rows of 128 bytes are K indices (8-row groups
+// 1024 bytes apart = stride byte offset), 64-element MN blocks `mn_block` bytes apart (leading byte offset).
+__device__ __forceinline__ uint64_t umma_desc_sw128_mn(uint32_t saddr, uint32_t mn_block) {
+  return uint64_t((saddr & 0x3FFFFu) >> 4) | (uint64_t(mn_block >> 4) << 16) | (uint64_t(1024 >> 4) << 32) |
+         (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+// Instruction descriptor, kind::f16: fp32 accumulator, bf16 A and B, M 128; B K-major or MN-major.
+__host__ __device__ constexpr uint32_t umma_idesc_bf16_m128(int N, int b_mn_major) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(b_mn_major) << 16) | (uint32_t(N >> 3) << 17) |
+         (uint32_t(128 >> 4) << 24);
+}
+// A from tensor memory: lane = row, one 32-bit column = two consecutive bf16 K elements.
+__device__ __forceinline__ void umma_bf16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
+                                             uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+#define WC_R8(a, i) "=r"((a)[i]), "=r"((a)[i + 1]), "=r"((a)[i + 2]), "=r"((a)[i + 3]), "=r"((a)[i + 4]), \
+                    "=r"((a)[i + 5]), "=r"((a)[i + 6]), "=r"((a)[i + 7])
+#define WC_I8(a, i) "r"((a)[i]), "r"((a)[i + 1]), "r"((a)[i + 2]), "r"((a)[i + 3]), "r"((a)[i + 4]), \
+                    "r"((a)[i + 5]), "r"((a)[i + 6]), "r"((a)[i + 7])
+// 32 consecutive columns of this thread's lane, complete on return
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+      "tcgen05.wait::ld.sync.aligned;\n"
+      : WC_R8(r, 0), WC_R8(r, 8), WC_R8(r, 16), WC_R8(r, 24)
+      : "r"(taddr)
+      : "memory");
+}
+// 64 consecutive columns, complete on return
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n"
+      "tcgen05.wait::ld.sync.aligned;\n"
+      : WC_R8(r, 0), WC_R8(r, 8), WC_R8(r, 16), WC_R8(r, 24), WC_R8(r, 32), WC_R8(r, 40), WC_R8(r, 48), WC_R8(r, 56)
+      : "r"(taddr)
+      : "memory");
+}
+// stores 32 consecutive columns; tmem_st_wait() completes them
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};\n" ::WC_I8(r, 0),
+      WC_I8(r, 8), WC_I8(r, 16), WC_I8(r, 24), "r"(taddr)
+      : "memory");
+}
+#undef WC_R8
+#undef WC_I8
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+// generic-proxy shared-memory writes before this are visible to the tensor core and copy engine after it
+__device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
+
 }  // namespace wc
