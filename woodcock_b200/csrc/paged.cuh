@@ -1012,7 +1012,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
 // (kTwo: an item has 256 rows), or alternate key tiles of one row tile, joined at the item's end
 // (128 rows). A row's output is rescaled only when its running maximum grows by more than 2^8: P is
 // then at most 2^8 instead of 1, and the final division by the sum takes the same factor out.
-constexpr int PM_THREADS = 320;
+constexpr int PM_THREADS = 384;  // producer, products, two idle warps (registers); 2 x 4 softmax warps
 constexpr int PM_KT = 128;
 
 template <int D, bool kTwo>
@@ -1097,9 +1097,11 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
   PagedWalk<M, KT> w;
   const bool work = w.begin(p, kinds, min_per, sh);
 
-  if (!work) {
-    // nothing to do
-  } else if (warp == 0) {  // ---- K and V tiles, in the order that the products take them
+  // registers: launched with 168 a thread (64512); 88 for the first four warps, 208 for the softmax warps
+  // (128 x 88 + 256 x 208 = 64512): a row's 128 scores stay in registers
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n");
+  if (warp == 0 && work) {  // ---- K and V tiles, in the order that the products take them
     const int psize = 1 << p.page_log2;
     const int box = min(psize, KT), parts = KT / box;
     const int part = lane / HALVES, half = lane % HALVES;
@@ -1135,105 +1137,122 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
     if (lane == 0)
       for (int q = max(0, cnt - NST); q < cnt; ++q)
         if (!mbar_wait(kv_full + q % NST, (q / NST) & 1)) raise_error(p.err, kErrTimeout);
-  } else if (warp == 1) {  // ---- products
-    if (lane == 0) {
-      constexpr uint32_t id_s = umma_idesc_bf16_m128(KT, 0), id_o = umma_idesc_bf16_m128(D, 1);
-      int cnt = 0;                                        // ring position of the next tile taken
-      int items[2] = {0, 0}, np[2] = {0, 0};              // per slot: items, weights waited for
-      auto stage = [&]() {
-        const int s = cnt % NST;
-        paged_wait(kv_full + s, (cnt / NST) & 1, dead, p.err);
-        ++cnt;
-        return s;
-      };
-      auto scores = [&](int slot, int qslot, int s) {
-        tc_fence_after();
-        const uint32_t a = smem_addr(qs + qslot * 128 * D * 2), b = smem_addr(ring + size_t(s) * L::kTile);
+  } else if (warp == 1 && work) {  // ---- products: the warp walks together, one lane issues
+    constexpr uint32_t id_s = umma_idesc_bf16_m128(KT, 0), id_o = umma_idesc_bf16_m128(D, 1);
+    const bool issuer = elect_one();
+    const uint32_t q_lo = umma_lo(smem_addr(qs), 1), k_lo = umma_lo(smem_addr(ring), 1);
+    const uint32_t v_lo = umma_lo(smem_addr(ring), (KT * 128) >> 4);
+    int st = 0;               // ring stage of the next tile taken
+    uint32_t ring_ph = 0;     // and its phase
+    uint32_t p_ph = 0, o_ph = 0, q_ph = 0;  // phases by slot, as bits
+    uint32_t used = 0;        // slots with an item before
+    auto take = [&]() {
+      const int s = st;
+      paged_wait(kv_full + s, ring_ph, dead, p.err);
+      if (++st == NST) {
+        st = 0;
+        ring_ph ^= 1;
+      }
+      return s;
+    };
+    auto queries = [&](int slot) {
+      paged_wait(q_full + slot, (q_ph >> slot) & 1, dead, p.err);
+      q_ph ^= 1u << slot;
+    };
+    auto scores = [&](int slot, int qslot, int s) {
+      tc_fence_after();
+      if (issuer) {
+        const uint32_t a = q_lo + qslot * (128 * D * 2 / 16), b = k_lo + s * (L::kTile / 16), d = tmem + slot * 128;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          umma_bf16(tmem + slot * 128, umma_desc_sw128(a + (kk / 4) * (128 * 128) + (kk % 4) * 32),
-                    umma_desc_sw128(b + (kk / 4) * (KT * 128) + (kk % 4) * 32), id_s, kk != 0);
+          umma_ss(d, a + (kk / 4) * (128 * 128 / 16) + (kk % 4) * 2, b + (kk / 4) * (KT * 128 / 16) + (kk % 4) * 2, id_s,
+                  kk != 0);
         umma_commit(s_full + slot);
-      };
-      auto output = [&](int slot, int s, bool first) {
-        paged_wait(p_full + slot, np[slot] & 1, dead, p.err);
-        ++np[slot];
-        if (first && items[slot] > 0) paged_wait(o_empty + slot, (items[slot] - 1) & 1, dead, p.err);
-        tc_fence_after();
-        const uint32_t b = smem_addr(ring + size_t(s) * L::kTile);
-#pragma unroll
-        for (int kk = 0; kk < KT / 16; ++kk)
-          umma_bf16_ta(tmem + kColO + slot * D, tmem + slot * 128 + kk * 8,
-                       umma_desc_sw128_mn(b + kk * 16 * 128, KT * 128), id_o, !first || kk != 0);
-      };
-      int nitem = 0;
-      do {
-        const int nt = w.kt1 - w.kt0;
-        if constexpr (kTwo) {
-          const bool two = w.g.n * p.rep - w.qt * M > 128;
-          int ks = stage();
-          paged_wait(q_full, nitem & 1, dead, p.err);
-          scores(0, 0, ks);
-          if (two) {
-            paged_wait(q_full + 1, items[1] & 1, dead, p.err);
-            scores(1, 1, ks);
-          }
-          umma_commit(kv_empty + ks);
-          for (int t = 0; t < nt && !*dead; ++t) {
-            const int vs = stage();
-            const bool more = t + 1 < nt;
-            output(0, vs, t == 0);
-            if (!two) umma_commit(kv_empty + vs);
-            if (more) {
-              ks = stage();
-              scores(0, 0, ks);
-            } else {
-              umma_commit(o_full);
-            }
-            if (two) {
-              output(1, vs, t == 0);
-              umma_commit(kv_empty + vs);
-              if (more) scores(1, 1, ks);
-              else umma_commit(o_full + 1);
-            }
-            if (more) umma_commit(kv_empty + ks);
-          }
-          ++items[0];
-          if (two) ++items[1];
-        } else {
-          int ks[2];
-          ks[0] = stage();
-          paged_wait(q_full, nitem & 1, dead, p.err);
-          scores(0, 0, ks[0]);
-          umma_commit(kv_empty + ks[0]);
-          if (nt > 1) {
-            ks[1] = stage();
-            scores(1, 0, ks[1]);
-            umma_commit(kv_empty + ks[1]);
-          }
-          for (int t = 0; t < nt && !*dead; ++t) {
-            const int vs = stage(), slot = t & 1;
-            output(slot, vs, t < 2);
-            umma_commit(kv_empty + vs);
-            if (t + 2 < nt) {
-              const int k2 = stage();
-              scores(slot, 0, k2);
-              umma_commit(kv_empty + k2);
-            } else {
-              umma_commit(o_full + slot);
-            }
-          }
-          ++items[0];
-          if (nt > 1) ++items[1];
+      }
+    };
+    auto output = [&](int slot, int s, bool first) {
+      paged_wait(p_full + slot, (p_ph >> slot) & 1, dead, p.err);
+      p_ph ^= 1u << slot;
+      if (first) {
+        if ((used >> slot) & 1) {
+          paged_wait(o_empty + slot, (o_ph >> slot) & 1, dead, p.err);
+          o_ph ^= 1u << slot;
         }
-        ++nitem;
-      } while (!*dead && w.next(p, kinds));
-      umma_commit(drain);  // tensor memory is given back only when nothing writes it any more
-      if (!mbar_wait(drain, 0)) raise_error(p.err, kErrTimeout);
-    }
+        used |= 1u << slot;
+      }
+      tc_fence_after();
+      if (issuer) {
+        const uint32_t b = v_lo + s * (L::kTile / 16), d = tmem + kColO + slot * D, a = tmem + slot * 128;
+#pragma unroll
+        for (int kk = 0; kk < KT / 16; ++kk) umma_ts(d, a + kk * 8, b + kk * (16 * 128 / 16), id_o, !first || kk != 0);
+      }
+    };
+    auto done = [&](uint64_t* bar) {
+      if (issuer) umma_commit(bar);
+    };
+    do {
+      const int nt = w.kt1 - w.kt0;
+      if constexpr (kTwo) {
+        const bool two = w.g.n * p.rep - w.qt * M > 128;
+        int ks = take();
+        queries(0);
+        scores(0, 0, ks);
+        if (two) {
+          queries(1);
+          scores(1, 1, ks);
+        }
+        done(kv_empty + ks);
+        for (int t = 0; t < nt && !*dead; ++t) {
+          const int vs = take();
+          const bool more = t + 1 < nt;
+          output(0, vs, t == 0);
+          if (!two) done(kv_empty + vs);
+          if (more) {
+            ks = take();
+            scores(0, 0, ks);
+          } else {
+            done(o_full);
+          }
+          if (two) {
+            output(1, vs, t == 0);
+            done(kv_empty + vs);
+            if (more) scores(1, 1, ks);
+            else done(o_full + 1);
+          }
+          if (more) done(kv_empty + ks);
+        }
+      } else {
+        int ks = take();
+        queries(0);
+        scores(0, 0, ks);
+        done(kv_empty + ks);
+        if (nt > 1) {
+          ks = take();
+          scores(1, 0, ks);
+          done(kv_empty + ks);
+        }
+        for (int t = 0; t < nt && !*dead; ++t) {
+          const int vs = take(), slot = t & 1;
+          output(slot, vs, t < 2);
+          done(kv_empty + vs);
+          if (t + 2 < nt) {
+            ks = take();
+            scores(slot, 0, ks);
+            done(kv_empty + ks);
+          } else {
+            done(o_full + slot);
+          }
+        }
+      }
+    } while (!*dead && w.next(p, kinds));
+    done(drain);  // tensor memory is given back only when nothing writes it any more
+    if (!mbar_wait(drain, 0)) raise_error(p.err, kErrTimeout);
     __syncwarp();
+  }
   } else {  // ---- softmax: thread = row of its slot
-    const int slot = (warp - 2) >> 2, qd = warp & 3, r128 = qd * 32 + lane;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;\n");
+    if (work) {
+    const int slot = (warp - 4) >> 2, qd = warp & 3, r128 = qd * 32 + lane;
     const uint32_t lanes = tmem + (uint32_t(qd * 32) << 16);
     const uint32_t ts = lanes + slot * 128, to = lanes + kColO + slot * D;
     const float sl2 = p.scale_log2;
@@ -1275,16 +1294,11 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
       const int edge = min(w.g.klen, w.g.prefix ? w.g.klen
                                                 : w.g.klen - w.g.n + (p.tree ? 0 : (w.qt * M + (kTwo ? slot * 128 : 0)) / p.rep + 1));
       float m = -INFINITY, l = 0.f;
-      PagedWalk<M, KT> nx = w;
-      more = nx.next(p, kinds);
-      const bool load_next = more && (!kTwo || slot == 0 || both(nx));
       const int step = kTwo ? 1 : 2;
       for (int t = kTwo ? 0 : slot; t < nt && active; t += step) {
         paged_wait(s_full + slot, ns & 1, dead, p.err);
         ++ns;
         tc_fence_after();
-        // the item's queries have been used for the last time: the next item's take their place
-        if (load_next && t + 1 == nt) load_q(nx);
         uint32_t s0[64], s1[64];
         tmem_ld64(ts, s0);
         tmem_ld64(ts + 64, s1);
@@ -1382,8 +1396,13 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full + slot);
       }
-      if (kTwo && !active && load_next) load_q(nx);
       vcnt += 2 * nt;
+      // The item's queries have been used for the last time where the last scores were waited for (in
+      // the alternating form that is the last tile's slot): the next item's take their place while the
+      // last product runs.
+      PagedWalk<M, KT> nx = w;
+      more = nx.next(p, kinds);
+      if (more && (kTwo ? slot == 0 || both(nx) : ((nt - 1) & 1) == slot)) load_q(nx);
       // ---- the item's result
       float f0 = 1.f, f1 = 0.f;
       if constexpr (!kTwo) {  // the slots' states joined; each group of warps takes half of the columns
@@ -1476,6 +1495,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
       w = nx;
       ++nitem;
     } while (more);
+    }
   }
   tc_fence_before();
   __syncthreads();

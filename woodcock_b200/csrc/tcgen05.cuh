@@ -58,25 +58,40 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// MN-major operand written by TMA with the 128-byte swizzle: rows of 128 bytes are K indices (8-row groups
-// 1024 bytes apart = stride byte offset), 64-element MN blocks `mn_block` bytes apart (leading byte offset).
-__device__ __forceinline__ uint64_t umma_desc_sw128_mn(uint32_t saddr, uint32_t mn_block) {
-  return uint64_t((saddr & 0x3FFFFu) >> 4) | (uint64_t(mn_block >> 4) << 16) | (uint64_t(1024 >> 4) << 32) |
-         (uint64_t(1) << 46) | (uint64_t(2) << 61);
-}
+// The MN-major operand of a TMA tile with the 128-byte swizzle has rows of 128 bytes as K indices (8-row
+// groups 1024 bytes apart = stride byte offset) and 64-element MN blocks `leading` * 16 bytes apart.
 // Instruction descriptor, kind::f16: fp32 accumulator, bf16 A and B, M 128; B K-major or MN-major.
 __host__ __device__ constexpr uint32_t umma_idesc_bf16_m128(int N, int b_mn_major) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(b_mn_major) << 16) | (uint32_t(N >> 3) << 17) |
          (uint32_t(128 >> 4) << 24);
 }
-// A from tensor memory: lane = row, one 32-bit column = two consecutive bf16 K elements.
-__device__ __forceinline__ void umma_bf16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
-                                             uint32_t accumulate) {
+// A shared-memory descriptor as its address field (low word) and its constant high word: the address
+// of a later slice of the same tile is a 32-bit addition away.
+__device__ __forceinline__ uint32_t umma_lo(uint32_t saddr, uint32_t leading) {
+  return ((saddr & 0x3FFFFu) >> 4) | (leading << 16);
+}
+constexpr uint32_t kUmmaHiSw128 = (1024u >> 4) | (1u << 14) | (2u << 29);  // stride 1024 bytes, version 1, 128B swizzle
+// kind::f16 products of one thread, operands given by their descriptors' words
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t alo, uint32_t blo, uint32_t idesc, bool acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "{\n .reg .pred p;\n .reg .b64 a, b;\n setp.ne.b32 p, %4, 0;\n mov.b64 a, {%1, %5};\n mov.b64 b, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n}\n" ::"r"(d),
+      "r"(alo), "r"(blo), "r"(idesc), "r"(uint32_t(acc)), "r"(kUmmaHiSw128)
       : "memory");
+}
+// the same with A in tensor memory: lane = row, one 32-bit column = two consecutive bf16 K elements
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t blo, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 b;\n setp.ne.b32 p, %4, 0;\n mov.b64 b, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(blo), "r"(idesc), "r"(uint32_t(acc)), "r"(kUmmaHiSw128)
+      : "memory");
+}
+// one lane of a converged warp
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+  return r != 0;
 }
 #define WC_R8(a, i) "=r"((a)[i]), "=r"((a)[i + 1]), "=r"((a)[i + 2]), "=r"((a)[i + 3]), "=r"((a)[i + 4]), \
                     "=r"((a)[i + 5]), "=r"((a)[i + 6]), "=r"((a)[i + 7])
