@@ -226,7 +226,7 @@ Launch plan_launch(const wc_ctx* ctx, const wc_pages& g, long long rows) {
 
 struct Layout {
   Launch own, prefix;
-  size_t part_o[2], part_ml[2], desc[2], whole_o[2], whole_ml[2], bytes;
+  size_t part_o[2], part_ml[2], rec, desc[2], whole_o[2], whole_ml[2], bytes;
 };
 
 size_t take(size_t& at, size_t bytes) {
@@ -251,8 +251,10 @@ Layout layout(const wc_ctx* ctx, const wc_paged_attention_args& a) {
     const size_t items = size_t((long long)b.rows * rep / x.M) + (kind ? a.groups : b.requests) + 2;
     l.part_o[kind] = take(at, slots * g.head_dim * sizeof(float));
     l.part_ml[kind] = take(at, slots * sizeof(float2));
-    l.desc[kind] = take(at, items * g.kv_heads * sizeof(int4));
-    if (a.groups) {
+    if (!a.groups) {
+      l.rec = take(at, x.blocks * sizeof(PagedRec));
+    } else {
+      l.desc[kind] = take(at, items * g.kv_heads * sizeof(int2));
       l.whole_o[kind] = take(at, size_t(b.rows) * b.heads * g.head_dim * sizeof(float));
       l.whole_ml[kind] = take(at, size_t(b.rows) * b.heads * sizeof(float2));
     }
@@ -299,38 +301,40 @@ CUtensorMap page_map(const wc_pages& g, const PagePool& pool, int rows) {
 }
 
 template <int D, int RG>
-void launch_few(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, const PagedAttnParams& p, int kinds, const Launch& l) {
-  const size_t smem = PfLayout<D>::bytes();
-  static_assert(PfLayout<D>::bytes() <= kSmemOptinBytes, "shared memory");
+void launch_few(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, const PagedAttnParams& p, int kinds, const Launch& l,
+                 bool late) {
+  const size_t smem = PfLayout<D, 16 * RG>::bytes();
+  static_assert(PfLayout<D, 16 * RG>::bytes() <= kSmemOptinBytes, "shared memory");
   opt_in(ctx, paged_few_kernel<D, RG>, smem);
   launch_on(ctx, st, "paged_few", paged_few_kernel<D, RG>, dim3(l.blocks), dim3(PF_THREADS), smem, true, 1,
-            page_map(g, p.K, PF_KT), page_map(g, p.V, PF_KT), p, kinds, l.min_per);
+            page_map(g, p.K, PF_KT), page_map(g, p.V, PF_KT), p, kinds, l.min_per, late);
 }
 
 template <int D, bool kTwo>
-void launch_many(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, const PagedAttnParams& p, int kinds, const Launch& l) {
+void launch_many(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, const PagedAttnParams& p, int kinds, const Launch& l,
+                 bool late) {
   const size_t smem = PmLayout<D, kTwo>::bytes();
   static_assert(PmLayout<D, kTwo>::bytes() <= kSmemOptinBytes, "shared memory");
   opt_in(ctx, paged_many_kernel<D, kTwo>, smem);
   launch_on(ctx, st, "paged_many", paged_many_kernel<D, kTwo>, dim3(l.blocks), dim3(PM_THREADS), smem, true, 1,
-            page_map(g, p.K, PM_KT), page_map(g, p.V, PM_KT), p, kinds, l.min_per);
+            page_map(g, p.K, PM_KT), page_map(g, p.V, PM_KT), p, kinds, l.min_per, late);
 }
 
 template <typename S, int D>
 void launch_attention(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, const PagedAttnParams& p, int kinds,
-                      const Launch& l) {
+                      const Launch& l, bool late) {
   if constexpr (sizeof(S) == 4) {
     opt_in(ctx, paged_simt_kernel<S, D>, paged_simt_smem<D>());
     launch_on(ctx, st, "paged_simt", paged_simt_kernel<S, D>, dim3(l.blocks), dim3(PS_THREADS), paged_simt_smem<D>(),
-              true, 1, p, kinds, l.min_per);
+              true, 1, p, kinds, l.min_per, late);
   } else if (l.variant == kFew16) {
-    launch_few<D, 1>(ctx, st, g, p, kinds, l);
+    launch_few<D, 1>(ctx, st, g, p, kinds, l, late);
   } else if (l.variant == kFew32) {
-    launch_few<D, 2>(ctx, st, g, p, kinds, l);
+    launch_few<D, 2>(ctx, st, g, p, kinds, l, late);
   } else if (l.variant == kMany128) {
-    launch_many<D, false>(ctx, st, g, p, kinds, l);
+    launch_many<D, false>(ctx, st, g, p, kinds, l, late);
   } else {
-    launch_many<D, true>(ctx, st, g, p, kinds, l);
+    launch_many<D, true>(ctx, st, g, p, kinds, l, late);
   }
 }
 
@@ -342,14 +346,23 @@ void attend(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, PagedAttnParams p, 
     const Launch& x = kind ? l.prefix : l.own;
     p.part_o = reinterpret_cast<float*>(ws + l.part_o[kind]);
     p.part_ml = reinterpret_cast<float2*>(ws + l.part_ml[kind]);
-    launch_attention<S, D>(ctx, st, g, p, kind ? kPrefixRows : kOwnRows, x);
+    // The own rows' kernel needs nothing of the prefixes': it may start beside it, and waits for it at
+    // its end, so that the joining kernel comes after both.
+    launch_attention<S, D>(ctx, st, g, p, kind ? kPrefixRows : kOwnRows, x, p.G && !kind && ctx->pdl);
     c.part_o[kind] = p.part_o;
     c.part_ml[kind] = p.part_ml;
     c.M[kind] = x.M;
     c.blocks[kind] = x.blocks;
   }
-  c.a = p;
-  launch_on(ctx, st, "paged_combine", paged_combine_kernel<S, D>, dim3(p.T), dim3(PJ_THREADS), 0, true, 1, c);
+  if (!p.G) {
+    launch_on(ctx, st, "paged_join", paged_join_kernel<S, D>, dim3(l.own.blocks, l.own.M / PJ_ROWS),
+              dim3(PJ_ROWS * D / 4), 0, true, 1, p, l.own.M);
+  } else {
+    c.a = p;
+    const int heads = PC_JOIN / (D / 4);  // a block's
+    launch_on(ctx, st, "paged_combine", paged_combine_kernel<S, D>, dim3(p.T, (p.H + heads - 1) / heads),
+              dim3(PC_JOIN), 0, true, 1, c);
+  }
 }
 
 }  // namespace
@@ -408,9 +421,9 @@ extern "C" wc_status wc_paged_attention(wc_ctx* ctx, void* stream, const wc_page
     p.rep = b.heads / g.kv_heads;
     p.scale_log2 = a->scale * kLog2e;
     p.out = a->out;
-    p.desc_own = reinterpret_cast<int4*>(ws + l.desc[0]);
-    p.desc_prefix = reinterpret_cast<int4*>(ws + l.desc[1]);
+    p.rec = reinterpret_cast<PagedRec*>(ws + l.rec);
     for (int i = 0; i < 2; ++i) {
+      p.desc[i] = reinterpret_cast<int2*>(ws + l.desc[i]);
       p.whole_o[i] = reinterpret_cast<float*>(ws + l.whole_o[i]);
       p.whole_ml[i] = reinterpret_cast<float2*>(ws + l.whole_ml[i]);
     }

@@ -258,6 +258,11 @@ __global__ void __launch_bounds__(PC_THREADS) paged_compact_kernel(const __grid_
 // block order by the combine kernel: no atomics, the same result every time.
 enum PagedKinds : int { kOwnRows = 1, kPrefixRows = 2 };
 
+// A divided item as the joining kernel needs it; count 0: none.
+struct PagedRec {
+  int tok0, rows, qt, head, count, pad[3];  // rows: the segment's, times rep
+};
+
 struct PagedAttnParams {
   const void* q;
   long long q_row, q_head;
@@ -278,9 +283,9 @@ struct PagedAttnParams {
   // workspace
   float* part_o;                // [blocks][2][M][D]
   float2* part_ml;              // [blocks][2][M]
-  int4* desc_own;               // per item: {first block, number of blocks, redo rows 0-127, redo rows 128-255}
-  int4* desc_prefix;
-  float* whole_o[2];            // with prefixes: items of one block, [T][H][D] (own, prefix)
+  PagedRec* rec;                // [blocks], without prefixes: the divided item that begins in the block
+  int2* desc[2];                // with prefixes, per item (own, prefix): {first block, number of blocks}
+  float* whole_o[2];            // with prefixes: items of one block, [T][H][D]
   float2* whole_ml[2];          // [T][H]
   int* err;
 };
@@ -338,22 +343,28 @@ __device__ __forceinline__ long long paged_head_tiles(const PagedAttnParams& p, 
   return n;
 }
 
-// One block's walk over its range of key tiles, item by item.
-template <int M, int KT>
+// One block's walk over its range of the line, item by item. An item counts kOver units beyond its key
+// tiles, for what it costs whatever its length (its queries, its result, the way there); a block whose
+// range holds only such units of an item passes it over.
+template <int M, int KT, int kOver>
 struct PagedWalk {
   PagedSeg g;
   int head, qt, qts;    // the item
   int kt0, kt1, ktn;    // this block's key tiles [kt0, kt1) of the item's ktn
   int first, count;     // the blocks that share the item
-  int seg, nseg;
-  long long pos, end;   // tiles of the line: the item's first one here, the block's end
-  int per;
+  int seg, nseg, per;
+  long long pos, end;   // units of the line: the item's first one here, the block's end
+
+  __device__ static long long units(const PagedAttnParams& p, const PagedSeg& g) {
+    const int qts = (g.n * p.rep + M - 1) / M;
+    return paged_head_tiles<M, KT>(p, g) + (long long)qts * kOver;
+  }
 
   // Block-collective; `sh` holds kWalkShared words. False: the block has no work.
   __device__ bool begin(const PagedAttnParams& p, int kinds, int min_per, long long* sh) {
     nseg = ((kinds & kPrefixRows) ? p.G : 0) + ((kinds & kOwnRows) ? p.B : 0);
     const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, nw = (nt + 31) >> 5;
-    long long total = 0;
+    long long total = 0, w = 0, x = 0;
     pos = 0;
     for (int pass = 0; pass < 2; ++pass) {
       if (pass) {
@@ -365,28 +376,30 @@ struct PagedWalk {
       long long base = 0;
       for (int s0 = 0; s0 < nseg; s0 += nt) {
         const int s = s0 + tid;
-        long long w = 0;
-        if (s < nseg) w = paged_head_tiles<M, KT>(p, paged_seg(p, kinds, s)) * p.Hk;
-        long long x = w;
+        if (!pass || nseg > nt) {  // one round of segments: the first pass has it all
+          w = 0;
+          if (s < nseg) w = units(p, paged_seg(p, kinds, s)) * p.Hk;
+          x = w;
 #pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-          const long long y = __shfl_up_sync(0xffffffffu, x, o);
-          if (lane >= o) x += y;
+          for (int o = 1; o < 32; o *= 2) {
+            const long long y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+          }
+          if (lane == 31) sh[warp] = x;
+          __syncthreads();
         }
-        if (lane == 31) sh[warp] = x;
-        __syncthreads();
         long long before = base, all = 0;
         for (int i = 0; i < nw; ++i) {
           if (i < warp) before += sh[i];
           all += sh[i];
         }
-        const long long a = before + x - w;  // the segment's first tile
+        const long long a = before + x - w;  // the segment's first unit
         if (pass && a <= pos && pos < a + w) {
           sh[32] = s;
           sh[33] = pos - a;
         }
         base += all;
-        __syncthreads();
+        if (pass || nseg > nt) __syncthreads();
       }
       total = base;
     }
@@ -394,38 +407,41 @@ struct PagedWalk {
     long long off = sh[33];
     g = paged_seg(p, kinds, seg);
     qts = (g.n * p.rep + M - 1) / M;
-    const long long ph = paged_head_tiles<M, KT>(p, g);
+    const long long ph = units(p, g);
     head = int(off / ph);
     off -= head * ph;
     qt = 0;
-    while (off >= (ktn = paged_item_tiles<M, KT>(p, g, qt))) {
-      off -= ktn;
+    while (off >= (ktn = paged_item_tiles<M, KT>(p, g, qt)) + kOver) {
+      off -= ktn + kOver;
       ++qt;
     }
-    place(int(off));
-    return true;
+    return place(int(off)) || next(p, kinds);
   }
-  __device__ void place(int off) {
-    kt0 = off;
-    kt1 = int(min((long long)ktn, off + (end - pos)));
-    first = int((pos - off) / per);
-    count = int((pos - off + ktn - 1) / per) - first + 1;
+  // The item's tiles in this block's range; false: only units that hold no tiles.
+  __device__ bool place(int off) {
+    const long long item = pos - off;  // the item's first unit
+    kt0 = max(0, off - kOver);
+    kt1 = int(min((long long)ktn, end - item - kOver));
+    first = int((item + kOver) / per);
+    count = int((item + kOver + ktn - 1) / per) - first + 1;
+    pos = min(end, item + kOver + ktn);
+    return kt1 > kt0;
   }
   __device__ bool next(const PagedAttnParams& p, int kinds) {
-    pos += kt1 - kt0;
-    if (pos >= end) return false;
-    if (++qt == qts) {
-      qt = 0;
-      if (++head == p.Hk) {
-        head = 0;
-        do {
-          g = paged_seg(p, kinds, ++seg);
-        } while (g.n == 0);
-        qts = (g.n * p.rep + M - 1) / M;
+    do {
+      if (pos >= end) return false;
+      if (++qt == qts) {
+        qt = 0;
+        if (++head == p.Hk) {
+          head = 0;
+          do {
+            g = paged_seg(p, kinds, ++seg);
+          } while (g.n == 0);
+          qts = (g.n * p.rep + M - 1) / M;
+        }
       }
-    }
-    ktn = paged_item_tiles<M, KT>(p, g, qt);
-    place(0);
+      ktn = paged_item_tiles<M, KT>(p, g, qt);
+    } while (!place(0));
     return true;
   }
   // Number of the item among those of its kind and head: distinct, below T rep / M + segments + 1.
@@ -434,7 +450,17 @@ struct PagedWalk {
   }
   // Where this block's share of a divided item goes: slot 0 when the item began in an earlier block.
   __device__ int slot() const { return kt0 > 0 ? 0 : 1; }
+  // One thread, once per item: what the joining kernel needs to know of it.
+  __device__ void report(const PagedAttnParams& p) const {
+    if (kt0 > 0) return;
+    if (p.G > 0) p.desc[g.prefix][item(p) * p.Hk + head] = make_int2(first, count);
+    else if (count > 1) p.rec[blockIdx.x] = PagedRec{g.tok0, g.n * p.rep, qt, head, count, {}};
+  }
 };
+// Before the first report of a block.
+__device__ __forceinline__ void paged_no_rec(const PagedAttnParams& p) {
+  if (p.G == 0 && threadIdx.x == 0) p.rec[blockIdx.x] = PagedRec{};
+}
 constexpr int kWalkShared = 34;
 
 // What one query row sees: keys below `lim`, and with a tree the new rows in `bits`.
@@ -503,7 +529,7 @@ constexpr size_t paged_simt_smem() {
 
 template <typename S, int D>
 __global__ void __launch_bounds__(PS_THREADS)
-    paged_simt_kernel(const __grid_constant__ PagedAttnParams p, int kinds, int min_per) {
+    paged_simt_kernel(const __grid_constant__ PagedAttnParams p, int kinds, int min_per, bool late) {
   constexpr int M = PS_M, KT = PS_KT, LD = D + 4, LS = KT + 4;
   constexpr int RPT = D / 64;  // rows per thread of P V: two (D 128), one (D 64)
   extern __shared__ __align__(16) float ps_smem[];
@@ -513,10 +539,14 @@ __global__ void __launch_bounds__(PS_THREADS)
   float* ss = qs + M * D;
   long long* sh = reinterpret_cast<long long*>(ss + M * LS);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (!late) pdl_wait();
   pdl_launch_dependents();
-  pdl_wait();
-  PagedWalk<M, KT> w;
-  if (!w.begin(p, kinds, min_per, sh)) return;
+  PagedWalk<M, KT, 1> w;
+  paged_no_rec(p);
+  if (!w.begin(p, kinds, min_per, sh)) {
+    if (late) pdl_wait();
+    return;
+  }
   do {
     __syncthreads();
     for (int c = tid; c < M * (D / 8); c += PS_THREADS) {
@@ -600,8 +630,7 @@ __global__ void __launch_bounds__(PS_THREADS)
         }
       }
     }
-    if (w.kt0 == 0 && tid == 0)
-      (w.g.prefix ? p.desc_prefix : p.desc_own)[w.item(p) * p.Hk + w.head] = make_int4(w.first, w.count, 0, 0);
+    if (tid == 0) w.report(p);
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
       const int ri = D == 64 ? lane / 16 : i;
@@ -631,6 +660,45 @@ __global__ void __launch_bounds__(PS_THREADS)
       }
     }
   } while (w.next(p, kinds));
+  if (late) pdl_wait();
+}
+
+// A row's state over keys [k0, k1), key by key and without those that it does not see: the slow way,
+// warp-collective, for rows beside a value that is not finite.
+template <int D>
+__device__ __forceinline__ void paged_redo_row(const PagedAttnParams& p, const PagedSeg& g, const PagedRow& r, int head,
+                                               int k0, int k1, int lane, float& M, float& L, float (&o)[D / 32]) {
+  constexpr int E = D / 32;
+  M = -INFINITY;
+  L = 0.f;
+  float q[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    o[e] = 0.f;
+    q[e] = bf16_bits_to_f32(static_cast<const uint16_t*>(p.q)[r.tok * p.q_row + r.h * p.q_head + lane * E + e]);
+  }
+#pragma unroll 1
+  for (int key = k0; key < min(k1, g.klen); ++key) {
+    if (!r.sees(key)) continue;
+    const int page = paged_page(p, g, key >> p.page_log2), pr = key & ((1 << p.page_log2) - 1);
+    float v[E] = {}, z = 0.f;
+    if (page >= 0) {
+      const uint16_t* kp = static_cast<const uint16_t*>(p.K.ptr) + page * p.K.page + head * p.K.head + pr * p.K.row + lane * E;
+      const uint16_t* vp = static_cast<const uint16_t*>(p.V.ptr) + page * p.V.page + head * p.V.head + pr * p.V.row + lane * E;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        z = fmaf(q[e], bf16_bits_to_f32(kp[e]), z);
+        v[e] = bf16_bits_to_f32(vp[e]);
+      }
+    }
+    z = warp_sum(z) * p.scale_log2;
+    const float mn = fmaxf(M, z), mg = mn == -INFINITY ? 0.f : mn;
+    const float wa = exp2f(M - mg), wb = exp2f(z - mg);
+    M = mn;
+    L = L * wa + wb;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = o[e] * wa + wb * v[e];
+  }
 }
 
 // ---------------------------------------------------------------------------- few rows: streamed pages
@@ -644,19 +712,26 @@ __global__ void __launch_bounds__(PS_THREADS)
 constexpr int PF_CONSUMERS = 8;
 constexpr int PF_THREADS = 32 * (PF_CONSUMERS + 1);
 constexpr int PF_KT = 64;
+constexpr int PF_OVER = 1;
 
-template <int D>
+template <int D, int M>
 struct PfLayout {
   static constexpr int kTile = PF_KT * D * 2;          // K or V of one tile
   static constexpr int kStage = 2 * kTile;
   static constexpr int kJoin = 4 * 16 * D * 4;         // four 16-row partial outputs
-  static constexpr int kTail = 8 * kWalkShared + 256 + 8 * 16 * 8 + 32 * 8;
-  // An even number: a stage then always belongs to the same set of warps, whose waits see each of its
-  // phases. (With an odd ring a set would meet a stage every other use, and a wait by parity would take
-  // the use before last, which another set reads, for its own.)
-  static constexpr int kStages = (int(kSmemOptinBytes) - 1024 - kJoin - kTail) / kStage & ~1;
-  static constexpr size_t bytes() { return 1024 + size_t(kStages) * kStage + kJoin + kTail; }
+  static constexpr int kQRow = (D + 8) * 2;            // a query row, padded against bank conflicts
+  static constexpr int kQ = 2 * M * kQRow;             // two items' queries
+  static constexpr int kTail = 8 * kWalkShared + 256 + 8 * 16 * 8 + M * 8 + 2 * 64;
+  static constexpr int kStages = (int(kSmemOptinBytes) - 1024 - kJoin - kQ - kTail) / kStage;
+  static constexpr size_t bytes() { return 1024 + size_t(kStages) * kStage + kJoin + kQ + kTail; }
 };
+
+// An item as the producer hands it to the other warps.
+struct PfItem {
+  PagedSeg g;
+  int head, qt, kt0, kt1, count, slot, pad[5];
+};
+static_assert(sizeof(PfItem) == 64, "item queue");
 
 // Waits give up after a bound; then `dead` lets the block's other waits pass, so that it ends.
 __device__ __forceinline__ void paged_wait(uint64_t* bar, uint32_t parity, volatile int* dead, int* err) {
@@ -701,35 +776,48 @@ struct PageWindow {
 template <int D, int RG>
 __global__ void __launch_bounds__(PF_THREADS, 1)
     paged_few_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
-                     const __grid_constant__ PagedAttnParams p, int kinds, int min_per) {
-  using L = PfLayout<D>;
-  constexpr int M = 16 * RG, KT = PF_KT, NST = L::kStages, NK = D / 16, ND = D / 8;
-  constexpr int kWarpsPerTile = RG == 1 ? 4 : 8;
+                     const __grid_constant__ PagedAttnParams p, int kinds, int min_per, bool late) {
+  constexpr int M = 16 * RG, KT = PF_KT, NK = D / 16, ND = D / 8;
+  using L = PfLayout<D, M>;
+  constexpr int NST = L::kStages;
   extern __shared__ unsigned char pf_raw[];
   unsigned char* sm = pf_raw + ((1024u - (smem_addr(pf_raw) & 1023u)) & 1023u);
   float* join = reinterpret_cast<float*>(sm + size_t(NST) * L::kStage);
-  unsigned char* tail = reinterpret_cast<unsigned char*>(join) + L::kJoin;
+  unsigned char* qbuf = reinterpret_cast<unsigned char*>(join) + L::kJoin;
+  unsigned char* tail = qbuf + L::kQ;
   long long* sh = reinterpret_cast<long long*>(tail);
-  uint64_t* full = reinterpret_cast<uint64_t*>(tail + 8 * kWalkShared);
+  uint64_t* it_full = reinterpret_cast<uint64_t*>(tail + 8 * kWalkShared);  // [2] items handed over
+  uint64_t* it_empty = it_full + 2;
+  uint64_t* full = it_full + 4;
   uint64_t* empty = full + NST;
   volatile int* dead = reinterpret_cast<volatile int*>(tail + 8 * kWalkShared + 248);
+  volatile int* stop = dead + 1;
   float2* wml = reinterpret_cast<float2*>(tail + 8 * kWalkShared + 256);  // [8 warps][16 rows]
   float2* rml = wml + 8 * 16;                                            // [M]
-  static_assert(16 * NST <= 248, "barriers");
+  PfItem* items = reinterpret_cast<PfItem*>(rml + M);                    // [2]
+  static_assert(32 + 16 * NST <= 248, "barriers");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int s = 0; s < NST; ++s) {
       mbar_init(full + s, 1);
-      mbar_init(empty + s, kWarpsPerTile);
+      mbar_init(empty + s, PF_CONSUMERS);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(it_full + s, 1);
+      mbar_init(it_empty + s, PF_CONSUMERS);
     }
     mbar_fence_init();
     *dead = 0;
   }
+  if (!late) pdl_wait();
   pdl_launch_dependents();
-  pdl_wait();
-  PagedWalk<M, KT> w;
+  PagedWalk<M, KT, PF_OVER> w;
+  paged_no_rec(p);
   __syncthreads();
-  if (!w.begin(p, kinds, min_per, sh)) return;
+  if (!w.begin(p, kinds, min_per, sh)) {
+    if (late) pdl_wait();
+    return;
+  }
 
   if (warp == PF_CONSUMERS) {  // ---- producer
     const int psize = 1 << p.page_log2;
@@ -737,8 +825,27 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     constexpr int HALVES = D / 64;
     const int part = lane / (2 * HALVES), half = (lane >> 1) % HALVES;
     const bool isv = lane & 1, issue = part < parts;
-    int cnt = 0;
+    int cnt = 0, nitem = 0;
+    bool more = true;
     do {
+      // the item and its query rows (those past the segment's keep what the buffer holds: nobody reads them)
+      const int b = nitem & 1;
+      if (lane == 0) {
+        w.report(p);
+        if (nitem >= 2) paged_wait(it_empty + b, ((nitem >> 1) - 1) & 1, dead, p.err);
+        items[b] = PfItem{w.g, w.head, w.qt, w.kt0, w.kt1, w.count, w.slot(), {}};
+        const int rows = min(M, w.g.n * p.rep - w.qt * M);
+        if (!*dead) mbar_arrive_expect_tx(it_full + b, rows * D * 2);
+      }
+      __syncwarp();
+      if (*dead) break;
+      {
+        const PagedRow r = paged_row(p, w.g, w.head, w.qt * M + lane);
+        if (lane < M && r.valid)
+          bulk_g2s(qbuf + (b * M + lane) * L::kQRow,
+                   static_cast<const uint16_t*>(p.q) + r.tok * p.q_row + r.h * p.q_head, D * 2, it_full + b);
+      }
+      ++nitem;
       PageWindow win;
       win.start(p, w.g, (w.kt0 * KT) >> p.page_log2, lane);
       for (int kt = w.kt0; kt < w.kt1; ++kt, ++cnt) {
@@ -757,11 +864,24 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
                       isv ? &tv : &tk, half * 64, (kt * KT) & (psize - 1), w.head, page, full + s);
         __syncwarp();
       }
-    } while (!*dead && w.next(p, kinds));
-    // shared memory must outlive the copies
-    if (lane == 0)
+      more = !*dead && w.next(p, kinds);
+    } while (more);
+    if (lane == 0) {
+      const int b = nitem & 1;
+      if (nitem >= 2) paged_wait(it_empty + b, ((nitem >> 1) - 1) & 1, dead, p.err);
+      const bool closed = !*dead;
+      if (closed) {  // an item without blocks ends the line
+        items[b].count = 0;
+        mbar_arrive(it_full + b);
+      }
+      // shared memory must outlive the copies
       for (int q = max(0, cnt - NST); q < cnt; ++q)
         if (!mbar_wait(full + q % NST, (q / NST) & 1)) raise_error(p.err, kErrTimeout);
+      for (int q = max(0, nitem - (closed ? 1 : 2)); q < nitem; ++q)  // the closing item's buffer was empty
+        if (!mbar_wait(it_full + (q & 1), (q >> 1) & 1)) raise_error(p.err, kErrTimeout);
+    }
+    __syncwarp();
+    if (late) pdl_wait();
     return;
   }
 
@@ -771,21 +891,23 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   const int slice = RG == 1 ? (warp & 3) : (warp >> 1);
   const float sl2 = p.scale_log2;
   int cnt = 0;
-  do {
-    const PagedRow ra = paged_row(p, w.g, w.head, w.qt * M + rg * 16 + g);
-    const PagedRow rb = paged_row(p, w.g, w.head, w.qt * M + rg * 16 + g + 8);
+  for (int nitem = 0;; ++nitem) {
+    // One thread says for all of them whether the line goes on: the warps meet at the item's end, so
+    // none may leave alone. The barrier also frees the joining space of the item before.
+    const int b = nitem & 1;
+    paged_wait(it_full + b, (nitem >> 1) & 1, dead, p.err);
+    if (tid == 0) *stop = *dead || items[b].count == 0;
+    named_sync(1, 32 * PF_CONSUMERS);
+    if (*stop) break;
+    const PfItem it = items[b];
+    const PagedRow ra = paged_row(p, it.g, it.head, it.qt * M + rg * 16 + g);
+    const PagedRow rb = paged_row(p, it.g, it.head, it.qt * M + rg * 16 + g + 8);
     uint32_t qa[NK][4];
-    {
-      const uint16_t* qp0 = static_cast<const uint16_t*>(p.q) + ra.tok * p.q_row + ra.h * p.q_head + 2 * t;
-      const uint16_t* qp1 = static_cast<const uint16_t*>(p.q) + rb.tok * p.q_row + rb.h * p.q_head + 2 * t;
 #pragma unroll
-      for (int kk = 0; kk < NK; ++kk) {
-        qa[kk][0] = ra.valid ? *reinterpret_cast<const uint32_t*>(qp0 + kk * 16) : 0u;
-        qa[kk][1] = rb.valid ? *reinterpret_cast<const uint32_t*>(qp1 + kk * 16) : 0u;
-        qa[kk][2] = ra.valid ? *reinterpret_cast<const uint32_t*>(qp0 + kk * 16 + 8) : 0u;
-        qa[kk][3] = rb.valid ? *reinterpret_cast<const uint32_t*>(qp1 + kk * 16 + 8) : 0u;
-      }
-    }
+    for (int kk = 0; kk < NK; ++kk)
+      ldsm_x4(qa[kk], qbuf + (b * M + rg * 16 + (lane & 15)) * L::kQRow + kk * 32 + (lane >> 4) * 16);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(it_empty + b);
     // rows that pad the tile count as seeing everything: their results go nowhere
     const int lim0 = ra.valid ? ra.lim : 0x7fffffff, lim1 = rb.valid ? rb.lim : 0x7fffffff;
     const int lim = min(lim0, lim1);
@@ -796,10 +918,16 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
-    for (int kt = w.kt0; kt < w.kt1; ++kt, ++cnt) {
-      if (RG == 1 && (cnt & 1) != (warp >> 2)) continue;
+    for (int kt = it.kt0; kt < it.kt1; ++kt, ++cnt) {
       const int s = cnt % NST;
       paged_wait(full + s, (cnt / NST) & 1, dead, p.err);
+      if (RG == 1 && (cnt & 1) != (warp >> 2)) {
+        // The other set's tile. Its phases are waited for and passed on all the same: a set that met a
+        // stage only every other use could take an earlier use, which a wait by parity does not tell
+        // apart, for its own.
+        if (lane == 0) mbar_arrive(empty + s);
+        continue;
+      }
       const unsigned char* kb = sm + size_t(s) * L::kStage + slice * 16 * 128;  // the slice's first key
       const unsigned char* vb = kb + L::kTile;
       // ---- S = Q K^T, 16 keys: the dims in two chains of each n-tile
@@ -967,12 +1095,10 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       }
     }
     named_sync(1, 32 * PF_CONSUMERS);
-    if (w.kt0 == 0 && tid == 0)
-      (w.g.prefix ? p.desc_prefix : p.desc_own)[w.item(p) * p.Hk + w.head] = make_int4(w.first, w.count, 0, 0);
     for (int c = tid; c < M * (D / 4); c += 32 * PF_CONSUMERS) {
       const int row = c / (D / 4), col = (c % (D / 4)) * 4;
-      const int rho = w.qt * M + row;
-      if (rho >= w.g.n * p.rep) continue;
+      const int rho = it.qt * M + row;
+      if (rho >= it.g.n * p.rep) continue;
       float y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int q = 0; q < 4; q += RG) {
@@ -984,23 +1110,23 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       }
       const float2 ml = rml[row];
       const int i = rho / p.rep;
-      const long long to = (long long)(w.g.tok0 + i) * p.H + w.head * p.rep + (rho - i * p.rep);
-      if (w.count == 1 && p.G == 0) {
+      const long long to = (long long)(it.g.tok0 + i) * p.H + it.head * p.rep + (rho - i * p.rep);
+      if (it.count == 1 && p.G == 0) {
         const float inv = ml.y > 0.f ? 1.f / ml.y : (ml.y == 0.f ? 0.f : ml.y);
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] *= inv;
         store4(static_cast<uint16_t*>(p.out) + to * D + col, y);
-      } else if (w.count == 1) {
-        store4(p.whole_o[w.g.prefix] + to * D + col, y);
-        if (col == 0) p.whole_ml[w.g.prefix][to] = ml;
+      } else if (it.count == 1) {
+        store4(p.whole_o[it.g.prefix] + to * D + col, y);
+        if (col == 0) p.whole_ml[it.g.prefix][to] = ml;
       } else {
-        const long long pt = ((long long)blockIdx.x * 2 + w.slot()) * M + row;
+        const long long pt = ((long long)blockIdx.x * 2 + it.slot) * M + row;
         store4(p.part_o + pt * D + col, y);
         if (col == 0) p.part_ml[pt] = ml;
       }
     }
-    named_sync(1, 32 * PF_CONSUMERS);  // the joining space is free for the next item
-  } while (w.next(p, kinds));
+  }
+  if (late) pdl_wait();
 }
 
 // ---------------------------------------------------------------------------- many rows: tensor memory
@@ -1014,6 +1140,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
 // then at most 2^8 instead of 1, and the final division by the sum takes the same factor out.
 constexpr int PM_THREADS = 384;  // producer, products, two idle warps (registers); 2 x 4 softmax warps
 constexpr int PM_KT = 128;
+constexpr int PM_OVER = 1;
 
 template <int D, bool kTwo>
 struct PmLayout {
@@ -1041,7 +1168,7 @@ __device__ __forceinline__ uint32_t seen_bits(const PagedRow& r, int k0) {
 template <int D, bool kTwo>
 __global__ void __launch_bounds__(PM_THREADS, 1)
     paged_many_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
-                      const __grid_constant__ PagedAttnParams p, int kinds, int min_per) {
+                      const __grid_constant__ PagedAttnParams p, int kinds, int min_per, bool late) {
   using L = PmLayout<D, kTwo>;
   constexpr int M = kTwo ? 256 : 128, KT = PM_KT, NST = L::kStages, HALVES = D / 64;
   constexpr uint32_t kColO = 256;
@@ -1088,13 +1215,15 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
   }
+  if (!late) pdl_wait();
   pdl_launch_dependents();
-  pdl_wait();
+  paged_no_rec(p);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tslot;
-  PagedWalk<M, KT> w;
+  using Walk = PagedWalk<M, KT, PM_OVER>;
+  Walk w;
   const bool work = w.begin(p, kinds, min_per, sh);
 
   // registers: launched with 168 a thread (64512); 88 for the first four warps, 208 for the softmax warps
@@ -1261,7 +1390,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
     int nitem = 0;
 
     // this thread's query row, 16 bytes at a time, into the slot's swizzled tile
-    auto load_q = [&](const PagedWalk<M, KT>& x) {
+    auto load_q = [&](const Walk& x) {
       const int rho = x.qt * M + (kTwo ? slot * 128 : 0) + r128;
       const PagedRow r = paged_row(p, x.g, x.head, rho);
       const uint16_t* src = static_cast<const uint16_t*>(p.q) + r.tok * p.q_row + r.h * p.q_head;
@@ -1281,7 +1410,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
       if (lane == 0) mbar_arrive(q_full + (kTwo ? slot : 0));
     };
     // whether an item's rows reach the second slot's tile; only then are its queries loaded and waited for
-    auto both = [&](const PagedWalk<M, KT>& x) { return x.g.n * p.rep - x.qt * M > 128; };
+    auto both = [&](const Walk& x) { return x.g.n * p.rep - x.qt * M > 128; };
     if (slot == 0 || (kTwo && both(w))) load_q(w);
     bool more;
     do {
@@ -1400,7 +1529,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
       // The item's queries have been used for the last time where the last scores were waited for (in
       // the alternating form that is the last tile's slot): the next item's take their place while the
       // last product runs.
-      PagedWalk<M, KT> nx = w;
+      Walk nx = w;
       more = nx.next(p, kinds);
       if (more && (kTwo ? slot == 0 || both(nx) : ((nt - 1) & 1) == slot)) load_q(nx);
       // ---- the item's result
@@ -1425,18 +1554,9 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
         paged_wait(o_full + slot, no[0] & 1, dead, p.err);
         ++no[0];
       }
+      if (warp == 4 && lane == 0) w.report(p);
       // every warp of the slot raised its mark before the product that o_full reports
       const bool again = kTwo ? active && redo[slot] == nitem : redo[0] == nitem || redo[1] == nitem;
-      if (w.kt0 == 0 && qd == 0 && lane == 0) {
-        int4* d = (w.g.prefix ? p.desc_prefix : p.desc_own) + w.item(p) * p.Hk + w.head;
-        if (slot == 0) {
-          *reinterpret_cast<int2*>(d) = make_int2(w.first, w.count);
-          d->z = again;
-        } else if (kTwo) {
-          d->w = again;
-        }
-      }
-      if (again) m = __int_as_float(0x7fc00000);  // a state that the joining kernel does not take
       if (active || !kTwo) {
         tc_fence_after();
         const bool direct = w.count == 1 && p.G == 0;
@@ -1463,7 +1583,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
               for (int j = 0; j < 32; ++j) y[j] = fmaf(__uint_as_float(v[j]), g1, y[j]);
             }
           }
-          if (r.valid) {
+          if (r.valid && !again) {
             if (direct) {
               uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at * D + c);
 #pragma unroll
@@ -1487,9 +1607,30 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
             if (two) mbar_arrive(o_empty + 1);
           }
         }
-        if (r.valid && !direct && (kTwo || slot == 0)) {
+        if (r.valid && !again && !direct && (kTwo || slot == 0)) {
           if (w.count == 1) p.whole_ml[w.g.prefix][at] = make_float2(m, l);
           else p.part_ml[pt] = make_float2(m, l);
+        }
+        if (again && (kTwo || slot == 0)) {
+#pragma unroll 1
+          for (int i = 0; i < 32; ++i) {
+            const int row = (kTwo ? slot * 128 : 0) + qd * 32 + i;
+            const PagedRow ri = paged_row(p, w.g, w.head, w.qt * M + row);
+            if (!ri.valid) break;
+            float mi, li, oi[D / 32];
+            paged_redo_row<D>(p, w.g, ri, w.head, w.kt0 * KT, w.kt1 * KT, lane, mi, li, oi);
+            const long long to = (long long)ri.tok * p.H + ri.h;
+            const long long pi = ((long long)blockIdx.x * 2 + w.slot()) * M + row;
+            const float iv = li > 0.f ? 1.f / li : (li == 0.f ? 0.f : li);
+#pragma unroll
+            for (int e = 0; e < D / 32; ++e) {
+              const int c = lane * (D / 32) + e;
+              if (direct) static_cast<uint16_t*>(p.out)[to * D + c] = f32_to_bf16_bits(oi[e] * iv);
+              else (w.count == 1 ? p.whole_o[w.g.prefix] + to * D : p.part_o + pi * D)[c] = oi[e];
+            }
+            if (!direct && lane == 0)
+              (w.count == 1 ? p.whole_ml[w.g.prefix] + to : p.part_ml + pi)[0] = make_float2(mi, li);
+          }
         }
       }
       w = nx;
@@ -1503,148 +1644,125 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u) : "memory");
   }
+  if (late) pdl_wait();
 }
 
 // ---------------------------------------------------------------------------- joining
-// One block per row, one warp per query head: the states of the row's prefix and own items, each
-// whole or in parts, joined in order: with M = max m_i, o = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i.
-struct PagedCombineParams {
-  PagedAttnParams a;
-  const float* part_o[2];    // own, prefix
-  const float2* part_ml[2];
-  int M[2];
-  int blocks[2];  // blocks of the launch that wrote them
-};
-
-constexpr int PJ_THREADS = 256;
-
-// A row's state over a segment, key by key and without the keys that it does not see: the slow way
-// for rows beside a value that is not finite.
-template <typename S, int D>
-__device__ __noinline__ void paged_redo_row(const PagedAttnParams& p, int kind, int seg, int t, int h, int lane,
-                                            float& M, float& L, float (&o)[D / 32]) {
-  constexpr int E = D / 32;
-  const PagedSeg g = paged_seg(p, kind, seg);
-  const PagedRow r = paged_row(p, g, h / p.rep, (t - g.tok0) * p.rep + h % p.rep);
-  if (!r.valid) return;
-  auto get = [](const S* x) { return sizeof(S) == 2 ? bf16_bits_to_f32(uint16_t(*x)) : float(*x); };
-  float q[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) q[e] = get(static_cast<const S*>(p.q) + t * p.q_row + h * p.q_head + lane * E + e);
-  for (int key = 0; key < g.klen; ++key) {
-    if (!r.sees(key)) continue;
-    const int page = paged_page(p, g, key >> p.page_log2), pr = key & ((1 << p.page_log2) - 1);
-    float k[E] = {}, v[E] = {}, z = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      if (page >= 0) {
-        k[e] = get(static_cast<const S*>(p.K.ptr) + page * p.K.page + (h / p.rep) * p.K.head + pr * p.K.row + lane * E + e);
-        v[e] = get(static_cast<const S*>(p.V.ptr) + page * p.V.page + (h / p.rep) * p.V.head + pr * p.V.row + lane * E + e);
-      }
-      z = fmaf(q[e], k[e], z);
-    }
-    z = warp_sum(z) * p.scale_log2;
-    const float mn = fmaxf(M, z), mg = mn == -INFINITY ? 0.f : mn;
-    const float wa = exp2f(M - mg), wb = exp2f(z - mg);
-    M = mn;
-    L = L * wa + wb;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = o[e] * wa + wb * v[e];
-  }
+// States (m, l, o) of one row over different keys: with M = max m_i, o = sum 2^(m_i - M) o_i /
+// sum 2^(m_i - M) l_i, taken in the order of the keys. Both kernels read a few states that are still
+// in L2; they are bound by the latency of the loads that depend on one another, so each thread first
+// finds where its states are, then has all of their loads in flight.
+template <typename S>
+__device__ __forceinline__ void paged_store_out(void* out, long long at, const float (&o)[4], float L) {
+  const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+  const float y[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+  store4(static_cast<S*>(out) + at, y);
 }
 
+// Without prefixes: block (x, y) joins rows [8 y, 8 y + 8) of the divided item that began in block x
+// of the attention; D / 4 threads a row.
+constexpr int PJ_ROWS = 8;
 template <typename S, int D>
-__global__ void __launch_bounds__(PJ_THREADS) paged_combine_kernel(const __grid_constant__ PagedCombineParams c) {
-  const PagedAttnParams& p = c.a;
-  constexpr int E = D / 32;
+__global__ void __launch_bounds__(PJ_ROWS* D / 4)
+    paged_join_kernel(const __grid_constant__ PagedAttnParams p, int M) {
   pdl_launch_dependents();
   pdl_wait();
-  const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const PagedRec rec = p.rec[blockIdx.x];
+  const int row = blockIdx.y * PJ_ROWS + int(threadIdx.x) / (D / 4), col = (threadIdx.x % (D / 4)) * 4;
+  const int rho = rec.qt * M + row;
+  if (rec.count < 2 || rho >= rec.rows) return;
+  const long long at = ((long long)blockIdx.x * 2 + 1) * M + row;  // later parts: the next blocks' first slots
+  const float2* pm = p.part_ml + at;
+  const float* po = p.part_o + at * D + col;
+  float top = pm[0].x;
+#pragma unroll 8
+  for (int i = 1; i < rec.count; ++i) top = fmaxf(top, pm[(long long)i * 2 * M - M].x);
+  const float mg = top == -INFINITY ? 0.f : top;
+  float L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = 0; i < rec.count; ++i) {
+    const long long r = i ? (long long)i * 2 * M - M : 0;
+    const float2 ml = pm[r];
+    const float4 x = *reinterpret_cast<const float4*>(po + r * D);
+    const float f = exp2f(ml.x - mg);
+    L += ml.y * f;
+    o[0] += x.x * f;
+    o[1] += x.y * f;
+    o[2] += x.z * f;
+    o[3] += x.w * f;
+  }
+  const int i = rho / p.rep;
+  paged_store_out<S>(p.out, ((long long)(rec.tok0 + i) * p.H + rec.head * p.rep + (rho - i * p.rep)) * D + col, o, L);
+}
+
+// With prefixes: a row and query head per D / 4 threads; its prefix item's states, then its own.
+struct PagedCombineParams {
+  PagedAttnParams a;
+  const float* part_o[2];  // own, prefix
+  const float2* part_ml[2];
+  int M[2];
+  int blocks[2];           // blocks of the launch that wrote them
+};
+
+constexpr int PC_JOIN = 256;
+template <typename S, int D>
+__global__ void __launch_bounds__(PC_JOIN) paged_combine_kernel(const __grid_constant__ PagedCombineParams c) {
+  const PagedAttnParams& p = c.a;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int t = blockIdx.x, col = (threadIdx.x % (D / 4)) * 4;
   const int b = request_of_row(p.offsets, t, p.T, p.B);
   if (b >= p.B) return;
-  int grp = -1;
-  if (p.G > 0) {
-    int n = 0;
-    for (int g0 = 0; g0 < p.G; g0 += PJ_THREADS) {
-      const int g = g0 + int(threadIdx.x);
-      n += __syncthreads_count(g < p.G && p.groups[g + 1] <= b);
-    }
-    if (n < p.G && p.groups[n] <= b) grp = n;
+  int grp = 0;
+  for (int g0 = 0; g0 < p.G; g0 += PC_JOIN) {
+    const int g = g0 + int(threadIdx.x);
+    grp += __syncthreads_count(g < p.G && p.groups[g + 1] <= b);
   }
-  for (int h = warp; h < p.H; h += PJ_THREADS / 32) {
-    float M = -INFINITY, L = 0.f, o[E] = {};
-    bool write = p.G > 0, redo = false;
-    for (int kind = 1; kind >= 0; --kind) {
-      if (kind && grp < 0) continue;
-      const int tok0 = paged_row0(p, kind ? min(max(p.groups[grp], 0), p.B) : b);
-      const int rho = (t - tok0) * p.rep + h % p.rep;
-      if (rho < 0) continue;  // offsets that do not increase
-      const int m = c.M[kind], qt = rho / m;
-      const int item = int((long long)tok0 * p.rep / m) + (kind ? grp : b) + qt;
-      const int4 d = (kind ? p.desc_prefix : p.desc_own)[item * p.Hk + h / p.rep];
-      if (d.x < 0 || d.y < 1 || d.y > c.blocks[kind] || d.x > c.blocks[kind] - d.y) continue;  // never written
-      if (d.y > 1) write = true;
-      if (!write) {
-        redo = (rho - qt * m < 128 ? d.z : d.w) == 1;
-        continue;
-      }
-      const float2* pm;
-      const float* po;
-      long long step;  // rows from one part to the next (the first part is its block's second slot)
-      if (d.y == 1) {
-        const long long at = (long long)t * p.H + h;
-        pm = p.whole_ml[kind] + at;
-        po = p.whole_o[kind] + at * D;
-        step = 0;
-      } else {
-        const long long at = ((long long)d.x * 2 + 1) * m + (rho - qt * m);
-        pm = c.part_ml[kind] + at;
-        po = c.part_o[kind] + at * D;
-        step = 2 * m;
-      }
-      auto row_of = [&](int i) { return i ? i * step - m : 0ll; };
-      float mk = M;
-      bool bad = false;
-      for (int i = lane; i < d.y; i += 32) {
-        const float x = pm[row_of(i)].x;
-        mk = fmaxf(mk, x);
-        bad |= x != x;
-      }
-      redo |= __any_sync(0xffffffffu, bad) != 0;
-      mk = warp_max(mk);
-      const float mg = mk == -INFINITY ? 0.f : mk, wa = exp2f(M - mg);
-      L *= wa;
+  if (grp >= p.G || p.groups[grp] > b) grp = -1;
+  const int h = blockIdx.y * (PC_JOIN / (D / 4)) + int(threadIdx.x) / (D / 4);
+  if (h >= p.H) return;
+  const float2* pm[2];
+  const float* po[2];
+  long long step[2], less[2];
+  int count[2] = {0, 0};
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] *= wa;
-      M = mk;
+  for (int kind = 0; kind < 2; ++kind) {
+    if (kind && grp < 0) continue;
+    const int tok0 = paged_row0(p, kind ? min(max(p.groups[grp], 0), p.B) : b);
+    const int rho = (t - tok0) * p.rep + h % p.rep, m = c.M[kind], qt = rho / m;
+    if (rho < 0) continue;  // offsets that do not increase
+    const int2 d = p.desc[kind][(int((long long)tok0 * p.rep / m) + (kind ? grp : b) + qt) * p.Hk + h / p.rep];
+    if (d.x < 0 || d.y < 1 || d.y > c.blocks[kind] || d.x > c.blocks[kind] - d.y) continue;  // never written
+    count[kind] = d.y;
+    const bool one = d.y == 1;
+    const long long at = one ? (long long)t * p.H + h : ((long long)d.x * 2 + 1) * m + (rho - qt * m);
+    pm[kind] = (one ? p.whole_ml[kind] : c.part_ml[kind]) + at;
+    po[kind] = (one ? p.whole_o[kind] : c.part_o[kind]) + at * D + col;
+    step[kind] = 2 * m;
+    less[kind] = m;
+  }
+  float top = -INFINITY;
+#pragma unroll
+  for (int kind = 1; kind >= 0; --kind)
 #pragma unroll 4
-      for (int i = 0; i < d.y; ++i) {
-        const long long r = row_of(i);
-        const float2 ml = pm[r];
-        const float wb = exp2f(ml.x - mg);
-        L += ml.y * wb;
+    for (int i = 0; i < count[kind]; ++i) top = fmaxf(top, pm[kind][i ? i * step[kind] - less[kind] : 0].x);
+  const float mg = top == -INFINITY ? 0.f : top;
+  float L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] += po[r * D + lane * E + e] * wb;
-      }
+  for (int kind = 1; kind >= 0; --kind)
+#pragma unroll 4
+    for (int i = 0; i < count[kind]; ++i) {
+      const long long r = i ? i * step[kind] - less[kind] : 0;
+      const float2 ml = pm[kind][r];
+      const float4 x = *reinterpret_cast<const float4*>(po[kind] + r * D);
+      const float f = exp2f(ml.x - mg);
+      L += ml.y * f;
+      o[0] += x.x * f;
+      o[1] += x.y * f;
+      o[2] += x.z * f;
+      o[3] += x.w * f;
     }
-    if (redo) {
-      L = 0.f;
-      M = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = 0.f;
-      if (grp >= 0) paged_redo_row<S, D>(p, kPrefixRows, grp, t, h, lane, M, L, o);
-      paged_redo_row<S, D>(p, kOwnRows, b, t, h, lane, M, L, o);
-      write = true;
-    }
-    if (!write) continue;
-    const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
-    S* dst = static_cast<S*>(p.out) + ((long long)t * p.H + h) * D + lane * E;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      if constexpr (sizeof(S) == 2) dst[e] = f32_to_bf16_bits(o[e] * inv);
-      else dst[e] = o[e] * inv;
-    }
-  }
+  paged_store_out<S>(p.out, ((long long)t * p.H + h) * D + col, o, L);
 }
 
 }  // namespace wc
