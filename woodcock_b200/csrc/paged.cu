@@ -283,17 +283,18 @@ void opt_in(const wc_ctx* ctx, K kernel, size_t bytes) {
   d = true;
 }
 
-// K or V pages as a 4-D tensor (dim, row, head, page); a copy takes `rows` rows of one page and half
-// a row of head_dim 128 (128 bytes, the swizzle's width).
-CUtensorMap page_map(const wc_pages& g, const PagePool& pool, int rows) {
+// K or V pages as a 5-D tensor (64 dims, row, half row, head, page); a copy takes `rows` rows of one page,
+// and `halves` of the half rows of head_dim 128 (128 bytes, the swizzle's width), one after the other.
+CUtensorMap page_map(const wc_pages& g, const PagePool& pool, int rows, int halves) {
   CUtensorMap m;
-  const cuuint64_t dims[4] = {cuuint64_t(g.head_dim), cuuint64_t(g.page_size), cuuint64_t(g.kv_heads),
+  const cuuint64_t dims[5] = {64, cuuint64_t(g.page_size), cuuint64_t(g.head_dim / 64), cuuint64_t(g.kv_heads),
                               cuuint64_t(g.pages)};
-  const long long st[3] = {pool.row, g.kv_heads > 1 ? pool.head : 64, g.pages > 1 ? pool.page : 64};
-  const cuuint64_t strides[3] = {cuuint64_t(st[0]) * 2, cuuint64_t(st[1]) * 2, cuuint64_t(st[2]) * 2};
-  const cuuint32_t box[4] = {64, cuuint32_t(std::min(rows, g.page_size)), 1, 1};
-  const cuuint32_t es[4] = {1, 1, 1, 1};
-  const CUresult r = encode_tiled()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, pool.ptr, dims, strides, box, es,
+  const long long st[4] = {pool.row, 64, g.kv_heads > 1 ? pool.head : 64, g.pages > 1 ? pool.page : 64};
+  const cuuint64_t strides[4] = {cuuint64_t(st[0]) * 2, cuuint64_t(st[1]) * 2, cuuint64_t(st[2]) * 2,
+                                 cuuint64_t(st[3]) * 2};
+  const cuuint32_t box[5] = {64, cuuint32_t(std::min(rows, g.page_size)), cuuint32_t(halves), 1, 1};
+  const cuuint32_t es[5] = {1, 1, 1, 1, 1};
+  const CUresult r = encode_tiled()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, pool.ptr, dims, strides, box, es,
                                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) fail(WC_ERR_INVALID, "paged: the pages' strides cannot be described to the copy engine");
@@ -307,7 +308,7 @@ void launch_few(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, const PagedAttn
   static_assert(PfLayout<D, 16 * RG>::bytes() <= kSmemOptinBytes, "shared memory");
   opt_in(ctx, paged_few_kernel<D, RG>, smem);
   launch_on(ctx, st, "paged_few", paged_few_kernel<D, RG>, dim3(l.blocks), dim3(PF_THREADS), smem, true, 1,
-            page_map(g, p.K, PF_KT), page_map(g, p.V, PF_KT), p, kinds, l.min_per, late);
+            page_map(g, p.K, PF_KT, D / 64), page_map(g, p.V, PF_KT, D / 64), p, kinds, l.min_per, late);
 }
 
 template <int D, bool kTwo>
@@ -317,7 +318,7 @@ void launch_many(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, const PagedAtt
   static_assert(PmLayout<D, kTwo>::bytes() <= kSmemOptinBytes, "shared memory");
   opt_in(ctx, paged_many_kernel<D, kTwo>, smem);
   launch_on(ctx, st, "paged_many", paged_many_kernel<D, kTwo>, dim3(l.blocks), dim3(PM_THREADS), smem, true, 1,
-            page_map(g, p.K, PM_KT), page_map(g, p.V, PM_KT), p, kinds, l.min_per, late);
+            page_map(g, p.K, PM_KT, 1), page_map(g, p.V, PM_KT, D / 64), p, kinds, l.min_per, late);
 }
 
 template <typename S, int D>

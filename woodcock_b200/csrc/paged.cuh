@@ -821,9 +821,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
 
   if (warp == PF_CONSUMERS) {  // ---- producer
     const int psize = 1 << p.page_log2;
-    const int box = min(psize, KT), parts = KT / box;  // copies of one half row block per tile
-    constexpr int HALVES = D / 64;
-    const int part = lane / (2 * HALVES), half = (lane >> 1) % HALVES;
+    const int box = min(psize, KT), parts = KT / box;  // copies of K and of V per tile
+    const int part = lane >> 1;
     const bool isv = lane & 1, issue = part < parts;
     int cnt = 0, nitem = 0;
     bool more = true;
@@ -860,8 +859,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         __syncwarp();
         if (*dead) break;
         if (issue)
-          tma_load_4d(sm + size_t(s) * L::kStage + (isv ? L::kTile : 0) + half * (KT * 128) + part * box * 128,
-                      isv ? &tv : &tk, half * 64, (kt * KT) & (psize - 1), w.head, page, full + s);
+          tma_load_5d(sm + size_t(s) * L::kStage + (isv ? L::kTile : 0) + part * box * (D * 2), isv ? &tv : &tk, 0,
+                      (kt * KT) & (psize - 1), 0, w.head, page, full + s);
         __syncwarp();
       }
       more = !*dead && w.next(p, kinds);
@@ -890,6 +889,9 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   const int rg = RG == 1 ? 0 : (warp & 1);
   const int slice = RG == 1 ? (warp & 3) : (warp >> 1);
   const float sl2 = p.scale_log2;
+  // a copy's rows lie together, half rows of 128 bytes one after the other
+  const int box = min(1 << p.page_log2, KT), hstride = box * 128;
+  const int slice_at = (slice * 16 / box) * box * (D * 2) + (slice * 16 % box) * 128;
   int cnt = 0;
   for (int nitem = 0;; ++nitem) {
     // One thread says for all of them whether the line goes on: the warps meet at the item's end, so
@@ -928,7 +930,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         if (lane == 0) mbar_arrive(empty + s);
         continue;
       }
-      const unsigned char* kb = sm + size_t(s) * L::kStage + slice * 16 * 128;  // the slice's first key
+      const unsigned char* kb = sm + size_t(s) * L::kStage + slice_at;  // the slice's first key
       const unsigned char* vb = kb + L::kTile;
       // ---- S = Q K^T, 16 keys: the dims in two chains of each n-tile
       float sc[2][4], sx[2][4];
@@ -942,7 +944,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         for (int j = 0; j < 2; ++j) {
           uint32_t b[4];
           const int chunk = (i & 1) * 4 + (lane >> 3);
-          ldsm_x4(b, kb + (i >> 1) * (KT * 128) + (j * 8 + (lane & 7)) * 128 + ((chunk ^ (lane & 7)) << 4));
+          ldsm_x4(b, kb + (i >> 1) * hstride + (j * 8 + (lane & 7)) * 128 + ((chunk ^ (lane & 7)) << 4));
           mma_bf16_16816r(sc[j], qa[2 * i], b[0], b[1]);
           mma_bf16_16816r(sx[j], qa[2 * i + 1], b[2], b[3]);
         }
@@ -998,7 +1000,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         for (int h = 0; h < D / 64; ++h)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const uint4 x = *reinterpret_cast<const uint4*>(vr + h * (KT * 128) + c * 16);
+            const uint4 x = *reinterpret_cast<const uint4*>(vr + h * hstride + c * 16);
             const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -1017,7 +1019,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         for (int dj = 0; dj < ND; dj += 2) {
           uint32_t b[4];
           const int key = lane & 15, chunk = dj + (lane >> 4);
-          ldsm_x4_trans(b, vb + (chunk >> 3) * (KT * 128) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4));
+          ldsm_x4_trans(b, vb + (chunk >> 3) * hstride + key * 128 + (((chunk & 7) ^ (key & 7)) << 4));
           mma_bf16_16816r(o[dj], a, b[0], b[1]);
           mma_bf16_16816r(o[dj + 1], a, b[2], b[3]);
         }
@@ -1030,7 +1032,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           const float p0 = __shfl_sync(0xffffffffu, x0, from), p1 = __shfl_sync(0xffffffffu, x1, from);
 #pragma unroll
           for (int dj = 0; dj < ND; ++dj) {
-            const uint32_t v = *reinterpret_cast<const uint32_t*>(vb + (dj >> 3) * (KT * 128) + c * 128 +
+            const uint32_t v = *reinterpret_cast<const uint32_t*>(vb + (dj >> 3) * hstride + c * 128 +
                                                                   (((dj & 7) ^ (c & 7)) << 4) + 4 * t);
             const float v0 = __uint_as_float(v << 16), v1 = __uint_as_float(v & 0xffff0000u);
             if (p0 != 0.f) {
@@ -1127,6 +1129,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     }
   }
   if (late) pdl_wait();
+}
+
+// 32 bytes to a 32-byte aligned address in one store
+__device__ __forceinline__ void store32(float* dst, const float* y) {
+  asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"l"(dst), "f"(y[0]), "f"(y[1]), "f"(y[2]),
+               "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7])
+               : "memory");
 }
 
 // ---------------------------------------------------------------------------- many rows: tensor memory
@@ -1230,47 +1239,54 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
   // (128 x 88 + 256 x 208 = 64512): a row's 128 scores stay in registers
   if (warp < 4) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n");
-  if (warp == 0 && work) {  // ---- K and V tiles, in the order that the products take them
+  if ((warp == 0 || warp == 2) && work) {  // ---- K tiles (warp 0) and V tiles (warp 2)
+    const bool isv = warp == 2;
     const int psize = 1 << p.page_log2;
     const int box = min(psize, KT), parts = KT / box;
-    const int part = lane / HALVES, half = lane % HALVES;
-    int cnt = 0;
-    auto load = [&](PageWindow& win, const CUtensorMap* map, int kt) {
-      const int s = cnt % NST;
-      const int first = (kt * KT) >> p.page_log2;
-      win.seek(p, first, lane);
-      const int page = __shfl_sync(0xffffffffu, win.cur, (first - win.base + part) & 31);
-      if (lane == 0) {
-        if (cnt >= NST) paged_wait(kv_empty + s, ((cnt / NST) - 1) & 1, dead, p.err);
-        if (!*dead) mbar_arrive_expect_tx(kv_full + s, L::kTile);
-      }
-      __syncwarp();
-      if (*dead) return;
-      if (part < parts)
-        tma_load_4d(ring + size_t(s) * L::kTile + half * (KT * 128) + part * box * 128, map, half * 64,
-                    (kt * KT) & (psize - 1), w.head, page, kv_full + s);
-      __syncwarp();
-      ++cnt;
-    };
+    // K: half rows apart, so that the tile's 128 keys have one stride as the product wants it; V: a
+    // copy's rows together
+    const int part = isv ? lane : lane / HALVES, half = isv ? 0 : lane % HALVES;
+    const int at = isv ? part * box * (D * 2) : half * (KT * 128) + part * box * 128;
+    int base = 0, last = -1;
     do {
-      PageWindow wk, wv;
-      wk.start(p, w.g, (w.kt0 * KT) >> p.page_log2, lane);
-      wv = wk;
-      constexpr int kAhead = kTwo ? 1 : 2;  // K tiles that are taken before the first V tile
-      for (int i = 0; i < kAhead && w.kt0 + i < w.kt1; ++i) load(wk, &tk, w.kt0 + i);
-      for (int kt = w.kt0; kt < w.kt1 && !*dead; ++kt) {
-        load(wv, &tv, kt);
-        if (kt + kAhead < w.kt1) load(wk, &tk, kt + kAhead);
+      const int nt = w.kt1 - w.kt0;
+      PageWindow win;
+      win.start(p, w.g, (w.kt0 * KT) >> p.page_log2, lane);
+      for (int t = 0; t < nt; ++t) {
+        // The tile's place in the ring, in the order that the products take the tiles: K0 V0 K1 V1 ...,
+        // or with alternating slots K0 K1 V0 K2 V1 ... The two warps meet at a stage in turns; since the
+        // products free the stages in order, the use before last is over when this warp's last one was.
+        const int pos = base + (kTwo ? 2 * t + isv : isv ? t + min(t + 2, nt) : t < 2 ? t : 2 * t - 1);
+        const int s = pos % NST;
+        const int first = ((w.kt0 + t) * KT) >> p.page_log2;
+        win.seek(p, first, lane);
+        const int page = __shfl_sync(0xffffffffu, win.cur, (first - win.base + part) & 31);
+        if (lane == 0) {
+          if (pos >= NST) paged_wait(kv_empty + s, ((pos / NST) - 1) & 1, dead, p.err);
+          if (!*dead) mbar_arrive_expect_tx(kv_full + s, L::kTile);
+        }
+        __syncwarp();
+        if (*dead) break;
+        if (part < parts)
+          tma_load_5d(ring + size_t(s) * L::kTile + at, isv ? &tv : &tk, 0, ((w.kt0 + t) * KT) & (psize - 1), half,
+                      w.head, page, kv_full + s);
+        __syncwarp();
+        last = pos;
       }
+      base += 2 * nt;
     } while (!*dead && w.next(p, kinds));
+    // shared memory must outlive the copies: the last one is waited for here, those before it by the
+    // products that the block waits for, unless the block has given up
     if (lane == 0)
-      for (int q = max(0, cnt - NST); q < cnt; ++q)
+      for (int q = max(0, last - (*dead ? NST - 1 : 0)); q <= last; ++q)
         if (!mbar_wait(kv_full + q % NST, (q / NST) & 1)) raise_error(p.err, kErrTimeout);
   } else if (warp == 1 && work) {  // ---- products: the warp walks together, one lane issues
     constexpr uint32_t id_s = umma_idesc_bf16_m128(KT, 0), id_o = umma_idesc_bf16_m128(D, 1);
     const bool issuer = elect_one();
     const uint32_t q_lo = umma_lo(smem_addr(qs), 1), k_lo = umma_lo(smem_addr(ring), 1);
-    const uint32_t v_lo = umma_lo(smem_addr(ring), (KT * 128) >> 4);
+    const int vlog = min(p.page_log2, 7);  // keys of one copy of V
+    const uint32_t v_lo = umma_lo(smem_addr(ring), (128u << vlog) >> 4);
+    const uint32_t v_more = (((D - 64) * 2) << vlog) / 16;  // from a copy's last key to the next one's first
     int st = 0;               // ring stage of the next tile taken
     uint32_t ring_ph = 0;     // and its phase
     uint32_t p_ph = 0, o_ph = 0, q_ph = 0;  // phases by slot, as bits
@@ -1313,7 +1329,8 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
       if (issuer) {
         const uint32_t b = v_lo + s * (L::kTile / 16), d = tmem + kColO + slot * D, a = tmem + slot * 128;
 #pragma unroll
-        for (int kk = 0; kk < KT / 16; ++kk) umma_ts(d, a + kk * 8, b + kk * (16 * 128 / 16), id_o, !first || kk != 0);
+        for (int kk = 0; kk < KT / 16; ++kk)
+          umma_ts(d, a + kk * 8, b + kk * (16 * 128 / 16) + uint32_t((kk * 16) >> vlog) * v_more, id_o, !first || kk != 0);
       }
     };
     auto done = [&](uint64_t* bar) {
@@ -1385,37 +1402,44 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
     const uint32_t lanes = tmem + (uint32_t(qd * 32) << 16);
     const uint32_t ts = lanes + slot * 128, to = lanes + kColO + slot * D;
     const float sl2 = p.scale_log2;
+    const bool wide_out = (reinterpret_cast<unsigned long long>(p.out) & 31) == 0;
     int ns = 0, no[2] = {0, 0};  // scores and outputs waited for
     int vcnt = 0;                // ring position of the item's first K tile
     int nitem = 0;
 
-    // this thread's query row, 16 bytes at a time, into the slot's swizzled tile
-    auto load_q = [&](const Walk& x) {
-      const int rho = x.qt * M + (kTwo ? slot * 128 : 0) + r128;
-      const PagedRow r = paged_row(p, x.g, x.head, rho);
-      const uint16_t* src = static_cast<const uint16_t*>(p.q) + r.tok * p.q_row + r.h * p.q_head;
-      unsigned char* dst = qs + (kTwo ? slot : 0) * (128 * D * 2) + r128 * 128;
-      uint4 v[8];
-#pragma unroll
-      for (int h = 0; h < HALVES; ++h) {
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-          v[c] = r.valid ? *reinterpret_cast<const uint4*>(src + h * 64 + c * 8) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-          *reinterpret_cast<uint4*>(dst + h * (128 * 128) + ((c ^ (r128 & 7)) << 4)) = v[c];
+    // Query rows of an item into the slot's swizzled tile, asynchronously: 16 or 8 lanes copy a row, whose
+    // place the lane that owns it knows.
+    auto copy_q = [&](const Walk& x) {
+      constexpr int CH = D / 8, RPI = 32 / CH;  // 16-byte pieces of a row, rows per step
+      const PagedRow r = paged_row(p, x.g, x.head, x.qt * M + (kTwo ? slot * 128 : 0) + r128);
+      const long long mine = r.valid ? r.tok * p.q_row + r.h * p.q_head : -1;
+      const int c = lane % CH;
+      unsigned char* dst = qs + (kTwo ? slot : 0) * (128 * D * 2) + (c / 8) * (128 * 128) + qd * 32 * 128;
+#pragma unroll 4
+      for (int k = 0; k < 32; k += RPI) {
+        const int row = k + lane / CH;
+        const long long from = __shfl_sync(0xffffffffu, mine, row);
+        cp_async16(dst + row * 128 + (((c & 7) ^ (row & 7)) << 4),
+                   static_cast<const uint16_t*>(p.q) + (from < 0 ? 0 : from) + c * 8, from < 0 ? 0 : 16);
       }
+      cp_async_commit();
+    };
+    auto copied_q = [&]() {
+      cp_async_wait<0>();
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full + (kTwo ? slot : 0));
     };
-    // whether an item's rows reach the second slot's tile; only then are its queries loaded and waited for
+    // whether an item's rows reach the second slot's tile; only then are its queries copied and waited for
     auto both = [&](const Walk& x) { return x.g.n * p.rep - x.qt * M > 128; };
-    if (slot == 0 || (kTwo && both(w))) load_q(w);
+    if (slot == 0 || (kTwo && both(w))) {
+      copy_q(w);
+      copied_q();
+    }
     bool more;
     do {
       const int nt = w.kt1 - w.kt0;
-      const bool two = kTwo ? both(w) : nt > 1;
+      const bool two = kTwo ? both(w) : nt > 1;  // the second slot has work
       const bool active = slot == 0 || two;
       const PagedRow r = paged_row(p, w.g, w.head, w.qt * M + (kTwo ? slot * 128 : 0) + r128);
       const int lim = r.valid ? r.lim : 0x7fffffff;  // rows that pad the tile see everything, for nobody
@@ -1493,14 +1517,15 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
           const int vpos = vcnt + (kTwo ? 2 * t + 1 : min(2 * t + 2, nt + t));
           const int vs = vpos % NST;
           paged_wait(kv_full + vs, (vpos / NST) & 1, dead, p.err);
-          unsigned char* vrow = ring + size_t(vs) * L::kTile + r128 * 128;
+          const int vbox = min(1 << p.page_log2, KT), hstride = vbox * 128;
+          unsigned char* vrow = ring + size_t(vs) * L::kTile + r128 * 128 + (r128 / vbox) * (vbox * (D - 64) * 2);
           if (key0 + r128 >= w.g.klen) {
             if (slot == 0 || !kTwo) {  // slot 1 of a shared tile multiplies after slot 0
 #pragma unroll
               for (int h = 0; h < HALVES; ++h)
 #pragma unroll
                 for (int c = 0; c < 8; ++c)
-                  *reinterpret_cast<uint4*>(vrow + h * (KT * 128) + c * 16) = make_uint4(0, 0, 0, 0);
+                  *reinterpret_cast<uint4*>(vrow + h * hstride + c * 16) = make_uint4(0, 0, 0, 0);
             }
           } else {
             uint32_t worst = 0;
@@ -1508,7 +1533,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
             for (int h = 0; h < HALVES; ++h)
 #pragma unroll
               for (int c = 0; c < 8; ++c) {
-                const uint4 x = *reinterpret_cast<const uint4*>(vrow + h * (KT * 128) + c * 16);
+                const uint4 x = *reinterpret_cast<const uint4*>(vrow + h * hstride + c * 16);
                 const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -1526,12 +1551,13 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
         if (lane == 0) mbar_arrive(p_full + slot);
       }
       vcnt += 2 * nt;
-      // The item's queries have been used for the last time where the last scores were waited for (in
-      // the alternating form that is the last tile's slot): the next item's take their place while the
+      // The item's queries have been used for the last time where the last scores were waited for (with
+      // alternating slots, by the slot of the last tile): the next item's take their place while the
       // last product runs.
       Walk nx = w;
       more = nx.next(p, kinds);
-      if (more && (kTwo ? slot == 0 || both(nx) : ((nt - 1) & 1) == slot)) load_q(nx);
+      const bool load = more && (kTwo ? slot == 0 || both(nx) : ((nt - 1) & 1) == slot);
+      if (load) copy_q(nx);
       // ---- the item's result
       float f0 = 1.f, f1 = 0.f;
       if constexpr (!kTwo) {  // the slots' states joined; each group of warps takes half of the columns
@@ -1554,6 +1580,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
         paged_wait(o_full + slot, no[0] & 1, dead, p.err);
         ++no[0];
       }
+      if (load) copied_q();
       if (warp == 4 && lane == 0) w.report(p);
       // every warp of the slot raised its mark before the product that o_full reports
       const bool again = kTwo ? active && redo[slot] == nitem : redo[0] == nitem || redo[1] == nitem;
@@ -1585,15 +1612,21 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
           }
           if (r.valid && !again) {
             if (direct) {
-              uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at * D + c);
+              uint16_t* dst = static_cast<uint16_t*>(p.out) + at * D + c;
+              float v8[16];
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-                dst[j] = make_uint4(pack_bf16(y[8 * j], y[8 * j + 1]), pack_bf16(y[8 * j + 2], y[8 * j + 3]),
-                                    pack_bf16(y[8 * j + 4], y[8 * j + 5]), pack_bf16(y[8 * j + 6], y[8 * j + 7]));
-            } else {
-              float4* dst = reinterpret_cast<float4*>(po + c);
+              for (int j = 0; j < 16; ++j) v8[j] = __uint_as_float(pack_bf16(y[2 * j], y[2 * j + 1]));
+              if (wide_out) {
+                store32(reinterpret_cast<float*>(dst), v8);
+                store32(reinterpret_cast<float*>(dst) + 8, v8 + 8);
+              } else {
 #pragma unroll
-              for (int j = 0; j < 8; ++j) dst[j] = make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
+                for (int j = 0; j < 4; ++j)
+                  reinterpret_cast<float4*>(dst)[j] = make_float4(v8[4 * j], v8[4 * j + 1], v8[4 * j + 2], v8[4 * j + 3]);
+              }
+            } else {  // scratch: 256-byte aligned rows
+#pragma unroll
+              for (int j = 0; j < 4; ++j) store32(po + c + 8 * j, y + 8 * j);
             }
           }
         }
@@ -1633,8 +1666,8 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
           }
         }
       }
-      w = nx;
       ++nitem;
+      w = nx;
     } while (more);
     }
   }
