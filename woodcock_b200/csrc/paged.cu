@@ -149,7 +149,10 @@ extern "C" wc_status wc_paged_append(wc_ctx* ctx, void* stream, const wc_paged_a
     p.H = b.heads;
     p.Hk = g.kv_heads;
     p.err = ctx->d_err;
-    for (int i = 0; i < g.head_dim / 2; ++i) p.freq[i] = std::pow(a->base, -2.0 * i / g.head_dim);
+    // base^(-2i/D): eight powers, the rest by products (an error of a few 2^-53)
+    const double step = std::pow(a->base, -2.0 / g.head_dim);
+    for (int i = 0; i < g.head_dim / 2; ++i)
+      p.freq[i] = i % 8 ? p.freq[i - 1] * step : std::pow(a->base, -2.0 * i / g.head_dim);
     const cudaStream_t st = stream_of(ctx, stream);
     const bool sb = a->src_dtype == WC_BF16, pb = g.dtype == WC_BF16;
     if (sb && pb) launch_append<uint16_t, uint16_t>(ctx, st, p, g.head_dim);

@@ -712,7 +712,7 @@ __device__ __forceinline__ void paged_redo_row(const PagedAttnParams& p, const P
 constexpr int PF_CONSUMERS = 8;
 constexpr int PF_THREADS = 32 * (PF_CONSUMERS + 1);
 constexpr int PF_KT = 64;
-constexpr int PF_OVER = 1;
+constexpr int PF_OVER = 4;
 
 template <int D, int M>
 struct PfLayout {
@@ -1149,7 +1149,7 @@ __device__ __forceinline__ void store32(float* dst, const float* y) {
 // then at most 2^8 instead of 1, and the final division by the sum takes the same factor out.
 constexpr int PM_THREADS = 384;  // producer, products, two idle warps (registers); 2 x 4 softmax warps
 constexpr int PM_KT = 128;
-constexpr int PM_OVER = 1;
+constexpr int PM_OVER = 3;
 
 template <int D, bool kTwo>
 struct PmLayout {

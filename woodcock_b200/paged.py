@@ -23,6 +23,7 @@ from __future__ import annotations
 
 import ctypes as C
 import struct
+from functools import lru_cache
 
 import torch
 
@@ -38,6 +39,8 @@ _APPEND = struct.Struct("@" + _PAGES + _BATCH + "3P6q4Pdf2i0q")
 _ATTENTION = struct.Struct("@" + _PAGES + _BATCH + "P2qPPq2P2i2PQfi0q")
 _COMPACT = struct.Struct("@" + _PAGES + "Pq2i2Pq2Pi0q")
 
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
 
 def _fail(what: str):
     raise ValueError(what)
@@ -45,32 +48,32 @@ def _fail(what: str):
 
 def _stream(device: int) -> int:
     # the default stream's handle is 0, which the library reads as "the context's"; 1 names it
-    return torch._C._cuda_getCurrentRawStream(device) or 1
+    return _raw_stream(device) or 1
 
 
 def _pages(k: torch.Tensor, v: torch.Tensor, layers: bool = False) -> tuple:
-    if k.dtype not in _CODES or v.dtype != k.dtype:
+    code, n = _CODES.get(k.dtype), k.shape
+    if code is None or v.dtype is not k.dtype:
         _fail("pages must be fp32 or bf16, k and v alike")
-    if k.dim() != 4 + layers or v.shape != k.shape:
+    if len(n) != 4 + layers or v.shape != n:
         _fail(f"pages must be {'[layers]' if layers else ''}[pages][kv_heads][page_size][head_dim], k and v alike")
     ks, vs = k.stride(), v.stride()
     if ks[-1] != 1 or vs[-1] != 1:
         _fail("rows of the pages must be contiguous")
-    n = k.shape
     if n[-1] not in (64, 128) or n[-2] not in (16, 32, 64, 128, 256):
         _fail("head_dim must be 64 or 128, page_size a power of two from 16 to 256")
     if not k.is_cuda or v.device != k.device:
         _fail("pages must be on one CUDA device")
     if layers:
-        return (k.data_ptr(), v.data_ptr(), *ks[:4], *vs[:4], _CODES[k.dtype], n[1], n[3], n[2], n[4], n[0])
-    return (k.data_ptr(), v.data_ptr(), 0, *ks[:3], 0, *vs[:3], _CODES[k.dtype], n[0], n[2], n[1], n[3], 1)
+        return (k.data_ptr(), v.data_ptr(), *ks[:4], *vs[:4], code, n[1], n[3], n[2], n[4], n[0])
+    return (k.data_ptr(), v.data_ptr(), 0, ks[0], ks[1], ks[2], 0, vs[0], vs[1], vs[2], code, n[0], n[2], n[1], n[3], 1)
 
 
-def _ints(x, device, n: int | None, name: str) -> torch.Tensor:
+def _ints(x, device, n: int, name: str) -> torch.Tensor:
     if not (isinstance(x, torch.Tensor) and x.dtype is torch.int32 and x.device == device and x.dim() == 1
             and x.is_contiguous()):
         x = device_ints(x, device)
-    if n is not None and x.shape[0] != n:
+    if x.shape[0] != n:
         _fail(f"{name} must have {n} entries")
     return x
 
@@ -82,40 +85,44 @@ def _table(x, device, name: str) -> torch.Tensor:
         _fail(f"{name} must be [requests][pages of a request]")
     if x.dtype is not torch.int32 or x.device != device:
         x = x.to(device=device, dtype=torch.int32)
-    if x.shape[1] and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
-        x = x.contiguous()
+    if not x.is_contiguous():
+        n, st = x.shape, x.stride()
+        if n[1] and st[1] != 1 or n[0] > 1 and st[0] < n[1]:
+            x = x.contiguous()
     return x
 
 
-def _rows(x: torch.Tensor, dtype, device, heads: int | None, head_dim: int, rows: int | None, name: str) -> torch.Tensor:
-    if x.dim() != 3 or x.shape[2] != head_dim or (heads is not None and x.shape[1] != heads) or \
-            (rows is not None and x.shape[0] != rows):
+def _rows(x: torch.Tensor, dtype, device, heads: int | None, head_dim: int, rows: int | None, name: str) -> tuple:
+    """(the tensor whose memory is read, its first two strides, its shape)"""
+    n = x.shape
+    if len(n) != 3 or n[2] != head_dim or (heads is not None and n[1] != heads) or (rows is not None and n[0] != rows):
         _fail(f"{name} must be [rows][heads][head_dim] to match the pages and q")
     if x.dtype is not dtype or x.device != device:
         _fail(f"{name} must be {dtype} on {device}")
-    s, unit = x.stride(), 16 // x.element_size()
+    s, unit = x.stride(), 8 if dtype is torch.bfloat16 else 4
     if s[2] != 1 or s[0] % unit or s[1] % unit or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
-    return x
+        s = x.stride()
+    return x, s, n
 
 
-def _batch(q: torch.Tensor, table, kv_lens, q_offsets, device) -> tuple:
+def _batch(T: int, H: int, table, kv_lens, q_offsets, device) -> tuple:
     table = _table(table, device, "page_table")
-    B = table.shape[0]
+    B, cols = table.shape
     lens = _ints(kv_lens, device, B, "kv_lens")
     off = None if q_offsets is None else _ints(q_offsets, device, B + 1, "q_offsets")
-    if off is None and (q.shape[0] % B if B else q.shape[0]):
+    if off is None and (T % B if B else T):
         _fail("without q_offsets, q's rows must be a multiple of the requests")
-    args = (table.data_ptr(), table.stride(0) if B > 1 else table.shape[1], table.shape[1], B, lens.data_ptr(),
-            0 if off is None else off.data_ptr(), q.shape[0], q.shape[1])
-    return args, (table, lens, off), B
+    # the tensors come back too: a converted one must live until the launch
+    return (table.data_ptr(), table.stride(0) if B > 1 else cols, cols, B, lens.data_ptr(),
+            0 if off is None else off.data_ptr(), T, H), B, (table, lens, off)
 
 
-def _out(out, like: torch.Tensor, dtype) -> torch.Tensor:
+def _out(out, x: torch.Tensor, shape, dtype) -> torch.Tensor:
     if out is None:
-        return torch.empty(like.shape, dtype=dtype, device=like.device)
-    if out.shape != like.shape or out.dtype is not dtype or out.device != like.device or not out.is_contiguous():
-        _fail(f"out must be a contiguous {tuple(like.shape)} {dtype} tensor on {like.device}")
+        return x.new_empty(shape, dtype=dtype)
+    if out.shape != shape or out.dtype is not dtype or out.device != x.device or not out.is_contiguous():
+        _fail(f"out must be a contiguous {tuple(shape)} {dtype} tensor on {x.device}")
     return out
 
 
@@ -133,14 +140,14 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
     one call must not fall on the same page slot."""
     dev = k_pages.device
     pages = _pages(k_pages, v_pages)
-    D = k_pages.shape[3]
-    if q.dtype not in _CODES:
+    D, Hk, src = pages[14], pages[13], q.dtype
+    if src not in _CODES:
         _fail("q must be fp32 or bf16")
-    q = _rows(q, q.dtype, dev, None, D, None, "q")
-    T = q.shape[0]
-    k = _rows(k, q.dtype, dev, k_pages.shape[1], D, T, "k")
-    v = _rows(v, q.dtype, dev, k_pages.shape[1], D, T, "v")
-    batch, keep, B = _batch(q, page_table, kv_lens, q_offsets, dev)
+    q, qs, shape = _rows(q, src, dev, None, D, None, "q")
+    T = shape[0]
+    k, ks, _ = _rows(k, src, dev, Hk, D, T, "k")
+    v, vs, _ = _rows(v, src, dev, Hk, D, T, "v")
+    batch, B, keep = _batch(T, shape[1], page_table, kv_lens, q_offsets, dev)
     pos = None if positions is None else _ints(positions, dev, T, "positions")
     gains = []
     for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
@@ -150,51 +157,59 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
             if w.dtype is not torch.float32 or w.device != dev or not w.is_contiguous() or w.data_ptr() % 16:
                 w = w.to(device=dev, dtype=torch.float32, copy=True).contiguous()
         gains.append(w)
-    out = _out(out, q, k_pages.dtype)
+    qn, kn = gains
+    out = _out(out, q, shape, k_pages.dtype)
     if T == 0 or B == 0:
         return out
-    qs, ks, vs = q.stride(), k.stride(), v.stride()
     ctx = Context.get(dev)
-    args = _APPEND.pack(*pages, *batch, q.data_ptr(), k.data_ptr(), v.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0],
-                        vs[1], 0 if pos is None else pos.data_ptr(), *(0 if w is None else w.data_ptr() for w in gains),
-                        out.data_ptr(), base, eps, _CODES[q.dtype], 0)
-    ctx.check(lib().wc_paged_append(ctx.h, _stream(ctx.device.index), args))
+    ctx.check(lib().wc_paged_append(ctx.h, _stream(ctx.device.index), _APPEND.pack(
+        *pages, *batch, q.data_ptr(), k.data_ptr(), v.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1],
+        0 if pos is None else pos.data_ptr(), 0 if qn is None else qn.data_ptr(), 0 if kn is None else kn.data_ptr(),
+        out.data_ptr(), base, eps, _CODES[src], 0)))
     return out
+
+
+@lru_cache(maxsize=4096)
+def _workspace(device: int, code: int, pages: int, page_size: int, kv_heads: int, head_dim: int, cols: int,
+               requests: int, rows: int, heads: int, groups: int) -> int:
+    """Bytes of scratch for calls of these sizes (the library looks at no buffer for this)."""
+    n = C.c_uint64()
+    ctx = Context.get(device)
+    st = head_dim * page_size * kv_heads
+    strides = (0, st, head_dim * page_size, head_dim)
+    ctx.check(lib().wc_paged_attention_workspace(ctx.h, _ATTENTION.pack(
+        16, 16, *strides, *strides, code, pages, page_size, kv_heads, head_dim, 1, 16, cols, cols, requests, 16, 16,
+        rows, heads, 16, 0, 0, 0, 16, 0, 16, 16, groups, 0, 16, 0, 0, 1.0, 0), C.byref(n)))
+    return n.value
 
 
 def _attend(q, k_pages, v_pages, prefix, page_table, kv_lens, q_offsets, tree_mask, scale, out):
     dev = k_pages.device
     pages = _pages(k_pages, v_pages)
-    D = k_pages.shape[3]
-    q = _rows(q, k_pages.dtype, dev, None, D, None, "q")
-    T, H, _ = q.shape
-    batch, keep, B = _batch(q, page_table, kv_lens, q_offsets, dev)
+    D, kind = pages[14], k_pages.dtype
+    q, qs, shape = _rows(q, kind, dev, None, D, None, "q")
+    T, H, _ = shape
+    batch, B, keep = _batch(T, H, page_table, kv_lens, q_offsets, dev)
     if tree_mask is not None:
         if tree_mask.dtype is not torch.int64 or tree_mask.shape != (T,) or tree_mask.device != dev:
             _fail("tree_mask must be int64 [rows], a bit for each of the request's new rows")
         tree_mask = tree_mask.contiguous()
-    if prefix is None:
-        pre, ends = (0, 0, 0, 0, 0, 0), ()
-    else:
+    G, pre = 0, (0, 0, 0, 0, 0, 0)
+    if prefix is not None:
         table = _table(prefix[0], dev, "prefix_table")
-        G = table.shape[0]
-        ends = (table, _ints(prefix[1], dev, G, "prefix_lens"), _ints(prefix[2], dev, G + 1, "group_offsets"))
-        pre = (table.data_ptr(), table.stride(0) if G > 1 else table.shape[1], ends[1].data_ptr(), ends[2].data_ptr(),
-               G, table.shape[1])
-    out = _out(out, q, q.dtype)
+        G, cols = table.shape
+        plens, ends = _ints(prefix[1], dev, G, "prefix_lens"), _ints(prefix[2], dev, G + 1, "group_offsets")
+        pre = (table.data_ptr(), table.stride(0) if G > 1 else cols, plens.data_ptr(), ends.data_ptr(), G, cols)
+    out = _out(out, q, shape, kind)
     if T == 0 or B == 0:
         return out
-    scale = float(D ** -0.5 if scale is None else scale)
-    qs = q.stride()
     ctx = Context.get(dev)
-    head = (*pages, *batch, q.data_ptr(), qs[0], qs[1], 0 if tree_mask is None else tree_mask.data_ptr(), *pre,
-            out.data_ptr())
-    n = C.c_uint64()
-    ctx.check(lib().wc_paged_attention_workspace(ctx.h, _ATTENTION.pack(*head, 0, 0, scale, 0), C.byref(n)))
-    ws = torch.empty(n.value + 256, dtype=torch.uint8, device=dev)
-    at = -(-ws.data_ptr() // 256) * 256
-    ctx.check(lib().wc_paged_attention(ctx.h, _stream(ctx.device.index),
-                                       _ATTENTION.pack(*head, at, n.value, scale, 0)))
+    device = ctx.device.index
+    n = _workspace(device, pages[10], pages[11], pages[12], pages[13], D, batch[2], B, T, H, G)
+    ws = q.new_empty(n + 256, dtype=torch.uint8)
+    ctx.check(lib().wc_paged_attention(ctx.h, _stream(device), _ATTENTION.pack(
+        *pages, *batch, q.data_ptr(), qs[0], qs[1], 0 if tree_mask is None else tree_mask.data_ptr(), *pre,
+        out.data_ptr(), -(-ws.data_ptr() // 256) * 256, n, D ** -0.5 if scale is None else scale, 0)))
     return out
 
 
@@ -236,18 +251,19 @@ def paged_compact(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table, star
     dev = k_pages.device
     pages = _pages(k_pages, v_pages, layers=k_pages.dim() == 5)
     table = _table(page_table, dev, "page_table")
-    B = table.shape[0]
+    B, cols = table.shape
     starts = _ints(starts, dev, B, "starts")
     n_keep = _ints(n_keep, dev, B, "n_keep")
     keep = _table(keep, dev, "keep")
-    if keep.shape[0] != B or keep.shape[1] < 1:
+    most = keep.shape[1]
+    if keep.shape[0] != B or most < 1:
         _fail("keep must be [requests][at least 1]")
-    lens = torch.empty(B, dtype=torch.int32, device=dev)
+    lens = starts.new_empty(B)
     if B == 0:
         return lens
     ctx = Context.get(dev)
-    args = _COMPACT.pack(*pages, table.data_ptr(), table.stride(0) if B > 1 else table.shape[1], table.shape[1], B,
-                         starts.data_ptr(), keep.data_ptr(), keep.stride(0) if B > 1 else keep.shape[1],
-                         n_keep.data_ptr(), lens.data_ptr(), keep.shape[1])
-    ctx.check(lib().wc_paged_compact(ctx.h, _stream(ctx.device.index), args))
+    many = B > 1
+    ctx.check(lib().wc_paged_compact(ctx.h, _stream(ctx.device.index), _COMPACT.pack(
+        *pages, table.data_ptr(), table.stride(0) if many else cols, cols, B, starts.data_ptr(), keep.data_ptr(),
+        keep.stride(0) if many else most, n_keep.data_ptr(), lens.data_ptr(), most)))
     return lens
