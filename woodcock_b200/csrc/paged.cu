@@ -203,7 +203,7 @@ extern "C" wc_status wc_paged_compact(wc_ctx* ctx, void* stream, const wc_paged_
 
 namespace {
 
-enum Variant { kSimt, kFew16, kFew32, kMany128, kMany256 };
+enum Variant { kSimt, kFew, kMany128, kMany256 };
 
 struct Launch {
   Variant variant;
@@ -220,8 +220,8 @@ Launch plan_launch(const wc_ctx* ctx, const wc_pages& g, long long rows) {
     l.M = PS_M;
     l.blocks = ctx->num_sms * 2;
   } else {
-    l.variant = rows <= 16 ? kFew16 : rows <= 32 ? kFew32 : rows <= 128 ? kMany128 : kMany256;
-    l.M = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 128 ? 128 : 256;
+    l.variant = rows <= 16 ? kFew : rows <= 128 ? kMany128 : kMany256;
+    l.M = rows <= 16 ? 16 : rows <= 128 ? 128 : 256;
     l.blocks = ctx->num_sms;
   }
   return l;
@@ -304,13 +304,13 @@ CUtensorMap page_map(const wc_pages& g, const PagePool& pool, int rows, int halv
   return m;
 }
 
-template <int D, int RG>
+template <int D>
 void launch_few(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, const PagedAttnParams& p, int kinds, const Launch& l,
                  bool late) {
-  const size_t smem = PfLayout<D, 16 * RG>::bytes();
-  static_assert(PfLayout<D, 16 * RG>::bytes() <= kSmemOptinBytes, "shared memory");
-  opt_in(ctx, paged_few_kernel<D, RG>, smem);
-  launch_on(ctx, st, "paged_few", paged_few_kernel<D, RG>, dim3(l.blocks), dim3(PF_THREADS), smem, true, 1,
+  const size_t smem = PfLayout<D>::bytes();
+  static_assert(PfLayout<D>::bytes() <= kSmemOptinBytes, "shared memory");
+  opt_in(ctx, paged_few_kernel<D>, smem);
+  launch_on(ctx, st, "paged_few", paged_few_kernel<D>, dim3(l.blocks), dim3(PF_THREADS), smem, true, 1,
             page_map(g, p.K, PF_KT, D / 64), page_map(g, p.V, PF_KT, D / 64), p, kinds, l.min_per, late);
 }
 
@@ -331,10 +331,8 @@ void launch_attention(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, const Pag
     opt_in(ctx, paged_simt_kernel<S, D>, paged_simt_smem<D>());
     launch_on(ctx, st, "paged_simt", paged_simt_kernel<S, D>, dim3(l.blocks), dim3(PS_THREADS), paged_simt_smem<D>(),
               true, 1, p, kinds, l.min_per, late);
-  } else if (l.variant == kFew16) {
-    launch_few<D, 1>(ctx, st, g, p, kinds, l, late);
-  } else if (l.variant == kFew32) {
-    launch_few<D, 2>(ctx, st, g, p, kinds, l, late);
+  } else if (l.variant == kFew) {
+    launch_few<D>(ctx, st, g, p, kinds, l, late);
   } else if (l.variant == kMany128) {
     launch_many<D, false>(ctx, st, g, p, kinds, l, late);
   } else {

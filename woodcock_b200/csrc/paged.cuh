@@ -338,8 +338,20 @@ template <int M, int KT>
 __device__ __forceinline__ long long paged_head_tiles(const PagedAttnParams& p, const PagedSeg& g) {
   const int qts = (g.n * p.rep + M - 1) / M;
   if (g.prefix || p.tree) return (long long)qts * paged_item_tiles<M, KT>(p, g, 0);
+  // the last row of tile qt is ((qt + 1) M - 1) / rep: its quotient and remainder step from tile to tile
+  const int base = g.klen - g.n + 1, dq = M / p.rep, dr = M - dq * p.rep;
+  int q = (M - 1) / p.rep, r = (M - 1) - q * p.rep;
   long long n = 0;
-  for (int qt = 0; qt < qts; ++qt) n += paged_item_tiles<M, KT>(p, g, qt);
+  for (int qt = 0; qt < qts; ++qt) {
+    const int seen = min(max(base + min(g.n - 1, q), 0), g.klen);
+    n += max(1, (seen + KT - 1) / KT);
+    q += dq;
+    r += dr;
+    if (r >= p.rep) {
+      r -= p.rep;
+      ++q;
+    }
+  }
   return n;
 }
 
@@ -397,6 +409,7 @@ struct PagedWalk {
         if (pass && a <= pos && pos < a + w) {
           sh[32] = s;
           sh[33] = pos - a;
+          sh[34] = w;
         }
         base += all;
         if (pass || nseg > nt) __syncthreads();
@@ -407,7 +420,7 @@ struct PagedWalk {
     long long off = sh[33];
     g = paged_seg(p, kinds, seg);
     qts = (g.n * p.rep + M - 1) / M;
-    const long long ph = units(p, g);
+    const long long ph = sh[34] / p.Hk;
     head = int(off / ph);
     off -= head * ph;
     qt = 0;
@@ -461,7 +474,7 @@ struct PagedWalk {
 __device__ __forceinline__ void paged_no_rec(const PagedAttnParams& p) {
   if (p.G == 0 && threadIdx.x == 0) p.rec[blockIdx.x] = PagedRec{};
 }
-constexpr int kWalkShared = 34;
+constexpr int kWalkShared = 36;
 
 // What one query row sees: keys below `lim`, and with a tree the new rows in `bits`.
 struct PagedRow {
@@ -702,20 +715,21 @@ __device__ __forceinline__ void paged_redo_row(const PagedAttnParams& p, const P
 }
 
 // ---------------------------------------------------------------------------- few rows: streamed pages
-// Decoding steps and short chains: at most 32 rows against each key, so the pages' bytes bound the
+// Decoding steps and short chains: at most 16 rows against each key, so the pages' bytes bound the
 // time. One producer warp streams 64-key tiles of K and V (TMA, 128-byte swizzle, a page's rows per
-// copy) through a ring that fills most of shared memory; eight consumer warps cut every tile into
-// 16-key slices, so that a tile is held only for a quarter of its arithmetic and no two warps wait
-// for one another before the item's end: each keeps its own running maximum, sum and 16 x D output
-// (mma m16n8k16), joined in shared memory once per item. With 16 rows the tiles alternate between
-// two sets of four warps, with 32 rows each slice has a warp per 16 rows.
+// copy) through a ring that fills most of shared memory; two sets of four consumer warps take the
+// tiles in turn, a 16-key slice per warp, so that no two warps wait for one another before the item's
+// end: each keeps its own running maximum, sum and 16 x D output (mma m16n8k16), joined in shared
+// memory once per item. The producer also walks the line and hands the items over with their query
+// rows, one item ahead.
 constexpr int PF_CONSUMERS = 8;
 constexpr int PF_THREADS = 32 * (PF_CONSUMERS + 1);
-constexpr int PF_KT = 64;
+constexpr int PF_KT = 64, PF_M = 16;
 constexpr int PF_OVER = 4;
 
-template <int D, int M>
+template <int D>
 struct PfLayout {
+  static constexpr int M = PF_M;
   static constexpr int kTile = PF_KT * D * 2;          // K or V of one tile
   static constexpr int kStage = 2 * kTile;
   static constexpr int kJoin = 4 * 16 * D * 4;         // four 16-row partial outputs
@@ -773,12 +787,12 @@ struct PageWindow {
   }
 };
 
-template <int D, int RG>
+template <int D>
 __global__ void __launch_bounds__(PF_THREADS, 1)
     paged_few_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                      const __grid_constant__ PagedAttnParams p, int kinds, int min_per, bool late) {
-  constexpr int M = 16 * RG, KT = PF_KT, NK = D / 16, ND = D / 8;
-  using L = PfLayout<D, M>;
+  constexpr int M = PF_M, KT = PF_KT, NK = D / 16, ND = D / 8;
+  using L = PfLayout<D>;
   constexpr int NST = L::kStages;
   extern __shared__ unsigned char pf_raw[];
   unsigned char* sm = pf_raw + ((1024u - (smem_addr(pf_raw) & 1023u)) & 1023u);
@@ -886,8 +900,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
 
   // ---- consumers
   const int g = lane >> 2, t = lane & 3;
-  const int rg = RG == 1 ? 0 : (warp & 1);
-  const int slice = RG == 1 ? (warp & 3) : (warp >> 1);
+  const int slice = warp & 3;
   const float sl2 = p.scale_log2;
   // a copy's rows lie together, half rows of 128 bytes one after the other
   const int box = min(1 << p.page_log2, KT), hstride = box * 128;
@@ -902,12 +915,12 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     named_sync(1, 32 * PF_CONSUMERS);
     if (*stop) break;
     const PfItem it = items[b];
-    const PagedRow ra = paged_row(p, it.g, it.head, it.qt * M + rg * 16 + g);
-    const PagedRow rb = paged_row(p, it.g, it.head, it.qt * M + rg * 16 + g + 8);
+    const PagedRow ra = paged_row(p, it.g, it.head, it.qt * M + g);
+    const PagedRow rb = paged_row(p, it.g, it.head, it.qt * M + g + 8);
     uint32_t qa[NK][4];
 #pragma unroll
     for (int kk = 0; kk < NK; ++kk)
-      ldsm_x4(qa[kk], qbuf + (b * M + rg * 16 + (lane & 15)) * L::kQRow + kk * 32 + (lane >> 4) * 16);
+      ldsm_x4(qa[kk], qbuf + (b * M + (lane & 15)) * L::kQRow + kk * 32 + (lane >> 4) * 16);
     __syncwarp();
     if (lane == 0) mbar_arrive(it_empty + b);
     // rows that pad the tile count as seeing everything: their results go nowhere
@@ -923,7 +936,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     for (int kt = it.kt0; kt < it.kt1; ++kt, ++cnt) {
       const int s = cnt % NST;
       paged_wait(full + s, (cnt / NST) & 1, dead, p.err);
-      if (RG == 1 && (cnt & 1) != (warp >> 2)) {
+      if ((cnt & 1) != (warp >> 2)) {
         // The other set's tile. Its phases are waited for and passed on all the same: a set that met a
         // stage only every other use could take an earlier use, which a wait by parity does not tell
         // apart, for its own.
@@ -1062,11 +1075,11 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     for (int h = 0; h < 2; ++h) {
       float mx = -INFINITY, sum = 0.f;
 #pragma unroll
-      for (int q = 0; q < PF_CONSUMERS; q += RG) mx = fmaxf(mx, wml[(q + rg) * 16 + g + 8 * h].x);
+      for (int q = 0; q < PF_CONSUMERS; ++q) mx = fmaxf(mx, wml[q * 16 + g + 8 * h].x);
       const float mgx = mx == -INFINITY ? 0.f : mx;
 #pragma unroll
-      for (int q = 0; q < PF_CONSUMERS; q += RG) {
-        const float2 x = wml[(q + rg) * 16 + g + 8 * h];
+      for (int q = 0; q < PF_CONSUMERS; ++q) {
+        const float2 x = wml[q * 16 + g + 8 * h];
         sum += x.y * ex2_approx(x.x - mgx);
       }
       const float f = ex2_approx(m[h] - mgx);
@@ -1075,7 +1088,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         o[j][2 * h] *= f;
         o[j][2 * h + 1] *= f;
       }
-      if (warp < RG && t == 0) rml[rg * 16 + g + 8 * h] = make_float2(mx, sum);
+      if (warp == 0 && t == 0) rml[g + 8 * h] = make_float2(mx, sum);
     }
     float* mine = join + (warp & 3) * 16 * D;
     auto at = [&](int row, int col) { return row * D + (col ^ ((row & 3) << 3)); };  // spreads rows over the banks
@@ -1103,8 +1116,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       if (rho >= it.g.n * p.rep) continue;
       float y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int q = 0; q < 4; q += RG) {
-        const float4 x = *reinterpret_cast<const float4*>(join + (q + row / 16) * 16 * D + at(row % 16, col));
+      for (int q = 0; q < 4; ++q) {
+        const float4 x = *reinterpret_cast<const float4*>(join + q * 16 * D + at(row, col));
         y[0] += x.x;
         y[1] += x.y;
         y[2] += x.z;
@@ -1161,6 +1174,12 @@ struct PmLayout {
                                      : (int(kSmemOptinBytes) - 1024 - kQ - kTail) / kTile;
   static constexpr size_t bytes() { return 1024 + size_t(kQ) + size_t(kStages) * kTile + kTail; }
 };
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
 // Bits of the 32 keys from k0 on that a row sees.
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u); }
@@ -1235,10 +1254,6 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
   Walk w;
   const bool work = w.begin(p, kinds, min_per, sh);
 
-  // registers: launched with 168 a thread (64512); 88 for the first four warps, 208 for the softmax warps
-  // (128 x 88 + 256 x 208 = 64512): a row's 128 scores stay in registers
-  if (warp < 4) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n");
   if ((warp == 0 || warp == 2) && work) {  // ---- K tiles (warp 0) and V tiles (warp 2)
     const bool isv = warp == 2;
     const int psize = 1 << p.page_log2;
@@ -1394,10 +1409,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
     done(drain);  // tensor memory is given back only when nothing writes it any more
     if (!mbar_wait(drain, 0)) raise_error(p.err, kErrTimeout);
     __syncwarp();
-  }
-  } else {  // ---- softmax: thread = row of its slot
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;\n");
-    if (work) {
+  } else if (warp >= 4 && work) {  // ---- softmax: thread = row of its slot
     const int slot = (warp - 4) >> 2, qd = warp & 3, r128 = qd * 32 + lane;
     const uint32_t lanes = tmem + (uint32_t(qd * 32) << 16);
     const uint32_t ts = lanes + slot * 128, to = lanes + kColO + slot * D;
@@ -1448,68 +1460,13 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
                                                 : w.g.klen - w.g.n + (p.tree ? 0 : (w.qt * M + (kTwo ? slot * 128 : 0)) / p.rep + 1));
       float m = -INFINITY, l = 0.f;
       const int step = kTwo ? 1 : 2;
+      const bool rows = __any_sync(0xffffffffu, r.valid);
       for (int t = kTwo ? 0 : slot; t < nt && active; t += step) {
         paged_wait(s_full + slot, ns & 1, dead, p.err);
         ++ns;
         tc_fence_after();
-        uint32_t s0[64], s1[64];
-        tmem_ld64(ts, s0);
-        tmem_ld64(ts + 64, s1);
         const int key0 = (w.kt0 + t) * KT;
         const bool masked = key0 + KT > lim;
-        if (masked && r.valid) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const uint32_t see = seen_bits(r, key0 + 32 * q);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              uint32_t& x = q < 2 ? s0[(q & 1) * 32 + j] : s1[(q & 1) * 32 + j];
-              if (!((see >> j) & 1u)) x = 0xff800000u;
-            }
-          }
-        }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int j = 0; j < 64; j += 2) {
-          mx[0] = fmaxf(mx[0], __uint_as_float(s0[j]));
-          mx[1] = fmaxf(mx[1], __uint_as_float(s0[j + 1]));
-          mx[2] = fmaxf(mx[2], __uint_as_float(s1[j]));
-          mx[3] = fmaxf(mx[3], __uint_as_float(s1[j + 1]));
-        }
-        const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
-        const bool first = t < step;
-        if (first) {
-          m = mt;
-        } else if (__any_sync(0xffffffffu, mt > m + 8.f)) {
-          const float mn = mt > m + 8.f ? mt : m;
-          const float f = m == mn ? 1.f : ex2_approx(m - mn);
-          m = mn;
-          l *= f;
-#pragma unroll 1
-          for (int c = 0; c < D; c += 32) {
-            uint32_t v[32];
-            tmem_ld32(to + c, v);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * f);
-            tmem_st32(to + c, v);
-          }
-        }
-        const float mg = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          uint32_t pk[32];
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float a = ex2_approx(fmaf(__uint_as_float(q ? s1[2 * j] : s0[2 * j]), sl2, -mg));
-            const float b = ex2_approx(fmaf(__uint_as_float(q ? s1[2 * j + 1] : s0[2 * j + 1]), sl2, -mg));
-            sum[(j & 1) * 2] += a;
-            sum[(j & 1) * 2 + 1] += b;
-            pk[j] = pack_bf16(a, b);  // weights rounded to bf16, as the values are (2^-9 of each)
-          }
-          tmem_st32(ts + q * 32, pk);
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         // Values in masked places may be anything, and 0 x NaN would reach every row. Behind the last
         // key they are cleared; between keys (a later row, another branch) they mark the tile's rows
         // for the joining kernel, which sums such rows over the seen keys alone.
@@ -1544,6 +1501,73 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
             if (worst == 0x7f800000u) redo[slot] = nitem;
           }
           fence_proxy_async_smem();
+        }
+        if (rows) {  // a warp whose rows only pad the tile passes on
+          // The scores are read from tensor memory twice, 32 columns at a time: for the maximum and for
+          // the weights. The loops stay rolled: the tile's code is small enough to stay in the instruction
+          // caches beside the other warps', which is worth more than the loads it would save (unrolled,
+          // or with the next load under way: 6 to 20% more time).
+          if (__any_sync(0xffffffffu, masked)) {  // tensor memory is read and written by whole warps
+#pragma unroll 1
+            for (int c = 0; c < KT; c += 32) {
+              uint32_t v[32];
+              tmem_ld32(ts + c, v);
+              const uint32_t see = masked ? seen_bits(r, key0 + c) : 0xffffffffu;
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (!((see >> j) & 1u)) v[j] = 0xff800000u;
+              tmem_st32(ts + c, v);
+            }
+            tmem_st_wait();
+          }
+          float mt = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; c < KT; c += 32) {
+            uint32_t v[32];
+            tmem_ld32(ts + c, v);
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = fmaxf(__uint_as_float(v[e]), __uint_as_float(v[e + 4]));
+#pragma unroll
+            for (int j = 8; j < 32; j += 8)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[e] = max3(x[e], __uint_as_float(v[j + e]), __uint_as_float(v[j + e + 4]));
+            mt = max3(mt, fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+          }
+          mt *= sl2;
+          if (t < step) {
+            m = mt;
+          } else if (__any_sync(0xffffffffu, mt > m + 8.f)) {
+            const float mn = mt > m + 8.f ? mt : m;
+            const float f = m == mn ? 1.f : ex2_approx(m - mn);
+            m = mn;
+            l *= f;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              uint32_t v[32];
+              tmem_ld32(to + c, v);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * f);
+              tmem_st32(to + c, v);
+            }
+          }
+          const float mg = m == -INFINITY ? 0.f : m;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+          for (int c = 0; c < KT; c += 32) {
+            uint32_t v[32], pk[16];
+            tmem_ld32(ts + c, v);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float x = ex2_approx(fmaf(__uint_as_float(v[2 * j]), sl2, -mg));
+              const float y = ex2_approx(fmaf(__uint_as_float(v[2 * j + 1]), sl2, -mg));
+              sum[(j & 1) * 2] += x;
+              sum[(j & 1) * 2 + 1] += y;
+              pk[j] = pack_bf16(x, y);  // weights rounded to bf16, as the values are (2^-9 of each)
+            }
+            tmem_st16u(ts + c / 2, pk);  // over scores that both passes have read
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         }
         tmem_st_wait();
         tc_fence_before();
@@ -1669,7 +1693,6 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
       ++nitem;
       w = nx;
     } while (more);
-    }
   }
   tc_fence_before();
   __syncthreads();
