@@ -207,14 +207,13 @@ enum Variant { kSimt, kFew, kMany128, kMany256 };
 
 struct Launch {
   Variant variant;
-  int M, blocks, min_per;
+  int M, blocks;
 };
 
-// One launch: its row tile, blocks and the least key tiles a block takes on. `rows`: query rows per
+// One launch: its row tile and the blocks that share its key tiles. `rows`: query rows per
 // segment and KV head, on average.
 Launch plan_launch(const wc_ctx* ctx, const wc_pages& g, long long rows) {
   Launch l;
-  l.min_per = 1;
   if (g.dtype == WC_F32) {
     l.variant = kSimt;
     l.M = PS_M;
@@ -311,7 +310,7 @@ void launch_few(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, const PagedAttn
   static_assert(PfLayout<D>::bytes() <= kSmemOptinBytes, "shared memory");
   opt_in(ctx, paged_few_kernel<D>, smem);
   launch_on(ctx, st, "paged_few", paged_few_kernel<D>, dim3(l.blocks), dim3(PF_THREADS), smem, true, 1,
-            page_map(g, p.K, PF_KT, D / 64), page_map(g, p.V, PF_KT, D / 64), p, kinds, l.min_per, late);
+            page_map(g, p.K, PF_KT, D / 64), page_map(g, p.V, PF_KT, D / 64), p, kinds, late);
 }
 
 template <int D, bool kTwo>
@@ -321,7 +320,7 @@ void launch_many(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, const PagedAtt
   static_assert(PmLayout<D, kTwo>::bytes() <= kSmemOptinBytes, "shared memory");
   opt_in(ctx, paged_many_kernel<D, kTwo>, smem);
   launch_on(ctx, st, "paged_many", paged_many_kernel<D, kTwo>, dim3(l.blocks), dim3(PM_THREADS), smem, true, 1,
-            page_map(g, p.K, PM_KT, 1), page_map(g, p.V, PM_KT, D / 64), p, kinds, l.min_per, late);
+            page_map(g, p.K, PM_KT, 1), page_map(g, p.V, PM_KT, D / 64), p, kinds, late);
 }
 
 template <typename S, int D>
@@ -330,7 +329,7 @@ void launch_attention(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, const Pag
   if constexpr (sizeof(S) == 4) {
     opt_in(ctx, paged_simt_kernel<S, D>, paged_simt_smem<D>());
     launch_on(ctx, st, "paged_simt", paged_simt_kernel<S, D>, dim3(l.blocks), dim3(PS_THREADS), paged_simt_smem<D>(),
-              true, 1, p, kinds, l.min_per, late);
+              true, 1, p, kinds, late);
   } else if (l.variant == kFew) {
     launch_few<D>(ctx, st, g, p, kinds, l, late);
   } else if (l.variant == kMany128) {

@@ -355,6 +355,11 @@ __device__ __forceinline__ long long paged_head_tiles(const PagedAttnParams& p, 
   return n;
 }
 
+// a / b for a >= 0, b > 0: almost always of 32-bit values, whose division is several times shorter
+__device__ __forceinline__ long long paged_div(long long a, long long b) {
+  return ((a | b) >> 32) ? a / b : (long long)(uint32_t(a) / uint32_t(b));
+}
+
 // One block's walk over its range of the line, item by item. An item counts kOver units beyond its key
 // tiles, for what it costs whatever its length (its queries, its result, the way there); a block whose
 // range holds only such units of an item passes it over.
@@ -373,14 +378,14 @@ struct PagedWalk {
   }
 
   // Block-collective; `sh` holds kWalkShared words. False: the block has no work.
-  __device__ bool begin(const PagedAttnParams& p, int kinds, int min_per, long long* sh) {
+  __device__ bool begin(const PagedAttnParams& p, int kinds, long long* sh) {
     nseg = ((kinds & kPrefixRows) ? p.G : 0) + ((kinds & kOwnRows) ? p.B : 0);
     const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, nw = (nt + 31) >> 5;
     long long total = 0, w = 0, x = 0;
     pos = 0;
     for (int pass = 0; pass < 2; ++pass) {
       if (pass) {
-        per = int(max((long long)min_per, (total + gridDim.x - 1) / gridDim.x));
+        per = int(paged_div(total + gridDim.x - 1, gridDim.x));
         pos = (long long)blockIdx.x * per;
         end = min(pos + per, total);
         if (pos >= end) return false;
@@ -420,8 +425,8 @@ struct PagedWalk {
     long long off = sh[33];
     g = paged_seg(p, kinds, seg);
     qts = (g.n * p.rep + M - 1) / M;
-    const long long ph = sh[34] / p.Hk;
-    head = int(off / ph);
+    const long long ph = paged_div(sh[34], p.Hk);
+    head = int(paged_div(off, ph));
     off -= head * ph;
     qt = 0;
     while (off >= (ktn = paged_item_tiles<M, KT>(p, g, qt)) + kOver) {
@@ -435,8 +440,8 @@ struct PagedWalk {
     const long long item = pos - off;  // the item's first unit
     kt0 = max(0, off - kOver);
     kt1 = int(min((long long)ktn, end - item - kOver));
-    first = int((item + kOver) / per);
-    count = int((item + kOver + ktn - 1) / per) - first + 1;
+    first = int(paged_div(item + kOver, per));
+    count = int(paged_div(item + kOver + ktn - 1, per)) - first + 1;
     pos = min(end, item + kOver + ktn);
     return kt1 > kt0;
   }
@@ -459,7 +464,7 @@ struct PagedWalk {
   }
   // Number of the item among those of its kind and head: distinct, below T rep / M + segments + 1.
   __device__ int item(const PagedAttnParams& p) const {
-    return int((long long)g.tok0 * p.rep / M) + g.idx + qt;
+    return g.tok0 * p.rep / M + g.idx + qt;  // rows x heads is below 2^30
   }
   // Where this block's share of a divided item goes: slot 0 when the item began in an earlier block.
   __device__ int slot() const { return kt0 > 0 ? 0 : 1; }
@@ -475,6 +480,13 @@ __device__ __forceinline__ void paged_no_rec(const PagedAttnParams& p) {
   if (p.G == 0 && threadIdx.x == 0) p.rec[blockIdx.x] = PagedRec{};
 }
 constexpr int kWalkShared = 36;
+
+// An item as the warp that walks hands it to the others; count 0: the line's end.
+struct __align__(16) PagedItem {
+  PagedSeg g;
+  int head, qt, kt0, kt1, count, slot, pad[5];
+};
+static_assert(sizeof(PagedItem) == 64, "item queue");
 
 // What one query row sees: keys below `lim`, and with a tree the new rows in `bits`.
 struct PagedRow {
@@ -542,7 +554,7 @@ constexpr size_t paged_simt_smem() {
 
 template <typename S, int D>
 __global__ void __launch_bounds__(PS_THREADS)
-    paged_simt_kernel(const __grid_constant__ PagedAttnParams p, int kinds, int min_per, bool late) {
+    paged_simt_kernel(const __grid_constant__ PagedAttnParams p, int kinds, bool late) {
   constexpr int M = PS_M, KT = PS_KT, LD = D + 4, LS = KT + 4;
   constexpr int RPT = D / 64;  // rows per thread of P V: two (D 128), one (D 64)
   extern __shared__ __align__(16) float ps_smem[];
@@ -556,7 +568,7 @@ __global__ void __launch_bounds__(PS_THREADS)
   pdl_launch_dependents();
   PagedWalk<M, KT, 1> w;
   paged_no_rec(p);
-  if (!w.begin(p, kinds, min_per, sh)) {
+  if (!w.begin(p, kinds, sh)) {
     if (late) pdl_wait();
     return;
   }
@@ -740,12 +752,6 @@ struct PfLayout {
   static constexpr size_t bytes() { return 1024 + size_t(kStages) * kStage + kJoin + kQ + kTail; }
 };
 
-// An item as the producer hands it to the other warps.
-struct PfItem {
-  PagedSeg g;
-  int head, qt, kt0, kt1, count, slot, pad[5];
-};
-static_assert(sizeof(PfItem) == 64, "item queue");
 
 // Waits give up after a bound; then `dead` lets the block's other waits pass, so that it ends.
 __device__ __forceinline__ void paged_wait(uint64_t* bar, uint32_t parity, volatile int* dead, int* err) {
@@ -790,7 +796,7 @@ struct PageWindow {
 template <int D>
 __global__ void __launch_bounds__(PF_THREADS, 1)
     paged_few_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
-                     const __grid_constant__ PagedAttnParams p, int kinds, int min_per, bool late) {
+                     const __grid_constant__ PagedAttnParams p, int kinds, bool late) {
   constexpr int M = PF_M, KT = PF_KT, NK = D / 16, ND = D / 8;
   using L = PfLayout<D>;
   constexpr int NST = L::kStages;
@@ -808,7 +814,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   volatile int* stop = dead + 1;
   float2* wml = reinterpret_cast<float2*>(tail + 8 * kWalkShared + 256);  // [8 warps][16 rows]
   float2* rml = wml + 8 * 16;                                            // [M]
-  PfItem* items = reinterpret_cast<PfItem*>(rml + M);                    // [2]
+  PagedItem* items = reinterpret_cast<PagedItem*>(rml + M);                    // [2]
   static_assert(32 + 16 * NST <= 248, "barriers");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -828,7 +834,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   PagedWalk<M, KT, PF_OVER> w;
   paged_no_rec(p);
   __syncthreads();
-  if (!w.begin(p, kinds, min_per, sh)) {
+  if (!w.begin(p, kinds, sh)) {
     if (late) pdl_wait();
     return;
   }
@@ -846,7 +852,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       if (lane == 0) {
         w.report(p);
         if (nitem >= 2) paged_wait(it_empty + b, ((nitem >> 1) - 1) & 1, dead, p.err);
-        items[b] = PfItem{w.g, w.head, w.qt, w.kt0, w.kt1, w.count, w.slot(), {}};
+        items[b] = PagedItem{w.g, w.head, w.qt, w.kt0, w.kt1, w.count, w.slot(), {}};
         const int rows = min(M, w.g.n * p.rep - w.qt * M);
         if (!*dead) mbar_arrive_expect_tx(it_full + b, rows * D * 2);
       }
@@ -914,7 +920,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     if (tid == 0) *stop = *dead || items[b].count == 0;
     named_sync(1, 32 * PF_CONSUMERS);
     if (*stop) break;
-    const PfItem it = items[b];
+    const PagedItem it = items[b];
     const PagedRow ra = paged_row(p, it.g, it.head, it.qt * M + g);
     const PagedRow rb = paged_row(p, it.g, it.head, it.qt * M + g + 8);
     uint32_t qa[NK][4];
@@ -1168,7 +1174,7 @@ template <int D, bool kTwo>
 struct PmLayout {
   static constexpr int kTile = PM_KT * D * 2;  // a K or V tile
   static constexpr int kQ = (kTwo ? 2 : 1) * 128 * D * 2;
-  static constexpr int kTail = 8 * kWalkShared + 512 + (kTwo ? 0 : 2 * 128 * 8);
+  static constexpr int kTail = 8 * kWalkShared + 400 + 4 * 64 + (kTwo ? 0 : 4 * 128 * 8);
   static constexpr int kStages = (int(kSmemOptinBytes) - 1024 - kQ - kTail) / kTile > 12
                                      ? 12
                                      : (int(kSmemOptinBytes) - 1024 - kQ - kTail) / kTile;
@@ -1196,7 +1202,7 @@ __device__ __forceinline__ uint32_t seen_bits(const PagedRow& r, int k0) {
 template <int D, bool kTwo>
 __global__ void __launch_bounds__(PM_THREADS, 1)
     paged_many_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
-                      const __grid_constant__ PagedAttnParams p, int kinds, int min_per, bool late) {
+                      const __grid_constant__ PagedAttnParams p, int kinds, bool late) {
   using L = PmLayout<D, kTwo>;
   constexpr int M = kTwo ? 256 : 128, KT = PM_KT, NST = L::kStages, HALVES = D / 64;
   constexpr uint32_t kColO = 256;
@@ -1215,10 +1221,14 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
   uint64_t* o_full = bars + 30;              // [2]: the item's output complete
   uint64_t* o_empty = bars + 32;             // [2]: and read
   uint64_t* drain = bars + 34;
-  volatile int* dead = reinterpret_cast<volatile int*>(bars + 36);
-  uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + 37);
-  volatile int* redo = reinterpret_cast<volatile int*>(bars + 38);  // [2]: number of the item to be redone
-  float2* xml = reinterpret_cast<float2*>(tail + 8 * kWalkShared + 512);  // [slot][row]: the slots' states
+  uint64_t* x_full = bars + 35;              // the slots' states are in shared memory
+  uint64_t* it_full = bars + 36;             // [4]: an item handed over
+  uint64_t* it_empty = bars + 40;            // [4]: and read by all
+  volatile int* dead = reinterpret_cast<volatile int*>(bars + 44);
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + 45);
+  volatile int* redo = reinterpret_cast<volatile int*>(bars + 46);  // [2]: number of the item to be redone
+  PagedItem* queue = reinterpret_cast<PagedItem*>(tail + 8 * kWalkShared + 400);          // [4]
+  float2* xml = reinterpret_cast<float2*>(tail + 8 * kWalkShared + 400 + 4 * 64);         // [item & 1][slot][row]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int s = 0; s < NST; ++s) {
@@ -1232,6 +1242,11 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
       mbar_init(o_full + s, 1);
       mbar_init(o_empty + s, kTwo ? 4 : 8);
     }
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(it_full + s, 1);
+      mbar_init(it_empty + s, 10);  // V copies, products, 8 softmax warps
+    }
+    mbar_init(x_full, 8);
     mbar_init(drain, 1);
     mbar_fence_init();
     *dead = 0;
@@ -1252,9 +1267,21 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
   const uint32_t tmem = *tslot;
   using Walk = PagedWalk<M, KT, PM_OVER>;
   Walk w;
-  const bool work = w.begin(p, kinds, min_per, sh);
+  const bool work = w.begin(p, kinds, sh);
 
-  if ((warp == 0 || warp == 2) && work) {  // ---- K tiles (warp 0) and V tiles (warp 2)
+  // The next item of the line, as the walking warp left it.
+  auto take_item = [&](int n) {
+    paged_wait(it_full + (n & 3), (n >> 2) & 1, dead, p.err);
+    PagedItem it = queue[n & 3];
+    if (*dead) it.count = 0;
+    return it;
+  };
+  auto release_item = [&](int n) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(it_empty + (n & 3));
+  };
+
+  if ((warp == 0 || warp == 2) && work) {  // ---- K tiles (warp 0, which also walks) and V tiles (warp 2)
     const bool isv = warp == 2;
     const int psize = 1 << p.page_log2;
     const int box = min(psize, KT), parts = KT / box;
@@ -1263,17 +1290,32 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
     const int part = isv ? lane : lane / HALVES, half = isv ? 0 : lane % HALVES;
     const int at = isv ? part * box * (D * 2) : half * (KT * 128) + part * box * 128;
     int base = 0, last = -1;
-    do {
-      const int nt = w.kt1 - w.kt0;
+    bool more = true;
+    for (int n = 0; more; ++n) {
+      PagedItem it;
+      if (!isv) {
+        if (n >= 4) paged_wait(it_empty + (n & 3), ((n >> 2) - 1) & 1, dead, p.err);
+        it = PagedItem{w.g, w.head, w.qt, w.kt0, w.kt1, w.count, w.slot(), {}};
+        if (lane == 0) {
+          w.report(p);
+          queue[n & 3] = it;
+          mbar_arrive(it_full + (n & 3));
+        }
+      } else {
+        it = take_item(n);
+        release_item(n);
+        if (it.count == 0) break;
+      }
+      const int nt = it.kt1 - it.kt0;
       PageWindow win;
-      win.start(p, w.g, (w.kt0 * KT) >> p.page_log2, lane);
+      win.start(p, it.g, (it.kt0 * KT) >> p.page_log2, lane);
       for (int t = 0; t < nt; ++t) {
         // The tile's place in the ring, in the order that the products take the tiles: K0 V0 K1 V1 ...,
         // or with alternating slots K0 K1 V0 K2 V1 ... The two warps meet at a stage in turns; since the
         // products free the stages in order, the use before last is over when this warp's last one was.
         const int pos = base + (kTwo ? 2 * t + isv : isv ? t + min(t + 2, nt) : t < 2 ? t : 2 * t - 1);
         const int s = pos % NST;
-        const int first = ((w.kt0 + t) * KT) >> p.page_log2;
+        const int first = ((it.kt0 + t) * KT) >> p.page_log2;
         win.seek(p, first, lane);
         const int page = __shfl_sync(0xffffffffu, win.cur, (first - win.base + part) & 31);
         if (lane == 0) {
@@ -1283,13 +1325,22 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
         __syncwarp();
         if (*dead) break;
         if (part < parts)
-          tma_load_5d(ring + size_t(s) * L::kTile + at, isv ? &tv : &tk, 0, ((w.kt0 + t) * KT) & (psize - 1), half,
-                      w.head, page, kv_full + s);
+          tma_load_5d(ring + size_t(s) * L::kTile + at, isv ? &tv : &tk, 0, ((it.kt0 + t) * KT) & (psize - 1), half,
+                      it.head, page, kv_full + s);
         __syncwarp();
         last = pos;
       }
       base += 2 * nt;
-    } while (!*dead && w.next(p, kinds));
+      if (*dead) break;
+      if (!isv && !(more = w.next(p, kinds))) {
+        const int e = n + 1;
+        if (e >= 4) paged_wait(it_empty + (e & 3), ((e >> 2) - 1) & 1, dead, p.err);
+        if (lane == 0) {
+          queue[e & 3].count = 0;
+          mbar_arrive(it_full + (e & 3));
+        }
+      }
+    }
     // shared memory must outlive the copies: the last one is waited for here, those before it by the
     // products that the block waits for, unless the block has given up
     if (lane == 0)
@@ -1351,10 +1402,13 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
     auto done = [&](uint64_t* bar) {
       if (issuer) umma_commit(bar);
     };
-    do {
-      const int nt = w.kt1 - w.kt0;
+    for (int n = 0;; ++n) {
+      const PagedItem it = take_item(n);
+      release_item(n);
+      if (it.count == 0) break;
+      const int nt = it.kt1 - it.kt0;
       if constexpr (kTwo) {
-        const bool two = w.g.n * p.rep - w.qt * M > 128;
+        const bool two = it.g.n * p.rep - it.qt * M > 128;
         int ks = take();
         queries(0);
         scores(0, 0, ks);
@@ -1405,7 +1459,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
           }
         }
       }
-    } while (!*dead && w.next(p, kinds));
+    }
     done(drain);  // tensor memory is given back only when nothing writes it any more
     if (!mbar_wait(drain, 0)) raise_error(p.err, kErrTimeout);
     __syncwarp();
@@ -1421,7 +1475,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
 
     // Query rows of an item into the slot's swizzled tile, asynchronously: 16 or 8 lanes copy a row, whose
     // place the lane that owns it knows.
-    auto copy_q = [&](const Walk& x) {
+    auto copy_q = [&](const PagedItem& x) {
       constexpr int CH = D / 8, RPI = 32 / CH;  // 16-byte pieces of a row, rows per step
       const PagedRow r = paged_row(p, x.g, x.head, x.qt * M + (kTwo ? slot * 128 : 0) + r128);
       const long long mine = r.valid ? r.tok * p.q_row + r.h * p.q_head : -1;
@@ -1443,13 +1497,13 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
       if (lane == 0) mbar_arrive(q_full + (kTwo ? slot : 0));
     };
     // whether an item's rows reach the second slot's tile; only then are its queries copied and waited for
-    auto both = [&](const Walk& x) { return x.g.n * p.rep - x.qt * M > 128; };
-    if (slot == 0 || (kTwo && both(w))) {
+    auto both = [&](const PagedItem& x) { return x.g.n * p.rep - x.qt * M > 128; };
+    PagedItem w = take_item(0);
+    if (w.count && (slot == 0 || (kTwo && both(w)))) {
       copy_q(w);
       copied_q();
     }
-    bool more;
-    do {
+    for (; w.count; ++nitem) {
       const int nt = w.kt1 - w.kt0;
       const bool two = kTwo ? both(w) : nt > 1;  // the second slot has work
       const bool active = slot == 0 || two;
@@ -1578,22 +1632,23 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
       // The item's queries have been used for the last time where the last scores were waited for (with
       // alternating slots, by the slot of the last tile): the next item's take their place while the
       // last product runs.
-      Walk nx = w;
-      more = nx.next(p, kinds);
-      const bool load = more && (kTwo ? slot == 0 || both(nx) : ((nt - 1) & 1) == slot);
+      const PagedItem nx = take_item(nitem + 1);
+      const bool load = nx.count && (kTwo ? slot == 0 || both(nx) : ((nt - 1) & 1) == slot);
       if (load) copy_q(nx);
       // ---- the item's result
       float f0 = 1.f, f1 = 0.f;
       if constexpr (!kTwo) {  // the slots' states joined; each group of warps takes half of the columns
-        xml[slot * 128 + r128] = make_float2(m, l);
-        named_sync(1, 256);
-        const float2 a = xml[r128], b = xml[128 + r128];
+        float2* x = xml + (nitem & 1) * 256;  // by turns: the item before last has been read by all
+        x[slot * 128 + r128] = make_float2(m, l);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(x_full);
+        paged_wait(x_full, nitem & 1, dead, p.err);
+        const float2 a = x[r128], b = x[128 + r128];
         m = fmaxf(a.x, b.x);
         const float mg = m == -INFINITY ? 0.f : m;
         f0 = ex2_approx(a.x - mg);
         f1 = ex2_approx(b.x - mg);
         l = a.y * f0 + b.y * f1;
-        named_sync(1, 256);
         paged_wait(o_full, no[0] & 1, dead, p.err);
         ++no[0];
         if (two) {
@@ -1605,7 +1660,6 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
         ++no[0];
       }
       if (load) copied_q();
-      if (warp == 4 && lane == 0) w.report(p);
       // every warp of the slot raised its mark before the product that o_full reports
       const bool again = kTwo ? active && redo[slot] == nitem : redo[0] == nitem || redo[1] == nitem;
       if (active || !kTwo) {
@@ -1613,7 +1667,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
         const bool direct = w.count == 1 && p.G == 0;
         const float inv = direct ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;
         const long long at = (long long)r.tok * p.H + r.h;
-        const long long pt = ((long long)blockIdx.x * 2 + w.slot()) * M + (kTwo ? slot * 128 : 0) + r128;
+        const long long pt = ((long long)blockIdx.x * 2 + w.slot) * M + (kTwo ? slot * 128 : 0) + r128;
         float* po = w.count == 1 ? p.whole_o[w.g.prefix] + at * D : p.part_o + pt * D;
         const int c0 = kTwo ? 0 : slot * (D / 2), c1 = kTwo ? D : c0 + D / 2;
 #pragma unroll 1
@@ -1677,7 +1731,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
             float mi, li, oi[D / 32];
             paged_redo_row<D>(p, w.g, ri, w.head, w.kt0 * KT, w.kt1 * KT, lane, mi, li, oi);
             const long long to = (long long)ri.tok * p.H + ri.h;
-            const long long pi = ((long long)blockIdx.x * 2 + w.slot()) * M + row;
+            const long long pi = ((long long)blockIdx.x * 2 + w.slot) * M + row;
             const float iv = li > 0.f ? 1.f / li : (li == 0.f ? 0.f : li);
 #pragma unroll
             for (int e = 0; e < D / 32; ++e) {
@@ -1690,9 +1744,9 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
           }
         }
       }
-      ++nitem;
+      release_item(nitem);
       w = nx;
-    } while (more);
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -1787,7 +1841,7 @@ __global__ void __launch_bounds__(PC_JOIN) paged_combine_kernel(const __grid_con
     const int tok0 = paged_row0(p, kind ? min(max(p.groups[grp], 0), p.B) : b);
     const int rho = (t - tok0) * p.rep + h % p.rep, m = c.M[kind], qt = rho / m;
     if (rho < 0) continue;  // offsets that do not increase
-    const int2 d = p.desc[kind][(int((long long)tok0 * p.rep / m) + (kind ? grp : b) + qt) * p.Hk + h / p.rep];
+    const int2 d = p.desc[kind][(tok0 * p.rep / m + (kind ? grp : b) + qt) * p.Hk + h / p.rep];
     if (d.x < 0 || d.y < 1 || d.y > c.blocks[kind] || d.x > c.blocks[kind] - d.y) continue;  // never written
     count[kind] = d.y;
     const bool one = d.y == 1;
