@@ -81,14 +81,52 @@ __device__ __forceinline__ int request_of_row(const int* offsets, int t, int T, 
 
 constexpr int PA_THREADS = 128;
 
-// One block per row; D / 16 lanes share a head, eight pairs each.
+// Eight elements as they lie in memory.
+template <typename S>
+struct __align__(16) Raw8 {
+  uint4 w[sizeof(S) / 2];
+};
+__device__ __forceinline__ void unpack8(const Raw8<float>& r, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    x[4 * i] = __uint_as_float(r.w[i].x);
+    x[4 * i + 1] = __uint_as_float(r.w[i].y);
+    x[4 * i + 2] = __uint_as_float(r.w[i].z);
+    x[4 * i + 3] = __uint_as_float(r.w[i].w);
+  }
+}
+__device__ __forceinline__ void unpack8(const Raw8<uint16_t>& r, float (&x)[8]) {
+  const uint32_t w[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+
+// One block per row; D / 16 lanes share a head, eight pairs each. Bound by HBM on prompts (each value is
+// read once and written once), by the chain request -> length -> page -> store on single rows: the
+// first heads' values are on their way before that chain begins, and the next heads' while one step's
+// are turned.
 template <typename S, typename P, int D>
 __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_constant__ PagedAppendParams p) {
   constexpr int LPH = D / 16, HPB = PA_THREADS / LPH;  // lanes per head, heads per step
   __shared__ __align__(16) float cs[2][D / 2];
   pdl_launch_dependents();
   pdl_wait();
-  const int t = blockIdx.x;
+  const int t = blockIdx.x, sub = threadIdx.x % LPH;  // pairs [8 sub, 8 sub + 8)
+  const int nh = p.H + 2 * p.Hk;
+  auto fetch = [&](int h, Raw8<S>& lo, Raw8<S>& hi) {
+    if (h >= nh) return;
+    const S* x = h < p.H ? static_cast<const S*>(p.q) + t * p.q_row + h * p.q_head
+                         : (h < p.H + p.Hk ? static_cast<const S*>(p.k) + t * p.k_row + (h - p.H) * p.k_head
+                                           : static_cast<const S*>(p.v) + t * p.v_row + (h - p.H - p.Hk) * p.v_head);
+    lo = *reinterpret_cast<const Raw8<S>*>(x + 8 * sub);
+    hi = *reinterpret_cast<const Raw8<S>*>(x + D / 2 + 8 * sub);
+  };
+  Raw8<S> lo = {}, hi = {};
+  int h = int(threadIdx.x) / LPH;
+  fetch(h, lo, hi);
   const int b = request_of_row(p.offsets, t, p.T, p.B);
   if (b >= p.B) return;  // a row behind the last request
   const int row0 = p.offsets ? p.offsets[b] : b * (p.T / p.B);
@@ -101,12 +139,11 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_c
     if (threadIdx.x == 0) raise_error(p.err, page < 0 && (slot < 0 || pi >= p.table_cols) ? kErrCapacity : kErrPage);
     page = -1;  // k and v are not written
   }
-  const int pos = p.positions ? p.positions[t] : slot;
   if (threadIdx.x < D / 2) {
     // The angle in 64 bits: at position 10^6 a 32-bit product would be off by 0.06. Reduced to
     // [-pi, pi] before it is rounded, so the cosine is within 2^-22 of the exact one.
     constexpr double kTwoPi = 6.283185307179586476925287;
-    const double a = double(pos) * p.freq[threadIdx.x];
+    const double a = double(p.positions ? p.positions[t] : slot) * p.freq[threadIdx.x];
     const float r = float(a - kTwoPi * rint(a * (1.0 / kTwoPi)));
     float s, c;
     sincosf(r, &s, &c);
@@ -114,41 +151,32 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_c
     cs[1][threadIdx.x] = s;
   }
   __syncthreads();
-  const int sub = threadIdx.x % LPH;  // pairs [8 sub, 8 sub + 8)
   float c8[8], s8[8];
   load8(cs[0] + 8 * sub, c8);
   load8(cs[1] + 8 * sub, s8);
   const int r = slot & ((1 << p.page_log2) - 1);
-  const int nh = p.H + 2 * p.Hk;
-  for (int h0 = 0; h0 < nh; h0 += HPB) {
-    const int h = h0 + int(threadIdx.x) / LPH;
-    const bool live = h < nh;
+  for (int h0 = 0; h0 < nh; h0 += HPB, h += HPB) {
+    float a[8], c[8];
+    unpack8(lo, a);
+    unpack8(hi, c);
+    fetch(h + HPB, lo, hi);
     const bool isq = h < p.H, isk = !isq && h < p.H + p.Hk;
-    float a[8] = {}, c[8] = {};
-    if (live) {
-      const S* x = isq ? static_cast<const S*>(p.q) + t * p.q_row + h * p.q_head
-                       : (isk ? static_cast<const S*>(p.k) + t * p.k_row + (h - p.H) * p.k_head
-                              : static_cast<const S*>(p.v) + t * p.v_row + (h - p.H - p.Hk) * p.v_head);
-      load8(x + 8 * sub, a);
-      load8(x + D / 2 + 8 * sub, c);
-    }
     const float* w = isq ? p.q_norm : (isk ? p.k_norm : nullptr);
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + c[i] * c[i];
 #pragma unroll
     for (int o = 1; o < LPH; o *= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (!live) continue;
+    if (h >= nh) continue;
     if (w) {
       const float inv = 1.f / sqrtf(ss / float(D) + p.eps);
-      float wa[8], wc8[8];
-      load8(w + 8 * sub, wa);
-      load8(w + D / 2 + 8 * sub, wc8);
+      float g[8];
+      load8(w + 8 * sub, g);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        a[i] *= inv * wa[i];
-        c[i] *= inv * wc8[i];
-      }
+      for (int i = 0; i < 8; ++i) a[i] *= inv * g[i];
+      load8(w + D / 2 + 8 * sub, g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c[i] *= inv * g[i];
     }
     if (isq || isk) {
 #pragma unroll
@@ -225,13 +253,15 @@ __global__ void __launch_bounds__(PC_THREADS) paged_compact_kernel(const __grid_
     return;
   }
   if (layer == 0 && threadIdx.x == 0) p.lens_out[b] = start + nk;
+  int first = 0;  // the rows before the first gap stay where they are
+  while (first < nk && s_src[first] == s_dst[first] && s_sr[first] == s_dr[first]) ++first;
   const int units = 2 * p.Hk * p.row_chunks;
   for (int u = threadIdx.x; u < units; u += PC_THREADS) {
     const int chunk = u % p.row_chunks, hv = u / p.row_chunks, head = hv >> 1;
     const PagePool& pool = (hv & 1) ? p.V : p.K;
     char* base = static_cast<char*>(pool.ptr) +
                  ((((hv & 1) ? p.v_layer : p.k_layer) * layer + head * pool.head) << p.esize_log2) + chunk * 16;
-    for (int i0 = 0; i0 < nk; i0 += 8) {
+    for (int i0 = first; i0 < nk; i0 += 8) {
       uint4 x[8];
       const int m = min(8, nk - i0);
 #pragma unroll
