@@ -369,6 +369,113 @@ def test_a_pool_whose_offsets_pass_32_bits():
     assert torch.equal(v[at], n[0].to(BF))
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("H, Hk, D", [(32, 1, 128), (71, 1, 64), (24, 2, 64)])
+@pytest.mark.parametrize("rows", [1, 3, 37])
+def test_many_query_heads_per_kv_head(dtype, H, Hk, D, rows):
+    from woodcock_b200 import ops
+
+    c = Case(50, [rows, 200, 97], [rows] * 3, H, Hk, D, 16, dtype)
+    check(c, ops.paged_attention(c.q, c.k, c.v, c.table, c.kv))
+
+
+@pytest.mark.parametrize("page", [16, 32, 128, 256])
+@pytest.mark.parametrize("rows", [20, 300])
+@pytest.mark.parametrize("D", [64, 128])
+def test_pages_of_every_size_on_the_tensor_cores(page, rows, D):
+    from woodcock_b200 import ops
+
+    c = Case(51, [rows, rows + 333, 2 * rows + 1], [rows] * 3, 16, 8, D, page, BF)
+    check(c, ops.paged_attention(c.q, c.k, c.v, c.table, c.kv))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows", [1, 18])
+def test_more_requests_than_a_block_has_threads(dtype, rows):
+    from woodcock_b200 import ops
+
+    B = 700
+    lens = [(i * 37) % 90 + rows for i in range(B)]
+    c = Case(52, lens, [rows] * B, 2, 1, 64, 16, dtype, prefix=[5 + i % 40 for i in range(350)])
+    some = [0, 1, 255, 256, 383, 384, 511, 699]
+    out = ops.paged_attention(c.q, c.k, c.v, c.table, c.kv)
+    for b in some:
+        check_one(c, out, b, rows)
+    out = ops.paged_attention(c.q, c.k, c.v, c.table, c.kv, q_offsets=c.off)
+    for b in some:
+        check_one(c, out, b, rows)
+    groups = list(range(0, 701, 2))
+    out = ops.shared_prefix_attention(c.q, c.k, c.v, c.ptable, i32(c.prefix), i32(groups), c.table, c.kv, q_offsets=c.off)
+    for b in some:
+        check_one(c, out, b, rows, groups)
+
+
+def check_one(c, out, b, rows, groups=None):
+    """One request of a uniform batch, without the cost of all the others."""
+    o, a, es, n = want_rows(c, b, b * rows, None, None if groups is None else b // 2)
+    h = half_step(c.dtype)
+    tol = (h * o.abs() + (h + 2.0 ** -12 + 2 * es) * a) if c.dtype is BF else (2 * es + n * 2.0 ** -24 + 2.0 ** -19) * a
+    assert ((out[b * rows: (b + 1) * rows].double() - o).abs() <= tol + 1e-30).all(), b
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_trees_with_fewer_keys_than_rows_and_with_too_many_rows(dtype):
+    from woodcock_b200 import ops
+    from woodcock_b200._lib import WcError
+    from woodcock_b200.context import Context
+
+    # rows without a slot: bit i still names new row i, whose key may lie before the first
+    c = Case(53, [2, 30], [4, 30], 16, 8, 128, 16, dtype)
+    bits = tree_bits([4, 30])
+    check(c, ops.paged_attention(c.q, c.k, c.v, c.table, c.kv, q_offsets=c.off, tree_mask=bits), bits)
+    Context.get(0).synchronize()
+    c = Case(54, [90], [65], 16, 8, 128, 16, dtype)
+    ops.paged_attention(c.q, c.k, c.v, c.table, c.kv, tree_mask=torch.ones(65, dtype=torch.int64, device="cuda"))
+    torch.cuda.synchronize()
+    with pytest.raises(WcError):
+        Context.get(0).synchronize()
+    Context.get(0).synchronize()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows", [2, 30, 200])
+def test_a_query_row_of_nan_stays_alone(dtype, rows):
+    from woodcock_b200 import ops
+
+    c = Case(55, [rows + 70] * 3, [rows] * 3, 16, 8, 128, 32, dtype)
+    want = ops.paged_attention(c.q, c.k, c.v, c.table, c.kv)
+    c.q[rows + 1, 5] = math.nan
+    got = ops.paged_attention(c.q, c.k, c.v, c.table, c.kv)
+    assert torch.isnan(got[rows + 1, 5].float()).all()
+    got[rows + 1, 5] = want[rows + 1, 5]
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("rows", [33, 150])
+def test_poisoned_values_in_many_items_and_long_contexts(rows):
+    """Every request holds a later row of NaN: all items of a block are summed again, divided ones too."""
+    from woodcock_b200 import ops
+
+    B = 40
+    lens = [rows + (4000 if b == 0 else 60 + b) for b in range(B)]
+    c = Case(56, lens, [rows] * B, 8, 8, 128, 64, BF, prefix=[300])
+    clean = ops.paged_attention(c.q, c.k, c.v, c.table, c.kv)
+    joined = ops.shared_prefix_attention(c.q, c.k, c.v, c.ptable, i32([300]), i32([0, B]), c.table, c.kv)
+    hole = rows // 3
+    for b, n in enumerate(lens):
+        key = n - rows + hole
+        at = c.table[b].long()[key // 64], slice(None), key % 64
+        c.k[at] = math.nan
+        c.v[at] = math.nan
+    for want, got in ((clean, ops.paged_attention(c.q, c.k, c.v, c.table, c.kv)),
+                      (joined, ops.shared_prefix_attention(c.q, c.k, c.v, c.ptable, i32([300]), i32([0, B]), c.table, c.kv))):
+        want, got = want.view(B, rows, 8, 128).float(), got.view(B, rows, 8, 128).float()
+        assert torch.isnan(got[:, hole:]).all()
+        # both within the tolerance of the formula: the rounded weights' (2^-8 of sum p |v|, at most max |v|) on
+        # one side and the output's rounding on both
+        assert (got[:, :hole] - want[:, :hole]).abs().max() <= 2.0 ** -8 * 5.5 + 2.0 ** -7 * want.abs().max()
+
+
 # ------------------------------------------------------------------------------------------------ shared prefixes
 
 
@@ -478,6 +585,24 @@ def test_append_agrees_with_the_contiguous_operators():
     got = ops.paged_append(q, k, v, c.k, c.v, c.table, c.kv, base=1e6, q_norm=w, k_norm=w)
     # ops.rope takes its angles from a 32-bit table: off by at most 2^-24 of an angle below 64
     torch.testing.assert_close(got, ops.rope(ops.rmsnorm(q, w, 1e-6), pos, 1e6), rtol=0, atol=64 * 2.0 ** -22)
+
+
+def test_append_for_more_requests_than_a_block_has_threads():
+    from woodcock_b200 import ops
+
+    B = 700
+    rows = [i % 3 for i in range(B)]
+    lens = [(i * 13) % 50 + r for i, r in enumerate(rows)]
+    c = Case(57, lens, rows, 4, 2, 64, 16, F32)
+    T = sum(rows)
+    k, v = c.randn(T, 2, 64), c.randn(T, 2, 64)
+    got = ops.paged_append(c.q, k, v, c.k, c.v, c.table, c.kv, q_offsets=c.off)
+    b = torch.repeat_interleave(torch.arange(B, device="cuda"), i32(rows).long())
+    within = torch.arange(T, device="cuda") - c.off.long()[b]
+    slot = c.kv.long()[b] - i32(rows).long()[b] + within
+    y, tol = want_rotated(c.q, None, slot, 1e6, 1e-6)
+    assert ((got.double() - y).abs() <= tol).all()
+    assert torch.equal(c.v[c.table.long()[b, slot // 16], :, slot % 16], v)
 
 
 def test_append_rows_without_a_slot():

@@ -149,10 +149,12 @@ extern "C" wc_status wc_paged_append(wc_ctx* ctx, void* stream, const wc_paged_a
     p.H = b.heads;
     p.Hk = g.kv_heads;
     p.err = ctx->d_err;
-    // base^(-2i/D): eight powers, the rest by products (an error of a few 2^-53)
-    const double step = std::pow(a->base, -2.0 / g.head_dim);
-    for (int i = 0; i < g.head_dim / 2; ++i)
-      p.freq[i] = i % 8 ? p.freq[i - 1] * step : std::pow(a->base, -2.0 * i / g.head_dim);
+    if (ctx->turn_base != a->base || ctx->turn_dim != g.head_dim) {
+      for (int i = 0; i < g.head_dim / 2; ++i) ctx->turn_freq[i] = std::pow(a->base, -2.0 * i / g.head_dim);
+      ctx->turn_base = a->base;
+      ctx->turn_dim = g.head_dim;
+    }
+    std::memcpy(p.freq, ctx->turn_freq, sizeof(p.freq));
     const cudaStream_t st = stream_of(ctx, stream);
     const bool sb = a->src_dtype == WC_BF16, pb = g.dtype == WC_BF16;
     if (sb && pb) launch_append<uint16_t, uint16_t>(ctx, st, p, g.head_dim);
@@ -207,13 +209,19 @@ enum Variant { kSimt, kFew, kMany128, kMany256 };
 
 struct Launch {
   Variant variant;
-  int M, blocks;
+  int M, blocks, least;
 };
 
-// One launch: its row tile and the blocks that share its key tiles. `rows`: query rows per
-// segment and KV head, on average.
-Launch plan_launch(const wc_ctx* ctx, const wc_pages& g, long long rows) {
+// One launch: its row tile, the blocks that share its key tiles and the units that a block takes at
+// least. `rows`: query rows per segment and KV head, on average; `prefixes`: beside shared prefixes,
+// where each part costs a row more states to join (eight chains of five rows under 1001 keys: 31.6 us
+// with parts of one tile, 24.8 with least 4, 29.0 with 8; one decoding step alone: 12.8, 13.2, 15.3).
+// bf16, 64 requests: 16 rows 168 us on the streamed kernel and 184 on tensor memory at 4000 keys, 35
+// and 50 at 300; 18 rows 211 and 172 at 4000 keys, 77 and 70 at 1000, 42 and 48 at 300 (the streamed
+// kernel then in a 32-row form, since removed).
+Launch plan_launch(const wc_ctx* ctx, const wc_pages& g, long long rows, bool prefixes) {
   Launch l;
+  l.least = 1;
   if (g.dtype == WC_F32) {
     l.variant = kSimt;
     l.M = PS_M;
@@ -222,6 +230,7 @@ Launch plan_launch(const wc_ctx* ctx, const wc_pages& g, long long rows) {
     l.variant = rows <= 16 ? kFew : rows <= 128 ? kMany128 : kMany256;
     l.M = rows <= 16 ? 16 : rows <= 128 ? 128 : 256;
     l.blocks = ctx->num_sms;
+    if (prefixes || l.variant != kFew) l.least = 4;
   }
   return l;
 }
@@ -244,8 +253,8 @@ Layout layout(const wc_ctx* ctx, const wc_paged_attention_args& a) {
   Layout l;
   std::memset(&l, 0, sizeof(l));
   const long long rows = (long long)b.rows * rep;
-  l.own = plan_launch(ctx, g, (rows + b.requests - 1) / b.requests);
-  l.prefix = plan_launch(ctx, g, a.groups ? (rows + a.groups - 1) / a.groups : 0);
+  l.own = plan_launch(ctx, g, (rows + b.requests - 1) / b.requests, a.groups > 0);
+  l.prefix = plan_launch(ctx, g, a.groups ? (rows + a.groups - 1) / a.groups : 0, true);
   size_t at = 0;
   for (int kind = 0; kind < (a.groups ? 2 : 1); ++kind) {
     const Launch& x = kind ? l.prefix : l.own;
@@ -310,7 +319,7 @@ void launch_few(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, const PagedAttn
   static_assert(PfLayout<D>::bytes() <= kSmemOptinBytes, "shared memory");
   opt_in(ctx, paged_few_kernel<D>, smem);
   launch_on(ctx, st, "paged_few", paged_few_kernel<D>, dim3(l.blocks), dim3(PF_THREADS), smem, true, 1,
-            page_map(g, p.K, PF_KT, D / 64), page_map(g, p.V, PF_KT, D / 64), p, kinds, late);
+            page_map(g, p.K, PF_KT, D / 64), page_map(g, p.V, PF_KT, D / 64), p, kinds, l.least, late);
 }
 
 template <int D, bool kTwo>
@@ -320,7 +329,7 @@ void launch_many(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, const PagedAtt
   static_assert(PmLayout<D, kTwo>::bytes() <= kSmemOptinBytes, "shared memory");
   opt_in(ctx, paged_many_kernel<D, kTwo>, smem);
   launch_on(ctx, st, "paged_many", paged_many_kernel<D, kTwo>, dim3(l.blocks), dim3(PM_THREADS), smem, true, 1,
-            page_map(g, p.K, PM_KT, 1), page_map(g, p.V, PM_KT, D / 64), p, kinds, late);
+            page_map(g, p.K, PM_KT, 1), page_map(g, p.V, PM_KT, D / 64), p, kinds, l.least, late);
 }
 
 template <typename S, int D>
@@ -329,7 +338,7 @@ void launch_attention(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, const Pag
   if constexpr (sizeof(S) == 4) {
     opt_in(ctx, paged_simt_kernel<S, D>, paged_simt_smem<D>());
     launch_on(ctx, st, "paged_simt", paged_simt_kernel<S, D>, dim3(l.blocks), dim3(PS_THREADS), paged_simt_smem<D>(),
-              true, 1, p, kinds, late);
+              true, 1, p, kinds, l.least, late);
   } else if (l.variant == kFew) {
     launch_few<D>(ctx, st, g, p, kinds, l, late);
   } else if (l.variant == kMany128) {

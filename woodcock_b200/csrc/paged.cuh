@@ -392,7 +392,8 @@ __device__ __forceinline__ long long paged_div(long long a, long long b) {
 
 // One block's walk over its range of the line, item by item. An item counts kOver units beyond its key
 // tiles, for what it costs whatever its length (its queries, its result, the way there); a block whose
-// range holds only such units of an item passes it over.
+// range holds only such units of an item passes it over. A block takes `least` units at least, where
+// more parts would cost the joining kernel more than they save.
 template <int M, int KT, int kOver>
 struct PagedWalk {
   PagedSeg g;
@@ -408,14 +409,14 @@ struct PagedWalk {
   }
 
   // Block-collective; `sh` holds kWalkShared words. False: the block has no work.
-  __device__ bool begin(const PagedAttnParams& p, int kinds, long long* sh) {
+  __device__ bool begin(const PagedAttnParams& p, int kinds, int least, long long* sh) {
     nseg = ((kinds & kPrefixRows) ? p.G : 0) + ((kinds & kOwnRows) ? p.B : 0);
     const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, nw = (nt + 31) >> 5;
     long long total = 0, w = 0, x = 0;
     pos = 0;
     for (int pass = 0; pass < 2; ++pass) {
       if (pass) {
-        per = int(paged_div(total + gridDim.x - 1, gridDim.x));
+        per = max(least, int(paged_div(total + gridDim.x - 1, gridDim.x)));
         pos = (long long)blockIdx.x * per;
         end = min(pos + per, total);
         if (pos >= end) return false;
@@ -584,7 +585,7 @@ constexpr size_t paged_simt_smem() {
 
 template <typename S, int D>
 __global__ void __launch_bounds__(PS_THREADS)
-    paged_simt_kernel(const __grid_constant__ PagedAttnParams p, int kinds, bool late) {
+    paged_simt_kernel(const __grid_constant__ PagedAttnParams p, int kinds, int least, bool late) {
   constexpr int M = PS_M, KT = PS_KT, LD = D + 4, LS = KT + 4;
   constexpr int RPT = D / 64;  // rows per thread of P V: two (D 128), one (D 64)
   extern __shared__ __align__(16) float ps_smem[];
@@ -598,7 +599,7 @@ __global__ void __launch_bounds__(PS_THREADS)
   pdl_launch_dependents();
   PagedWalk<M, KT, 1> w;
   paged_no_rec(p);
-  if (!w.begin(p, kinds, sh)) {
+  if (!w.begin(p, kinds, least, sh)) {
     if (late) pdl_wait();
     return;
   }
@@ -826,7 +827,7 @@ struct PageWindow {
 template <int D>
 __global__ void __launch_bounds__(PF_THREADS, 1)
     paged_few_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
-                     const __grid_constant__ PagedAttnParams p, int kinds, bool late) {
+                     const __grid_constant__ PagedAttnParams p, int kinds, int least, bool late) {
   constexpr int M = PF_M, KT = PF_KT, NK = D / 16, ND = D / 8;
   using L = PfLayout<D>;
   constexpr int NST = L::kStages;
@@ -864,7 +865,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   PagedWalk<M, KT, PF_OVER> w;
   paged_no_rec(p);
   __syncthreads();
-  if (!w.begin(p, kinds, sh)) {
+  if (!w.begin(p, kinds, least, sh)) {
     if (late) pdl_wait();
     return;
   }
@@ -879,6 +880,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     do {
       // the item and its query rows (those past the segment's keep what the buffer holds: nobody reads them)
       const int b = nitem & 1;
+      PageWindow win;
+      win.start(p, w.g, (w.kt0 * KT) >> p.page_log2, lane);
       if (lane == 0) {
         w.report(p);
         if (nitem >= 2) paged_wait(it_empty + b, ((nitem >> 1) - 1) & 1, dead, p.err);
@@ -895,8 +898,6 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
                    static_cast<const uint16_t*>(p.q) + r.tok * p.q_row + r.h * p.q_head, D * 2, it_full + b);
       }
       ++nitem;
-      PageWindow win;
-      win.start(p, w.g, (w.kt0 * KT) >> p.page_log2, lane);
       for (int kt = w.kt0; kt < w.kt1; ++kt, ++cnt) {
         const int s = cnt % NST;
         const int first = (kt * KT) >> p.page_log2;
@@ -1200,11 +1201,13 @@ constexpr int PM_THREADS = 384;  // producer, products, two idle warps (register
 constexpr int PM_KT = 128;
 constexpr int PM_OVER = 3;
 
+constexpr int kRedo = 16;  // words: 512 items are told apart
+
 template <int D, bool kTwo>
 struct PmLayout {
   static constexpr int kTile = PM_KT * D * 2;  // a K or V tile
   static constexpr int kQ = (kTwo ? 2 : 1) * 128 * D * 2;
-  static constexpr int kTail = 8 * kWalkShared + 400 + 4 * 64 + (kTwo ? 0 : 4 * 128 * 8);
+  static constexpr int kTail = 8 * kWalkShared + 384 + 4 * 64 + 2 * kRedo * 4 + (kTwo ? 0 : 4 * 128 * 8);
   static constexpr int kStages = (int(kSmemOptinBytes) - 1024 - kQ - kTail) / kTile > 12
                                      ? 12
                                      : (int(kSmemOptinBytes) - 1024 - kQ - kTail) / kTile;
@@ -1232,7 +1235,7 @@ __device__ __forceinline__ uint32_t seen_bits(const PagedRow& r, int k0) {
 template <int D, bool kTwo>
 __global__ void __launch_bounds__(PM_THREADS, 1)
     paged_many_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
-                      const __grid_constant__ PagedAttnParams p, int kinds, bool late) {
+                      const __grid_constant__ PagedAttnParams p, int kinds, int least, bool late) {
   using L = PmLayout<D, kTwo>;
   constexpr int M = kTwo ? 256 : 128, KT = PM_KT, NST = L::kStages, HALVES = D / 64;
   constexpr uint32_t kColO = 256;
@@ -1256,9 +1259,9 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
   uint64_t* it_empty = bars + 40;            // [4]: and read by all
   volatile int* dead = reinterpret_cast<volatile int*>(bars + 44);
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + 45);
-  volatile int* redo = reinterpret_cast<volatile int*>(bars + 46);  // [2]: number of the item to be redone
-  PagedItem* queue = reinterpret_cast<PagedItem*>(tail + 8 * kWalkShared + 400);          // [4]
-  float2* xml = reinterpret_cast<float2*>(tail + 8 * kWalkShared + 400 + 4 * 64);         // [item & 1][slot][row]
+  PagedItem* queue = reinterpret_cast<PagedItem*>(tail + 8 * kWalkShared + 384);  // [4]
+  uint32_t* redo = reinterpret_cast<uint32_t*>(queue + 4);  // [slot][kRedo]: items to be summed again, by number
+  float2* xml = reinterpret_cast<float2*>(redo + 2 * kRedo);  // [item & 1][slot][row]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int s = 0; s < NST; ++s) {
@@ -1280,8 +1283,8 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
     mbar_init(drain, 1);
     mbar_fence_init();
     *dead = 0;
-    redo[0] = redo[1] = -1;
   }
+  if (tid < 2 * kRedo) redo[tid] = 0;
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_addr(tslot)),
                  "r"(512u)
@@ -1297,7 +1300,9 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
   const uint32_t tmem = *tslot;
   using Walk = PagedWalk<M, KT, PM_OVER>;
   Walk w;
-  const bool work = w.begin(p, kinds, sh);
+  const bool work = w.begin(p, kinds, least, sh);
+  static_assert(sizeof(Walk) <= 8 * 32, "kept where the search has been");
+  if (tid == 0) *reinterpret_cast<Walk*>(sh) = w;  // the line's beginning, for a second walk
 
   // The next item of the line, as the walking warp left it.
   auto take_item = [&](int n) {
@@ -1552,8 +1557,8 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
         const int key0 = (w.kt0 + t) * KT;
         const bool masked = key0 + KT > lim;
         // Values in masked places may be anything, and 0 x NaN would reach every row. Behind the last
-        // key they are cleared; between keys (a later row, another branch) they mark the tile's rows
-        // for the joining kernel, which sums such rows over the seen keys alone.
+        // key they are cleared; between keys (a later row, another branch) they mark the slot's rows,
+        // which are summed again over the seen keys alone when the line is done.
         if (key0 + KT > edge) {
           const int vpos = vcnt + (kTwo ? 2 * t + 1 : min(2 * t + 2, nt + t));
           const int vs = vpos % NST;
@@ -1582,7 +1587,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
                   worst = max(worst, (xs[e] << 16) & 0x7f800000u);
                 }
               }
-            if (worst == 0x7f800000u) redo[slot] = nitem;
+            if (worst == 0x7f800000u) atomicOr(redo + slot * kRedo + (nitem >> 5) % kRedo, 1u << (nitem & 31));
           }
           fence_proxy_async_smem();
         }
@@ -1690,8 +1695,6 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
         ++no[0];
       }
       if (load) copied_q();
-      // every warp of the slot raised its mark before the product that o_full reports
-      const bool again = kTwo ? active && redo[slot] == nitem : redo[0] == nitem || redo[1] == nitem;
       if (active || !kTwo) {
         tc_fence_after();
         const bool direct = w.count == 1 && p.G == 0;
@@ -1718,7 +1721,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
               for (int j = 0; j < 32; ++j) y[j] = fmaf(__uint_as_float(v[j]), g1, y[j]);
             }
           }
-          if (r.valid && !again) {
+          if (r.valid) {
             if (direct) {
               uint16_t* dst = static_cast<uint16_t*>(p.out) + at * D + c;
               float v8[16];
@@ -1748,34 +1751,46 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
             if (two) mbar_arrive(o_empty + 1);
           }
         }
-        if (r.valid && !again && !direct && (kTwo || slot == 0)) {
+        if (r.valid && !direct && (kTwo || slot == 0)) {
           if (w.count == 1) p.whole_ml[w.g.prefix][at] = make_float2(m, l);
           else p.part_ml[pt] = make_float2(m, l);
-        }
-        if (again && (kTwo || slot == 0)) {
-#pragma unroll 1
-          for (int i = 0; i < 32; ++i) {
-            const int row = (kTwo ? slot * 128 : 0) + qd * 32 + i;
-            const PagedRow ri = paged_row(p, w.g, w.head, w.qt * M + row);
-            if (!ri.valid) break;
-            float mi, li, oi[D / 32];
-            paged_redo_row<D>(p, w.g, ri, w.head, w.kt0 * KT, w.kt1 * KT, lane, mi, li, oi);
-            const long long to = (long long)ri.tok * p.H + ri.h;
-            const long long pi = ((long long)blockIdx.x * 2 + w.slot) * M + row;
-            const float iv = li > 0.f ? 1.f / li : (li == 0.f ? 0.f : li);
-#pragma unroll
-            for (int e = 0; e < D / 32; ++e) {
-              const int c = lane * (D / 32) + e;
-              if (direct) static_cast<uint16_t*>(p.out)[to * D + c] = f32_to_bf16_bits(oi[e] * iv);
-              else (w.count == 1 ? p.whole_o[w.g.prefix] + to * D : p.part_o + pi * D)[c] = oi[e];
-            }
-            if (!direct && lane == 0)
-              (w.count == 1 ? p.whole_ml[w.g.prefix] + to : p.part_ml + pi)[0] = make_float2(mi, li);
-          }
         }
       }
       release_item(nitem);
       w = nx;
+    }
+    // Rows beside values that are not finite, once more from the line's beginning (nobody waits for these
+    // warps now, however long it takes); with alternating slots each takes every other row.
+    named_sync(1, 256);
+    uint32_t any = 0;
+    for (int i = 0; i < kRedo; ++i) any |= kTwo ? redo[slot * kRedo + i] : redo[i] | redo[kRedo + i];
+    if (any) {
+      Walk again = *reinterpret_cast<const Walk*>(sh);
+      int n = 0;
+      do {
+        const int word = (n >> 5) % kRedo;
+        if (!(((kTwo ? redo[slot * kRedo + word] : redo[word] | redo[kRedo + word]) >> (n & 31)) & 1u)) continue;
+        const bool direct = again.count == 1 && p.G == 0;
+#pragma unroll 1
+        for (int i = kTwo ? 0 : slot; i < 32; i += kTwo ? 1 : 2) {
+          const int row = (kTwo ? slot * 128 : 0) + qd * 32 + i;
+          const PagedRow r = paged_row(p, again.g, again.head, again.qt * M + row);
+          if (!r.valid) break;
+          float m, l, o[D / 32];
+          paged_redo_row<D>(p, again.g, r, again.head, again.kt0 * KT, again.kt1 * KT, lane, m, l, o);
+          const long long to = (long long)r.tok * p.H + r.h;
+          const long long pt = ((long long)blockIdx.x * 2 + again.slot()) * M + row;
+          const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+#pragma unroll
+          for (int e = 0; e < D / 32; ++e) {
+            const int c = lane * (D / 32) + e;
+            if (direct) static_cast<uint16_t*>(p.out)[to * D + c] = f32_to_bf16_bits(o[e] * inv);
+            else (again.count == 1 ? p.whole_o[again.g.prefix] + to * D : p.part_o + pt * D)[c] = o[e];
+          }
+          if (!direct && lane == 0)
+            (again.count == 1 ? p.whole_ml[again.g.prefix] + to : p.part_ml + pt)[0] = make_float2(m, l);
+        }
+      } while (++n, again.next(p, kinds));
     }
   }
   tc_fence_before();
