@@ -764,7 +764,8 @@ __device__ __forceinline__ void paged_redo_row(const PagedAttnParams& p, const P
 // tiles in turn, a 16-key slice per warp, so that no two warps wait for one another before the item's
 // end: each keeps its own running maximum, sum and 16 x D output (mma m16n8k16), joined in shared
 // memory once per item. The producer also walks the line and hands the items over with their query
-// rows, one item ahead.
+// rows, one item ahead. 64 requests of 6000 keys, pages of 64: 239 us, 6.6 TB/s; pages of 16 263 us
+// (4 KB copies).
 constexpr int PF_CONSUMERS = 8;
 constexpr int PF_THREADS = 32 * (PF_CONSUMERS + 1);
 constexpr int PF_KT = 64, PF_M = 16;
