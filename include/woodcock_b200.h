@@ -373,12 +373,14 @@ WC_API wc_status wc_gemm_bf16(wc_ctx* ctx, const void* A, const void* B, float* 
  *    hold its last keys. Rows behind q_offsets[requests] are neither read nor written.
  *  - Lengths, offsets and tables are device memory, so a captured graph may be replayed on new ones.
  *    A table entry outside the pool, a length beyond the table and offsets out of range are never
- *    followed: the keys count as absent, append drops the row, and the device error word is raised
- *    (wc_ctx_synchronize returns WC_ERR_DEVICE once the stream's work is done).
+ *    followed: such a page's keys and values read as zeros, a length is cut to what the table holds,
+ *    append drops the row, and the device error word is raised (wc_ctx_synchronize returns
+ *    WC_ERR_DEVICE once the stream's work is done).
  *  - head_dim 64 or 128; page_size a power of two from 16 to 256; pages of WC_F32 or WC_BF16;
- *    16-byte aligned pointers and strides.
+ *    16-byte aligned pointers and strides, no stride of zero. Outputs must not overlap inputs.
  *  - `stream`: the cudaStream_t to enqueue on (NULL: the context's; cudaStreamLegacy for the
- *    default stream). Nothing is allocated and no state is kept between calls. */
+ *    default stream). Nothing is allocated and no state is kept between calls. The first call on a
+ *    device sets kernel attributes: make one before a capture begins. */
 typedef struct {
   void *k, *v;
   int64_t k_stride[4], v_stride[4]; /* layer, page, head, row; in elements */

@@ -714,6 +714,9 @@ def test_refusals(dtype):
                {"tree_mask": torch.ones(3, dtype=torch.int64, device="cuda")}):
         with pytest.raises(ValueError):
             call(**kw)
+    one = c.k[:1].contiguous()
+    with pytest.raises(ValueError, match="overlap"):
+        call(k_pages=one.expand(3, 8, 16, 128), v_pages=one.expand(3, 8, 16, 128))
     with pytest.raises(ValueError):
         ops.paged_append(c.q, c.q, c.q, c.k, c.v, c.table, c.kv)  # k has q's heads
     with pytest.raises(ValueError):

@@ -52,7 +52,7 @@ void check_pages(const wc_pages& g) {
   for (int i = 0; i < 4; ++i) {
     if (sizes[i] == 1) continue;  // never stepped over
     need(g.k_stride[i] % unit == 0 && g.v_stride[i] % unit == 0, "paged: page strides must be multiples of 16 bytes");
-    need(g.k_stride[i] >= 0 && g.v_stride[i] >= 0, "paged: negative page stride");
+    need(g.k_stride[i] > 0 && g.v_stride[i] > 0, "paged: pages must not overlap");
   }
 }
 

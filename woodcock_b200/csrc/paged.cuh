@@ -786,7 +786,6 @@ struct PfLayout {
   static constexpr size_t bytes() { return 1024 + size_t(kStages) * kStage + kJoin + kQ + kTail; }
 };
 
-
 // Waits give up after a bound; then `dead` lets the block's other waits pass, so that it ends.
 __device__ __forceinline__ void paged_wait(uint64_t* bar, uint32_t parity, volatile int* dead, int* err) {
   if (*dead) return;
@@ -848,7 +847,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   volatile int* stop = dead + 1;
   float2* wml = reinterpret_cast<float2*>(tail + 8 * kWalkShared + 256);  // [8 warps][16 rows]
   float2* rml = wml + 8 * 16;                                            // [M]
-  PagedItem* items = reinterpret_cast<PagedItem*>(rml + M);                    // [2]
+  PagedItem* items = reinterpret_cast<PagedItem*>(rml + M);              // [2]
   static_assert(32 + 16 * NST <= 248, "barriers");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {

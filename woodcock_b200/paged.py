@@ -12,11 +12,12 @@ python/woodcock/target.py:159-175); a server keeps many requests' keys and value
   q, k, v and out (int32 [requests + 1]; None: rows / requests each); rows behind the last request
   are left alone.
 * Tables, lengths and offsets stay on the device, so a captured CUDA graph can be replayed on new
-  contents. A page number outside the pool, a length beyond its table or a row with no slot is never
-  followed; it raises the context's device error word (``Context.get(device).synchronize()`` after
-  the stream's work raises WcError).
+  contents (make one call before the capture). A page number outside the pool (its keys and values read
+  as zeros), a length beyond its table (cut to it) or a row with no slot (dropped) is never followed;
+  it raises the context's device error word (``Context.get(device).synchronize()`` after the
+  stream's work raises WcError).
 * Work runs on the caller's current stream of the tensors' device, in its order; scratch comes from
-  PyTorch's allocator for that one call.
+  PyTorch's allocator for that one call. Outputs must not overlap inputs.
 """
 
 from __future__ import annotations
