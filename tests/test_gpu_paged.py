@@ -721,8 +721,55 @@ def test_refusals(dtype):
         ops.paged_append(c.q, c.q, c.q, c.k, c.v, c.table, c.kv)  # k has q's heads
     with pytest.raises(ValueError):
         ops.paged_append(c.q, c.q[:, :8], c.q[:, :8], c.k, c.v, c.table, c.kv, q_norm=torch.ones(64, device="cuda"))
+    both = torch.zeros((5, 16, 128), dtype=dtype, device="cuda")  # an output among the inputs
+    for lo in (0, 1, 2):
+        with pytest.raises(ValueError, match="overlap"):
+            call(q=both[1:3], out=both[lo:lo + 2])
+    assert call(q=both[1:3], out=both[3:]).data_ptr() == both[3:].data_ptr()
+    kv = both[3:, :8]
+    for q, k, v, out in ((both[:2], kv, kv.clone(), both[1:3]), (c.q, kv, kv.clone(), both[3:]), (c.q, kv.clone(), kv, both[3:])):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.paged_append(q, k, v, c.k.clone(), c.v.clone(), c.table, c.kv, out=out)
+    with pytest.raises(ValueError, match="share"):
+        ops.paged_append(c.q, kv, kv, c.k, c.k, c.table, c.kv)
+    with pytest.raises(ValueError, match="share"):
+        ops.paged_compact(c.k, c.k, c.table, c.kv, i32([[0], [0]]), i32([0, 0]))
     assert call(q=c.q[:0], page_table=c.table[:0], kv_lens=c.kv[:0]).shape == (0, 16, 128)
     assert call(q=c.q[:0]).shape == (0, 16, 128)
+
+
+def test_threads_that_append_at_once_keep_their_own_bases():
+    import threading
+
+    from woodcock_b200 import ops
+
+    c = Case(33, [40, 50], [1, 1], 16, 8, 128, 16, F32)
+    k, v = torch.randn((2, 8, 128), device="cuda"), torch.randn((2, 8, 128), device="cuda")
+
+    def append(base):
+        return ops.paged_append(c.q, k, v, c.k.clone(), c.v.clone(), c.table, c.kv, base=base)
+
+    want = {base: append(base) for base in (1e4, 1e6)}
+    torch.cuda.synchronize()
+    assert not torch.equal(want[1e4], want[1e6])
+    got, errors = {1e4: [], 1e6: []}, []
+
+    def run(base):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                got[base] = [append(base) for _ in range(200)]
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # a thread's exceptions are the test's
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(base,)) for base in got]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for base, outs in got.items():
+        assert len(outs) == 200 and all(torch.equal(o, want[base]) for o in outs)
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])

@@ -105,9 +105,6 @@ struct wc_ctx {
   void* pw_scratch = nullptr;            // wc_probs_from_logits: parameters + row thresholds
   int pw_rows = 0;
   uint32_t* lin_xf = nullptr;  // input fragments of the ops-API linear
-  double turn_freq[64] = {};   // wc_paged_append: base^(-2i/D) of the last base and head dim
-  double turn_base = 0;
-  int turn_dim = 0;
   int lin_xf_k = 0;
   bool lin_xf_bf16 = false;
 };

@@ -85,7 +85,29 @@ void check_rows(const void* p, const int64_t* st, int dtype, const char* what) {
   need(aligned16(p) && st[0] % unit == 0 && st[1] % unit == 0 && st[0] >= 0 && st[1] >= 0, what);
 }
 
+// A dense output of n elements against strided rows that other blocks still read.
+void check_apart(const void* out, long long n, int out_dtype, const void* x, const int64_t* st, int dtype, int rows,
+                 int heads, int head_dim, const char* what) {
+  auto size = [](int type) { return type == WC_BF16 ? 2ll : 4ll; };
+  const uintptr_t o = reinterpret_cast<uintptr_t>(out), b = reinterpret_cast<uintptr_t>(x);
+  const long long last = (rows - 1) * st[0] + (heads - 1) * st[1] + head_dim;
+  need(o + n * size(out_dtype) <= b || b + last * size(dtype) <= o, what);
+}
+
 cudaStream_t stream_of(wc_ctx* ctx, void* s) { return s ? static_cast<cudaStream_t>(s) : ctx->stream; }
+
+// base^(-2i/D) of the calling thread's last base and head dim: the powers cost 3 us of a call, and
+// Python threads share a device's context.
+const double* turn_frequencies(double base, int head_dim) {
+  thread_local double freq[kPagedMaxHeadDim / 2], of_base = 0;
+  thread_local int of_dim = 0;
+  if (of_base != base || of_dim != head_dim) {
+    for (int i = 0; i < head_dim / 2; ++i) freq[i] = std::pow(base, -2.0 * i / head_dim);
+    of_base = base;
+    of_dim = head_dim;
+  }
+  return freq;
+}
 
 template <typename S, typename P, int D>
 void launch_append(wc_ctx* ctx, cudaStream_t st, const PagedAppendParams& p) {
@@ -114,6 +136,12 @@ extern "C" wc_status wc_paged_append(wc_ctx* ctx, void* stream, const wc_paged_a
     check_rows(a->k, a->k_stride, a->src_dtype, "paged_append: k must be 16-byte aligned, rows contiguous");
     check_rows(a->v, a->v_stride, a->src_dtype, "paged_append: v must be 16-byte aligned, rows contiguous");
     need(a->q_out && aligned16(a->q_out), "paged_append: q_out must be 16-byte aligned");
+    need(g.k != g.v, "paged_append: k and v must not share their pages");
+    const long long n = (long long)b.rows * b.heads * g.head_dim;
+    const char* apart = "paged_append: q_out must not overlap q, k or v";
+    check_apart(a->q_out, n, g.dtype, a->q, a->q_stride, a->src_dtype, b.rows, b.heads, g.head_dim, apart);
+    check_apart(a->q_out, n, g.dtype, a->k, a->k_stride, a->src_dtype, b.rows, g.kv_heads, g.head_dim, apart);
+    check_apart(a->q_out, n, g.dtype, a->v, a->v_stride, a->src_dtype, b.rows, g.kv_heads, g.head_dim, apart);
     need(!a->q_norm || aligned16(a->q_norm), "paged_append: q_norm must be 16-byte aligned");
     need(!a->k_norm || aligned16(a->k_norm), "paged_append: k_norm must be 16-byte aligned");
     need(a->base > 0 && std::isfinite(a->base), "paged_append: base must be positive");
@@ -149,12 +177,7 @@ extern "C" wc_status wc_paged_append(wc_ctx* ctx, void* stream, const wc_paged_a
     p.H = b.heads;
     p.Hk = g.kv_heads;
     p.err = ctx->d_err;
-    if (ctx->turn_base != a->base || ctx->turn_dim != g.head_dim) {
-      for (int i = 0; i < g.head_dim / 2; ++i) ctx->turn_freq[i] = std::pow(a->base, -2.0 * i / g.head_dim);
-      ctx->turn_base = a->base;
-      ctx->turn_dim = g.head_dim;
-    }
-    std::memcpy(p.freq, ctx->turn_freq, sizeof(p.freq));
+    std::memcpy(p.freq, turn_frequencies(a->base, g.head_dim), sizeof(p.freq));
     const cudaStream_t st = stream_of(ctx, stream);
     const bool sb = a->src_dtype == WC_BF16, pb = g.dtype == WC_BF16;
     if (sb && pb) launch_append<uint16_t, uint16_t>(ctx, st, p, g.head_dim);
@@ -172,7 +195,10 @@ extern "C" wc_status wc_paged_compact(wc_ctx* ctx, void* stream, const wc_paged_
     check_table(a->page_table, a->table_stride, a->table_cols, g.page_size, "paged_compact: bad page table");
     need(a->requests > 0 && a->starts && a->keep && a->n_keep && a->lens_out, "paged_compact: null argument");
     need(a->max_keep > 0 && a->keep_stride >= a->max_keep && a->keep_stride < (1ll << 31), "paged_compact: bad keep list");
+    need(a->lens_out + a->requests <= a->starts || a->starts + a->requests <= a->lens_out,
+         "paged_compact: lens_out must not overlap starts");
     if (a->max_keep > PC_MAXKEEP) fail(WC_ERR_UNSUPPORTED, "paged_compact: keep list longer than 64");
+    need(g.k != g.v, "paged_compact: k and v must not share their pages");
     if (g.layers > 65535) fail(WC_ERR_UNSUPPORTED, "paged_compact: more than 65535 layers");
     DeviceScope scope(ctx->device);
     PagedCompactParams p;
@@ -394,6 +420,8 @@ extern "C" wc_status wc_paged_attention(wc_ctx* ctx, void* stream, const wc_page
     if (b.rows == 0) return;
     check_rows(a->q, a->q_stride, g.dtype, "paged_attention: q must be 16-byte aligned, rows contiguous");
     need(a->out && aligned16(a->out), "paged_attention: out must be 16-byte aligned");
+    check_apart(a->out, (long long)b.rows * b.heads * g.head_dim, g.dtype, a->q, a->q_stride, g.dtype, b.rows, b.heads,
+                g.head_dim, "paged_attention: out must not overlap q");
     if (a->groups) {
       check_table(a->prefix_table, a->prefix_stride, a->prefix_cols, g.page_size, "paged_attention: bad prefix table");
       need(a->prefix_lens && a->group_offsets, "paged_attention: null prefix_lens or group_offsets");
