@@ -379,7 +379,7 @@ WC_API wc_status wc_gemm_bf16(wc_ctx* ctx, const void* A, const void* B, float* 
  *  - head_dim 64 or 128; page_size a power of two from 16 to 256; pages of WC_F32 or WC_BF16;
  *    16-byte aligned pointers and strides, no stride of zero. Outputs must not overlap inputs.
  *  - `stream`: the cudaStream_t to enqueue on (NULL: the context's; cudaStreamLegacy for the
- *    default stream). Nothing is allocated and no state is kept between calls. The first call on a
+ *    default stream). Nothing is allocated and no device state is kept between calls. The first call on a
  *    device sets kernel attributes: make one before a capture begins. */
 typedef struct {
   void *k, *v;
