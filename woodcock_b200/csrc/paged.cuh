@@ -409,7 +409,8 @@ struct PagedWalk {
     return paged_head_tiles<M, KT>(p, g) + (long long)qts * kOver;
   }
 
-  // Block-collective; `sh` holds kWalkShared words. False: the block has no work.
+  // Block-collective; `sh` holds kWalkShared words. False: the block has no work, and other warps may
+  // still be reading `sh`.
   __device__ bool begin(const PagedAttnParams& p, int kinds, int least, long long* sh) {
     nseg = ((kinds & kPrefixRows) ? p.G : 0) + ((kinds & kOwnRows) ? p.B : 0);
     const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, nw = (nt + 31) >> 5;
@@ -466,6 +467,14 @@ struct PagedWalk {
       ++qt;
     }
     return place(int(off)) || next(p, kinds);
+  }
+  // begin(), and the line's beginning kept in sh for a second walk. Only where there is work: there the
+  // search has ended in a barrier, while a block without work leaves between its reads of sh.
+  __device__ bool begin_kept(const PagedAttnParams& p, int kinds, int least, long long* sh) {
+    static_assert(sizeof(PagedWalk) <= 8 * 32, "kept where the search has been");
+    if (!begin(p, kinds, least, sh)) return false;
+    if (threadIdx.x == 0) *reinterpret_cast<PagedWalk*>(sh) = *this;
+    return true;
   }
   // The item's tiles in this block's range; false: only units that hold no tiles.
   __device__ bool place(int off) {
@@ -1305,9 +1314,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
   const uint32_t tmem = *tslot;
   using Walk = PagedWalk<M, KT, PM_OVER>;
   Walk w;
-  const bool work = w.begin(p, kinds, least, sh);
-  static_assert(sizeof(Walk) <= 8 * 32, "kept where the search has been");
-  if (tid == 0) *reinterpret_cast<Walk*>(sh) = w;  // the line's beginning, for a second walk
+  const bool work = w.begin_kept(p, kinds, least, sh);
 
   // The next item of the line, as the walking warp left it.
   auto take_item = [&](int n) {
