@@ -7,14 +7,16 @@
  * plain C: opaque handles, device or host pointers, sizes and a status code.
  *
  * Conventions
- *  - One context per GPU; a context is not thread-safe. All work is enqueued on
- *    the context's stream (set by wc_ctx_create / wc_ctx_set_stream).
+ *  - One context per GPU. wc_paged_* calls on streams of the caller's may come from several threads
+ *    at once, and beside one thread's other calls; those are one thread's at a time. All work is enqueued
+ *    on the context's stream (set by wc_ctx_create / wc_ctx_set_stream) unless a call names another.
  *  - Activation buffers ("_dev" pointers) are caller-owned device memory, row-major
  *    as in the reference (x[L][d], q[L][H][D], K/V[T][Hk][D], mask[L][T], 1 = visible).
  *  - The library owns weights, KV arenas and workspaces behind its handles.
  *  - No function aborts or throws: each returns wc_status; wc_last_error(ctx)
- *    describes the most recent failure. Device-side failures (bounds, timeouts)
- *    are raised through a device error word checked at the round's sync.
+ *    describes the calling thread's most recent failure (any thread's, where it had none).
+ *    Device-side failures (bounds, timeouts) are raised through a device error word checked at
+ *    the round's sync.
  *  - dtype codes: WC_F32 = 0, WC_BF16 = 1.
  */
 #ifndef WOODCOCK_B200_H_

@@ -1,0 +1,21 @@
+"""Threads that share a context: each is told its own failure, none of the shared words is raced on."""
+
+from __future__ import annotations
+
+import subprocess
+
+
+from conftest import REPO
+
+
+def test_failures_and_launches_of_threads(tmp_path):
+    cmd = ["g++", "-std=c++17", "-O1", "-I", "/usr/local/cuda/include", "-I", str(REPO / "include"),
+           str(REPO / "tests" / "host_threads.cpp"), "-o", str(tmp_path / "t")]
+    flags = ["-fsanitize=thread"]
+    (tmp_path / "e.cpp").write_text("int main() { return 0; }\n")
+    if subprocess.run(["g++", *flags, str(tmp_path / "e.cpp"), "-o", str(tmp_path / "e")], capture_output=True).returncode \
+            or subprocess.run([str(tmp_path / "e")], capture_output=True).returncode:
+        flags = []  # no sanitizer: the messages and counts are still compared
+    subprocess.run([*cmd, *flags], check=True, capture_output=True)
+    r = subprocess.run([str(tmp_path / "t")], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "ThreadSanitizer" not in r.stderr, r.stdout + r.stderr[:2000]

@@ -6,12 +6,14 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdlib>
 #include <exception>
 #include <map>
 #include <mutex>
 #include <new>
 #include <string>
+#include <thread>
 #include <utility>
 #include <vector>
 
@@ -36,6 +38,33 @@ struct WcError {
   } while (0)
 
 }  // namespace
+
+// The last failure's message, by thread: paged calls of several threads share a context. A thread that
+// had no failure of its own is told the latest of any.
+class LastError {
+ public:
+  void set(const char* msg) noexcept {
+    try {
+      std::lock_guard<std::mutex> lock(mu_);
+      latest_ = msg;
+      of_[std::this_thread::get_id()] = latest_;
+    } catch (...) {  // no memory for the words: the status still stands
+    }
+  }
+  const char* get() const noexcept {  // valid until the calling thread's next failure
+    try {
+      std::lock_guard<std::mutex> lock(mu_);
+      return of_.emplace(std::this_thread::get_id(), latest_).first->second.c_str();
+    } catch (...) {
+      return "host allocation failed";
+    }
+  }
+
+ private:
+  mutable std::mutex mu_;
+  mutable std::map<std::thread::id, std::string> of_;
+  std::string latest_;
+};
 
 // ============================================================================ context
 
@@ -71,11 +100,11 @@ struct wc_ctx {
   cudaStream_t stream = nullptr;
   bool own_stream = false;
   int num_sms = 148;
-  std::string err;
+  LastError err;
   int* d_err = nullptr;  // device error word of the ops API
-  uint64_t launches = 0;
-  bool capturing = false;
-  uint64_t capture_launches = 0;
+  std::atomic<uint64_t> launches{0};
+  std::atomic<bool> capturing{false};  // on `stream`
+  std::atomic<uint64_t> capture_launches{0};
   std::map<std::pair<int, uint32_t>, RopeTable> rope;
   double* pw = nullptr;
   double* qw = nullptr;
@@ -117,13 +146,13 @@ wc_status guard(wc_ctx* ctx, F&& f) {
     f();
     return WC_OK;
   } catch (const WcError& e) {
-    if (ctx) ctx->err = e.msg;
+    if (ctx) ctx->err.set(e.msg.c_str());
     return e.st;
   } catch (const std::bad_alloc&) {
-    if (ctx) ctx->err = "host allocation failed";
+    if (ctx) ctx->err.set("host allocation failed");
     return WC_ERR_OOM;
   } catch (const std::exception& e) {
-    if (ctx) ctx->err = e.what();
+    if (ctx) ctx->err.set(e.what());
     return WC_ERR_IO;
   }
 }
@@ -146,15 +175,15 @@ void prof_end(wc_ctx* ctx, int kind) {
   ctx->prof->open[kind] = nullptr;
 }
 
-void count_launch(wc_ctx* ctx) {
-  if (ctx->capturing) ++ctx->capture_launches;
+void count_launch(wc_ctx* ctx, cudaStream_t stream) {
+  if (ctx->capturing && stream == ctx->stream) ++ctx->capture_launches;
   else ++ctx->launches;
 }
 
 void check_launch(wc_ctx* ctx, const char* what) {
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) fail(WC_ERR_CUDA, std::string("launch of ") + what + " failed: " + cudaGetErrorString(e));
-  count_launch(ctx);
+  count_launch(ctx, ctx->stream);
 }
 
 // Launch with optional programmatic dependent launch (the kernel must pdl_wait() before it
@@ -185,7 +214,7 @@ void launch_on(wc_ctx* ctx, cudaStream_t stream, const char* what, void (*kernel
   cfg.numAttrs = na;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
   if (e != cudaSuccess) fail(WC_ERR_CUDA, std::string("launch of ") + what + ": " + cudaGetErrorString(e));
-  count_launch(ctx);
+  count_launch(ctx, stream);
 }
 
 // The same on the context's stream.

@@ -673,7 +673,7 @@ extern "C" void wc_ctx_destroy(wc_ctx* ctx) {
   delete ctx;
 }
 
-extern "C" const char* wc_last_error(const wc_ctx* ctx) { return ctx ? ctx->err.c_str() : "null context"; }
+extern "C" const char* wc_last_error(const wc_ctx* ctx) { return ctx ? ctx->err.get() : "null context"; }
 
 extern "C" wc_status wc_ctx_synchronize(wc_ctx* ctx) {
   if (!ctx) return WC_ERR_INVALID;
@@ -690,7 +690,7 @@ extern "C" wc_status wc_ctx_synchronize(wc_ctx* ctx) {
   });
 }
 
-extern "C" uint64_t wc_ctx_launch_count(const wc_ctx* ctx) { return ctx ? ctx->launches : 0; }
+extern "C" uint64_t wc_ctx_launch_count(const wc_ctx* ctx) { return ctx ? ctx->launches.load() : 0; }
 extern "C" wc_status wc_ctx_wait_selftest(wc_ctx* ctx, int iterations) {
   if (!ctx || iterations < 1 || iterations > (1 << 20)) return WC_ERR_INVALID;
   return guard(ctx, [&] {
@@ -2300,7 +2300,7 @@ extern "C" wc_status wc_drafter_head_softmax(wc_drafter* d, const float* out, in
                                              float* probs) {
   if (!d || !out || !probs || rows <= 0) return WC_ERR_INVALID;
   if (!(temperature > 0.f)) {
-    d->ctx->err = "the draft distribution needs a temperature > 0 (greedy drafting uses 1)";
+    d->ctx->err.set("the draft distribution needs a temperature > 0 (greedy drafting uses 1)");
     return WC_ERR_INVALID;
   }
   const wc_status st = wc_drafter_logits(d, out, rows, probs);  // logits into the output, then in place
