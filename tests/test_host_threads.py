@@ -3,7 +3,8 @@
 from __future__ import annotations
 
 import subprocess
-
+import threading
+import time
 
 from conftest import REPO
 
@@ -19,3 +20,26 @@ def test_failures_and_launches_of_threads(tmp_path):
     subprocess.run([*cmd, *flags], check=True, capture_output=True)
     r = subprocess.run([str(tmp_path / "t")], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0 and "ThreadSanitizer" not in r.stderr, r.stdout + r.stderr[:2000]
+
+
+def test_threads_that_ask_first_get_one_context(monkeypatch):
+    from woodcock_b200.context import Context
+
+    made, got, start = [], [], threading.Barrier(8)
+
+    def init(self, device=0):
+        time.sleep(0.05)
+        made.append(device)
+
+    def ask():
+        start.wait()
+        got.append(Context.get(5))
+
+    monkeypatch.setattr(Context, "__init__", init)
+    monkeypatch.setattr(Context, "_by_device", {})
+    threads = [threading.Thread(target=ask) for _ in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert made == [5] and len({id(c) for c in got}) == 1

@@ -9,6 +9,7 @@ stream and the caller's stream after the work it enqueued.
 from __future__ import annotations
 
 import ctypes as C
+import threading
 from contextlib import contextmanager
 
 import torch
@@ -18,6 +19,7 @@ from ._lib import check, lib
 
 class Context:
     _by_device: dict[int, "Context"] = {}
+    _making = threading.Lock()  # one context per device, whichever thread asks first
 
     def __init__(self, device: int = 0):
         if not torch.cuda.is_available():
@@ -39,7 +41,9 @@ class Context:
             device = device.index or 0
         device = 0 if device is None else int(device)
         if device not in cls._by_device:
-            cls._by_device[device] = cls(device)
+            with cls._making:
+                if device not in cls._by_device:
+                    cls._by_device[device] = cls(device)
         return cls._by_device[device]
 
     def check(self, status: int) -> None:
