@@ -379,7 +379,10 @@ WC_API wc_status wc_gemm_bf16(wc_ctx* ctx, const void* A, const void* B, float* 
  *    append drops the row, and the device error word is raised (wc_ctx_synchronize returns
  *    WC_ERR_DEVICE once the stream's work is done).
  *  - head_dim 64 or 128; page_size a power of two from 16 to 256; pages of WC_F32 or WC_BF16;
- *    16-byte aligned pointers and strides, no stride of zero. Outputs must not overlap inputs.
+ *    16-byte aligned pointers and strides, no stride of zero.
+ *  - What a call writes (q_out, out, lens_out, the workspace, the pages of append and compact) must not
+ *    overlap what it reads, nor itself: refused. K and V may be cut from one buffer; they are told apart
+ *    where their strides are equal.
  *  - `stream`: the cudaStream_t to enqueue on (NULL: the context's; cudaStreamLegacy for the
  *    default stream). Nothing is allocated and no device state is kept between calls. The first call on a
  *    device sets kernel attributes: make one before a capture begins. */

@@ -6,7 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_gpu_paged import BF, Case, check, i32
+from test_gpu_paged import BF, F32, Case, check, i32
 
 pytestmark = pytest.mark.gpu
 
@@ -61,3 +61,118 @@ def test_threads_that_are_refused_at_once_are_told_their_own_reasons():
         t.join()
     for what, words in told.items():
         assert len(words) == 300 and all(what in w for w in words), (what, set(words))
+
+
+def windows(x, step):
+    """The pool with its pages `step` elements apart, each reaching into the next."""
+    return x.as_strided(x.shape, (step, *x.stride()[1:]))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_written_memory_that_overlaps_is_refused(dtype):
+    from woodcock_b200 import ops
+
+    c = Case(62, [40, 50], [1, 1], 16, 8, 128, 16, dtype)
+    n = torch.randn((2, 8, 128), generator=c.g, device="cuda").to(dtype)
+    page = c.k[0].numel()
+    zeros = i32([0, 0])
+
+    def append(k, v, q=c.q, kn=n, vn=n, **kw):
+        return ops.paged_append(q, kn, vn, k, v, c.table, c.kv, **kw)
+
+    def compact(k, v, keep=None):
+        return ops.paged_compact(k, v, c.table, zeros, i32([[0], [0]]) if keep is None else keep, zeros)
+
+    both = torch.zeros((2 * c.k.shape[0], *c.k.shape[1:]), dtype=dtype, device="cuda")
+    half = c.k.shape[0]
+    for k, v, what in (
+            (windows(c.k, page // 2), c.v, "overlap"),                # pages that reach into the next
+            (c.k, windows(c.v, page - 128), "overlap"),
+            (both[:half], both[1: half + 1], "share"),                # K and V a page apart in one buffer
+            (both[: half], both[half - 1: 2 * half - 1], "share"),
+            (both.view(half, 2, 8, 16, 128)[:, 0], both.view(half, 2, 8, 16, 128)[:, 0], "share")):
+        for call in (append, compact):
+            with pytest.raises(ValueError, match=what):
+                call(k, v)
+    flat = torch.zeros(2 * half * page + 2 * 16 * 128, dtype=dtype, device="cuda")
+    pools = flat[: 2 * half * page].view(2, half, 8, 16, 128)
+    k, v = pools[0], pools[1]
+    inside = flat[2 * half * page - 2048: 2 * half * page + 2048].view(2, 16, 128)  # its first half in V's last page
+    with pytest.raises(ValueError, match="overlap"):
+        append(k, v, out=inside)
+    with pytest.raises(ValueError, match="overlap"):
+        append(k, v, q=inside)
+    for kn, vn in ((k[0, :, :2].transpose(0, 1), n), (n, v[3, :, 4:6].transpose(0, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            append(k, v, kn=kn, vn=vn)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.paged_attention(c.q, k, v, c.table, c.kv, out=inside)
+    with pytest.raises(ValueError, match="overlap"):  # page numbers inside the pages
+        ops.paged_compact(k, v, k.view(torch.int32)[0, 0, :2, : c.table.shape[1]], zeros, i32([[0], [0]]), zeros)
+    # what lies apart is not refused: behind the pages, and K and V side by side in one buffer
+    out = flat[2 * half * page:].view(2, 16, 128)
+    assert append(k, v, out=out) is out
+    assert ops.paged_attention(c.q, k, v, c.table, c.kv, out=out) is out
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("layout", ["halves", "page", "head", "row", "shifted"])
+def test_k_and_v_in_one_buffer(dtype, layout):
+    """Pools cut from one buffer: halves of it, or K and V of a page, a head or a row side by side."""
+    from woodcock_b200 import ops
+
+    c = Case(63, [40, 5, 90], [2, 2, 2], 8, 4, 64, 16, dtype)
+    P, Hk, page, D = c.k.shape
+    shape = {"halves": (2, P, Hk, page, D), "page": (P, 2, Hk, page, D), "head": (P, Hk, 2, page, D),
+             "row": (P, Hk, page, 2, D), "shifted": (P + 4, 2, Hk, page, D)}[layout]
+    buf = torch.full(shape, 3.0, dtype=dtype, device="cuda")
+    axis = {"halves": 0, "page": 1, "head": 2, "row": 3, "shifted": 1}[layout]
+    k, v = buf.select(axis, 0), buf.select(axis, 1)
+    if layout == "shifted":
+        k, v = k[:P], v[4:]
+    k.copy_(c.k)
+    v.copy_(c.v)
+    new = [c.randn(6, h, D) for h in (8, 4, 4)]
+    a = ops.paged_append(*new, c.k, c.v, c.table, c.kv)
+    b = ops.paged_append(*new, k, v, c.table, c.kv)
+    assert torch.equal(a, b)
+    c.q = a
+    out = ops.paged_attention(a, k, v, c.table, c.kv)
+    check(c, out)
+    assert torch.equal(out, ops.paged_attention(a, c.k, c.v, c.table, c.kv))
+    args = c.table, i32([38, 3, 88]), i32([[0, 1], [1, 0], [1, 0]]), i32([2, 1, 1])
+    assert torch.equal(ops.paged_compact(k, v, *args), ops.paged_compact(c.k, c.v, *args))
+    assert torch.equal(k.nan_to_num(7.0), c.k.nan_to_num(7.0)) and torch.equal(v.nan_to_num(7.0), c.v.nan_to_num(7.0))
+
+
+def test_a_workspace_over_what_the_call_reads_or_writes_is_refused():
+    import ctypes as C
+
+    from woodcock_b200 import ops, paged
+    from woodcock_b200._lib import WC_ERR_INVALID, WC_OK, lib
+    from woodcock_b200.context import Context
+
+    ctx = Context.get(0)
+    c = Case(64, [40, 50], [1, 1], 16, 8, 128, 16, BF)
+    pages = paged._pages(c.k, c.v)
+    batch, _, _ = paged._batch(2, 16, c.table, c.kv, None, c.k.device)
+    need = C.c_uint64()
+    out = torch.zeros((2, 16, 128), dtype=BF, device="cuda")
+
+    def args(ws, n, to=out):
+        return paged._ATTENTION.pack(*pages, *batch, c.q.data_ptr(), *c.q.stride()[:2], 0, 0, 0, 0, 0, 0, 0, to.data_ptr(), ws, n,
+                                     128 ** -0.5, 0)
+
+    assert lib().wc_paged_attention_workspace(ctx.h, args(16, 0), C.byref(need)) == WC_OK
+    n = need.value
+    buf = torch.zeros(2 * n + 512, dtype=torch.uint8, device="cuda")
+    ws = -(-buf.data_ptr() // 256) * 256
+    stream = paged._stream(0)
+    for to in (ws, ws + n - 256):
+        over = buf[to - buf.data_ptr():][: out.numel() * 2].view(BF).view(out.shape)
+        assert lib().wc_paged_attention(ctx.h, stream, args(ws, n, over)) == WC_ERR_INVALID
+    for x in (c.q, c.k, c.v):
+        assert lib().wc_paged_attention(ctx.h, stream, args(-(-x.data_ptr() // 256) * 256, n)) == WC_ERR_INVALID
+    over = buf[ws + n - buf.data_ptr():][: out.numel() * 2].view(BF).view(out.shape)  # right behind it
+    assert lib().wc_paged_attention(ctx.h, stream, args(ws, n, over)) == WC_OK
+    assert torch.equal(over, ops.paged_attention(c.q, c.k, c.v, c.table, c.kv))

@@ -3,8 +3,10 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <initializer_list>
 
 #include "host.h"
+#include "overlap.h"
 #include "paged.cuh"
 
 using namespace wc;
@@ -30,6 +32,8 @@ struct DeviceScope {
 void need(bool ok, const char* what) {
   if (!ok) fail(WC_ERR_INVALID, what);
 }
+
+long long element(int dtype) { return dtype == WC_BF16 ? 2 : 4; }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
@@ -63,7 +67,7 @@ void check_table(const int* table, long long stride, int cols, int page_size, co
 
 PagePool pool(const wc_pages& g, const void* base, const int64_t* st, int layer) {
   PagePool r;
-  r.ptr = static_cast<char*>(const_cast<void*>(base)) + st[0] * layer * (g.dtype == WC_BF16 ? 2 : 4);
+  r.ptr = static_cast<char*>(const_cast<void*>(base)) + st[0] * layer * element(g.dtype);
   r.page = st[1];
   r.head = st[2];
   r.row = st[3];
@@ -85,13 +89,50 @@ void check_rows(const void* p, const int64_t* st, int dtype, const char* what) {
   need(aligned16(p) && st[0] % unit == 0 && st[1] % unit == 0 && st[0] >= 0 && st[1] >= 0, what);
 }
 
-// A dense output of n elements against strided rows that other blocks still read.
-void check_apart(const void* out, long long n, int out_dtype, const void* x, const int64_t* st, int dtype, int rows,
-                 int heads, int head_dim, const char* what) {
-  auto size = [](int type) { return type == WC_BF16 ? 2ll : 4ll; };
-  const uintptr_t o = reinterpret_cast<uintptr_t>(out), b = reinterpret_cast<uintptr_t>(x);
-  const long long last = (rows - 1) * st[0] + (heads - 1) * st[1] + head_dim;
-  need(o + n * size(out_dtype) <= b || b + last * size(dtype) <= o, what);
+// What a call writes must lie apart from what its blocks read, and from itself: nothing orders them.
+struct Run {
+  const void* p;
+  long long bytes;
+};
+
+// Strided rows [rows][heads][head_dim] as the range from their first byte to their last.
+Run rows_run(const void* p, const int64_t* st, int dtype, int rows, int heads, int head_dim) {
+  return {p, ((rows - 1) * st[0] + (heads - 1) * st[1] + head_dim) * element(dtype)};
+}
+
+Run ints_run(const int* p, long long n) { return {p, p ? n * 4 : 0}; }
+Run table_run(const int* p, long long stride, int cols, int n) { return ints_run(p, n > 0 ? (n - 1) * stride + cols : 0); }
+
+void check_apart(const Run& out, std::initializer_list<Run> in, const char* what) {
+  const uintptr_t o = reinterpret_cast<uintptr_t>(out.p);
+  for (const Run& x : in) {
+    const uintptr_t b = reinterpret_cast<uintptr_t>(x.p);
+    need(!b || x.bytes <= 0 || o + out.bytes <= b || b + x.bytes <= o, what);
+  }
+}
+
+// The places of one layer's pages (layer >= 0), or of all layers'.
+Strided places(const wc_pages& g, const void* base, const int64_t* st, int layer) {
+  const long long e = element(g.dtype);
+  Strided s;
+  s.at = reinterpret_cast<uintptr_t>(base) + (layer > 0 ? st[0] * layer * e : 0);
+  s.run = g.head_dim * e;
+  if (layer < 0) s.add(g.layers, st[0] * e);
+  s.add(g.pages, st[1] * e);
+  s.add(g.kv_heads, st[2] * e);
+  s.add(g.page_size, st[3] * e);
+  s.close();
+  return s;
+}
+
+// Pages that a call writes.
+void check_written(const Strided& K, const Strided& V) {
+  need(K.nested && V.nested, "paged: pages must not overlap");
+  need(!meets(K, V), "paged: k and v must not share their pages");
+}
+
+void check_pages_apart(const Strided& K, const Strided& V, std::initializer_list<Run> runs, const char* what) {
+  for (const Run& x : runs) need(!meets_run(K, x.p, x.bytes) && !meets_run(V, x.p, x.bytes), what);
 }
 
 cudaStream_t stream_of(wc_ctx* ctx, void* s) { return s ? static_cast<cudaStream_t>(s) : ctx->stream; }
@@ -136,12 +177,18 @@ extern "C" wc_status wc_paged_append(wc_ctx* ctx, void* stream, const wc_paged_a
     check_rows(a->k, a->k_stride, a->src_dtype, "paged_append: k must be 16-byte aligned, rows contiguous");
     check_rows(a->v, a->v_stride, a->src_dtype, "paged_append: v must be 16-byte aligned, rows contiguous");
     need(a->q_out && aligned16(a->q_out), "paged_append: q_out must be 16-byte aligned");
-    need(g.k != g.v, "paged_append: k and v must not share their pages");
-    const long long n = (long long)b.rows * b.heads * g.head_dim;
-    const char* apart = "paged_append: q_out must not overlap q, k or v";
-    check_apart(a->q_out, n, g.dtype, a->q, a->q_stride, a->src_dtype, b.rows, b.heads, g.head_dim, apart);
-    check_apart(a->q_out, n, g.dtype, a->k, a->k_stride, a->src_dtype, b.rows, g.kv_heads, g.head_dim, apart);
-    check_apart(a->q_out, n, g.dtype, a->v, a->v_stride, a->src_dtype, b.rows, g.kv_heads, g.head_dim, apart);
+    const Strided K = places(g, g.k, g.k_stride, a->layer), V = places(g, g.v, g.v_stride, a->layer);
+    check_written(K, V);
+    const Run out{a->q_out, (long long)b.rows * b.heads * g.head_dim * element(g.dtype)};
+    const Run q = rows_run(a->q, a->q_stride, a->src_dtype, b.rows, b.heads, g.head_dim),
+              k = rows_run(a->k, a->k_stride, a->src_dtype, b.rows, g.kv_heads, g.head_dim),
+              v = rows_run(a->v, a->v_stride, a->src_dtype, b.rows, g.kv_heads, g.head_dim),
+              table = table_run(b.page_table, b.table_stride, b.table_cols, b.requests),
+              lens = ints_run(b.kv_lens, b.requests), offsets = ints_run(b.q_offsets, b.requests + 1ll),
+              positions = ints_run(a->positions, b.rows), qn{a->q_norm, g.head_dim * 4ll}, kn{a->k_norm, g.head_dim * 4ll};
+    check_apart(out, {q, k, v, table, lens, offsets, positions, qn, kn}, "paged_append: q_out must not overlap an input");
+    check_pages_apart(K, V, {out, q, k, v, table, lens, offsets, positions, qn, kn},
+                      "paged_append: the pages must not overlap q_out or an input");
     need(!a->q_norm || aligned16(a->q_norm), "paged_append: q_norm must be 16-byte aligned");
     need(!a->k_norm || aligned16(a->k_norm), "paged_append: k_norm must be 16-byte aligned");
     need(a->base > 0 && std::isfinite(a->base), "paged_append: base must be positive");
@@ -195,10 +242,16 @@ extern "C" wc_status wc_paged_compact(wc_ctx* ctx, void* stream, const wc_paged_
     check_table(a->page_table, a->table_stride, a->table_cols, g.page_size, "paged_compact: bad page table");
     need(a->requests > 0 && a->starts && a->keep && a->n_keep && a->lens_out, "paged_compact: null argument");
     need(a->max_keep > 0 && a->keep_stride >= a->max_keep && a->keep_stride < (1ll << 31), "paged_compact: bad keep list");
-    need(a->lens_out + a->requests <= a->starts || a->starts + a->requests <= a->lens_out,
-         "paged_compact: lens_out must not overlap starts");
     if (a->max_keep > PC_MAXKEEP) fail(WC_ERR_UNSUPPORTED, "paged_compact: keep list longer than 64");
-    need(g.k != g.v, "paged_compact: k and v must not share their pages");
+    const Strided K = places(g, g.k, g.k_stride, -1), V = places(g, g.v, g.v_stride, -1);
+    check_written(K, V);
+    const Run lens = ints_run(a->lens_out, a->requests), starts = ints_run(a->starts, a->requests),
+              n_keep = ints_run(a->n_keep, a->requests),
+              keep = table_run(a->keep, a->keep_stride, a->max_keep, a->requests),
+              table = table_run(a->page_table, a->table_stride, a->table_cols, a->requests);
+    check_apart(lens, {starts, keep, n_keep, table}, "paged_compact: lens_out must not overlap an input");
+    check_pages_apart(K, V, {lens, starts, keep, n_keep, table},
+                      "paged_compact: the pages must not overlap lens_out or an input");
     if (g.layers > 65535) fail(WC_ERR_UNSUPPORTED, "paged_compact: more than 65535 layers");
     DeviceScope scope(ctx->device);
     PagedCompactParams p;
@@ -420,8 +473,6 @@ extern "C" wc_status wc_paged_attention(wc_ctx* ctx, void* stream, const wc_page
     if (b.rows == 0) return;
     check_rows(a->q, a->q_stride, g.dtype, "paged_attention: q must be 16-byte aligned, rows contiguous");
     need(a->out && aligned16(a->out), "paged_attention: out must be 16-byte aligned");
-    check_apart(a->out, (long long)b.rows * b.heads * g.head_dim, g.dtype, a->q, a->q_stride, g.dtype, b.rows, b.heads,
-                g.head_dim, "paged_attention: out must not overlap q");
     if (a->groups) {
       check_table(a->prefix_table, a->prefix_stride, a->prefix_cols, g.page_size, "paged_attention: bad prefix table");
       need(a->prefix_lens && a->group_offsets, "paged_attention: null prefix_lens or group_offsets");
@@ -429,6 +480,17 @@ extern "C" wc_status wc_paged_attention(wc_ctx* ctx, void* stream, const wc_page
     const Layout l = layout(ctx, *a);
     if (!a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 256 || a->workspace_bytes < l.bytes)
       fail(WC_ERR_CAPACITY, "paged_attention: workspace missing, misaligned or too small");
+    const Run out{a->out, (long long)b.rows * b.heads * g.head_dim * element(g.dtype)},
+        scratch{a->workspace, (long long)l.bytes}, q = rows_run(a->q, a->q_stride, g.dtype, b.rows, b.heads, g.head_dim),
+        table = table_run(b.page_table, b.table_stride, b.table_cols, b.requests), lens = ints_run(b.kv_lens, b.requests),
+        offsets = ints_run(b.q_offsets, b.requests + 1ll), tree{a->tree_mask, a->tree_mask ? b.rows * 8ll : 0},
+        ptable = table_run(a->prefix_table, a->prefix_stride, a->prefix_cols, a->groups),
+        plens = ints_run(a->prefix_lens, a->groups), ends = ints_run(a->group_offsets, a->groups ? a->groups + 1ll : 0);
+    check_apart(out, {q, table, lens, offsets, tree, ptable, plens, ends}, "paged_attention: out must not overlap an input");
+    check_apart(scratch, {out, q, table, lens, offsets, tree, ptable, plens, ends},
+                "paged_attention: the workspace must not overlap out or an input");
+    check_pages_apart(places(g, g.k, g.k_stride, a->layer), places(g, g.v, g.v_stride, a->layer), {out, scratch},
+                      "paged_attention: out and the workspace must not overlap the pages");
     DeviceScope scope(ctx->device);
     char* ws = static_cast<char*>(a->workspace);
     PagedAttnParams p;

@@ -17,7 +17,9 @@ python/woodcock/target.py:159-175); a server keeps many requests' keys and value
   it raises the context's device error word (``Context.get(device).synchronize()`` after the
   stream's work raises WcError).
 * Work runs on the caller's current stream of the tensors' device, in its order; scratch comes from
-  PyTorch's allocator for that one call. Outputs must not overlap inputs.
+  PyTorch's allocator for that one call. What a call writes (its output, the pages of append and
+  compact) must not overlap what it reads, nor itself: refused with ValueError. K and V may be cut from
+  one buffer (halves, or side by side in a page, a head or a row).
 """
 
 from __future__ import annotations
