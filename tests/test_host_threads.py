@@ -43,3 +43,32 @@ def test_threads_that_ask_first_get_one_context(monkeypatch):
     for t in threads:
         t.join()
     assert made == [5] and len({id(c) for c in got}) == 1
+
+
+def test_a_paged_call_makes_its_context_within_the_device(monkeypatch):
+    """Making a context selects its device; the one that was current comes back."""
+    import torch
+
+    from woodcock_b200 import paged
+    from woodcock_b200.context import Context
+
+    current = [0]
+
+    class device:
+        def __init__(self, d):
+            self.d = d.index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.d
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    def init(self, index=0):
+        current[0] = index  # as the library does
+
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(Context, "__init__", init)
+    monkeypatch.setattr(Context, "_by_device", {})
+    a = paged._context(torch.device("cuda", 3))
+    assert current == [0] and paged._context(torch.device("cuda", 3)) is a and Context.get(3) is a

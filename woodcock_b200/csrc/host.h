@@ -239,6 +239,22 @@ void dfree(void* p) {
   if (p) cudaFree(p);
 }
 
+// A call's device where it is not the current one; the current one comes back at its end.
+struct DeviceScope {
+  int before = -1;
+  explicit DeviceScope(int device) {
+    int cur = 0;
+    CUDA_TRY(cudaGetDevice(&cur));
+    if (cur != device) {
+      CUDA_TRY(cudaSetDevice(device));
+      before = cur;
+    }
+  }
+  ~DeviceScope() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
+
 // cuTensorMapEncodeTiled through the runtime's driver entry point (no libcuda link).
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,

@@ -13,22 +13,6 @@ using namespace wc;
 
 namespace {
 
-// Work goes to the caller's stream, which may belong to another device than the current one.
-struct DeviceScope {
-  int before = -1;
-  explicit DeviceScope(int device) {
-    int cur = 0;
-    CUDA_TRY(cudaGetDevice(&cur));
-    if (cur != device) {
-      CUDA_TRY(cudaSetDevice(device));
-      before = cur;
-    }
-  }
-  ~DeviceScope() {
-    if (before >= 0) cudaSetDevice(before);
-  }
-};
-
 void need(bool ok, const char* what) {
   if (!ok) fail(WC_ERR_INVALID, what);
 }

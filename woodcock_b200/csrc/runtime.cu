@@ -678,6 +678,7 @@ extern "C" const char* wc_last_error(const wc_ctx* ctx) { return ctx ? ctx->err.
 extern "C" wc_status wc_ctx_synchronize(wc_ctx* ctx) {
   if (!ctx) return WC_ERR_INVALID;
   return guard(ctx, [&] {
+    DeviceScope scope(ctx->device);
     CUDA_TRY(cudaStreamSynchronize(ctx->stream));
     int e = 0;
     CUDA_TRY(cudaMemcpy(&e, ctx->d_err, sizeof(int), cudaMemcpyDeviceToHost));

@@ -49,6 +49,14 @@ def _fail(what: str):
     raise ValueError(what)
 
 
+def _context(device: torch.device) -> Context:
+    ctx = Context._by_device.get(device.index)
+    if ctx is None:  # making one selects its device: the caller's stays the current one
+        with torch.cuda.device(device):
+            ctx = Context.get(device)
+    return ctx
+
+
 def _stream(device: int) -> int:
     # the default stream's handle is 0, which the library reads as "the context's"; 1 names it
     return _raw_stream(device) or 1
@@ -164,7 +172,7 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
     out = _out(out, q, shape, k_pages.dtype)
     if T == 0 or B == 0:
         return out
-    ctx = Context.get(dev)
+    ctx = _context(dev)
     ctx.check(lib().wc_paged_append(ctx.h, _stream(ctx.device.index), _APPEND.pack(
         *pages, *batch, q.data_ptr(), k.data_ptr(), v.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1],
         0 if pos is None else pos.data_ptr(), 0 if qn is None else qn.data_ptr(), 0 if kn is None else kn.data_ptr(),
@@ -177,7 +185,7 @@ def _workspace(device: int, code: int, pages: int, page_size: int, kv_heads: int
                requests: int, rows: int, heads: int, groups: int) -> int:
     """Bytes of scratch for calls of these sizes (the library looks at no buffer for this)."""
     n = C.c_uint64()
-    ctx = Context.get(device)
+    ctx = _context(torch.device("cuda", device))
     st = head_dim * page_size * kv_heads
     strides = (0, st, head_dim * page_size, head_dim)
     ctx.check(lib().wc_paged_attention_workspace(ctx.h, _ATTENTION.pack(
@@ -206,7 +214,7 @@ def _attend(q, k_pages, v_pages, prefix, page_table, kv_lens, q_offsets, tree_ma
     out = _out(out, q, shape, kind)
     if T == 0 or B == 0:
         return out
-    ctx = Context.get(dev)
+    ctx = _context(dev)
     device = ctx.device.index
     n = _workspace(device, pages[10], pages[11], pages[12], pages[13], D, batch[2], B, T, H, G)
     ws = q.new_empty(n + 256, dtype=torch.uint8)
@@ -264,7 +272,7 @@ def paged_compact(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table, star
     lens = starts.new_empty(B)
     if B == 0:
         return lens
-    ctx = Context.get(dev)
+    ctx = _context(dev)
     many = B > 1
     ctx.check(lib().wc_paged_compact(ctx.h, _stream(ctx.device.index), _COMPACT.pack(
         *pages, table.data_ptr(), table.stride(0) if many else cols, cols, B, starts.data_ptr(), keep.data_ptr(),
