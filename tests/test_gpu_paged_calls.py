@@ -176,3 +176,71 @@ def test_a_workspace_over_what_the_call_reads_or_writes_is_refused():
     over = buf[ws + n - buf.data_ptr():][: out.numel() * 2].view(BF).view(out.shape)  # right behind it
     assert lib().wc_paged_attention(ctx.h, stream, args(ws, n, over)) == WC_OK
     assert torch.equal(over, ops.paged_attention(c.q, c.k, c.v, c.table, c.kv))
+
+
+FIRST_USE = """
+import sys
+sys.path[:0] = [{tests!r}, {repo!r}]
+import torch
+from test_gpu_paged import BF, F32, Case, check, i32
+from woodcock_b200 import ops
+
+c = Case(70, [40], [1], 16, 8, 128, 16, BF)
+ops.paged_attention(c.q, c.k, c.v, c.table, c.kv)
+torch.cuda.synchronize()
+for c in (Case(71, [300, 200], [130, 20], 16, 8, 128, 16, BF, prefix=[100]), Case(72, [300], [300], 16, 8, 64, 16, BF, prefix=[100]),
+          Case(73, [90, 80], [3, 3], 4, 2, 64, 16, F32, prefix=[100]), Case(74, [90, 80], [20, 3], 4, 2, 64, 16, BF, prefix=[100])):
+    B, new = len(c.lens), [c.randn(sum(c.rows), h, c.D) for h in (c.H, c.Hk, c.Hk)]
+    k, v, plens, ends = c.k.clone(), c.v.clone(), i32([100]), i32([0, B])
+    starts, keep, n = i32([0] * B), i32([[0, 2]] * B), i32([2] * B)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        own = ops.paged_attention(c.q, c.k, c.v, c.table, c.kv, q_offsets=c.off)
+        joined = ops.shared_prefix_attention(c.q, c.k, c.v, c.ptable, plens, ends, c.table, c.kv, q_offsets=c.off)
+        q = ops.paged_append(*new, k, v, c.table, c.kv, q_offsets=c.off)
+        lens = ops.paged_compact(k, v, c.table, starts, keep, n)
+    g.replay()
+    torch.cuda.synchronize()
+    check(c, own)
+    check(c, joined, groups=[0, B])
+    k2, v2 = c.k.clone(), c.v.clone()
+    assert torch.equal(q, ops.paged_append(*new, k2, v2, c.table, c.kv, q_offsets=c.off))
+    assert torch.equal(lens, ops.paged_compact(k2, v2, c.table, starts, keep, n))
+    assert torch.equal(k.nan_to_num(7.0), k2.nan_to_num(7.0)) and torch.equal(v.nan_to_num(7.0), v2.nan_to_num(7.0))
+print("captured")
+"""
+
+
+def test_a_capture_may_hold_sizes_that_no_call_had_before():
+    """One call of any size comes before a capture; the captured calls reach other kernels for the first time."""
+    import subprocess
+    import sys
+
+    from conftest import REPO
+
+    r = subprocess.run([sys.executable, "-c", FIRST_USE.format(tests=str(REPO / "tests"), repo=str(REPO))],
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+def test_a_padded_batch_in_a_step():
+    """Rows that pad a batch behind the last request hold NaN and are left alone by every operator of the step."""
+    from woodcock_b200 import ops
+
+    c = Case(65, [40, 5, 90], [2, 1, 3], 16, 8, 128, 16, BF)
+    T, pad = 6, 5
+    full = [torch.full((T + pad, h, 128), float("nan"), dtype=BF, device="cuda") for h in (16, 8, 8)]
+    new = [c.randn(T, h, 128) for h in (16, 8, 8)]
+    for x, y in zip(full, new):
+        x[:T] = y
+    k, v, out = c.k.clone(), c.v.clone(), torch.full((T + pad, 16, 128), 5.0, dtype=BF, device="cuda")
+    a = ops.paged_append(*new, c.k, c.v, c.table, c.kv, q_offsets=c.off)
+    assert ops.paged_append(*full, k, v, c.table, c.kv, q_offsets=c.off, out=out) is out
+    assert torch.equal(out[:T], a) and (out[T:] == 5).all()
+    assert torch.equal(k.nan_to_num(7.0), c.k.nan_to_num(7.0)) and torch.equal(v.nan_to_num(7.0), c.v.nan_to_num(7.0))
+    c.q = a
+    full[0][:T] = a
+    got = ops.paged_attention(full[0], c.k, c.v, c.table, c.kv, q_offsets=c.off, out=torch.full_like(out, 5.0))
+    check(c, got)
+    assert (got[T:] == 5).all()
