@@ -372,11 +372,12 @@ WC_API wc_status wc_gemm_bf16(wc_ctx* ctx, const void* A, const void* B, float* 
  *    request b is row j % page_size of page page_table[b][j / page_size].
  *  - kv_lens[b] counts request b's keys, its new rows included; its new rows are rows
  *    q_offsets[b] .. q_offsets[b + 1] of q, k, v and out (q_offsets NULL: rows / requests each) and
- *    hold its last keys. Rows behind q_offsets[requests] are neither read nor written.
+ *    hold its last keys. Rows behind q_offsets[requests] are not written and what they hold does not
+ *    matter, but they are memory: append may load them.
  *  - Lengths, offsets and tables are device memory, so a captured graph may be replayed on new ones.
  *    A table entry outside the pool, a length beyond the table and offsets out of range are never
  *    followed: such a page's keys and values read as zeros, a length is cut to what the table holds,
- *    append drops the row, and the device error word is raised (wc_ctx_synchronize returns
+ *    append drops the row's k and v, and the device error word is raised (wc_ctx_synchronize returns
  *    WC_ERR_DEVICE once the stream's work is done).
  *  - head_dim 64 or 128; page_size a power of two from 16 to 256; pages of WC_F32 or WC_BF16;
  *    16-byte aligned pointers and strides, no stride of zero.
@@ -439,7 +440,9 @@ typedef struct {
 } wc_paged_attention_args;
 /* out = softmax(scale q K^T + mask) V for every row: over all keys of the group's prefix, the request's
  * keys before its new rows, and the new rows that the mask shows. A row that sees nothing gives 0.
- * Sums and softmax statistics are fp32; bf16 pages: weights rounded to bf16 for the second product. */
+ * Sums and softmax statistics are fp32; bf16 pages: weights rounded to bf16 for the second product (at
+ * most 2^-8 of each; wc_attention keeps them as two bf16 terms). The kernel follows from rows / requests
+ * over the whole call: where a few requests have most rows, a call of their own is faster. */
 WC_API wc_status wc_paged_attention(wc_ctx* ctx, void* stream, const wc_paged_attention_args* args);
 /* Bytes of workspace that wc_paged_attention needs for these arguments (buffers are not looked at). */
 WC_API wc_status wc_paged_attention_workspace(wc_ctx* ctx, const wc_paged_attention_args* args, uint64_t* bytes);

@@ -281,7 +281,10 @@ struct Launch {
 // with parts of one tile, 24.8 with least 4, 29.0 with 8; one decoding step alone: 12.8, 13.2, 15.3).
 // bf16, 64 requests: 16 rows 168 us on the streamed kernel and 184 on tensor memory at 4000 keys, 35
 // and 50 at 300; 18 rows 211 and 172 at 4000 keys, 77 and 70 at 1000, 42 and 48 at 300 (the streamed
-// kernel then in a 32-row form, since removed).
+// kernel then in a 32-row form, since removed). All of these are uniform batches; the mean tells little of
+// one that mixes: 255 steps over 2000 keys 343 us, one chunk of 1024 rows over 8192 keys 89 us (256-row
+// tiles), both in one call (mean 10 a head) 868 us, the chunk among 255 idle slots 489 us; 63 steps 97 us,
+// with the chunk (mean 34, 128-row tiles) 165 us.
 Launch plan_launch(const wc_ctx* ctx, const wc_pages& g, long long rows, bool prefixes) {
   Launch l;
   l.least = 1;

@@ -107,7 +107,7 @@ __device__ __forceinline__ void unpack8(const Raw8<uint16_t>& r, float (&x)[8]) 
 // One block per row; D / 16 lanes share a head, eight pairs each. Bound by HBM on prompts (each value is
 // read once and written once), by the chain request -> length -> page -> store on single rows: the
 // first heads' values are on their way before that chain begins, and the next heads' while one step's
-// are turned. 10.4 thousand prompt rows of 48 heads: 65 us, 4.9 TB/s, the issue slots 64% used (77 us
+// are turned. 13.0 thousand prompt rows of 48 heads: 65 us, 4.9 TB/s, the issue slots 64% used (77 us
 // without the early loads; 256 threads a block 105 us); 64 single rows: 3.9 us.
 template <typename S, typename P, int D>
 __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_constant__ PagedAppendParams p) {
@@ -204,7 +204,10 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_c
 // Rows start + keep[i] -> start + i of every layer, new length start + n_keep. keep is strictly
 // increasing from keep[0] >= 0 (checked), so keep[i] >= i: each thread moves one 16-byte column
 // chunk of all rows in order, up to eight rows read before they are written, and a row is read
-// before any later step overwrites it. 64 paths of 5 over 28 layers: 13.8 us, 4.3 TB/s of 256-byte rows.
+// before any later step overwrites it. 64 paths of 5 over 28 layers: 13.8 us, 4.3 TB/s:
+// 1792 blocks of 54 registers a thread are three waves, and each walks the chain start -> list -> page
+// -> row anew (profile: DRAM at 23% of nominal, 43% of the warps; stalls on that chain, the barrier and
+// the lists in shared memory).
 constexpr int PC_THREADS = 256;
 constexpr int PC_MAXKEEP = 64;
 
@@ -1072,8 +1075,9 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         clean = !__any_sync(0xffffffffu, worst == 0x7f800000u);
       }
       if (clean) {
-        // ---- O += P V; the weights are rounded to bf16, as the values are: relative 2^-9 each, the
-        // size of the output's own rounding
+        // ---- O += P V; the weights are rounded to bf16, as the values are: at most 2^-8 of each, as much
+        // as the output's own rounding. The row's sum takes them unrounded. Two bf16 terms, as the
+        // contiguous kernels keep, would double this product.
         const uint32_t a[4] = {pack_bf16(sc[0][0], sc[0][1]), pack_bf16(sc[0][2], sc[0][3]),
                                pack_bf16(sc[1][0], sc[1][1]), pack_bf16(sc[1][2], sc[1][3])};
 #pragma unroll
@@ -1664,7 +1668,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1)
               const float y = ex2_approx(fmaf(__uint_as_float(v[2 * j + 1]), sl2, -mg));
               sum[(j & 1) * 2] += x;
               sum[(j & 1) * 2 + 1] += y;
-              pk[j] = pack_bf16(x, y);  // weights rounded to bf16, as the values are (2^-9 of each)
+              pk[j] = pack_bf16(x, y);  // rounded to bf16, as the values are: at most 2^-8 of each, whatever m
             }
             tmem_st16u(ts + c / 2, pk);  // over scores that both passes have read
           }

@@ -13,13 +13,14 @@ python/woodcock/target.py:159-175); a server keeps many requests' keys and value
   are left alone.
 * Tables, lengths and offsets stay on the device, so a captured CUDA graph can be replayed on new
   contents (make one call before the capture). A page number outside the pool (its keys and values read
-  as zeros), a length beyond its table (cut to it) or a row with no slot (dropped) is never followed;
-  it raises the context's device error word (``Context.get(device).synchronize()`` after the
-  stream's work raises WcError).
+  as zeros), a length beyond its table (cut to it) or a row with no slot (its k and v are dropped) is never
+  followed; it raises the context's device error word (``Context.get(device).synchronize()`` after
+  the stream's work raises WcError).
 * Work runs on the caller's current stream of the tensors' device, in its order; scratch comes from
   PyTorch's allocator for that one call. What a call writes (its output, the pages of append and
   compact) must not overlap what it reads, nor itself: refused with ValueError. K and V may be cut from
-  one buffer (halves, or side by side in a page, a head or a row).
+  one buffer (halves, or side by side in a page, a head or a row). Several threads may call these
+  operators at once, each with buffers of its own.
 """
 
 from __future__ import annotations
@@ -233,8 +234,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     verification chains, draft trees and prompts may share a call. New row i of a request sees the keys
     before the new rows and new rows 0..i; with ``tree_mask`` (int64 [rows], at most 64 new rows a
     request) those new rows whose bit is set. A row that sees nothing gives 0; masked places may hold
-    anything, NaN and infinities included. Statistics and sums are fp32. scale: positive, default
-    head_dim ** -0.5."""
+    anything, NaN and infinities included. Statistics and sums are fp32; with bf16 pages the softmax
+    weights are rounded to bf16 once (at most 2^-8 of each; ops.attention, which takes and returns fp32,
+    keeps two bf16 terms). scale: positive, default head_dim ** -0.5.
+
+    The kernel follows from rows / requests over the whole call, so where a few prompts have most of the
+    rows and steps most of the requests, one call for each kind is faster than one for both."""
     return _attend(q, k_pages, v_pages, None, page_table, kv_lens, q_offsets, tree_mask, scale, out)
 
 
