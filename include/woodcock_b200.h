@@ -464,6 +464,102 @@ typedef struct {
  * share the pages that their moved rows lie in. */
 WC_API wc_status wc_paged_compact(wc_ctx* ctx, void* stream, const wc_paged_compact_args* args);
 
+/* The attention weight that each key gathers: fp32 [pages][kv_heads][page_size] (any strides, rows contiguous)
+ * beside the pages, in the same page order. */
+typedef struct {
+  float* p;
+  int64_t stride[3]; /* layer, page, head; in elements */
+} wc_mass;
+
+typedef struct {
+  wc_pages pages; /* v is not looked at */
+  wc_paged_batch batch;
+  const void* q; /* [rows][heads][head_dim] of the pages' dtype */
+  int64_t q_stride[2];
+  wc_mass mass;
+  void* workspace; /* 256-byte aligned; used by this call alone until its work is done */
+  uint64_t workspace_bytes;
+  float scale;
+  int layer, add;
+} wc_paged_mass_args;
+/* mass[b][kv head][key] = was + the sum over request b's new rows and the kv head's query heads of
+ * softmax(scale q K^T)[key]: the weights of wc_paged_attention without a tree. A row gives each key that
+ * it sees its weight, one that sees nothing none. `was` is what the key gathered before; 0 for the keys
+ * that are new in this call (the request's last ones, one for each of its rows), and for all of them where
+ * `add` is 0. Statistics and sums are fp32, added in the same order every time. Requests must not share
+ * pages; where their keys are far more than the pool holds, nothing is written and the device error word is
+ * raised. The pages themselves are only read. */
+WC_API wc_status wc_paged_mass(wc_ctx* ctx, void* stream, const wc_paged_mass_args* args);
+/* Bytes of workspace that wc_paged_mass needs for these arguments (buffers are not looked at). */
+WC_API wc_status wc_paged_mass_workspace(wc_ctx* ctx, const wc_paged_mass_args* args, uint64_t* bytes);
+
+typedef struct {
+  wc_pages pages; /* every layer */
+  wc_mass mass;
+  const int* page_table;
+  int64_t table_stride;
+  int table_cols, requests;
+  const int* kv_lens; /* [requests], alike in all layers */
+  const int* budgets; /* [requests] or NULL: `budget` for each */
+  int* lens_out;      /* [requests]: min(kv_lens, budget) */
+  void* workspace;
+  uint64_t workspace_bytes;
+  int budget, sinks, recent;
+} wc_paged_evict_args;
+/* Where a request has more keys than its budget, each layer and kv head keeps `budget` of them: the first
+ * `sinks`, the last `recent`, and of those between the ones of the largest mass (ties: the lower key; a mass
+ * that is no number ranks last). They move to keys 0 .. budget - 1 in their order, with their mass; what
+ * lies behind is left as it was. A request whose budget is below sinks + recent, whose length is beyond its
+ * table or one of whose pages is outside the pool keeps its rows and its length, and raises the device
+ * error word. Requests must not share pages. */
+WC_API wc_status wc_paged_evict(wc_ctx* ctx, void* stream, const wc_paged_evict_args* args);
+/* Bytes of workspace that wc_paged_evict needs for these arguments (buffers are not looked at; with `budgets`
+ * the table's capacity stands for the largest). */
+WC_API wc_status wc_paged_evict_workspace(wc_ctx* ctx, const wc_paged_evict_args* args, uint64_t* bytes);
+
+/* ------------------------------------------------------------------ beam search
+ * (no counterpart in the reference, which keeps one continuation per request.) As for the paged operators:
+ * the caller owns every buffer, work is enqueued on `stream`, device memory may change between replays
+ * of a captured graph. */
+typedef struct {
+  const void* logits; /* [requests][beams][vocab], tokens contiguous */
+  int64_t request_stride, beam_stride; /* in elements */
+  const float* scores;     /* [requests][beams]: the beams' log probabilities; -inf: a dead beam */
+  const uint8_t* finished; /* [requests][beams], 1: the beam has ended; or NULL */
+  float* out_scores;       /* [requests][n], best first */
+  int *out_parents, *out_tokens;
+  void* workspace;
+  uint64_t workspace_bytes;
+  int dtype, requests, beams, vocab, n, pad;
+} wc_beam_select_args;
+/* The n best continuations of each request over its beams and the vocabulary, by
+ * scores[w] + log_softmax(logits[w])[token], ties to the lower beam, then to the lower token; ranked in 64 bits,
+ * given in 32. A beam that has ended offers itself alone, with its score and token `pad`; a token at -inf,
+ * a dead beam and a beam of which nothing is left offer nothing. Places for which no candidate is left hold
+ * score -inf, parent 0, token 0. A beam with a logit (where they are looked at) or score that is NaN or +inf
+ * offers nothing and raises the device error word. n and beams at most 64, beams x vocab below 2^31. */
+WC_API wc_status wc_beam_select(wc_ctx* ctx, void* stream, const wc_beam_select_args* args);
+WC_API wc_status wc_beam_select_workspace(wc_ctx* ctx, const wc_beam_select_args* args, uint64_t* bytes);
+
+typedef struct {
+  wc_pages pages;
+  const int* page_table; /* [requests * beams][table_cols]: every beam is a request of the paged operators */
+  int64_t table_stride;
+  int table_cols, requests, beams;
+  const int* kv_lens; /* [requests * beams], alike for the beams of a request */
+  const int* parents; /* [requests][beams]: the beam that each beam continues from now on */
+  int* table_out;     /* [requests * beams][table_cols], rows out_stride ints apart */
+  int64_t out_stride;
+} wc_beam_reorder_args;
+/* Every beam takes over its parent's keys, in every layer. Full pages are shared: table_out names the parent's.
+ * The page that is being filled must be another one for each beam: the first child of a parent (the lowest
+ * beam) keeps it; the request's i-th further child gets the page of the i-th beam without a child, and the
+ * filled rows are copied there. Pages behind it stay with their beams. Lengths stay as they are. A request
+ * with a parent out of range, beams of unequal length, a length beyond the table, or a page being filled
+ * that is outside the pool or in two beams' tables is left as it is (its table copied) and raises the device
+ * error word. Beams at most 64. */
+WC_API wc_status wc_beam_reorder(wc_ctx* ctx, void* stream, const wc_beam_reorder_args* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -139,6 +139,13 @@ SIGNATURES = {
     "wc_paged_attention": (S, [P, P, P]),
     "wc_paged_attention_workspace": (S, [P, P, C.POINTER(C.c_uint64)]),
     "wc_paged_compact": (S, [P, P, P]),
+    "wc_paged_mass": (S, [P, P, P]),
+    "wc_paged_mass_workspace": (S, [P, P, C.POINTER(C.c_uint64)]),
+    "wc_paged_evict": (S, [P, P, P]),
+    "wc_paged_evict_workspace": (S, [P, P, C.POINTER(C.c_uint64)]),
+    "wc_beam_select": (S, [P, P, P]),
+    "wc_beam_select_workspace": (S, [P, P, C.POINTER(C.c_uint64)]),
+    "wc_beam_reorder": (S, [P, P, P]),
     "wc_decoder_save_state": (S, [P]),
     "wc_decoder_restore_state": (S, [P]),
     "wc_decoder_round_logits": (S, [P, C.c_int, P, P, I32P, C.POINTER(C.c_uint64)]),

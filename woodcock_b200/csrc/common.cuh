@@ -21,7 +21,9 @@ enum DeviceError : int {
   kErrTree = 16,          // malformed tree (parent >= child)
   kErrTimeout = 32,       // a bounded wait (mbarrier / pipeline) expired
   kErrSample = 64,        // a sampled draw found no token with positive probability
-  kErrPage = 128,         // a page table entry outside the pool
+  kErrPage = 128,         // a page table entry outside the pool, or a page in two places that are written
+  kErrLogits = 256,       // a logit or score that is no number
+  kErrBudget = 512,       // a budget below what is protected
 };
 
 __device__ __forceinline__ void raise_error(int* err, int bit) {

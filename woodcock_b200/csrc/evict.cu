@@ -1,0 +1,234 @@
+// Entry points of the gathered attention weight and of the eviction by it: argument checks, workspace layout
+// and launches of the kernels in evict.cuh.
+#include <cmath>
+#include <cstring>
+
+#include "evict.cuh"
+#include "paged_host.h"
+
+using namespace wc;
+
+namespace {
+
+// The mass of one layer's keys (layer >= 0), or of all layers'.
+Strided mass_places(const wc_pages& g, const wc_mass& m, int layer) {
+  Strided s;
+  s.at = reinterpret_cast<uintptr_t>(m.p) + (layer > 0 ? m.stride[0] * layer * 4 : 0);
+  s.run = g.page_size * 4ll;
+  if (layer < 0) s.add(g.layers, m.stride[0] * 4);
+  s.add(g.pages, m.stride[1] * 4);
+  s.add(g.kv_heads, m.stride[2] * 4);
+  s.close();
+  return s;
+}
+
+void check_mass(const wc_pages& g, const wc_mass& m) {
+  need(m.p != nullptr && reinterpret_cast<uintptr_t>(m.p) % 4 == 0, "paged: null or misaligned mass");
+  const int sizes[3] = {g.layers, g.pages, g.kv_heads};
+  for (int i = 0; i < 3; ++i) need(sizes[i] == 1 || m.stride[i] > 0, "paged: mass pages must not overlap");
+}
+
+wc_pages keys_only(wc_pages g) {
+  g.v = g.k;
+  std::memcpy(g.v_stride, g.k_stride, sizeof(g.v_stride));
+  return g;
+}
+
+struct MassLayout {
+  int blocks;
+  size_t row_ml, part_ml, rec, tiles, bytes;
+};
+
+MassLayout mass_layout(const wc_ctx* ctx, const wc_paged_mass_args& a) {
+  const wc_paged_batch& b = a.batch;
+  MassLayout l;
+  std::memset(&l, 0, sizeof(l));
+  size_t at = 0;
+  l.blocks = ctx->num_sms * 2;
+  l.row_ml = take(at, size_t(b.rows) * b.heads * sizeof(float2));
+  l.part_ml = take(at, size_t(l.blocks) * 2 * MS_M * sizeof(float2));
+  l.rec = take(at, l.blocks * sizeof(PagedRec));
+  l.tiles = take(at, (size_t(b.requests) + 1) * sizeof(long long));
+  l.bytes = at;
+  return l;
+}
+
+void check_mass_args(const wc_paged_mass_args& a) {
+  check_pages(keys_only(a.pages));
+  check_batch(a.pages, a.batch);
+  need(a.layer >= 0 && a.layer < a.pages.layers, "paged_mass: layer out of range");
+  need(std::isfinite(a.scale) && a.scale > 0, "paged_mass: scale must be positive");
+}
+
+template <typename S, int D>
+void gather_mass(wc_ctx* ctx, cudaStream_t st, const MassParams& p) {
+  opt_in(ctx, mass_rows_kernel<S, D>, mass_simt_smem<D>());
+  opt_in(ctx, mass_keys_kernel<S, D>, mass_simt_smem<D>());
+  launch_on(ctx, st, "mass_rows", mass_rows_kernel<S, D>, dim3(p.blocks), dim3(MS_THREADS), mass_simt_smem<D>(), true, 1, p);
+  launch_on(ctx, st, "mass_join", mass_join_kernel<MS_M, MS_KT>, dim3(p.blocks + 1), dim3(256), 0, true, 1, p);
+  launch_on(ctx, st, "mass_keys", mass_keys_kernel<S, D>, dim3(ctx->num_sms * 2), dim3(MS_THREADS), mass_simt_smem<D>(),
+            true, 1, p);
+}
+
+}  // namespace
+
+extern "C" wc_status wc_paged_mass_workspace(wc_ctx* ctx, const wc_paged_mass_args* a, uint64_t* bytes) {
+  if (!ctx || !a || !bytes) return WC_ERR_INVALID;
+  return guard(ctx, [&] {
+    check_mass_args(*a);
+    *bytes = mass_layout(ctx, *a).bytes;
+  });
+}
+
+extern "C" wc_status wc_paged_mass(wc_ctx* ctx, void* stream, const wc_paged_mass_args* a) {
+  if (!ctx || !a) return WC_ERR_INVALID;
+  return guard(ctx, [&] {
+    check_mass_args(*a);
+    const wc_pages g = keys_only(a->pages);
+    const wc_paged_batch& b = a->batch;
+    check_mass(g, a->mass);
+    if (b.rows == 0) return;
+    check_rows(a->q, a->q_stride, g.dtype, "paged_mass: q must be 16-byte aligned, rows contiguous");
+    const MassLayout l = mass_layout(ctx, *a);
+    if (!a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 256 || a->workspace_bytes < l.bytes)
+      fail(WC_ERR_CAPACITY, "paged_mass: workspace missing, misaligned or too small");
+    const Run scratch{a->workspace, (long long)l.bytes},
+        q = rows_run(a->q, a->q_stride, g.dtype, b.rows, b.heads, g.head_dim),
+        table = table_run(b.page_table, b.table_stride, b.table_cols, b.requests), lens = ints_run(b.kv_lens, b.requests),
+        offsets = ints_run(b.q_offsets, b.requests + 1ll);
+    check_apart(scratch, {q, table, lens, offsets}, "paged_mass: the workspace must not overlap an input");
+    const Strided K = places(g, g.k, g.k_stride, a->layer), mass = mass_places(g, a->mass, a->layer);
+    need(mass.nested, "paged: mass pages must not overlap");
+    need(!meets(K, mass), "paged_mass: mass must not overlap the pages");
+    need(!meets_run(K, scratch.p, scratch.bytes), "paged_mass: the workspace must not overlap the pages");
+    for (const Run& x : {scratch, q, table, lens, offsets})
+      need(!meets_run(mass, x.p, x.bytes), "paged_mass: mass must not overlap the workspace or an input");
+    DeviceScope scope(ctx->device);
+    char* ws = static_cast<char*>(a->workspace);
+    MassParams p;
+    std::memset(&p, 0, sizeof(p));
+    p.a.q = a->q;
+    p.a.q_row = a->q_stride[0];
+    p.a.q_head = a->q_stride[1];
+    p.a.K = pool(g, g.k, g.k_stride, a->layer);
+    p.a.pages = g.pages;
+    p.a.page_log2 = log2i(g.page_size);
+    p.a.table = b.page_table;
+    p.a.table_ld = int(b.table_stride);
+    p.a.table_cols = b.table_cols;
+    p.a.lens = b.kv_lens;
+    p.a.offsets = b.q_offsets;
+    p.a.T = b.rows;
+    p.a.B = b.requests;
+    p.a.H = b.heads;
+    p.a.Hk = g.kv_heads;
+    p.a.rep = b.heads / g.kv_heads;
+    p.a.scale_log2 = a->scale * kLog2e;
+    p.a.rec = reinterpret_cast<PagedRec*>(ws + l.rec);
+    p.a.err = ctx->d_err;
+    p.mass = {a->mass.p + a->mass.stride[0] * a->layer, a->mass.stride[0], a->mass.stride[1], a->mass.stride[2]};
+    p.add = a->add;
+    p.row_ml = reinterpret_cast<float2*>(ws + l.row_ml);
+    p.part_ml = reinterpret_cast<float2*>(ws + l.part_ml);
+    p.tiles = reinterpret_cast<long long*>(ws + l.tiles);
+    p.blocks = l.blocks;
+    const cudaStream_t st = stream_of(ctx, stream);
+    if (g.dtype == WC_BF16) {
+      if (g.head_dim == 64) gather_mass<uint16_t, 64>(ctx, st, p);
+      else gather_mass<uint16_t, 128>(ctx, st, p);
+    } else {
+      if (g.head_dim == 64) gather_mass<float, 64>(ctx, st, p);
+      else gather_mass<float, 128>(ctx, st, p);
+    }
+  });
+}
+
+// ============================================================================ eviction
+
+namespace {
+
+void check_evict_args(const wc_paged_evict_args& a) {
+  check_pages(a.pages);
+  check_table(a.page_table, a.table_stride, a.table_cols, a.pages.page_size, "paged_evict: bad page table");
+  need(a.requests > 0 && a.requests < (1 << 24), "paged_evict: bad request count");
+  need(a.sinks >= 0 && a.recent >= 0 && a.sinks < (1 << 30) && a.recent < (1 << 30), "paged_evict: negative sinks or recent");
+  need(a.budgets || a.budget >= a.sinks + a.recent, "paged_evict: budget below sinks + recent");
+  need((long long)a.pages.layers * a.requests * a.pages.kv_heads < (1ll << 31), "paged_evict: batch too large");
+}
+
+int evict_most(const wc_paged_evict_args& a) {
+  const int cap = a.table_cols * a.pages.page_size;
+  return a.budgets ? cap : std::min(cap, a.budget);
+}
+
+}  // namespace
+
+extern "C" wc_status wc_paged_evict_workspace(wc_ctx* ctx, const wc_paged_evict_args* a, uint64_t* bytes) {
+  if (!ctx || !a || !bytes) return WC_ERR_INVALID;
+  return guard(ctx, [&] {
+    check_evict_args(*a);
+    *bytes = uint64_t(a->pages.layers) * a->requests * a->pages.kv_heads * (evict_most(*a) + 1) * sizeof(int);
+  });
+}
+
+extern "C" wc_status wc_paged_evict(wc_ctx* ctx, void* stream, const wc_paged_evict_args* a) {
+  if (!ctx || !a) return WC_ERR_INVALID;
+  return guard(ctx, [&] {
+    const wc_pages& g = a->pages;
+    check_evict_args(*a);
+    check_mass(g, a->mass);
+    need(a->kv_lens && a->lens_out, "paged_evict: null kv_lens or lens_out");
+    const int most = evict_most(*a);
+    const long long lists = (long long)g.layers * a->requests * g.kv_heads;
+    const long long bytes = lists * (most + 1) * (long long)sizeof(int);
+    if (!a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 256 || a->workspace_bytes < uint64_t(bytes))
+      fail(WC_ERR_CAPACITY, "paged_evict: workspace missing, misaligned or too small");
+    const Strided K = places(g, g.k, g.k_stride, -1), V = places(g, g.v, g.v_stride, -1), mass = mass_places(g, a->mass, -1);
+    check_written(K, V);
+    need(mass.nested, "paged: mass pages must not overlap");
+    need(!meets(K, mass) && !meets(V, mass), "paged_evict: mass must not overlap the pages");
+    const Run scratch{a->workspace, bytes}, out = ints_run(a->lens_out, a->requests),
+              table = table_run(a->page_table, a->table_stride, a->table_cols, a->requests),
+              lens = ints_run(a->kv_lens, a->requests), budgets = ints_run(a->budgets, a->requests);
+    check_apart(out, {table, lens, budgets, scratch}, "paged_evict: lens_out must not overlap an input or the workspace");
+    check_apart(scratch, {table, lens, budgets}, "paged_evict: the workspace must not overlap an input");
+    check_pages_apart(K, V, {out, table, lens, budgets, scratch},
+                      "paged_evict: the pages must not overlap lens_out, the workspace or an input");
+    for (const Run& x : {out, table, lens, budgets, scratch})
+      need(!meets_run(mass, x.p, x.bytes), "paged_evict: mass must not overlap lens_out, the workspace or an input");
+    DeviceScope scope(ctx->device);
+    EvictParams p;
+    std::memset(&p, 0, sizeof(p));
+    p.K = pool(g, g.k, g.k_stride, 0);
+    p.V = pool(g, g.v, g.v_stride, 0);
+    p.k_layer = g.k_stride[0];
+    p.v_layer = g.v_stride[0];
+    p.mass = {a->mass.p, a->mass.stride[0], a->mass.stride[1], a->mass.stride[2]};
+    p.pages = g.pages;
+    p.page_log2 = log2i(g.page_size);
+    p.B = a->requests;
+    p.Hk = g.kv_heads;
+    p.layers = g.layers;
+    p.esize_log2 = g.dtype == WC_BF16 ? 1 : 2;
+    p.row_chunks = (g.head_dim << p.esize_log2) / 16;
+    p.table = a->page_table;
+    p.table_ld = int(a->table_stride);
+    p.table_cols = a->table_cols;
+    p.lens = a->kv_lens;
+    p.budgets = a->budgets;
+    p.budget = a->budget;
+    p.sinks = a->sinks;
+    p.recent = a->recent;
+    p.lens_out = a->lens_out;
+    p.list = static_cast<int*>(a->workspace);
+    p.most = most;
+    p.cache = std::min(a->table_cols * g.page_size, EV_CACHE);
+    p.splits = 1;
+    p.err = ctx->d_err;
+    const cudaStream_t st = stream_of(ctx, stream);
+    opt_in(ctx, evict_select_kernel, EV_CACHE * sizeof(float));
+    launch_on(ctx, st, "evict_select", evict_select_kernel, dim3(unsigned(lists)), dim3(EV_THREADS), p.cache * sizeof(float),
+              true, 1, p);
+    launch_on(ctx, st, "evict_move", evict_move_kernel, dim3(unsigned(lists), 2 * p.splits), dim3(EM_THREADS), 0, true, 1, p);
+  });
+}

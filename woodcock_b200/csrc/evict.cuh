@@ -1,0 +1,502 @@
+// Keys that a long session keeps: the attention weight that each key gathers, and the eviction of those
+// that gather least.
+#pragma once
+
+#include "common.cuh"
+#include "paged_walk.cuh"
+
+namespace wc {
+
+// The gathered weight of each key, fp32 [pages][kv_heads][page_size] beside the pages, rows contiguous.
+struct MassPool {
+  float* ptr;
+  long long layer, page, head;
+};
+
+// ---------------------------------------------------------------------------- the weight a key gathers
+// mass_j (+)= sum over new rows i and query heads h of the key's head of p_ih(j),
+// p_ih(j) = 2^(s_ih(j) - M_ih) / L_ih over the keys that row i sees. A weight needs its row's maximum and sum
+// over all keys first, so the scores are needed twice.
+struct MassParams {
+  PagedAttnParams a;     // q, K pages, batch
+  MassPool mass;
+  int add;               // 0: the sums of all keys start anew
+  // workspace
+  float2* row_ml;        // [T][H]: maximum (log2 units) and 1 / sum
+  float2* part_ml;       // [blocks][2][16]: of divided items
+  long long* tiles;      // [B + 1]: key tiles before each request (all of its heads')
+  int blocks;            // of the statistics' launch
+};
+
+// What a weight is before the sums are joined: rows that see nothing keep 0.
+__device__ __forceinline__ float2 mass_row(float m, float l) {
+  return make_float2(m == -INFINITY ? 0.f : m, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l));
+}
+
+// The first kernel's scores, one row tile against one key tile: 16 rows x 64 keys, a key and four rows a
+// thread. qs [16][D], ks [64][D + 4].
+template <int D>
+__device__ __forceinline__ void mass_scores(const float* qs, const float* ks, int sk, int sr, float (&s)[4]) {
+#pragma unroll 8
+  for (int d = 0; d < D; d += 4) {
+    const float4 k4 = *reinterpret_cast<const float4*>(ks + sk * (D + 4) + d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 q4 = *reinterpret_cast<const float4*>(qs + (sr + i) * D + d);
+      s[i] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, s[i]))));
+    }
+  }
+}
+
+constexpr int MS_THREADS = 256, MS_M = 16, MS_KT = 64;
+
+template <typename S, int D>
+__device__ __forceinline__ void mass_load_q(const PagedAttnParams& p, const PagedSeg& g, int head, int rho0, float* qs) {
+  for (int c = threadIdx.x; c < MS_M * (D / 8); c += MS_THREADS) {
+    const int m = c / (D / 8), col = (c % (D / 8)) * 8;
+    const PagedRow r = paged_row(p, g, head, rho0 + m);
+    float x[8] = {};
+    if (r.valid) load8(static_cast<const S*>(p.q) + r.tok * p.q_row + r.h * p.q_head + col, x);
+    store8(qs + m * D + col, x);
+  }
+}
+template <typename S, int D>
+__device__ __forceinline__ void mass_load_k(const PagedAttnParams& p, const PagedSeg& g, int head, int kt, float* ks) {
+  for (int c = threadIdx.x; c < MS_KT * (D / 8); c += MS_THREADS) {
+    const int kr = c / (D / 8), cc = (c % (D / 8)) * 8, key = kt * MS_KT + kr;
+    float x[8] = {};
+    const int page = key < g.klen ? paged_page(p, g, key >> p.page_log2) : -1;
+    if (page >= 0)
+      load8(static_cast<const S*>(p.K.ptr) + page * p.K.page + head * p.K.head +
+                (key & ((1 << p.page_log2) - 1)) * p.K.row + cc, x);
+    store8(ks + kr * (D + 4) + cc, x);
+  }
+}
+
+template <int D>
+constexpr size_t mass_simt_smem() {
+  return sizeof(float) * (size_t(MS_KT) * (D + 4) + MS_M * D + MS_M * (MS_KT + 4)) + 8 * kWalkShared;
+}
+
+// Every row's maximum and sum, on the CUDA cores. Items as in paged attention; a divided one leaves its parts.
+template <typename S, int D>
+__global__ void __launch_bounds__(MS_THREADS) mass_rows_kernel(const __grid_constant__ MassParams mp) {
+  const PagedAttnParams& p = mp.a;
+  constexpr int M = MS_M, KT = MS_KT, LS = KT + 4;
+  extern __shared__ __align__(16) float ms_smem[];
+  float* ks = ms_smem;
+  float* qs = ks + KT * (D + 4);
+  float* ss = qs + M * D;
+  long long* sh = reinterpret_cast<long long*>(ss + M * LS);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_wait();
+  pdl_launch_dependents();
+  PagedWalk<M, KT, 1> w;
+  paged_no_rec(p);
+  if (!w.begin(p, kOwnRows, 1, sh)) return;
+  do {
+    __syncthreads();
+    mass_load_q<S, D>(p, w.g, w.head, w.qt * M, qs);
+    const int sk = tid & 63, sr = (tid >> 6) * 4;
+    PagedRow rows[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) rows[i] = paged_row(p, w.g, w.head, w.qt * M + 2 * warp + i);
+    float m2[2] = {-INFINITY, -INFINITY}, l2[2] = {0.f, 0.f};
+    for (int kt = w.kt0; kt < w.kt1; ++kt) {
+      __syncthreads();
+      mass_load_k<S, D>(p, w.g, w.head, kt, ks);
+      __syncthreads();
+      float s[4] = {};
+      mass_scores<D>(qs, ks, sk, sr, s);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ss[(sr + i) * LS + sk] = s[i];
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float z[2], mx = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          z[h] = ss[(2 * warp + i) * LS + lane + 32 * h] * p.scale_log2;
+          if (!rows[i].sees(kt * KT + lane + 32 * h)) z[h] = -INFINITY;
+          mx = fmaxf(mx, z[h]);
+        }
+        mx = fmaxf(warp_max(mx), m2[i]);
+        const float mg = mx == -INFINITY ? 0.f : mx;
+        l2[i] = l2[i] * exp2f(m2[i] - mg) + warp_sum(exp2f(z[0] - mg) + exp2f(z[1] - mg));
+        m2[i] = mx;
+      }
+    }
+    if (tid == 0) w.report(p);
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (!rows[i].valid) continue;
+        if (w.count == 1) mp.row_ml[(long long)rows[i].tok * p.H + rows[i].h] = mass_row(m2[i], l2[i]);
+        else mp.part_ml[((long long)blockIdx.x * 2 + w.slot()) * M + 2 * warp + i] = make_float2(m2[i], l2[i]);
+      }
+    }
+  } while (w.next(p, kOwnRows));
+}
+
+// Key tiles of requests that share no pages, at most.
+__host__ __device__ __forceinline__ long long mass_most_tiles(int pages, int page_log2, int B, int Hk, int KT) {
+  return (((long long)pages << page_log2) / KT + B) * Hk;
+}
+
+// Joins the parts of divided items, one block an item and a warp a row; the last block counts the key tiles
+// before each request.
+template <int M, int KT>
+__global__ void __launch_bounds__(256) mass_join_kernel(const __grid_constant__ MassParams mp) {
+  const PagedAttnParams& p = mp.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_wait();
+  pdl_launch_dependents();
+  if (int(blockIdx.x) == mp.blocks) {
+    __shared__ long long sums[8];
+    long long base = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 256) {
+      const int b = b0 + tid;
+      long long w = 0;
+      if (b < p.B) {
+        const PagedSeg g = paged_seg(p, kOwnRows, b);
+        if (g.n > 0) w = (long long)((g.klen + KT - 1) / KT) * p.Hk;
+      }
+      long long x = w;
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const long long y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      if (lane == 31) sums[warp] = x;
+      __syncthreads();
+      long long before = base;
+      for (int i = 0; i < 8; ++i) {
+        if (i < warp) before += sums[i];
+        base += sums[i];
+      }
+      if (b < p.B) mp.tiles[b] = before + x - w;
+      __syncthreads();
+    }
+    if (tid == 0) {
+      // more than the pool holds: requests share pages, whose sums two blocks would write
+      const bool shared = base > mass_most_tiles(p.pages, p.page_log2, p.B, p.Hk, KT);
+      if (shared) raise_error(p.err, kErrPage);
+      mp.tiles[p.B] = shared ? 0 : base;
+    }
+    return;
+  }
+  const PagedRec rec = p.rec[blockIdx.x];
+  if (rec.count == 0) return;
+  for (int r = warp; r < M; r += 8) {
+    const int rho = rec.qt * M + r;
+    if (rho >= rec.rows) break;
+    float m = -INFINITY, l = 0.f;
+    for (int i = lane; i < rec.count; i += 32) {
+      const float2 y = mp.part_ml[((long long)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * M + r];
+      const float mn = fmaxf(m, y.x), mg = mn == -INFINITY ? 0.f : mn;
+      l = l * exp2f(m - mg) + y.y * exp2f(y.x - mg);
+      m = mn;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
+      const float mn = fmaxf(m, m2), mg = mn == -INFINITY ? 0.f : mn;
+      l = l * exp2f(m - mg) + l2 * exp2f(m2 - mg);
+      m = mn;
+    }
+    if (lane == 0) {
+      const int i = rho / p.rep;
+      mp.row_ml[(long long)(rec.tok0 + i) * p.H + rec.head * p.rep + rho - i * p.rep] = mass_row(m, l);
+    }
+  }
+}
+
+// The request whose tiles hold tile `at` (warp-collective; tiles[] ascends, tiles[B] is above `at`).
+__device__ __forceinline__ int mass_request(const long long* tiles, int B, long long at, int lane) {
+  int lo = 0, hi = B;  // tiles[lo] <= at < tiles[hi]
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32, i = min(lo + (lane + 1) * step, hi);
+    const uint32_t above = __ballot_sync(0xffffffffu, tiles[i] > at);
+    const int f = __ffs(above) - 1;  // lane 31's is hi at the latest
+    const int nhi = min(lo + (f + 1) * step, hi);
+    lo = lo + f * step;
+    hi = nhi;
+  }
+  return lo;
+}
+
+// Sums over the rows, a key tile and head at a time: every row tile that sees the keys, in order.
+template <typename S, int D>
+__global__ void __launch_bounds__(MS_THREADS) mass_keys_kernel(const __grid_constant__ MassParams mp) {
+  const PagedAttnParams& p = mp.a;
+  constexpr int M = MS_M, KT = MS_KT;
+  extern __shared__ __align__(16) float ms_smem[];
+  float* ks = ms_smem;
+  float* qs = ks + KT * (D + 4);
+  float* ss = qs + M * D;  // [4][KT]
+  __shared__ float2 ml[M];
+  __shared__ int lim[M];
+  const int tid = threadIdx.x, lane = tid & 31;
+  pdl_wait();
+  pdl_launch_dependents();
+  const long long total = mp.tiles[p.B];
+  const int sk = tid & 63, sr = (tid >> 6) * 4;
+  for (long long at = blockIdx.x; at < total; at += gridDim.x) {
+    const int b = mass_request(mp.tiles, p.B, at, lane);
+    const PagedSeg g = paged_seg(p, kOwnRows, b);
+    const int nt = (g.klen + KT - 1) / KT;
+    const int head = int((at - mp.tiles[b]) / nt), kt = int((at - mp.tiles[b]) - (long long)head * nt);
+    __syncthreads();
+    mass_load_k<S, D>(p, g, head, kt, ks);
+    const int key = kt * KT + sk, rows = g.n * p.rep;
+    // the first row that sees the tile's first key
+    const int first = max(0, kt * KT - (g.klen - g.n)) * p.rep / M * M;
+    float sum = 0.f;
+    for (int rho0 = first; rho0 < rows; rho0 += M) {
+      __syncthreads();
+      mass_load_q<S, D>(p, g, head, rho0, qs);
+      if (tid < M) {
+        const PagedRow r = paged_row(p, g, head, rho0 + tid);
+        ml[tid] = r.valid ? mp.row_ml[(long long)r.tok * p.H + r.h] : make_float2(0.f, 0.f);
+        lim[tid] = r.lim;
+      }
+      __syncthreads();
+      float s[4] = {};
+      mass_scores<D>(qs, ks, sk, sr, s);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (key < lim[sr + i]) sum += exp2f(s[i] * p.scale_log2 - ml[sr + i].x) * ml[sr + i].y;
+    }
+    ss[(tid >> 6) * KT + sk] = sum;
+    __syncthreads();
+    if (tid < KT && key < g.klen) {
+      const int page = paged_page(p, g, key >> p.page_log2);
+      if (page >= 0) {
+        float* to = mp.mass.ptr + page * mp.mass.page + head * mp.mass.head + (key & ((1 << p.page_log2) - 1));
+        const float was = mp.add && key < g.klen - g.n ? *to : 0.f;
+        *to = was + ((ss[tid] + ss[KT + tid]) + (ss[2 * KT + tid] + ss[3 * KT + tid]));
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------- eviction
+// Of n keys the first `sinks` and the last `recent` stay, and of those between the ones of the largest mass,
+// ties to the lower key, until m are left; they move together in order. The selection writes the list of
+// kept keys and moves their sums; a second kernel moves the rows.
+constexpr int EV_THREADS = 512;
+constexpr int EV_CACHE = 16384;  // sums held in shared memory; those behind are read again in every pass
+constexpr int EM_THREADS = 256;
+
+struct EvictParams {
+  PagePool K, V;
+  long long k_layer, v_layer;
+  MassPool mass;
+  int pages, page_log2, B, Hk, layers, row_chunks, esize_log2;
+  const int* table;
+  int table_ld, table_cols;
+  const int* lens;
+  const int* budgets;  // [B] or null: `budget`
+  int budget, sinks, recent;
+  int* lens_out;
+  int* list;           // [layers][B][Hk][1 + most]: how many rows stay in place, then the kept keys
+  int most;
+  int cache;           // sums in shared memory
+  int splits;          // blocks of a list and pool: each moves a part of every row
+  int* err;
+};
+
+struct EvictJob {
+  int n, m;  // keys, and how many stay; n <= m: nothing to do
+};
+__device__ __forceinline__ EvictJob evict_job(const EvictParams& p, int b, int& bad) {
+  EvictJob j;
+  j.n = p.lens[b];
+  j.m = p.budgets ? p.budgets[b] : p.budget;
+  if (j.n < 0 || j.n > (p.table_cols << p.page_log2)) bad |= kErrCapacity;
+  if (j.m < p.sinks + p.recent || j.m < 0) bad |= kErrBudget;
+  if (bad) j.m = j.n = max(j.n, 0);
+  return j;
+}
+
+// Larger mass, larger key; no number is below all others.
+__device__ __forceinline__ uint32_t mass_key(float x) {
+  return x != x ? 0u : uint32_t(argmax_key(x + 0.f, 0) >> 32);
+}
+
+__global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const __grid_constant__ EvictParams p) {
+  constexpr int BINS = 2048, WARPS = EV_THREADS / 32;
+  extern __shared__ float ev_cache[];
+  __shared__ int hist[BINS];
+  __shared__ int s_warp[2][WARPS];
+  __shared__ int s_bin, s_left;
+  __shared__ int s_bad, s_still;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int h = blockIdx.x % p.Hk, lb = blockIdx.x / p.Hk, b = lb % p.B, layer = lb / p.B;
+  pdl_wait();
+  pdl_launch_dependents();
+  int bad = 0;
+  const EvictJob job = evict_job(p, b, bad);
+  const int n = job.n, m = job.m, mask = (1 << p.page_log2) - 1;
+  const int* row = p.table + (long long)b * p.table_ld;
+  if (tid == 0) s_bad = s_still = 0;
+  __syncthreads();
+  if (!bad && n > m)  // a page outside the pool: the request stays as it is
+    for (int c = tid; c < (n + mask) >> p.page_log2; c += EV_THREADS)
+      if (row[c] < 0 || row[c] >= p.pages) s_bad = kErrPage;
+  __syncthreads();
+  bad |= s_bad;
+  if (layer == 0 && h == 0 && tid == 0) {
+    if (bad) raise_error(p.err, bad);
+    p.lens_out[b] = bad ? p.lens[b] : min(n, m);
+  }
+  if (bad || n <= m) return;
+  float* base = p.mass.ptr + layer * p.mass.layer + h * p.mass.head;
+  auto at = [&](int j) { return base + row[j >> p.page_log2] * p.mass.page + (j & mask); };
+  const int lo = p.sinks, hi = n - p.recent;
+  int left = m - p.sinks - p.recent;  // to be taken of [lo, hi), fewer than there are
+  for (int j = lo + tid; j < hi && j - lo < p.cache; j += EV_THREADS) ev_cache[j - lo] = *at(j);
+  auto value = [&](int j) { return j - lo < p.cache ? ev_cache[j - lo] : *at(j); };
+  // The key of the last one taken, from its upper bits down: 11, 11, 10
+  uint32_t prefix = 0;
+  int shift = 32;
+  for (int pass = 0; pass < 3; ++pass) {
+    const int bits = pass < 2 ? 11 : 10;
+    shift -= bits;
+    __syncthreads();
+    for (int i = tid; i < BINS; i += EV_THREADS) hist[i] = 0;
+    __syncthreads();
+    for (int j = lo + tid; j < hi; j += EV_THREADS) {
+      const uint32_t k = mass_key(value(j));
+      if (pass == 0 || (k >> (shift + bits)) == prefix) atomicAdd(hist + ((k >> shift) & ((1 << bits) - 1)), 1);
+    }
+    __syncthreads();
+    // counts from the top: thread t has bins [4 t', 4 t' + 4) of the reversed order
+    int c[4], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      c[i] = hist[BINS - 1 - (4 * tid + i)];
+      sum += c[i];
+    }
+    int x = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) s_warp[0][warp] = x;
+    __syncthreads();
+    int above = x - sum;
+    for (int i = 0; i < warp; ++i) above += s_warp[0][i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (above < left && above + c[i] >= left) {
+        s_bin = BINS - 1 - (4 * tid + i);
+        s_left = left - above;
+      }
+      above += c[i];
+    }
+    __syncthreads();
+    if (left > 0) {
+      prefix = (prefix << bits) | uint32_t(s_bin);
+      left = s_left;
+    }
+  }
+  // `left` of those equal to the key, the lowest first, and all above it, in order
+  const bool any = m > p.sinks + p.recent;
+  int* list = p.list + (long long)blockIdx.x * (p.most + 1);
+  int kept = 0, equal = 0, still = 0;
+  for (int j0 = 0; j0 < n; j0 += EV_THREADS) {
+    const int j = j0 + tid;
+    float x = 0.f;
+    bool in = false, tie = false;
+    if (j < n) {
+      x = *at(j);
+      if (j < lo || j >= hi) {
+        in = true;
+      } else if (any) {
+        const uint32_t k = mass_key(x);
+        in = k > prefix;
+        tie = k == prefix;
+      }
+    }
+    const uint32_t ties = __ballot_sync(0xffffffffu, tie);
+    const uint32_t ins = __ballot_sync(0xffffffffu, in);
+    if (lane == 0) {
+      s_warp[0][warp] = __popc(ties);
+      s_warp[1][warp] = __popc(ins);
+    }
+    __syncthreads();  // all of this step's sums are read, and none of a later one's is written to
+    int te = equal, ki = kept, tie_all = 0, in_all = 0;
+    for (int i = 0; i < WARPS; ++i) {
+      if (i < warp) {
+        te += s_warp[0][i];
+        ki += s_warp[1][i];
+      }
+      tie_all += s_warp[0][i];
+      in_all += s_warp[1][i];
+    }
+    const uint32_t below = (1u << lane) - 1;
+    te += __popc(ties & below);                        // equal ones before
+    ki += __popc(ins & below) + min(te, left) - min(equal, left);
+    // of the ties before this one, those of earlier steps are in `kept` already
+    if (in || (tie && te < left)) {
+      list[1 + ki] = j;
+      if (ki != j) *at(ki) = x;
+      else ++still;  // keys before the first gap
+    }
+    kept += in_all + min(equal + tie_all, left) - min(equal, left);
+    equal += tie_all;
+    __syncthreads();
+  }
+  still = __reduce_add_sync(0xffffffffu, still);
+  if (lane == 0) atomicAdd(&s_still, still);
+  __syncthreads();
+  if (tid == 0) list[0] = s_still;
+}
+
+// Moves the kept rows of one list together, K or V, or a part of every row's columns: kept row i comes from
+// row list[i] >= i, so a step's rows are read before any is written, and no later step reads a row that
+// an earlier one wrote.
+__global__ void __launch_bounds__(EM_THREADS) evict_move_kernel(const __grid_constant__ EvictParams p) {
+  constexpr int U = 8;
+  const int tid = threadIdx.x;
+  const int h = blockIdx.x % p.Hk, lb = blockIdx.x / p.Hk, b = lb % p.B, layer = lb / p.B;
+  const int isv = blockIdx.y & 1, split = blockIdx.y >> 1;
+  pdl_wait();
+  pdl_launch_dependents();
+  int bad = 0;
+  const EvictJob job = evict_job(p, b, bad);
+  if (bad || job.n <= job.m) return;
+  const int mask = (1 << p.page_log2) - 1;
+  const int* row = p.table + (long long)b * p.table_ld;
+  for (int c = tid; c < (job.n + mask) >> p.page_log2; c += EM_THREADS) bad |= row[c] < 0 || row[c] >= p.pages;
+  if (__syncthreads_or(bad)) return;
+  const int* list = p.list + (long long)blockIdx.x * (p.most + 1) + 1;
+  const PagePool& pool = isv ? p.V : p.K;
+  const int chunks = p.row_chunks / p.splits, rows_step = EM_THREADS / chunks;
+  char* base = static_cast<char*>(pool.ptr) +
+               (((isv ? p.v_layer : p.k_layer) * layer + h * pool.head) << p.esize_log2) +
+               (split * chunks + tid % chunks) * 16;
+  auto at = [&](int j) {
+    return reinterpret_cast<uint4*>(base + ((row[j >> p.page_log2] * pool.page + (j & mask) * pool.row) << p.esize_log2));
+  };
+  const int first = list[-1];
+  for (int i0 = first; i0 < job.m; i0 += U * rows_step) {
+    uint4 x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * rows_step + tid / chunks;
+      if (i < job.m) x[u] = *at(list[i]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * rows_step + tid / chunks;
+      if (i < job.m) *at(i) = x[u];
+    }
+  }
+}
+
+}  // namespace wc

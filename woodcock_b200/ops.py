@@ -9,11 +9,14 @@ import ctypes as C
 import torch
 
 from ._lib import WC_BF16, WC_F32, lib
+from .beam import beam_reorder, beam_select
 from .context import Context, device_ints, ptr
-from .paged import paged_append, paged_attention, paged_compact, shared_prefix_attention
+from .paged import (paged_append, paged_attention, paged_compact, paged_evict, paged_mass,
+                    shared_prefix_attention)
 
-__all__ = ["Weight", "argmax", "attention", "linear", "paged_append", "paged_attention", "paged_compact", "rmsnorm",
-           "rope", "shared_prefix_attention", "silu_mul", "softmax"]
+__all__ = ["Weight", "argmax", "attention", "beam_reorder", "beam_select", "linear", "paged_append", "paged_attention",
+           "paged_compact", "paged_evict", "paged_mass", "rmsnorm", "rope", "shared_prefix_attention", "silu_mul",
+           "softmax"]
 
 
 class Weight:

@@ -16,9 +16,11 @@ python/woodcock/target.py:159-175); a server keeps many requests' keys and value
   as zeros), a length beyond its table (cut to it) or a row with no slot (its k and v are dropped) is never
   followed; it raises the context's device error word (``Context.get(device).synchronize()`` after
   the stream's work raises WcError).
+* ``mass_pages`` (fp32 [pages][kv_heads][page_size]) hold the attention weight that each key has gathered, beside
+  the pages and addressed by the same tables; rows contiguous, any other strides.
 * Work runs on the caller's current stream of the tensors' device, in its order; scratch comes from
-  PyTorch's allocator for that one call. What a call writes (its output, the pages of append and
-  compact) must not overlap what it reads, nor itself: refused with ValueError. K and V may be cut from
+  PyTorch's allocator for that one call. What a call writes (its output, the pages of append,
+  compact and evict, the mass) must not overlap what it reads, nor itself: refused with ValueError. K and V may be cut from
   one buffer (halves, or side by side in a page, a head or a row). Several threads may call these
   operators at once, each with buffers of its own.
 """
@@ -42,6 +44,8 @@ _BATCH = "Pq2i2P2i"
 _APPEND = struct.Struct("@" + _PAGES + _BATCH + "3P6q4Pdf2i0q")
 _ATTENTION = struct.Struct("@" + _PAGES + _BATCH + "P2qPPq2P2i2PQfi0q")
 _COMPACT = struct.Struct("@" + _PAGES + "Pq2i2Pq2Pi0q")
+_MASS = struct.Struct("@" + _PAGES + _BATCH + "P2qP3qPQf2i0q")
+_EVICT = struct.Struct("@" + _PAGES + "P3qPq2i4PQ3i0q")
 
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
@@ -283,3 +287,99 @@ def paged_compact(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table, star
         *pages, table.data_ptr(), table.stride(0) if many else cols, cols, B, starts.data_ptr(), keep.data_ptr(),
         keep.stride(0) if many else most, n_keep.data_ptr(), lens.data_ptr(), most)))
     return lens
+
+
+def _mass(mass: torch.Tensor, pages: torch.Tensor) -> tuple:
+    n = pages.shape[:-1]
+    if mass.dtype is not torch.float32 or mass.shape != n or mass.device != pages.device:
+        _fail(f"mass_pages must be fp32 {list(n)} on {pages.device}: the pages without head_dim")
+    s = mass.stride()
+    if s[-1] != 1:
+        _fail("rows of mass_pages must be contiguous")
+    return (mass.data_ptr(), *s[:3]) if len(n) == 4 else (mass.data_ptr(), 0, *s[:2])
+
+
+@lru_cache(maxsize=4096)
+def _mass_workspace(device: int, code: int, pages: int, page_size: int, kv_heads: int, head_dim: int, cols: int,
+                    requests: int, rows: int, heads: int) -> int:
+    n = C.c_uint64()
+    ctx = _context(torch.device("cuda", device))
+    st = head_dim * page_size * kv_heads
+    strides = (0, st, head_dim * page_size, head_dim)
+    ctx.check(lib().wc_paged_mass_workspace(ctx.h, _MASS.pack(
+        16, 16, *strides, *strides, code, pages, page_size, kv_heads, head_dim, 1, 16, cols, cols, requests, 16, 16,
+        rows, heads, 16, 0, 0, 16, 0, 0, 0, 0, 0, 1.0, 0, 0), C.byref(n)))
+    return n.value
+
+
+def paged_mass(q: torch.Tensor, k_pages: torch.Tensor, mass_pages: torch.Tensor, page_table, kv_lens, q_offsets=None,
+               scale: float | None = None, add: bool = True) -> torch.Tensor:
+    """Adds up the attention weight that each key gathers, for paged_evict; returns mass_pages.
+
+    mass[b][kv head][key] = was + the sum over request b's new rows and the kv head's query heads of
+    softmax(scale q K^T)[key], the weights that paged_attention gives without a tree_mask. q as there
+    ([rows][heads][head_dim] of the pages' dtype). ``was`` is what the key gathered before: 0 for the keys that
+    are new in this call (a page may hold anything before), and with ``add=False`` for all of them. Rows need not
+    be all that were appended: after a verification the accepted ones, behind a prompt its last ones. A row that
+    sees nothing adds nothing. Statistics and sums are fp32, in the same order every time.
+
+    Requests must not share pages: with a common prompt each needs keys of its own. Where their keys are far
+    more than the pool holds, nothing is written and the device error word is raised."""
+    dev = k_pages.device
+    pages = _pages(k_pages, k_pages)
+    D, kind = pages[14], k_pages.dtype
+    mass = _mass(mass_pages, k_pages)
+    q, qs, shape = _rows(q, kind, dev, None, D, None, "q")
+    T, H, _ = shape
+    batch, B, keep = _batch(T, H, page_table, kv_lens, q_offsets, dev)
+    if T == 0 or B == 0:
+        return mass_pages
+    ctx = _context(dev)
+    device = ctx.device.index
+    n = _mass_workspace(device, pages[10], pages[11], pages[12], pages[13], D, batch[2], B, T, H)
+    ws = q.new_empty(n + 256, dtype=torch.uint8)
+    ctx.check(lib().wc_paged_mass(ctx.h, _stream(device), _MASS.pack(
+        *pages, *batch, q.data_ptr(), qs[0], qs[1], *mass, -(-ws.data_ptr() // 256) * 256, n,
+        D ** -0.5 if scale is None else scale, 0, bool(add))))
+    return mass_pages
+
+
+def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, mass_pages: torch.Tensor, page_table, kv_lens, budget,
+                sinks: int = 0, recent: int = 0) -> torch.Tensor:
+    """Brings every request within its budget of keys; returns the new lengths min(kv_lens, budget) (int32).
+
+    Each layer and kv head of a request with more keys keeps ``budget`` of them (an int, or int32 [requests]): the
+    first ``sinks``, the last ``recent``, and of those between the ones of the largest mass (ties: the lower key;
+    a NaN ranks last). They become keys 0 .. budget - 1 in their order, with their mass; what lies behind is left as
+    it was. Keys keep the rotation they were appended with, so later rows need explicit positions.
+
+    Pages [layers][pages][kv_heads][page_size][head_dim] with mass [layers][pages][kv_heads][page_size], or one
+    layer's. A request whose budget is below sinks + recent keeps everything and raises the device error word.
+    Requests must not share pages."""
+    dev = k_pages.device
+    pages = _pages(k_pages, v_pages, layers=k_pages.dim() == 5)
+    mass = _mass(mass_pages, k_pages)
+    table = _table(page_table, dev, "page_table")
+    B, cols = table.shape
+    lens = _ints(kv_lens, dev, B, "kv_lens")
+    most, budgets = cols * pages[12], None
+    if isinstance(budget, int):
+        if budget < sinks + recent:
+            _fail("budget must not be below sinks + recent")
+        budget = min(budget, 0x7FFFFFFF)
+        most = min(most, budget)
+    else:
+        budgets, budget = _ints(budget, dev, B, "budget"), 0
+    if not 0 <= sinks < 1 << 30 or not 0 <= recent < 1 << 30:
+        _fail("sinks and recent must not be negative")
+    out = lens.new_empty(B)
+    if B == 0:
+        return out
+    ctx = _context(dev)
+    n = pages[15] * B * pages[13] * (most + 1) * 4
+    ws = k_pages.new_empty(n + 256, dtype=torch.uint8)
+    ctx.check(lib().wc_paged_evict(ctx.h, _stream(ctx.device.index), _EVICT.pack(
+        *pages, *mass, table.data_ptr(), table.stride(0) if B > 1 else cols, cols, B, lens.data_ptr(),
+        0 if budgets is None else budgets.data_ptr(), out.data_ptr(), -(-ws.data_ptr() // 256) * 256, n, budget, sinks,
+        recent)))
+    return out
