@@ -490,7 +490,8 @@ typedef struct {
  * pages; where their keys are far more than the pool holds, nothing is written and the device error word is
  * raised. The pages themselves are only read. */
 WC_API wc_status wc_paged_mass(wc_ctx* ctx, void* stream, const wc_paged_mass_args* args);
-/* Bytes of workspace that wc_paged_mass needs for these arguments (buffers are not looked at). */
+/* Bytes of workspace that wc_paged_mass needs for these arguments (buffers are not looked at, but for
+ * whether there are q_offsets). */
 WC_API wc_status wc_paged_mass_workspace(wc_ctx* ctx, const wc_paged_mass_args* args, uint64_t* bytes);
 
 typedef struct {

@@ -34,9 +34,11 @@ wc_pages keys_only(wc_pages g) {
   return g;
 }
 
+// Which kernels a call may need: the number of a request's rows is device data where offsets are given.
 struct MassLayout {
-  int blocks;
-  size_t row_ml, part_ml, rec, tiles, bytes;
+  bool few, many;        // requests of at most 16 rows a KV head, of more
+  int blocks, few_blocks, per, width;
+  size_t row_ml, part_ml, rec, tiles, few_part, scores, bytes;
 };
 
 MassLayout mass_layout(const wc_ctx* ctx, const wc_paged_mass_args& a) {
@@ -44,6 +46,19 @@ MassLayout mass_layout(const wc_ctx* ctx, const wc_paged_mass_args& a) {
   MassLayout l;
   std::memset(&l, 0, sizeof(l));
   size_t at = 0;
+  const wc_pages& g = a.pages;
+  const long long rep = b.heads / g.kv_heads, each = rep * (b.q_offsets ? b.rows : b.rows / b.requests);
+  l.few = g.dtype == WC_BF16 && (b.q_offsets || each <= 16);
+  l.many = g.dtype != WC_BF16 || each > 16;
+  if (l.few) {
+    l.few_blocks = ctx->num_sms * MF_PER_SM;
+    l.width = int(std::min(16ll, (each + 1) & ~1ll));
+    const long long units = mass_most_tiles(g.pages, log2i(g.page_size), b.requests, g.kv_heads, MF_KT) +
+                            (long long)b.requests * g.kv_heads * MF_OVER;
+    l.per = int((units + l.few_blocks - 1) / l.few_blocks);
+    l.few_part = take(at, size_t(l.few_blocks) * 2 * MF_M * sizeof(float2));
+    l.scores = take(at, size_t(l.few_blocks) * l.per * MF_KT * l.width * sizeof(float));
+  }
   l.blocks = ctx->num_sms * 2;
   l.row_ml = take(at, size_t(b.rows) * b.heads * sizeof(float2));
   l.part_ml = take(at, size_t(l.blocks) * 2 * MS_M * sizeof(float2));
@@ -60,8 +75,24 @@ void check_mass_args(const wc_paged_mass_args& a) {
   need(std::isfinite(a.scale) && a.scale > 0, "paged_mass: scale must be positive");
 }
 
+template <int D>
+void gather_few(wc_ctx* ctx, cudaStream_t st, MassParams p, const MassLayout& l, char* ws) {
+  p.kinds = kOwnRows | kFewRows;
+  p.part_ml = reinterpret_cast<float2*>(ws + l.few_part);
+  p.scores = reinterpret_cast<float*>(ws + l.scores);
+  p.per = l.per;
+  p.width = l.width;
+  launch_on(ctx, st, "mass_few_rows", l.width <= 8 ? mass_few_rows_kernel<D, 1> : mass_few_rows_kernel<D, 2>,
+            dim3(l.few_blocks), dim3(MF_THREADS), 0, true, 1, p);
+  launch_on(ctx, st, "mass_few_keys", mass_few_keys_kernel, dim3(l.few_blocks), dim3(MF_THREADS), 0, true, 1, p);
+}
+
 template <typename S, int D>
-void gather_mass(wc_ctx* ctx, cudaStream_t st, const MassParams& p) {
+void gather_mass(wc_ctx* ctx, cudaStream_t st, MassParams p, const MassLayout& l, char* ws) {
+  if constexpr (sizeof(S) == 2)
+    if (l.few) gather_few<D>(ctx, st, p, l, ws);
+  if (!l.many) return;
+  p.kinds = kOwnRows | (l.few ? kManyRows : 0);
   opt_in(ctx, mass_rows_kernel<S, D>, mass_simt_smem<D>());
   opt_in(ctx, mass_keys_kernel<S, D>, mass_simt_smem<D>());
   launch_on(ctx, st, "mass_rows", mass_rows_kernel<S, D>, dim3(p.blocks), dim3(MS_THREADS), mass_simt_smem<D>(), true, 1, p);
@@ -134,11 +165,11 @@ extern "C" wc_status wc_paged_mass(wc_ctx* ctx, void* stream, const wc_paged_mas
     p.blocks = l.blocks;
     const cudaStream_t st = stream_of(ctx, stream);
     if (g.dtype == WC_BF16) {
-      if (g.head_dim == 64) gather_mass<uint16_t, 64>(ctx, st, p);
-      else gather_mass<uint16_t, 128>(ctx, st, p);
+      if (g.head_dim == 64) gather_mass<uint16_t, 64>(ctx, st, p, l, ws);
+      else gather_mass<uint16_t, 128>(ctx, st, p, l, ws);
     } else {
-      if (g.head_dim == 64) gather_mass<float, 64>(ctx, st, p);
-      else gather_mass<float, 128>(ctx, st, p);
+      if (g.head_dim == 64) gather_mass<float, 64>(ctx, st, p, l, ws);
+      else gather_mass<float, 128>(ctx, st, p, l, ws);
     }
   });
 }

@@ -26,6 +26,9 @@ struct MassParams {
   float2* part_ml;       // [blocks][2][16]: of divided items
   long long* tiles;      // [B + 1]: key tiles before each request (all of its heads')
   int blocks;            // of the statistics' launch
+  int kinds;             // which requests' rows
+  float* scores;         // few rows: [blocks][per][64 keys][width], log2 units
+  int per, width;        // key tiles of a block at most, scores of a key at most
 };
 
 // What a weight is before the sums are joined: rows that see nothing keep 0.
@@ -93,7 +96,7 @@ __global__ void __launch_bounds__(MS_THREADS) mass_rows_kernel(const __grid_cons
   pdl_launch_dependents();
   PagedWalk<M, KT, 1> w;
   paged_no_rec(p);
-  if (!w.begin(p, kOwnRows, 1, sh)) return;
+  if (!w.begin(p, mp.kinds, 1, sh)) return;
   do {
     __syncthreads();
     mass_load_q<S, D>(p, w.g, w.head, w.qt * M, qs);
@@ -135,7 +138,7 @@ __global__ void __launch_bounds__(MS_THREADS) mass_rows_kernel(const __grid_cons
         else mp.part_ml[((long long)blockIdx.x * 2 + w.slot()) * M + 2 * warp + i] = make_float2(m2[i], l2[i]);
       }
     }
-  } while (w.next(p, kOwnRows));
+  } while (w.next(p, mp.kinds));
 }
 
 // Key tiles of requests that share no pages, at most.
@@ -158,7 +161,7 @@ __global__ void __launch_bounds__(256) mass_join_kernel(const __grid_constant__ 
       const int b = b0 + tid;
       long long w = 0;
       if (b < p.B) {
-        const PagedSeg g = paged_seg(p, kOwnRows, b);
+        const PagedSeg g = paged_seg(p, mp.kinds, b);
         if (g.n > 0) w = (long long)((g.klen + KT - 1) / KT) * p.Hk;
       }
       long long x = w;
@@ -243,7 +246,7 @@ __global__ void __launch_bounds__(MS_THREADS) mass_keys_kernel(const __grid_cons
   const int sk = tid & 63, sr = (tid >> 6) * 4;
   for (long long at = blockIdx.x; at < total; at += gridDim.x) {
     const int b = mass_request(mp.tiles, p.B, at, lane);
-    const PagedSeg g = paged_seg(p, kOwnRows, b);
+    const PagedSeg g = paged_seg(p, mp.kinds, b);
     const int nt = (g.klen + KT - 1) / KT;
     const int head = int((at - mp.tiles[b]) / nt), kt = int((at - mp.tiles[b]) - (long long)head * nt);
     __syncthreads();
@@ -279,6 +282,192 @@ __global__ void __launch_bounds__(MS_THREADS) mass_keys_kernel(const __grid_cons
     }
     __syncthreads();
   }
+}
+
+// ---- few rows (bf16 pages, at most 16 a KV head: steps and accepted chains)
+// K's bytes bound the time, so it is read once. The first kernel takes scores (keys as the products' rows,
+// mma m16n8k16) and keeps them, 4 bytes a key and row beside the key's 2 head_dim; the second, on the same
+// shares, turns them into weights and adds them up. K goes from memory to registers without a detour: a
+// product sums over head_dim in any order, so a lane's 16 consecutive bytes of a key serve as the places
+// that the operand's layout gives it, if the query's are taken alike. A warp has 16 keys at a time, 4 KB on
+// their way.
+constexpr int MF_THREADS = 256, MF_M = 16, MF_KT = 64, MF_OVER = 2, MF_PER_SM = 2;
+
+template <int D, int NT>
+__global__ void __launch_bounds__(MF_THREADS, MF_PER_SM) mass_few_rows_kernel(const __grid_constant__ MassParams mp) {
+  const PagedAttnParams& p = mp.a;
+  constexpr int NV = D / 32;  // 16-byte pieces of a key in a lane
+  __shared__ long long sh[kWalkShared];
+  __shared__ float2 wml[MF_THREADS / 32][8 * NT];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3;
+  pdl_wait();
+  pdl_launch_dependents();
+  PagedWalk<MF_M, MF_KT, MF_OVER> w;
+  if (!w.begin(p, mp.kinds, 1, sh)) return;
+  if (w.per > mp.per) {  // more keys than the pool holds: requests share pages
+    if (tid == 0) raise_error(p.err, kErrPage);
+    return;
+  }
+  float* buf = mp.scores + (long long)blockIdx.x * mp.per * MF_KT * mp.width;
+  do {
+    const int R = min(w.g.n * p.rep, 8 * NT), stride = (R + 1) & ~1;
+    uint4 q[NT][NV];
+    int lim[NT][2];
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const PagedRow r = paged_row(p, w.g, w.head, t * 8 + g8);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        q[t][i] = r.valid ? *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + r.tok * p.q_row +
+                                                            r.h * p.q_head + i * 32 + t4 * 8)
+                          : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        lim[t][e] = paged_row(p, w.g, w.head, t * 8 + 2 * t4 + e).lim;
+        m[t][e] = -INFINITY;
+        l[t][e] = 0.f;
+      }
+    }
+    const int end = min(w.kt1 * MF_KT, w.g.klen);
+    int key0 = w.kt0 * MF_KT + warp * 16;
+    int page = key0 < end ? paged_page(p, w.g, key0 >> p.page_log2) : -1;
+    for (; key0 < end; key0 += 16 * (MF_THREADS / 32)) {
+      uint4 a[NV], b[NV];
+      if (page >= 0) {
+        const uint16_t* k = static_cast<const uint16_t*>(p.K.ptr) + page * p.K.page + w.head * p.K.head +
+                            ((key0 & ((1 << p.page_log2) - 1)) + g8) * p.K.row + t4 * 8;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          a[i] = ldg_stream(reinterpret_cast<const uint4*>(k + i * 32));
+          b[i] = ldg_stream(reinterpret_cast<const uint4*>(k + 8 * p.K.row + i * 32));
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) a[i] = b[i] = make_uint4(0, 0, 0, 0);
+      }
+      const int next = key0 + 16 * (MF_THREADS / 32);
+      page = next < end ? paged_page(p, w.g, next >> p.page_log2) : -1;
+      float c[NT][4];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        c[t][0] = c[t][1] = c[t][2] = c[t][3] = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          mma_bf16_16816(c[t], make_uint4(a[i].x, b[i].x, a[i].y, b[i].y), q[t][i].x, q[t][i].y);
+          mma_bf16_16816(c[t], make_uint4(a[i].z, b[i].z, a[i].w, b[i].w), q[t][i].z, q[t][i].w);
+        }
+      }
+      float* to = buf + (key0 - w.kt0 * MF_KT + g8) * stride + 2 * t4;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float z0 = key0 + g8 < lim[t][e] ? c[t][e] * p.scale_log2 : -INFINITY;
+          const float z1 = key0 + g8 + 8 < lim[t][e] ? c[t][2 + e] * p.scale_log2 : -INFINITY;
+          c[t][e] = z0;
+          c[t][2 + e] = z1;
+          const float mn = fmaxf(m[t][e], fmaxf(z0, z1)), mg = mn == -INFINITY ? 0.f : mn;
+          l[t][e] = l[t][e] * ex2_approx(m[t][e] - mg) + (ex2_approx(z0 - mg) + ex2_approx(z1 - mg));
+          m[t][e] = mn;
+        }
+        if (t * 8 + 2 * t4 < R) {
+          *reinterpret_cast<float2*>(to + t * 8) = make_float2(c[t][0], c[t][1]);
+          *reinterpret_cast<float2*>(to + 8 * stride + t * 8) = make_float2(c[t][2], c[t][3]);
+        }
+      }
+    }
+    // one state a row: the lanes that share it, then the warps
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int o = 4; o < 32; o *= 2) {
+          const float m2 = __shfl_xor_sync(0xffffffffu, m[t][e], o), l2 = __shfl_xor_sync(0xffffffffu, l[t][e], o);
+          const float mn = fmaxf(m[t][e], m2), mg = mn == -INFINITY ? 0.f : mn;
+          l[t][e] = l[t][e] * ex2_approx(m[t][e] - mg) + l2 * ex2_approx(m2 - mg);
+          m[t][e] = mn;
+        }
+        if (g8 == 0) wml[warp][t * 8 + 2 * t4 + e] = make_float2(m[t][e], l[t][e]);
+      }
+    __syncthreads();
+    if (tid < R) {
+      float M = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int i = 0; i < MF_THREADS / 32; ++i) {
+        const float2 y = wml[i][tid];
+        const float mn = fmaxf(M, y.x), mg = mn == -INFINITY ? 0.f : mn;
+        L = L * ex2_approx(M - mg) + y.y * ex2_approx(y.x - mg);
+        M = mn;
+      }
+      const PagedRow r = paged_row(p, w.g, w.head, tid);
+      if (w.count == 1) mp.row_ml[(long long)r.tok * p.H + r.h] = mass_row(M, L);
+      else mp.part_ml[((long long)blockIdx.x * 2 + w.slot()) * MF_M + tid] = make_float2(M, L);
+    }
+    __syncthreads();
+    buf += (w.kt1 - w.kt0) * MF_KT * mp.width;
+  } while (w.next(p, mp.kinds));
+}
+
+// The scores' weights, added up: a thread a key, on the shares of the kernel before.
+__global__ void __launch_bounds__(MF_THREADS) mass_few_keys_kernel(const __grid_constant__ MassParams mp) {
+  const PagedAttnParams& p = mp.a;
+  __shared__ long long sh[kWalkShared];
+  __shared__ float2 ml[MF_M];
+  const int tid = threadIdx.x;
+  PagedWalk<MF_M, MF_KT, MF_OVER> w;
+  const bool work = w.begin(p, mp.kinds, 1, sh);  // of the lengths alone, which no kernel since has written
+  pdl_wait();
+  pdl_launch_dependents();
+  if (!work || w.per > mp.per) return;
+  const float* buf = mp.scores + (long long)blockIdx.x * mp.per * MF_KT * mp.width;
+  do {
+    const int R = min(w.g.n * p.rep, MF_M), stride = (R + 1) & ~1;
+    const int row = tid >> 4, part = tid & 15;
+    if (w.count == 1) {
+      if (tid < R) {
+        const PagedRow r = paged_row(p, w.g, w.head, tid);
+        ml[tid] = mp.row_ml[(long long)r.tok * p.H + r.h];
+      }
+    } else {
+      float M = -INFINITY, L = 0.f;
+      if (row < R)
+        for (int i = part; i < w.count; i += 16) {
+          const float2 y = mp.part_ml[((long long)(w.first + i) * 2 + (i == 0 ? 1 : 0)) * MF_M + row];
+          const float mn = fmaxf(M, y.x), mg = mn == -INFINITY ? 0.f : mn;
+          L = L * ex2_approx(M - mg) + y.y * ex2_approx(y.x - mg);
+          M = mn;
+        }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) {
+        const float m2 = __shfl_xor_sync(0xffffffffu, M, o), l2 = __shfl_xor_sync(0xffffffffu, L, o);
+        const float mn = fmaxf(M, m2), mg = mn == -INFINITY ? 0.f : mn;
+        L = L * ex2_approx(M - mg) + l2 * ex2_approx(m2 - mg);
+        M = mn;
+      }
+      if (part == 0) ml[row] = mass_row(M, L);
+    }
+    __syncthreads();
+    const int end = min(w.kt1 * MF_KT, w.g.klen);
+    for (int key = w.kt0 * MF_KT + tid; key < end; key += MF_THREADS) {
+      const float* z = buf + (key - w.kt0 * MF_KT) * stride;
+      float sum = 0.f;
+      for (int r = 0; r < R; r += 2) {
+        const float2 y = *reinterpret_cast<const float2*>(z + r);
+        sum += ex2_approx(y.x - ml[r].x) * ml[r].y;
+        if (r + 1 < R) sum += ex2_approx(y.y - ml[r + 1].x) * ml[r + 1].y;
+      }
+      const int page = paged_page(p, w.g, key >> p.page_log2);
+      if (page >= 0) {
+        float* to = mp.mass.ptr + page * mp.mass.page + w.head * mp.mass.head + (key & ((1 << p.page_log2) - 1));
+        const float was = mp.add && key < w.g.klen - w.g.n ? *to : 0.f;
+        *to = was + sum;
+      }
+    }
+    __syncthreads();
+    buf += (w.kt1 - w.kt0) * MF_KT * mp.width;
+  } while (w.next(p, mp.kinds));
 }
 
 // ---------------------------------------------------------------------------- eviction

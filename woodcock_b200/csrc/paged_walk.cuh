@@ -50,7 +50,12 @@ __device__ __forceinline__ void store8(uint16_t* p, const float (&x)[8]) {
 // ranges, one per block, so blocks carry equal work whatever the lengths. An item that crosses a
 // cut leaves partial states (running maximum in log2 units, sum, unnormalised output), joined in
 // block order by the combine kernel: no atomics, the same result every time.
-enum PagedKinds : int { kOwnRows = 1, kPrefixRows = 2 };
+enum PagedKinds : int {
+  kOwnRows = 1,
+  kPrefixRows = 2,
+  kFewRows = 4,   // requests of at most 16 query rows a KV head alone
+  kManyRows = 8,  // requests of more
+};
 
 // A divided item as the joining kernel needs it; count 0: none.
 struct PagedRec {
@@ -108,6 +113,8 @@ __device__ __forceinline__ PagedSeg paged_seg(const PagedAttnParams& p, int kind
   } else {
     g.tok0 = paged_row0(p, g.idx);
     g.n = max(0, paged_row0(p, g.idx + 1) - g.tok0);
+    if ((kinds & kFewRows) && g.n * p.rep > 16) g.n = 0;
+    if ((kinds & kManyRows) && g.n * p.rep <= 16) g.n = 0;
     g.klen = p.lens[g.idx];
     cap = p.table_cols << p.page_log2;
     if (p.tree && g.n > 64) raise_error(p.err, kErrRows);

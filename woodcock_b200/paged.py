@@ -301,13 +301,13 @@ def _mass(mass: torch.Tensor, pages: torch.Tensor) -> tuple:
 
 @lru_cache(maxsize=4096)
 def _mass_workspace(device: int, code: int, pages: int, page_size: int, kv_heads: int, head_dim: int, cols: int,
-                    requests: int, rows: int, heads: int) -> int:
+                    requests: int, ragged: int, rows: int, heads: int) -> int:
     n = C.c_uint64()
     ctx = _context(torch.device("cuda", device))
     st = head_dim * page_size * kv_heads
     strides = (0, st, head_dim * page_size, head_dim)
     ctx.check(lib().wc_paged_mass_workspace(ctx.h, _MASS.pack(
-        16, 16, *strides, *strides, code, pages, page_size, kv_heads, head_dim, 1, 16, cols, cols, requests, 16, 16,
+        16, 16, *strides, *strides, code, pages, page_size, kv_heads, head_dim, 1, 16, cols, cols, requests, 16, 16 * ragged,
         rows, heads, 16, 0, 0, 16, 0, 0, 0, 0, 0, 1.0, 0, 0), C.byref(n)))
     return n.value
 
@@ -336,7 +336,8 @@ def paged_mass(q: torch.Tensor, k_pages: torch.Tensor, mass_pages: torch.Tensor,
         return mass_pages
     ctx = _context(dev)
     device = ctx.device.index
-    n = _mass_workspace(device, pages[10], pages[11], pages[12], pages[13], D, batch[2], B, T, H)
+    n = _mass_workspace(device, pages[10], pages[11], pages[12], pages[13], D, batch[2], B,
+                        q_offsets is not None, T, H)
     ws = q.new_empty(n + 256, dtype=torch.uint8)
     ctx.check(lib().wc_paged_mass(ctx.h, _stream(device), _MASS.pack(
         *pages, *batch, q.data_ptr(), qs[0], qs[1], *mass, -(-ws.data_ptr() // 256) * 256, n,
