@@ -38,7 +38,8 @@ wc_pages keys_only(wc_pages g) {
 struct MassLayout {
   bool few, many;        // requests of at most 16 rows a KV head, of more
   int blocks, few_blocks, per, width;
-  size_t row_ml, part_ml, rec, tiles, few_part, scores, bytes;
+  MassModes rows, keys;
+  size_t row_ml, part_ml, rec, tiles, few_part, scores, part_sum, keys_rec, bytes;
 };
 
 MassLayout mass_layout(const wc_ctx* ctx, const wc_paged_mass_args& a) {
@@ -59,11 +60,21 @@ MassLayout mass_layout(const wc_ctx* ctx, const wc_paged_mass_args& a) {
     l.few_part = take(at, size_t(l.few_blocks) * 2 * MF_M * sizeof(float2));
     l.scores = take(at, size_t(l.few_blocks) * l.per * MF_KT * l.width * sizeof(float));
   }
-  l.blocks = ctx->num_sms * 2;
   l.row_ml = take(at, size_t(b.rows) * b.heads * sizeof(float2));
-  l.part_ml = take(at, size_t(l.blocks) * 2 * MS_M * sizeof(float2));
+  if (l.many && g.dtype == WC_BF16) {
+    const long long mean = (rep * b.rows + b.requests - 1) / b.requests;
+    l.blocks = ctx->num_sms;
+    l.rows = mean <= 128 ? kRows128 : kRows256;
+    l.keys = mean <= 256 ? kKeysWindow : kKeysPrompt;
+    l.part_sum = take(at, size_t(l.blocks) * 2 * MK_KEYS * sizeof(float));
+    l.keys_rec = take(at, l.blocks * sizeof(MassRec));
+  } else {
+    l.blocks = ctx->num_sms * 2;
+    l.tiles = take(at, (size_t(b.requests) + 1) * sizeof(long long));
+  }
+  const int M = g.dtype != WC_BF16 ? MS_M : l.rows == kRows128 ? 128 : 256;
+  l.part_ml = take(at, size_t(l.blocks) * 2 * M * sizeof(float2));
   l.rec = take(at, l.blocks * sizeof(PagedRec));
-  l.tiles = take(at, (size_t(b.requests) + 1) * sizeof(long long));
   l.bytes = at;
   return l;
 }
@@ -87,18 +98,43 @@ void gather_few(wc_ctx* ctx, cudaStream_t st, MassParams p, const MassLayout& l,
   launch_on(ctx, st, "mass_few_keys", mass_few_keys_kernel, dim3(l.few_blocks), dim3(MF_THREADS), 0, true, 1, p);
 }
 
+template <int D, int kMode>
+void launch_many(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, const MassParams& p) {
+  constexpr size_t smem = MmLayout<D, kMode>::bytes();
+  static_assert(smem <= kSmemOptinBytes, "shared memory");
+  opt_in(ctx, mass_many_kernel<D, kMode>, smem);
+  launch_on(ctx, st, "mass_many", mass_many_kernel<D, kMode>, dim3(p.blocks), dim3(MM_THREADS), smem, true, 1,
+            page_map(g, p.a.K, 128, 1), p);
+}
+
+template <int D>
+void gather_many(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, MassParams p, const MassLayout& l, char* ws) {
+  p.part_sum = reinterpret_cast<float*>(ws + l.part_sum);
+  p.keys_rec = reinterpret_cast<MassRec*>(ws + l.keys_rec);
+  if (l.rows == kRows128) launch_many<D, kRows128>(ctx, st, g, p);
+  else launch_many<D, kRows256>(ctx, st, g, p);
+  launch_on(ctx, st, "mass_join", l.rows == kRows128 ? mass_join_kernel<128, 128> : mass_join_kernel<256, 128>, dim3(p.blocks),
+            dim3(256), 0, true, 1, p);
+  if (l.keys == kKeysWindow) launch_many<D, kKeysWindow>(ctx, st, g, p);
+  else launch_many<D, kKeysPrompt>(ctx, st, g, p);
+  launch_on(ctx, st, "mass_fold", mass_fold_kernel, dim3(p.blocks), dim3(MK_KEYS), 0, true, 1, p);
+}
+
 template <typename S, int D>
-void gather_mass(wc_ctx* ctx, cudaStream_t st, MassParams p, const MassLayout& l, char* ws) {
-  if constexpr (sizeof(S) == 2)
+void gather_mass(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, MassParams p, const MassLayout& l, char* ws) {
+  if constexpr (sizeof(S) == 2) {
     if (l.few) gather_few<D>(ctx, st, p, l, ws);
-  if (!l.many) return;
-  p.kinds = kOwnRows | (l.few ? kManyRows : 0);
-  opt_in(ctx, mass_rows_kernel<S, D>, mass_simt_smem<D>());
-  opt_in(ctx, mass_keys_kernel<S, D>, mass_simt_smem<D>());
-  launch_on(ctx, st, "mass_rows", mass_rows_kernel<S, D>, dim3(p.blocks), dim3(MS_THREADS), mass_simt_smem<D>(), true, 1, p);
-  launch_on(ctx, st, "mass_join", mass_join_kernel<MS_M, MS_KT>, dim3(p.blocks + 1), dim3(256), 0, true, 1, p);
-  launch_on(ctx, st, "mass_keys", mass_keys_kernel<S, D>, dim3(ctx->num_sms * 2), dim3(MS_THREADS), mass_simt_smem<D>(),
-            true, 1, p);
+    p.kinds = kOwnRows | (l.few ? kManyRows : 0);
+    if (l.many) gather_many<D>(ctx, st, g, p, l, ws);
+  } else {
+    p.kinds = kOwnRows;
+    opt_in(ctx, mass_rows_kernel<S, D>, mass_simt_smem<D>());
+    opt_in(ctx, mass_keys_kernel<S, D>, mass_simt_smem<D>());
+    launch_on(ctx, st, "mass_rows", mass_rows_kernel<S, D>, dim3(p.blocks), dim3(MS_THREADS), mass_simt_smem<D>(), true, 1, p);
+    launch_on(ctx, st, "mass_join", mass_join_kernel<MS_M, MS_KT>, dim3(p.blocks + 1), dim3(256), 0, true, 1, p);
+    launch_on(ctx, st, "mass_keys", mass_keys_kernel<S, D>, dim3(ctx->num_sms * 2), dim3(MS_THREADS), mass_simt_smem<D>(),
+              true, 1, p);
+  }
 }
 
 }  // namespace
@@ -165,11 +201,11 @@ extern "C" wc_status wc_paged_mass(wc_ctx* ctx, void* stream, const wc_paged_mas
     p.blocks = l.blocks;
     const cudaStream_t st = stream_of(ctx, stream);
     if (g.dtype == WC_BF16) {
-      if (g.head_dim == 64) gather_mass<uint16_t, 64>(ctx, st, p, l, ws);
-      else gather_mass<uint16_t, 128>(ctx, st, p, l, ws);
+      if (g.head_dim == 64) gather_mass<uint16_t, 64>(ctx, st, g, p, l, ws);
+      else gather_mass<uint16_t, 128>(ctx, st, g, p, l, ws);
     } else {
-      if (g.head_dim == 64) gather_mass<float, 64>(ctx, st, p, l, ws);
-      else gather_mass<float, 128>(ctx, st, p, l, ws);
+      if (g.head_dim == 64) gather_mass<float, 64>(ctx, st, g, p, l, ws);
+      else gather_mass<float, 128>(ctx, st, g, p, l, ws);
     }
   });
 }

@@ -2,8 +2,11 @@
 // that gather least.
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "paged_walk.cuh"
+#include "tcgen05.cuh"
 
 namespace wc {
 
@@ -17,6 +20,10 @@ struct MassPool {
 // mass_j (+)= sum over new rows i and query heads h of the key's head of p_ih(j),
 // p_ih(j) = 2^(s_ih(j) - M_ih) / L_ih over the keys that row i sees. A weight needs its row's maximum and sum
 // over all keys first, so the scores are needed twice.
+struct MassRec {
+  int request, head, kt, count;  // count 0: none
+};
+
 struct MassParams {
   PagedAttnParams a;     // q, K pages, batch
   MassPool mass;
@@ -29,6 +36,9 @@ struct MassParams {
   int kinds;             // which requests' rows
   float* scores;         // few rows: [blocks][per][64 keys][width], log2 units
   int per, width;        // key tiles of a block at most, scores of a key at most
+  float* part_sum;       // many rows: [blocks][2][256], of divided key tiles
+  MassRec* keys_rec;     // [blocks]: the divided key tile that begins in the block
+  int key_blocks;
 };
 
 // What a weight is before the sums are joined: rows that see nothing keep 0.
@@ -146,10 +156,11 @@ __host__ __device__ __forceinline__ long long mass_most_tiles(int pages, int pag
   return (((long long)pages << page_log2) / KT + B) * Hk;
 }
 
-// Joins the parts of divided items, one block an item and a warp a row; the last block counts the key tiles
-// before each request.
+// Joins the parts of divided items, one block an item; where `tiles` is asked for, a last block counts the key
+// tiles before each request.
 template <int M, int KT>
 __global__ void __launch_bounds__(256) mass_join_kernel(const __grid_constant__ MassParams mp) {
+  constexpr int LANES = 256 / M;  // lanes a row
   const PagedAttnParams& p = mp.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_wait();
@@ -190,27 +201,25 @@ __global__ void __launch_bounds__(256) mass_join_kernel(const __grid_constant__ 
   }
   const PagedRec rec = p.rec[blockIdx.x];
   if (rec.count == 0) return;
-  for (int r = warp; r < M; r += 8) {
-    const int rho = rec.qt * M + r;
-    if (rho >= rec.rows) break;
-    float m = -INFINITY, l = 0.f;
-    for (int i = lane; i < rec.count; i += 32) {
+  const int r = tid / LANES, rho = rec.qt * M + r;
+  float m = -INFINITY, l = 0.f;
+  if (rho < rec.rows)
+    for (int i = tid % LANES; i < rec.count; i += LANES) {
       const float2 y = mp.part_ml[((long long)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * M + r];
       const float mn = fmaxf(m, y.x), mg = mn == -INFINITY ? 0.f : mn;
       l = l * exp2f(m - mg) + y.y * exp2f(y.x - mg);
       m = mn;
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
-      const float mn = fmaxf(m, m2), mg = mn == -INFINITY ? 0.f : mn;
-      l = l * exp2f(m - mg) + l2 * exp2f(m2 - mg);
-      m = mn;
-    }
-    if (lane == 0) {
-      const int i = rho / p.rep;
-      mp.row_ml[(long long)(rec.tok0 + i) * p.H + rec.head * p.rep + rho - i * p.rep] = mass_row(m, l);
-    }
+  for (int o = LANES / 2; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
+    const float mn = fmaxf(m, m2), mg = mn == -INFINITY ? 0.f : mn;
+    l = l * exp2f(m - mg) + l2 * exp2f(m2 - mg);
+    m = mn;
+  }
+  if (rho < rec.rows && tid % LANES == 0) {
+    const int i = rho / p.rep;
+    mp.row_ml[(long long)(rec.tok0 + i) * p.H + rec.head * p.rep + rho - i * p.rep] = mass_row(m, l);
   }
 }
 
@@ -468,6 +477,539 @@ __global__ void __launch_bounds__(MF_THREADS) mass_few_keys_kernel(const __grid_
     __syncthreads();
     buf += (w.kt1 - w.kt0) * MF_KT * mp.width;
   } while (w.next(p, mp.kinds));
+}
+
+// ---- many rows (bf16 pages, more than 16 a KV head: windows and prompts)
+// Scores on tensor memory, twice. First with the rows as the product's lanes, 128 keys as its columns: a
+// thread has a row and needs its maximum and sum alone. Then turned round: a thread has a key, the columns
+// are 128 rows, and the key's weights are added up where they are, without an exchange between threads.
+// Weights are 2^(s - L), L = M + log2(sum).
+//
+// Both kernels are one code: a lane operand A that stays for an item, a column operand B that streams, two
+// groups of four warps that read the products from tensor memory, two buffers each. kMode: rows of at most
+// 128 a request (the groups take alternate B tiles); rows of more (a group each half of 256 lanes); keys
+// (the same, 256 keys), with rings for prompts (Q streams) or for windows (K streams).
+// Bound by the exponential unit: 16 a clock, 1024 clocks for a product of 512.
+enum MassModes : int { kRows128 = 0, kRows256 = 1, kKeysPrompt = 2, kKeysWindow = 3 };
+constexpr int MM_THREADS = 384;  // K copies, products, 2 warps of Q copies; 2 x 4 warps of sums
+constexpr int MM_OVER = 2, MK_OVER = 2, MK_KEYS = 256;
+
+template <int D, int kMode>
+struct MmLayout {
+  static constexpr int KS = kMode == kKeysPrompt ? 2 : 4, QS = 6 - KS;  // tiles of 128 rows
+  static constexpr int kTile = 128 * D * 2;
+  static constexpr int kTail = 8 * kWalkShared + 256 + QS * 128 * 4 + 2 * 128 * 8;
+  static constexpr size_t bytes() { return 1024 + size_t(KS + QS) * kTile + kTail; }
+};
+
+// The line of key tiles (256 keys), each with the row tiles that see it: a block's share begins and ends anywhere.
+struct MassWalk {
+  PagedSeg g;
+  int seg, head, kt, nkt;
+  int QT, qf;         // row tiles of the request, the first that sees the key tile
+  int qt0, qt1;       // this block's
+  int first, count;   // the blocks that share the tile
+  int per;
+  long long pos, lo, hi;
+
+  __device__ __forceinline__ int first_row_tile(const PagedAttnParams& p, int k) const {
+    return int((long long)max(0, k * MK_KEYS - (g.klen - g.n)) * p.rep / 128);
+  }
+  __device__ __forceinline__ void enter(const PagedAttnParams& p) {  // a segment
+    nkt = (g.klen + MK_KEYS - 1) / MK_KEYS;
+    QT = (g.n * p.rep + 127) / 128;
+  }
+  __device__ __forceinline__ int plain_tiles() const {  // key tiles that every row tile sees
+    return g.klen < g.n ? 0 : min(nkt, (g.klen - g.n) / MK_KEYS + 1);
+  }
+  __device__ long long units(const PagedAttnParams& p) {  // of one head
+    if (g.n <= 0 || g.klen <= 0) return 0;
+    enter(p);
+    const int plain = plain_tiles();
+    long long u = (long long)plain * (QT + MK_OVER);
+    for (int k = plain; k < nkt; ++k) u += QT - first_row_tile(p, k) + MK_OVER;
+    return u;
+  }
+  // Block-collective; false: no work.
+  __device__ bool begin(const PagedAttnParams& p, int kinds, long long* sh) {
+    const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, nw = nt >> 5;
+    long long total = 0;
+    for (int pass = 0; pass < 2; ++pass) {
+      if (pass) {
+        per = int(max(1ll, (total + gridDim.x - 1) / gridDim.x));
+        lo = (long long)blockIdx.x * per;
+        hi = min(lo + per, total);
+        if (lo >= hi) return false;
+      }
+      long long base = 0;
+      for (int s0 = 0; s0 < p.B; s0 += nt) {
+        const int s = s0 + tid;
+        long long w = 0;
+        if (s < p.B) {
+          g = paged_seg(p, kinds, s);
+          w = units(p) * p.Hk;
+        }
+        long long x = w;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+          const long long y = __shfl_up_sync(0xffffffffu, x, o);
+          if (lane >= o) x += y;
+        }
+        if (lane == 31) sh[warp] = x;
+        __syncthreads();
+        long long before = base;
+        for (int i = 0; i < nw; ++i) {
+          if (i < warp) before += sh[i];
+          base += sh[i];
+        }
+        const long long a = before + x - w;
+        if (pass && a <= lo && lo < a + w) {
+          sh[32] = s;
+          sh[33] = a;
+          sh[34] = w;
+        }
+        __syncthreads();
+      }
+      total = base;
+    }
+    seg = int(sh[32]);
+    const long long ph = sh[34] / p.Hk;
+    g = paged_seg(p, kinds, seg);
+    enter(p);
+    head = int((lo - sh[33]) / ph);
+    pos = sh[33] + head * ph;
+    kt = int(min((long long)plain_tiles(), (lo - pos) / (QT + MK_OVER)));
+    pos += (long long)kt * (QT + MK_OVER);
+    for (;;) {
+      qf = first_row_tile(p, kt);
+      if (pos + QT - qf + MK_OVER > lo) break;
+      pos += QT - qf + MK_OVER;
+      ++kt;
+    }
+    return place() || next(p, kinds);
+  }
+  __device__ bool place() {
+    const long long at = pos + MK_OVER;
+    qt0 = qf + int(max(0ll, lo - at));
+    qt1 = int(min((long long)QT, qf + hi - at));
+    first = int(at / per);
+    count = int((at + QT - qf - 1) / per) - first + 1;
+    return qt1 > qt0;
+  }
+  __device__ bool next(const PagedAttnParams& p, int kinds) {
+    do {
+      pos += QT - qf + MK_OVER;
+      if (pos >= hi) return false;
+      if (++kt == nkt) {
+        kt = 0;
+        if (++head == p.Hk) {
+          head = 0;
+          do {
+            g = paged_seg(p, kinds, ++seg);
+          } while (g.n <= 0 || g.klen <= 0);
+          enter(p);
+        }
+      }
+      qf = first_row_tile(p, kt);
+    } while (!place());
+    return true;
+  }
+  __device__ int slot() const { return qt0 > qf ? 0 : 1; }
+};
+
+template <int D, int kMode>
+__global__ void __launch_bounds__(MM_THREADS, 1)
+    mass_many_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ MassParams mp) {
+  constexpr bool kKeys = kMode >= kKeysPrompt, kTwo = kMode != kRows128;
+  using L = MmLayout<D, kMode>;
+  using Walk = std::conditional_t<kKeys, MassWalk, PagedWalk<kTwo ? 256 : 128, 128, MM_OVER>>;
+  constexpr int M = kTwo ? 256 : 128, KS = L::KS, QS = L::QS, HALVES = D / 64;
+  const PagedAttnParams& p = mp.a;
+  extern __shared__ unsigned char mm_raw[];
+  unsigned char* sm = mm_raw + ((1024u - (smem_addr(mm_raw) & 1023u)) & 1023u);
+  unsigned char* ks = sm;                             // [KS][half][128 keys][128 B], swizzled
+  unsigned char* qs = sm + size_t(KS) * L::kTile;     // [QS][half][128 rows][128 B]
+  unsigned char* tail = qs + size_t(QS) * L::kTile;
+  long long* sh = reinterpret_cast<long long*>(tail);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(tail + 8 * kWalkShared);
+  uint64_t* k_full = bars;        // [4]
+  uint64_t* k_empty = bars + 4;   // [4]
+  uint64_t* q_full = bars + 8;    // [4]
+  uint64_t* q_empty = bars + 12;  // [4]
+  uint64_t* s_full = bars + 16;   // [4]: group * 2 + buffer
+  uint64_t* s_empty = bars + 20;  // [4]
+  uint64_t* x_full = bars + 24;   // [2]: the second group's states are in shared memory
+  uint64_t* x_empty = bars + 26;  // [2]: and read
+  uint64_t* drain = bars + 28;
+  volatile int* dead = reinterpret_cast<volatile int*>(bars + 29);
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + 30);
+  float* nl = reinterpret_cast<float*>(tail + 8 * kWalkShared + 256);  // [QS][128]: -L of the tile's rows
+  float2* xml = reinterpret_cast<float2*>(nl + QS * 128);              // [item & 1][row]
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(k_full + i, 1);
+      mbar_init(k_empty + i, 1);
+      mbar_init(q_full + i, 2);
+      mbar_init(q_empty + i, kKeys ? 9 : 1);
+      mbar_init(s_full + i, 1);
+      mbar_init(s_empty + i, 4);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(x_full + i, 4);
+      mbar_init(x_empty + i, 4);
+    }
+    mbar_init(drain, 1);
+    mbar_fence_init();
+    *dead = 0;
+  }
+  pdl_wait();
+  pdl_launch_dependents();
+  if constexpr (!kKeys) paged_no_rec(p);
+  else if (tid == 0) mp.keys_rec[blockIdx.x] = MassRec{0, 0, 0, 0};
+  Walk w;
+  bool work;
+  if constexpr (kKeys) work = w.begin(p, mp.kinds, sh);
+  else work = w.begin(p, mp.kinds, 1, sh);
+  if (!work) return;
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_addr(tslot)),
+                 "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tslot;
+
+  // An item: its A tiles (one or two in use), its B tiles, the K tiles' first key
+  struct Item {
+    int nb, key0, rho0;
+    bool two;
+  };
+  auto item_of = [&](const Walk& x) {
+    Item it;
+    if constexpr (kKeys) {
+      it.nb = x.qt1 - x.qt0;
+      it.key0 = x.kt * MK_KEYS;
+      it.rho0 = x.qt0 * 128;
+      it.two = x.g.klen - it.key0 > 128;
+    } else {
+      it.nb = x.kt1 - x.kt0;
+      it.key0 = x.kt0 * 128;
+      it.rho0 = x.qt * M;
+      it.two = kTwo && x.g.n * p.rep - it.rho0 > 128;
+    }
+    return it;
+  };
+
+  if (warp == 0) {  // ---- K tiles
+    const int psize = 1 << p.page_log2, box = min(psize, 128), parts = 128 / box;
+    const int part = lane / HALVES, half = lane % HALVES, at = half * (128 * 128) + part * box * 128;
+    int pos = 0;
+    do {
+      const Item it = item_of(w);
+      const int nt = kKeys ? 2 : it.nb;
+      PageWindow win;
+      win.start(p, w.g, it.key0 >> p.page_log2, lane);
+      for (int t = 0; t < nt; ++t, ++pos) {
+        const int s = pos % KS, first = (it.key0 + t * 128) >> p.page_log2;
+        win.seek(p, first, lane);
+        const int page = __shfl_sync(0xffffffffu, win.cur, (first - win.base + part) & 31);
+        if (lane == 0) {
+          if (pos >= KS) paged_wait(k_empty + s, ((pos / KS) - 1) & 1, dead, p.err);
+          if (!*dead) mbar_arrive_expect_tx(k_full + s, L::kTile);
+        }
+        __syncwarp();
+        if (*dead) break;
+        if (part < parts)
+          tma_load_5d(ks + size_t(s) * L::kTile + at, &tk, 0, (it.key0 + t * 128) & (psize - 1), half, w.head, page, k_full + s);
+        __syncwarp();
+      }
+    } while (!*dead && w.next(p, mp.kinds));
+    // shared memory must outlive the copies
+    if (lane == 0)
+      for (int q = max(0, pos - KS); q < pos; ++q)
+        if (!mbar_wait(k_full + q % KS, (q / KS) & 1)) raise_error(p.err, kErrTimeout);
+  } else if (warp == 1) {  // ---- products: the warp walks together, one lane issues
+    constexpr uint32_t id = umma_idesc_bf16_m128(128, 0);
+    const bool issuer = elect_one();
+    const uint32_t k_lo = umma_lo(smem_addr(ks), 1), q_lo = umma_lo(smem_addr(qs), 1);
+    int kpos = 0, qpos = 0;
+    int ns0 = 0, ns1 = 0;  // products of each group
+    auto product = [&](int group, int kslot, int qslot) {
+      const int i = group ? ns1++ : ns0++, buf = group * 2 + (i & 1);
+      if (i >= 2) paged_wait(s_empty + buf, ((i >> 1) - 1) & 1, dead, p.err);
+      tc_fence_after();
+      if (issuer) {
+        const uint32_t kt = k_lo + kslot * (L::kTile / 16), qt = q_lo + qslot * (L::kTile / 16);
+        const uint32_t a = kKeys ? kt : qt, b = kKeys ? qt : kt;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_ss(tmem + buf * 128, a + (kk / 4) * (128 * 128 / 16) + (kk % 4) * 2, b + (kk / 4) * (128 * 128 / 16) + (kk % 4) * 2,
+                  id, kk != 0);
+        umma_commit(s_full + buf);
+      }
+    };
+    auto done = [&](uint64_t* bar) {
+      if (issuer) umma_commit(bar);
+    };
+    do {
+      const Item it = item_of(w);
+      const int ka = kpos, qa = qpos;  // the item's A tiles
+      if constexpr (kKeys) {
+        for (int a = 0; a < 2; ++a, ++kpos) paged_wait(k_full + kpos % KS, (kpos / KS) & 1, dead, p.err);
+      } else {
+        for (int a = 0; a < (kTwo ? 2 : 1); ++a, ++qpos) paged_wait(q_full + qpos % QS, (qpos / QS) & 1, dead, p.err);
+      }
+      for (int t = 0; t < it.nb && !*dead; ++t) {
+        if constexpr (kKeys) {
+          const int s = qpos % QS;
+          paged_wait(q_full + s, (qpos / QS) & 1, dead, p.err);
+          ++qpos;
+          product(0, ka % KS, s);
+          if (it.two) product(1, (ka + 1) % KS, s);
+          done(q_empty + s);
+        } else {
+          const int s = kpos % KS;
+          paged_wait(k_full + s, (kpos / KS) & 1, dead, p.err);
+          ++kpos;
+          if constexpr (kTwo) {
+            product(0, s, qa % QS);
+            if (it.two) product(1, s, (qa + 1) % QS);
+          } else {
+            product(t & 1, s, qa % QS);
+          }
+          done(k_empty + s);
+        }
+      }
+      if constexpr (kKeys) {
+        for (int a = 0; a < 2; ++a) done(k_empty + (ka + a) % KS);
+      } else {
+        for (int a = 0; a < (kTwo ? 2 : 1); ++a) done(q_empty + (qa + a) % QS);
+      }
+    } while (!*dead && w.next(p, mp.kinds));
+    done(drain);  // tensor memory is given back only when nothing writes it any more
+    if (!mbar_wait(drain, 0)) raise_error(p.err, kErrTimeout);
+    __syncwarp();
+  } else if (warp < 4) {  // ---- Q tiles: two warps, 64 rows each, 16 or 8 lanes a row
+    constexpr int CH = D / 8, RPI = 32 / CH;
+    const int r0 = (warp - 2) * 64, c = lane % CH;
+    int pos = 0;
+    do {
+      const Item it = item_of(w);
+      const int nt = kKeys ? it.nb : kTwo ? 2 : 1;
+      for (int t = 0; t < nt && !*dead; ++t, ++pos) {
+        const int s = pos % QS;
+        long long from[2];
+        float minus_l[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const PagedRow r = paged_row(p, w.g, w.head, it.rho0 + t * 128 + r0 + e * 32 + lane);
+          from[e] = r.valid ? r.tok * p.q_row + r.h * p.q_head : -1;
+          if constexpr (kKeys) {
+            // 2^(s - M) / sum = 2^(s - (M - log2(1 / sum))); a row that sees nothing weighs nothing
+            const float2 ml = r.valid ? mp.row_ml[(long long)r.tok * p.H + r.h] : make_float2(0.f, 0.f);
+            minus_l[e] = log2f(ml.y) - ml.x;
+          }
+        }
+        if (pos >= QS) paged_wait(q_empty + s, ((pos / QS) - 1) & 1, dead, p.err);
+        if (*dead) break;
+        unsigned char* dst = qs + size_t(s) * L::kTile + (c / 8) * (128 * 128) + r0 * 128;
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll 4
+          for (int k = 0; k < 32; k += RPI) {
+            const int row = k + lane / CH;
+            const long long at = __shfl_sync(0xffffffffu, from[e], row);
+            cp_async16(dst + (e * 32 + row) * 128 + (((c & 7) ^ (row & 7)) << 4),
+                       static_cast<const uint16_t*>(p.q) + (at < 0 ? 0 : at) + c * 8, at < 0 ? 0 : 16);
+          }
+        cp_async_commit();
+        if constexpr (kKeys) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) nl[s * 128 + r0 + e * 32 + lane] = minus_l[e];
+        }
+        cp_async_wait<0>();
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full + s);
+      }
+    } while (!*dead && w.next(p, mp.kinds));
+  } else {  // ---- sums: a thread has a lane of its group's products
+    const int group = (warp - 4) >> 2, qd = warp & 3, r128 = qd * 32 + lane;
+    const uint32_t ts = tmem + (uint32_t(qd * 32) << 16) + group * 256;
+    const float sl2 = p.scale_log2;
+    int ns = 0, qpos = 0, nitem = 0;
+    auto scores = [&]() {  // waits for the group's next product; its columns
+      const int buf = ns & 1;
+      paged_wait(s_full + group * 2 + buf, (ns >> 1) & 1, dead, p.err);
+      tc_fence_after();
+      return ts + buf * 128;
+    };
+    auto scores_read = [&]() {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_empty + group * 2 + (ns & 1));
+      ++ns;
+    };
+    if constexpr (kKeys) {
+      do {
+        const Item it = item_of(w);
+        const bool active = group == 0 || it.two;
+        const int key = it.key0 + group * 128 + r128;
+        const bool mine = key < w.g.klen;
+        float* to = nullptr;
+        float was = 0.f;
+        if (mine && w.count == 1) {
+          const int page = paged_page(p, w.g, key >> p.page_log2);
+          if (page >= 0) {
+            to = mp.mass.ptr + page * mp.mass.page + w.head * mp.mass.head + (key & ((1 << p.page_log2) - 1));
+            if (mp.add && key < w.g.klen - w.g.n) was = *to;
+          }
+        }
+        // rows from this one on see the key
+        const long long see = (long long)max(0, key - (w.g.klen - w.g.n)) * p.rep;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < it.nb; ++t, ++qpos) {
+          const int s = qpos % QS;
+          paged_wait(q_full + s, (qpos / QS) & 1, dead, p.err);
+          if (active && !__any_sync(0xffffffffu, *dead)) {  // tensor memory is read by whole warps
+            const uint32_t cols = scores();
+            const float* row = nl + s * 128;
+            const int hide = int(min(see - (it.rho0 + t * 128), 128ll));  // columns before this one do not see the key
+            if (__any_sync(0xffffffffu, hide > 0)) {
+#pragma unroll 1
+              for (int c = 0; c < 128; c += 32) {
+                uint32_t v[32];
+                tmem_ld32(cols + c, v);
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                  const float4 l4 = *reinterpret_cast<const float4*>(row + c + i);
+                  const float x[4] = {l4.x, l4.y, l4.z, l4.w};
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    const float y = ex2_approx(fmaf(__uint_as_float(v[i + e]), sl2, x[e]));
+                    sum[e] += c + i + e >= hide ? y : 0.f;
+                  }
+                }
+              }
+            } else {
+#pragma unroll 1
+              for (int c = 0; c < 128; c += 32) {
+                uint32_t v[32];
+                tmem_ld32(cols + c, v);
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                  const float4 l4 = *reinterpret_cast<const float4*>(row + c + i);
+                  sum[0] += ex2_approx(fmaf(__uint_as_float(v[i]), sl2, l4.x));
+                  sum[1] += ex2_approx(fmaf(__uint_as_float(v[i + 1]), sl2, l4.y));
+                  sum[2] += ex2_approx(fmaf(__uint_as_float(v[i + 2]), sl2, l4.z));
+                  sum[3] += ex2_approx(fmaf(__uint_as_float(v[i + 3]), sl2, l4.w));
+                }
+              }
+            }
+            scores_read();
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(q_empty + s);
+        }
+        if (*dead) break;
+        const float total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (w.count == 1) {
+          if (to) *to = was + total;
+        } else {
+          mp.part_sum[((long long)blockIdx.x * 2 + w.slot()) * MK_KEYS + group * 128 + r128] = total;
+          if (warp == 4 && lane == 0 && w.slot() == 1) mp.keys_rec[blockIdx.x] = MassRec{w.seg, w.head, w.kt, w.count};
+        }
+      } while (w.next(p, mp.kinds));
+    } else {
+      do {
+        const Item it = item_of(w);
+        const PagedRow r = paged_row(p, w.g, w.head, it.rho0 + (kTwo ? group * 128 : 0) + r128);
+        const int lim = r.valid ? r.lim : 0x7fffffff;  // rows that pad the tile see everything, for nobody
+        float m = -INFINITY, l = 0.f;
+        if (!kTwo || group == 0 || it.two) {
+          for (int t = kTwo ? 0 : group; t < it.nb; t += kTwo ? 1 : 2) {
+            const uint32_t cols = scores();
+            if (__any_sync(0xffffffffu, *dead)) break;
+            const int key0 = it.key0 + t * 128;
+            const bool masked = __any_sync(0xffffffffu, key0 + 128 > lim);
+#pragma unroll 1
+            for (int c = 0; c < 128; c += 32) {
+              uint32_t v[32];
+              tmem_ld32(cols + c, v);
+              if (masked) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (key0 + c + i >= lim) v[i] = 0xff800000u;
+              }
+              float mx = fmaxf(__uint_as_float(v[0]), __uint_as_float(v[1]));
+#pragma unroll
+              for (int i = 2; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(v[i]));
+              const float mn = fmaxf(m, mx * sl2), mg = mn == -INFINITY ? 0.f : mn;
+              float sum[4] = {l * ex2_approx(m - mg), 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int i = 0; i < 32; ++i) sum[i & 3] += ex2_approx(fmaf(__uint_as_float(v[i]), sl2, -mg));
+              l = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+              m = mn;
+            }
+            scores_read();
+          }
+        }
+        if (*dead) break;
+        if (!kTwo) {  // the groups' states
+          const int xb = nitem & 1, xn = nitem >> 1;
+          if (group == 1) {
+            if (xn > 0) paged_wait(x_empty + xb, (xn - 1) & 1, dead, p.err);
+            xml[xb * 128 + r128] = make_float2(m, l);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(x_full + xb);
+          } else {
+            paged_wait(x_full + xb, xn & 1, dead, p.err);
+            const float2 y = xml[xb * 128 + r128];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(x_empty + xb);
+            const float mn = fmaxf(m, y.x), mg = mn == -INFINITY ? 0.f : mn;
+            l = l * ex2_approx(m - mg) + y.y * ex2_approx(y.x - mg);
+            m = mn;
+          }
+          ++nitem;
+        }
+        if (warp == 4 && lane == 0) w.report(p);
+        if (r.valid && (kTwo || group == 0)) {
+          if (w.count == 1) mp.row_ml[(long long)r.tok * p.H + r.h] = mass_row(m, l);
+          else mp.part_ml[((long long)blockIdx.x * 2 + w.slot()) * M + (kTwo ? group * 128 : 0) + r128] = make_float2(m, l);
+        }
+      } while (w.next(p, mp.kinds));
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+// Adds up the parts of divided key tiles, in order: one block a tile, a thread a key.
+__global__ void __launch_bounds__(MK_KEYS) mass_fold_kernel(const __grid_constant__ MassParams mp) {
+  const PagedAttnParams& p = mp.a;
+  pdl_wait();
+  pdl_launch_dependents();
+  const MassRec rec = mp.keys_rec[blockIdx.x];
+  if (rec.count == 0) return;
+  const PagedSeg g = paged_seg(p, mp.kinds, rec.request);
+  const int key = rec.kt * MK_KEYS + threadIdx.x;
+  if (key >= g.klen) return;
+  const int page = paged_page(p, g, key >> p.page_log2);
+  if (page < 0) return;
+  float sum = 0.f;
+  for (int i = 0; i < rec.count; ++i)
+    sum += mp.part_sum[((long long)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * MK_KEYS + threadIdx.x];
+  float* to = mp.mass.ptr + page * mp.mass.page + rec.head * mp.mass.head + (key & ((1 << p.page_log2) - 1));
+  *to = (mp.add && key < g.klen - g.n ? *to : 0.f) + sum;
 }
 
 // ---------------------------------------------------------------------------- eviction
