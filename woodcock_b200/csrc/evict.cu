@@ -39,7 +39,7 @@ struct MassLayout {
   bool few, many;        // requests of at most 16 rows a KV head, of more
   int blocks, few_blocks, per, width;
   MassModes rows, keys;
-  size_t row_ml, part_ml, rec, tiles, few_part, scores, part_sum, keys_rec, bytes;
+  size_t row_ml, part_ml, rec, tiles, few_ml, few_part, scores, part_sum, keys_rec, bytes;
 };
 
 MassLayout mass_layout(const wc_ctx* ctx, const wc_paged_mass_args& a) {
@@ -52,12 +52,13 @@ MassLayout mass_layout(const wc_ctx* ctx, const wc_paged_mass_args& a) {
   l.few = g.dtype == WC_BF16 && (b.q_offsets || each <= 16);
   l.many = g.dtype != WC_BF16 || each > 16;
   if (l.few) {
-    l.few_blocks = ctx->num_sms * MF_PER_SM;
-    l.width = int(std::min(16ll, (each + 1) & ~1ll));
+    l.few_blocks = ctx->num_sms;
+    l.width = int(std::min(16ll, each));
     const long long units = mass_most_tiles(g.pages, log2i(g.page_size), b.requests, g.kv_heads, MF_KT) +
                             (long long)b.requests * g.kv_heads * MF_OVER;
     l.per = int((units + l.few_blocks - 1) / l.few_blocks);
-    l.few_part = take(at, size_t(l.few_blocks) * 2 * MF_M * sizeof(float2));
+    l.few_ml = take(at, size_t(b.rows) * b.heads * MF_CONSUMERS * sizeof(float2));
+    l.few_part = take(at, size_t(l.few_blocks) * 2 * MF_M * MF_CONSUMERS * sizeof(float2));
     l.scores = take(at, size_t(l.few_blocks) * l.per * MF_KT * l.width * sizeof(float));
   }
   l.row_ml = take(at, size_t(b.rows) * b.heads * sizeof(float2));
@@ -86,16 +87,30 @@ void check_mass_args(const wc_paged_mass_args& a) {
   need(std::isfinite(a.scale) && a.scale > 0, "paged_mass: scale must be positive");
 }
 
+template <int D, int NT>
+void launch_few_rows(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, const MassParams& p, int blocks) {
+  constexpr size_t smem = MfLayout<D>::bytes();
+  static_assert(smem <= kSmemOptinBytes, "shared memory");
+  opt_in(ctx, mass_few_rows_kernel<D, NT>, smem);
+  launch_on(ctx, st, "mass_few_rows", mass_few_rows_kernel<D, NT>, dim3(blocks), dim3(MF_THREADS), smem, true, 1,
+            page_map(g, p.a.K, MF_KT, D / 64), p);
+}
+
 template <int D>
-void gather_few(wc_ctx* ctx, cudaStream_t st, MassParams p, const MassLayout& l, char* ws) {
+void gather_few(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, MassParams p, const MassLayout& l, char* ws) {
   p.kinds = kOwnRows | kFewRows;
+  p.row_ml = reinterpret_cast<float2*>(ws + l.few_ml);
   p.part_ml = reinterpret_cast<float2*>(ws + l.few_part);
   p.scores = reinterpret_cast<float*>(ws + l.scores);
   p.per = l.per;
   p.width = l.width;
-  launch_on(ctx, st, "mass_few_rows", l.width <= 8 ? mass_few_rows_kernel<D, 1> : mass_few_rows_kernel<D, 2>,
-            dim3(l.few_blocks), dim3(MF_THREADS), 0, true, 1, p);
-  launch_on(ctx, st, "mass_few_keys", mass_few_keys_kernel, dim3(l.few_blocks), dim3(MF_THREADS), 0, true, 1, p);
+  if (l.width <= 8) launch_few_rows<D, 1>(ctx, st, g, p, l.few_blocks);
+  else launch_few_rows<D, 2>(ctx, st, g, p, l.few_blocks);
+  // four sums at a time where they lie on 16 bytes
+  const bool wide = reinterpret_cast<uintptr_t>(p.mass.ptr) % 16 == 0 && (g.pages == 1 || p.mass.page % 4 == 0) &&
+                    (g.kv_heads == 1 || p.mass.head % 4 == 0);
+  launch_on(ctx, st, "mass_few_keys", mass_few_keys_kernel, dim3(l.few_blocks, MF_SPREAD), dim3(MF_KEYS_THREADS), 0, true, 1, p,
+            wide);
 }
 
 template <int D, int kMode>
@@ -123,7 +138,7 @@ void gather_many(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, MassParams p, 
 template <typename S, int D>
 void gather_mass(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, MassParams p, const MassLayout& l, char* ws) {
   if constexpr (sizeof(S) == 2) {
-    if (l.few) gather_few<D>(ctx, st, p, l, ws);
+    if (l.few) gather_few<D>(ctx, st, g, p, l, ws);
     p.kinds = kOwnRows | (l.few ? kManyRows : 0);
     if (l.many) gather_many<D>(ctx, st, g, p, l, ws);
   } else {

@@ -34,8 +34,8 @@ struct MassParams {
   long long* tiles;      // [B + 1]: key tiles before each request (all of its heads')
   int blocks;            // of the statistics' launch
   int kinds;             // which requests' rows
-  float* scores;         // few rows: [blocks][per][64 keys][width], log2 units
-  int per, width;        // key tiles of a block at most, scores of a key at most
+  float* scores;         // few rows: [blocks][per tiles][width rows][64 keys], log2 units
+  int per, width;        // key tiles of a block at most, rows of a tile at most
   float* part_sum;       // many rows: [blocks][2][256], of divided key tiles
   MassRec* keys_rec;     // [blocks]: the divided key tile that begins in the block
   int key_blocks;
@@ -294,32 +294,105 @@ __global__ void __launch_bounds__(MS_THREADS) mass_keys_kernel(const __grid_cons
 }
 
 // ---- few rows (bf16 pages, at most 16 a KV head: steps and accepted chains)
-// K's bytes bound the time, so it is read once. The first kernel takes scores (keys as the products' rows,
-// mma m16n8k16) and keeps them, 4 bytes a key and row beside the key's 2 head_dim; the second, on the same
-// shares, turns them into weights and adds them up. K goes from memory to registers without a detour: a
-// product sums over head_dim in any order, so a lane's 16 consecutive bytes of a key serve as the places
-// that the operand's layout gives it, if the query's are taken alike. A warp has 16 keys at a time, 4 KB on
-// their way.
-constexpr int MF_THREADS = 256, MF_M = 16, MF_KT = 64, MF_OVER = 2, MF_PER_SM = 2;
+// K's bytes bound the time, so it is read once. The first kernel takes scores (keys as the products' rows, mma
+// m16n8k16) and keeps them, 4 bytes a key and row beside the key's 2 head_dim; the second, on the same
+// shares, turns them into weights and adds them up. A producer streams tiles of 64 keys (TMA, 128-byte
+// swizzle) through a ring that fills shared memory: the bytes on their way do not depend on how an SM
+// happens to be split between L1 and shared memory. Two sets of four warps take the tiles in turn, 16 keys a
+// warp; four producers, since one takes about 800 clocks a tile whatever its bytes. Each warp keeps its own
+// maximum and sum. A product sums over head_dim in any order, so a lane's
+// 16 consecutive bytes of a key serve as the places that the operand's layout gives it, if the query's are
+// taken alike: no operand is rearranged.
+constexpr int MF_CONSUMERS = 8, MF_PRODUCERS = 4, MF_THREADS = 32 * (MF_CONSUMERS + MF_PRODUCERS), MF_M = 16, MF_KT = 64, MF_OVER = 2;
+constexpr int MF_SPREAD = 4, MF_KEYS_THREADS = 256;  // blocks of the second kernel for one of the first
+
+template <int D>
+struct MfLayout {
+  static constexpr int kStage = MF_KT * D * 2;
+  static constexpr int kTail = 8 * kWalkShared + 16 + 24 * 16;
+  static constexpr int kFit = (int(kSmemOptinBytes) - 1024 - kTail) / kStage;
+  // a multiple of the sets and of the producers: a stage is always of the same ones, which then see each phase
+  static constexpr int kStages = (kFit < 24 ? kFit : 24) / MF_PRODUCERS * MF_PRODUCERS;
+  static constexpr size_t bytes() { return 1024 + size_t(kStages) * kStage + kTail; }
+};
+
+// The warps' states of an item that lies in one block, and of a divided one's parts.
+__device__ __forceinline__ long long mass_whole_at(const PagedAttnParams& p, const PagedSeg& g, int head, int r) {
+  const int i = r / p.rep;
+  return ((long long)(g.tok0 + i) * p.H + head * p.rep + r - i * p.rep) * MF_CONSUMERS;
+}
 
 template <int D, int NT>
-__global__ void __launch_bounds__(MF_THREADS, MF_PER_SM) mass_few_rows_kernel(const __grid_constant__ MassParams mp) {
+__global__ void __launch_bounds__(MF_THREADS, 1)
+    mass_few_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ MassParams mp) {
   const PagedAttnParams& p = mp.a;
-  constexpr int NV = D / 32;  // 16-byte pieces of a key in a lane
-  __shared__ long long sh[kWalkShared];
-  __shared__ float2 wml[MF_THREADS / 32][8 * NT];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3;
+  using L = MfLayout<D>;
+  constexpr int NV = D / 32, NST = L::kStages;  // 16-byte pieces of a key in a lane
+  extern __shared__ unsigned char mf_raw[];
+  unsigned char* ring = mf_raw + ((1024u - (smem_addr(mf_raw) & 1023u)) & 1023u);
+  unsigned char* tail = ring + size_t(NST) * L::kStage;
+  long long* sh = reinterpret_cast<long long*>(tail);
+  volatile int* dead = reinterpret_cast<volatile int*>(tail + 8 * kWalkShared);
+  uint64_t* full = reinterpret_cast<uint64_t*>(tail + 8 * kWalkShared + 16);
+  uint64_t* empty = full + NST;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int s = 0; s < NST; ++s) {
+      mbar_init(full + s, 1);
+      mbar_init(empty + s, MF_CONSUMERS / 2);
+    }
+    mbar_fence_init();
+    *dead = 0;
+  }
   pdl_wait();
   pdl_launch_dependents();
+  __syncthreads();
   PagedWalk<MF_M, MF_KT, MF_OVER> w;
   if (!w.begin(p, mp.kinds, 1, sh)) return;
   if (w.per > mp.per) {  // more keys than the pool holds: requests share pages
     if (tid == 0) raise_error(p.err, kErrPage);
     return;
   }
+  int pos = 0, last = -1;  // tiles of the block before the item's; a producer's last one
+  if (warp >= MF_CONSUMERS) {  // ---- producers: every fourth tile
+    const int psize = 1 << p.page_log2, box = min(psize, MF_KT), parts = MF_KT / box;
+    do {
+      PageWindow win;
+      win.start(p, w.g, (w.kt0 * MF_KT) >> p.page_log2, lane);
+      const int nt = (min(w.kt1 * MF_KT, w.g.klen) - w.kt0 * MF_KT + MF_KT - 1) / MF_KT;
+      for (int t = (warp - pos) & (MF_PRODUCERS - 1); t < nt; t += MF_PRODUCERS) {
+        const int at = pos + t, s = at % NST, key0 = (w.kt0 + t) * MF_KT, first = key0 >> p.page_log2;
+        win.seek(p, first, lane);
+        const int page = __shfl_sync(0xffffffffu, win.cur, (first - win.base + lane) & 31);
+        if (lane == 0) {
+          if (at >= NST) paged_wait(empty + s, ((at / NST) - 1) & 1, dead, p.err);
+          if (!*dead) mbar_arrive_expect_tx(full + s, L::kStage);
+        }
+        __syncwarp();
+        if (*dead) break;
+        if (lane < parts)
+          tma_load_5d(ring + size_t(s) * L::kStage + lane * box * (D * 2), &tk, 0, key0 & (psize - 1), 0, w.head, page, full + s);
+        __syncwarp();
+        last = at;
+      }
+      pos += nt;
+    } while (!*dead && w.next(p, mp.kinds));
+    // shared memory must outlive the copies: the latest of this warp's, and those before it where nobody waited
+    if (lane == 0)
+      for (int q = max((warp - MF_CONSUMERS) & (MF_PRODUCERS - 1), last - NST + MF_PRODUCERS); q <= last; q += MF_PRODUCERS)
+        if (!mbar_wait(full + q % NST, (q / NST) & 1)) raise_error(p.err, kErrTimeout);
+    return;
+  }
+  // ---- scores: lane (g8, t4) has keys of a slice and 16-byte pieces t4, t4 + 4, ... of them. Which keys is free:
+  // neighbours in g8 are four rows apart, where the swizzle has them in different banks.
+  const int g8 = lane >> 2, t4 = lane & 3, kr = (g8 >> 1) | ((g8 & 1) << 2);
+  const int set = warp >> 2, slice = (warp & 3) * 16, vlog = min(p.page_log2, 6);
+  // the slice's rows in a tile: the copy that holds them, and the place in it
+  const int in_copy = (slice & ((1 << vlog) - 1)) + kr;
+  const int off = (slice >> vlog) * (D * 2 << vlog) + in_copy * 128, half = 128 << vlog;
   float* buf = mp.scores + (long long)blockIdx.x * mp.per * MF_KT * mp.width;
   do {
-    const int R = min(w.g.n * p.rep, 8 * NT), stride = (R + 1) & ~1;
+    const int R = min(w.g.n * p.rep, 8 * NT);
     uint4 q[NT][NV];
     int lim[NT][2];
     float m[NT][2], l[NT][2];
@@ -338,89 +411,73 @@ __global__ void __launch_bounds__(MF_THREADS, MF_PER_SM) mass_few_rows_kernel(co
         l[t][e] = 0.f;
       }
     }
-    const int end = min(w.kt1 * MF_KT, w.g.klen);
-    int key0 = w.kt0 * MF_KT + warp * 16;
-    int page = key0 < end ? paged_page(p, w.g, key0 >> p.page_log2) : -1;
-    for (; key0 < end; key0 += 16 * (MF_THREADS / 32)) {
+    const int nt = (min(w.kt1 * MF_KT, w.g.klen) - w.kt0 * MF_KT + MF_KT - 1) / MF_KT;
+    for (int t = (pos ^ set) & 1; t < nt; t += 2) {
+      const int s = (pos + t) % NST;
+      paged_wait(full + s, ((pos + t) / NST) & 1, dead, p.err);
+      const unsigned char* k = ring + size_t(s) * L::kStage + off;
       uint4 a[NV], b[NV];
-      if (page >= 0) {
-        const uint16_t* k = static_cast<const uint16_t*>(p.K.ptr) + page * p.K.page + w.head * p.K.head +
-                            ((key0 & ((1 << p.page_log2) - 1)) + g8) * p.K.row + t4 * 8;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          a[i] = ldg_stream(reinterpret_cast<const uint4*>(k + i * 32));
-          b[i] = ldg_stream(reinterpret_cast<const uint4*>(k + 8 * p.K.row + i * 32));
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) a[i] = b[i] = make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i / 2) * half + ((((i & 1) * 4 + t4) ^ kr) << 4);
+        a[i] = *reinterpret_cast<const uint4*>(k + c);
+        b[i] = *reinterpret_cast<const uint4*>(k + 8 * 128 + c);
       }
-      const int next = key0 + 16 * (MF_THREADS / 32);
-      page = next < end ? paged_page(p, w.g, next >> p.page_log2) : -1;
       float c[NT][4];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        c[t][0] = c[t][1] = c[t][2] = c[t][3] = 0.f;
+      for (int n = 0; n < NT; ++n) {
+        c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-          mma_bf16_16816(c[t], make_uint4(a[i].x, b[i].x, a[i].y, b[i].y), q[t][i].x, q[t][i].y);
-          mma_bf16_16816(c[t], make_uint4(a[i].z, b[i].z, a[i].w, b[i].w), q[t][i].z, q[t][i].w);
+          mma_bf16_16816(c[n], make_uint4(a[i].x, b[i].x, a[i].y, b[i].y), q[n][i].x, q[n][i].y);
+          mma_bf16_16816(c[n], make_uint4(a[i].z, b[i].z, a[i].w, b[i].w), q[n][i].z, q[n][i].w);
         }
       }
-      float* to = buf + (key0 - w.kt0 * MF_KT + g8) * stride + 2 * t4;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty + s);
+      const int key = (w.kt0 + t) * MF_KT + slice + kr;
+      float* to = buf + (size_t)t * MF_KT * mp.width + slice + kr;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float z0 = key0 + g8 < lim[t][e] ? c[t][e] * p.scale_log2 : -INFINITY;
-          const float z1 = key0 + g8 + 8 < lim[t][e] ? c[t][2 + e] * p.scale_log2 : -INFINITY;
-          c[t][e] = z0;
-          c[t][2 + e] = z1;
-          const float mn = fmaxf(m[t][e], fmaxf(z0, z1)), mg = mn == -INFINITY ? 0.f : mn;
-          l[t][e] = l[t][e] * ex2_approx(m[t][e] - mg) + (ex2_approx(z0 - mg) + ex2_approx(z1 - mg));
-          m[t][e] = mn;
+          const float z0 = key < lim[n][e] ? c[n][e] * p.scale_log2 : -INFINITY;
+          const float z1 = key + 8 < lim[n][e] ? c[n][2 + e] * p.scale_log2 : -INFINITY;
+          const int row = n * 8 + 2 * t4 + e;
+          if (row < R) {
+            to[row * MF_KT] = z0;
+            to[row * MF_KT + 8] = z1;
+          }
+          const float mn = fmaxf(m[n][e], fmaxf(z0, z1)), mg = mn == -INFINITY ? 0.f : mn;
+          l[n][e] = l[n][e] * ex2_approx(m[n][e] - mg) + (ex2_approx(z0 - mg) + ex2_approx(z1 - mg));
+          m[n][e] = mn;
         }
-        if (t * 8 + 2 * t4 < R) {
-          *reinterpret_cast<float2*>(to + t * 8) = make_float2(c[t][0], c[t][1]);
-          *reinterpret_cast<float2*>(to + 8 * stride + t * 8) = make_float2(c[t][2], c[t][3]);
-        }
-      }
     }
-    // one state a row: the lanes that share it, then the warps
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
         for (int o = 4; o < 32; o *= 2) {
-          const float m2 = __shfl_xor_sync(0xffffffffu, m[t][e], o), l2 = __shfl_xor_sync(0xffffffffu, l[t][e], o);
-          const float mn = fmaxf(m[t][e], m2), mg = mn == -INFINITY ? 0.f : mn;
-          l[t][e] = l[t][e] * ex2_approx(m[t][e] - mg) + l2 * ex2_approx(m2 - mg);
-          m[t][e] = mn;
+          const float m2 = __shfl_xor_sync(0xffffffffu, m[n][e], o), l2 = __shfl_xor_sync(0xffffffffu, l[n][e], o);
+          const float mn = fmaxf(m[n][e], m2), mg = mn == -INFINITY ? 0.f : mn;
+          l[n][e] = l[n][e] * ex2_approx(m[n][e] - mg) + l2 * ex2_approx(m2 - mg);
+          m[n][e] = mn;
         }
-        if (g8 == 0) wml[warp][t * 8 + 2 * t4 + e] = make_float2(m[t][e], l[t][e]);
+        const int row = n * 8 + 2 * t4 + e;
+        if (g8 == 0 && row < R) {
+          float2* at = w.count == 1 ? mp.row_ml + mass_whole_at(p, w.g, w.head, row)
+                                    : mp.part_ml + (((long long)blockIdx.x * 2 + w.slot()) * MF_M + row) * MF_CONSUMERS;
+          at[warp] = make_float2(m[n][e], l[n][e]);
+        }
       }
-    __syncthreads();
-    if (tid < R) {
-      float M = -INFINITY, L = 0.f;
-#pragma unroll
-      for (int i = 0; i < MF_THREADS / 32; ++i) {
-        const float2 y = wml[i][tid];
-        const float mn = fmaxf(M, y.x), mg = mn == -INFINITY ? 0.f : mn;
-        L = L * ex2_approx(M - mg) + y.y * ex2_approx(y.x - mg);
-        M = mn;
-      }
-      const PagedRow r = paged_row(p, w.g, w.head, tid);
-      if (w.count == 1) mp.row_ml[(long long)r.tok * p.H + r.h] = mass_row(M, L);
-      else mp.part_ml[((long long)blockIdx.x * 2 + w.slot()) * MF_M + tid] = make_float2(M, L);
-    }
-    __syncthreads();
-    buf += (w.kt1 - w.kt0) * MF_KT * mp.width;
+    buf += (size_t)nt * MF_KT * mp.width;
+    pos += nt;
   } while (w.next(p, mp.kinds));
 }
 
-// The scores' weights, added up: a thread a key, on the shares of the kernel before.
-__global__ void __launch_bounds__(MF_THREADS) mass_few_keys_kernel(const __grid_constant__ MassParams mp) {
+// The scores' weights, added up: a thread has four keys, MF_SPREAD blocks share what one block before had.
+__global__ void __launch_bounds__(MF_KEYS_THREADS) mass_few_keys_kernel(const __grid_constant__ MassParams mp, bool wide) {
   const PagedAttnParams& p = mp.a;
   __shared__ long long sh[kWalkShared];
   __shared__ float2 ml[MF_M];
@@ -432,50 +489,66 @@ __global__ void __launch_bounds__(MF_THREADS) mass_few_keys_kernel(const __grid_
   if (!work || w.per > mp.per) return;
   const float* buf = mp.scores + (long long)blockIdx.x * mp.per * MF_KT * mp.width;
   do {
-    const int R = min(w.g.n * p.rep, MF_M), stride = (R + 1) & ~1;
-    const int row = tid >> 4, part = tid & 15;
-    if (w.count == 1) {
-      if (tid < R) {
-        const PagedRow r = paged_row(p, w.g, w.head, tid);
-        ml[tid] = mp.row_ml[(long long)r.tok * p.H + r.h];
-      }
-    } else {
-      float M = -INFINITY, L = 0.f;
-      if (row < R)
-        for (int i = part; i < w.count; i += 16) {
-          const float2 y = mp.part_ml[((long long)(w.first + i) * 2 + (i == 0 ? 1 : 0)) * MF_M + row];
-          const float mn = fmaxf(M, y.x), mg = mn == -INFINITY ? 0.f : mn;
-          L = L * ex2_approx(M - mg) + y.y * ex2_approx(y.x - mg);
-          M = mn;
-        }
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, M, o), l2 = __shfl_xor_sync(0xffffffffu, L, o);
-        const float mn = fmaxf(M, m2), mg = mn == -INFINITY ? 0.f : mn;
-        L = L * ex2_approx(M - mg) + l2 * ex2_approx(m2 - mg);
+    const int R = min(w.g.n * p.rep, MF_M), row = tid >> 4, part = tid & 15;
+    float M = -INFINITY, L = 0.f;
+    if (row < R)
+      for (int i = part; i < w.count * MF_CONSUMERS; i += 16) {
+        const int block = i / MF_CONSUMERS;
+        const float2* at = w.count == 1 ? mp.row_ml + mass_whole_at(p, w.g, w.head, row)
+                                        : mp.part_ml + (((long long)(w.first + block) * 2 + (block == 0 ? 1 : 0)) * MF_M + row) * MF_CONSUMERS;
+        const float2 y = at[i % MF_CONSUMERS];
+        const float mn = fmaxf(M, y.x), mg = mn == -INFINITY ? 0.f : mn;
+        L = L * ex2_approx(M - mg) + y.y * ex2_approx(y.x - mg);
         M = mn;
       }
-      if (part == 0) ml[row] = mass_row(M, L);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, M, o), l2 = __shfl_xor_sync(0xffffffffu, L, o);
+      const float mn = fmaxf(M, m2), mg = mn == -INFINITY ? 0.f : mn;
+      L = L * ex2_approx(M - mg) + l2 * ex2_approx(m2 - mg);
+      M = mn;
+    }
+    if (part == 0) ml[row] = mass_row(M, L);
+    __syncthreads();
+    const int key_first = w.kt0 * MF_KT, end = min(w.kt1 * MF_KT, w.g.klen), old = w.g.klen - w.g.n;
+    for (int k = (blockIdx.y * MF_KEYS_THREADS + tid) * 4; key_first + k < end; k += MF_SPREAD * MF_KEYS_THREADS * 4) {
+      const int key = key_first + k;
+      const int page = paged_page(p, w.g, key >> p.page_log2);  // of all four: pages begin at multiples of 16
+      float* to = mp.mass.ptr + page * mp.mass.page + w.head * mp.mass.head + (key & ((1 << p.page_log2) - 1));
+      float was[4] = {0.f, 0.f, 0.f, 0.f};
+      const bool four = wide && key + 4 <= end;
+      if (page >= 0 && mp.add) {
+        if (four && key + 4 <= old) {
+          const float4 y = *reinterpret_cast<const float4*>(to);
+          was[0] = y.x, was[1] = y.y, was[2] = y.z, was[3] = y.w;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (key + e < min(old, end)) was[e] = to[e];
+        }
+      }
+      const float* z = buf + (size_t)(k / MF_KT) * MF_KT * mp.width + k % MF_KT;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+      for (int r = 0; r < R; ++r) {
+        const float4 y = *reinterpret_cast<const float4*>(z + r * MF_KT);
+        const float2 s = ml[r];
+        sum[0] += ex2_approx(y.x - s.x) * s.y;
+        sum[1] += ex2_approx(y.y - s.x) * s.y;
+        sum[2] += ex2_approx(y.z - s.x) * s.y;
+        sum[3] += ex2_approx(y.w - s.x) * s.y;
+      }
+      if (page < 0) continue;
+      if (four) {
+        *reinterpret_cast<float4*>(to) = make_float4(was[0] + sum[0], was[1] + sum[1], was[2] + sum[2], was[3] + sum[3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (key + e < end) to[e] = was[e] + sum[e];
+      }
     }
     __syncthreads();
-    const int end = min(w.kt1 * MF_KT, w.g.klen);
-    for (int key = w.kt0 * MF_KT + tid; key < end; key += MF_THREADS) {
-      const float* z = buf + (key - w.kt0 * MF_KT) * stride;
-      float sum = 0.f;
-      for (int r = 0; r < R; r += 2) {
-        const float2 y = *reinterpret_cast<const float2*>(z + r);
-        sum += ex2_approx(y.x - ml[r].x) * ml[r].y;
-        if (r + 1 < R) sum += ex2_approx(y.y - ml[r + 1].x) * ml[r + 1].y;
-      }
-      const int page = paged_page(p, w.g, key >> p.page_log2);
-      if (page >= 0) {
-        float* to = mp.mass.ptr + page * mp.mass.page + w.head * mp.mass.head + (key & ((1 << p.page_log2) - 1));
-        const float was = mp.add && key < w.g.klen - w.g.n ? *to : 0.f;
-        *to = was + sum;
-      }
-    }
-    __syncthreads();
-    buf += (w.kt1 - w.kt0) * MF_KT * mp.width;
+    buf += (size_t)((end - key_first + MF_KT - 1) / MF_KT) * MF_KT * mp.width;
   } while (w.next(p, mp.kinds));
 }
 
