@@ -37,9 +37,9 @@ wc_pages keys_only(wc_pages g) {
 // Which kernels a call may need: the number of a request's rows is device data where offsets are given.
 struct MassLayout {
   bool few, many;        // requests of at most 16 rows a KV head, of more
-  int blocks, few_blocks, per, width;
+  int blocks, few_blocks, per, width, most;
   MassModes rows, keys;
-  size_t row_ml, part_ml, rec, tiles, few_ml, few_part, scores, part_sum, keys_rec, bytes;
+  size_t row_ml, part_ml, rec, tiles, few_ml, few_part, scores, pieces, part_sum, keys_rec, bytes;
 };
 
 MassLayout mass_layout(const wc_ctx* ctx, const wc_paged_mass_args& a) {
@@ -57,6 +57,8 @@ MassLayout mass_layout(const wc_ctx* ctx, const wc_paged_mass_args& a) {
     const long long units = mass_most_tiles(g.pages, log2i(g.page_size), b.requests, g.kv_heads, MF_KT) +
                             (long long)b.requests * g.kv_heads * MF_OVER;
     l.per = int((units + l.few_blocks - 1) / l.few_blocks);
+    l.most = l.per / (1 + MF_OVER) + 4;  // an item's units but at both ends, and the list's end
+    l.pieces = take(at, size_t(l.few_blocks) * l.most * sizeof(MassPiece));
     l.few_ml = take(at, size_t(b.rows) * b.heads * MF_CONSUMERS * sizeof(float2));
     l.few_part = take(at, size_t(l.few_blocks) * 2 * MF_M * MF_CONSUMERS * sizeof(float2));
     l.scores = take(at, size_t(l.few_blocks) * l.per * MF_KT * l.width * sizeof(float));
@@ -88,12 +90,12 @@ void check_mass_args(const wc_paged_mass_args& a) {
 }
 
 template <int D, int NT>
-void launch_few_rows(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, const MassParams& p, int blocks) {
+void launch_few_rows(wc_ctx* ctx, cudaStream_t st, const MassParams& p, int blocks) {
   constexpr size_t smem = MfLayout<D>::bytes();
   static_assert(smem <= kSmemOptinBytes, "shared memory");
   opt_in(ctx, mass_few_rows_kernel<D, NT>, smem);
   launch_on(ctx, st, "mass_few_rows", mass_few_rows_kernel<D, NT>, dim3(blocks), dim3(MF_THREADS), smem, true, 1,
-            page_map(g, p.a.K, MF_KT, D / 64), p);
+            p);
 }
 
 template <int D>
@@ -104,8 +106,10 @@ void gather_few(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, MassParams p, c
   p.scores = reinterpret_cast<float*>(ws + l.scores);
   p.per = l.per;
   p.width = l.width;
-  if (l.width <= 8) launch_few_rows<D, 1>(ctx, st, g, p, l.few_blocks);
-  else launch_few_rows<D, 2>(ctx, st, g, p, l.few_blocks);
+  p.pieces = reinterpret_cast<MassPiece*>(ws + l.pieces);
+  p.most = l.most;
+  if (l.width <= 8) launch_few_rows<D, 1>(ctx, st, p, l.few_blocks);
+  else launch_few_rows<D, 2>(ctx, st, p, l.few_blocks);
   // four sums at a time where they lie on 16 bytes
   const bool wide = reinterpret_cast<uintptr_t>(p.mass.ptr) % 16 == 0 && (g.pages == 1 || p.mass.page % 4 == 0) &&
                     (g.kv_heads == 1 || p.mass.head % 4 == 0);

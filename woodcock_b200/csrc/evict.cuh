@@ -24,6 +24,15 @@ struct MassRec {
   int request, head, kt, count;  // count 0: none
 };
 
+// What one block of the few rows' first kernel had of an item, for the second; tiles 0: the list's end.
+struct MassPiece {
+  int request, head, key0, tiles;
+  int klen, old, rows;  // keys, those before the new ones, rows of the head
+  int at;               // of the item's first row, whole_ml's
+  int first, count;     // the blocks that share the item
+  int pad[2];
+};
+
 struct MassParams {
   PagedAttnParams a;     // q, K pages, batch
   MassPool mass;
@@ -36,6 +45,8 @@ struct MassParams {
   int kinds;             // which requests' rows
   float* scores;         // few rows: [blocks][per tiles][width rows][64 keys], log2 units
   int per, width;        // key tiles of a block at most, rows of a tile at most
+  MassPiece* pieces;     // [blocks][most]
+  int most;
   float* part_sum;       // many rows: [blocks][2][256], of divided key tiles
   MassRec* keys_rec;     // [blocks]: the divided key tile that begins in the block
   int key_blocks;
@@ -296,11 +307,10 @@ __global__ void __launch_bounds__(MS_THREADS) mass_keys_kernel(const __grid_cons
 // ---- few rows (bf16 pages, at most 16 a KV head: steps and accepted chains)
 // K's bytes bound the time, so it is read once. The first kernel takes scores (keys as the products' rows, mma
 // m16n8k16) and keeps them, 4 bytes a key and row beside the key's 2 head_dim; the second, on the same
-// shares, turns them into weights and adds them up. A producer streams tiles of 64 keys (TMA, 128-byte
-// swizzle) through a ring that fills shared memory: the bytes on their way do not depend on how an SM
-// happens to be split between L1 and shared memory. Two sets of four warps take the tiles in turn, 16 keys a
-// warp; four producers, since one takes about 800 clocks a tile whatever its bytes. Each warp keeps its own
-// maximum and sum. A product sums over head_dim in any order, so a lane's
+// shares, turns them into weights and adds them up. Four producer warps stream tiles of 64 keys
+// (cp.async, 16 bytes a lane) through a ring that fills shared memory: the bytes on their way do not depend
+// on how an SM happens to be split between L1 and shared memory, nor on the pages' size. Two sets of four warps take the tiles in turn, 16 keys a
+// warp; each warp keeps its own maximum and sum. A product sums over head_dim in any order, so a lane's
 // 16 consecutive bytes of a key serve as the places that the operand's layout gives it, if the query's are
 // taken alike: no operand is rearranged.
 constexpr int MF_CONSUMERS = 8, MF_PRODUCERS = 4, MF_THREADS = 32 * (MF_CONSUMERS + MF_PRODUCERS), MF_M = 16, MF_KT = 64, MF_OVER = 2;
@@ -316,15 +326,14 @@ struct MfLayout {
   static constexpr size_t bytes() { return 1024 + size_t(kStages) * kStage + kTail; }
 };
 
-// The warps' states of an item that lies in one block, and of a divided one's parts.
-__device__ __forceinline__ long long mass_whole_at(const PagedAttnParams& p, const PagedSeg& g, int head, int r) {
-  const int i = r / p.rep;
-  return ((long long)(g.tok0 + i) * p.H + head * p.rep + r - i * p.rep) * MF_CONSUMERS;
+// Where the warps' states of an item's rows lie that one block has whole: rows of 8, an item's in a row.
+__device__ __forceinline__ int mass_whole_at(const PagedAttnParams& p, const PagedSeg& g, int head) {
+  return g.tok0 * p.H + head * g.n * p.rep;
 }
 
 template <int D, int NT>
 __global__ void __launch_bounds__(MF_THREADS, 1)
-    mass_few_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ MassParams mp) {
+    mass_few_rows_kernel(const __grid_constant__ MassParams mp) {
   const PagedAttnParams& p = mp.a;
   using L = MfLayout<D>;
   constexpr int NV = D / 32, NST = L::kStages;  // 16-byte pieces of a key in a lane
@@ -338,7 +347,7 @@ __global__ void __launch_bounds__(MF_THREADS, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int s = 0; s < NST; ++s) {
-      mbar_init(full + s, 1);
+      mbar_init(full + s, 32);
       mbar_init(empty + s, MF_CONSUMERS / 2);
     }
     mbar_fence_init();
@@ -348,48 +357,56 @@ __global__ void __launch_bounds__(MF_THREADS, 1)
   pdl_launch_dependents();
   __syncthreads();
   PagedWalk<MF_M, MF_KT, MF_OVER> w;
-  if (!w.begin(p, mp.kinds, 1, sh)) return;
-  if (w.per > mp.per) {  // more keys than the pool holds: requests share pages
-    if (tid == 0) raise_error(p.err, kErrPage);
+  MassPiece* piece = mp.pieces + (long long)blockIdx.x * mp.most;
+  if (!w.begin(p, mp.kinds, 1, sh)) {
+    if (tid == 0) piece->tiles = 0;
     return;
   }
-  int pos = 0, last = -1;  // tiles of the block before the item's; a producer's last one
+  if (w.per > mp.per) {  // more keys than the pool holds: requests share pages
+    if (tid == 0) {
+      raise_error(p.err, kErrPage);
+      piece->tiles = 0;
+    }
+    return;
+  }
+  int pos = 0;  // tiles of the block before the item's
   if (warp >= MF_CONSUMERS) {  // ---- producers: every fourth tile
-    const int psize = 1 << p.page_log2, box = min(psize, MF_KT), parts = MF_KT / box;
+    constexpr int CH = D / 8, RPI = 32 / CH;  // 16-byte pieces of a row, rows a step
+    const int c = lane % CH, r0 = lane / CH;
+    unsigned char* mine = ring + (c / 8) * (MF_KT * 128);
     do {
       PageWindow win;
       win.start(p, w.g, (w.kt0 * MF_KT) >> p.page_log2, lane);
       const int nt = (min(w.kt1 * MF_KT, w.g.klen) - w.kt0 * MF_KT + MF_KT - 1) / MF_KT;
-      for (int t = (warp - pos) & (MF_PRODUCERS - 1); t < nt; t += MF_PRODUCERS) {
+      const uint16_t* head = static_cast<const uint16_t*>(p.K.ptr) + w.head * p.K.head + c * 8;
+      for (int t = (warp - pos) & (MF_PRODUCERS - 1); t < nt && !*dead; t += MF_PRODUCERS) {
         const int at = pos + t, s = at % NST, key0 = (w.kt0 + t) * MF_KT, first = key0 >> p.page_log2;
         win.seek(p, first, lane);
-        const int page = __shfl_sync(0xffffffffu, win.cur, (first - win.base + lane) & 31);
-        if (lane == 0) {
-          if (at >= NST) paged_wait(empty + s, ((at / NST) - 1) & 1, dead, p.err);
-          if (!*dead) mbar_arrive_expect_tx(full + s, L::kStage);
+        if (at >= NST) paged_wait(empty + s, ((at / NST) - 1) & 1, dead, p.err);
+        unsigned char* dst = mine + size_t(s) * L::kStage;
+#pragma unroll
+        for (int k = 0; k < MF_KT; k += 16) {  // 16 rows lie in one page
+          const int key = key0 + k, page = __shfl_sync(0xffffffffu, win.cur, ((key >> p.page_log2) - win.base) & 31);
+          const bool there = page < p.pages;
+          const uint16_t* src = head + (there ? page : 0) * p.K.page + ((key & ((1 << p.page_log2) - 1)) + r0) * p.K.row;
+#pragma unroll
+          for (int i = 0; i < 16; i += RPI) {
+            const int row = k + i + r0;
+            cp_async16(dst + row * 128 + (((c & 7) ^ (row & 7)) << 4), src + i * p.K.row, there ? 16 : 0);
+          }
         }
-        __syncwarp();
-        if (*dead) break;
-        if (lane < parts)
-          tma_load_5d(ring + size_t(s) * L::kStage + lane * box * (D * 2), &tk, 0, key0 & (psize - 1), 0, w.head, page, full + s);
-        __syncwarp();
-        last = at;
+        cp_async_arrive(full + s);
       }
       pos += nt;
     } while (!*dead && w.next(p, mp.kinds));
-    // shared memory must outlive the copies: the latest of this warp's, and those before it where nobody waited
-    if (lane == 0)
-      for (int q = max((warp - MF_CONSUMERS) & (MF_PRODUCERS - 1), last - NST + MF_PRODUCERS); q <= last; q += MF_PRODUCERS)
-        if (!mbar_wait(full + q % NST, (q / NST) & 1)) raise_error(p.err, kErrTimeout);
+    cp_async_commit();
+    cp_async_wait<0>();  // shared memory must outlive the copies
     return;
   }
   // ---- scores: lane (g8, t4) has keys of a slice and 16-byte pieces t4, t4 + 4, ... of them. Which keys is free:
   // neighbours in g8 are four rows apart, where the swizzle has them in different banks.
   const int g8 = lane >> 2, t4 = lane & 3, kr = (g8 >> 1) | ((g8 & 1) << 2);
-  const int set = warp >> 2, slice = (warp & 3) * 16, vlog = min(p.page_log2, 6);
-  // the slice's rows in a tile: the copy that holds them, and the place in it
-  const int in_copy = (slice & ((1 << vlog) - 1)) + kr;
-  const int off = (slice >> vlog) * (D * 2 << vlog) + in_copy * 128, half = 128 << vlog;
+  const int set = warp >> 2, slice = (warp & 3) * 16;
   float* buf = mp.scores + (long long)blockIdx.x * mp.per * MF_KT * mp.width;
   do {
     const int R = min(w.g.n * p.rep, 8 * NT);
@@ -412,14 +429,17 @@ __global__ void __launch_bounds__(MF_THREADS, 1)
       }
     }
     const int nt = (min(w.kt1 * MF_KT, w.g.klen) - w.kt0 * MF_KT + MF_KT - 1) / MF_KT;
+    if (tid == 0 && nt > 0)
+      *piece++ = MassPiece{w.g.idx, w.head, w.kt0 * MF_KT, nt, w.g.klen, w.g.klen - w.g.n, R, mass_whole_at(p, w.g, w.head),
+                           w.first, w.count, {}};
     for (int t = (pos ^ set) & 1; t < nt; t += 2) {
       const int s = (pos + t) % NST;
       paged_wait(full + s, ((pos + t) / NST) & 1, dead, p.err);
-      const unsigned char* k = ring + size_t(s) * L::kStage + off;
+      const unsigned char* k = ring + size_t(s) * L::kStage + (slice + kr) * 128;
       uint4 a[NV], b[NV];
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int c = (i / 2) * half + ((((i & 1) * 4 + t4) ^ kr) << 4);
+        const int c = (i / 2) * (MF_KT * 128) + ((((i & 1) * 4 + t4) ^ kr) << 4);
         a[i] = *reinterpret_cast<const uint4*>(k + c);
         b[i] = *reinterpret_cast<const uint4*>(k + 8 * 128 + c);
       }
@@ -466,7 +486,7 @@ __global__ void __launch_bounds__(MF_THREADS, 1)
         }
         const int row = n * 8 + 2 * t4 + e;
         if (g8 == 0 && row < R) {
-          float2* at = w.count == 1 ? mp.row_ml + mass_whole_at(p, w.g, w.head, row)
+          float2* at = w.count == 1 ? mp.row_ml + (mass_whole_at(p, w.g, w.head) + (long long)row) * MF_CONSUMERS
                                     : mp.part_ml + (((long long)blockIdx.x * 2 + w.slot()) * MF_M + row) * MF_CONSUMERS;
           at[warp] = make_float2(m[n][e], l[n][e]);
         }
@@ -474,33 +494,45 @@ __global__ void __launch_bounds__(MF_THREADS, 1)
     buf += (size_t)nt * MF_KT * mp.width;
     pos += nt;
   } while (w.next(p, mp.kinds));
+  if (tid == 0) piece->tiles = 0;
 }
 
-// The scores' weights, added up: a thread has four keys, MF_SPREAD blocks share what one block before had.
-__global__ void __launch_bounds__(MF_KEYS_THREADS) mass_few_keys_kernel(const __grid_constant__ MassParams mp, bool wide) {
+// The scores' weights, added up: a thread has four keys, MF_SPREAD blocks share what one block before had. Bound
+// by latency: piece -> states -> weights, a few pieces a block.
+__global__ void __launch_bounds__(MF_KEYS_THREADS, 4) mass_few_keys_kernel(const __grid_constant__ MassParams mp, bool wide) {
   const PagedAttnParams& p = mp.a;
-  __shared__ long long sh[kWalkShared];
-  __shared__ float2 ml[MF_M];
-  const int tid = threadIdx.x;
-  PagedWalk<MF_M, MF_KT, MF_OVER> w;
-  const bool work = w.begin(p, mp.kinds, 1, sh);  // of the lengths alone, which no kernel since has written
+  __shared__ float2 ml[2][MF_M];
+  const int tid = threadIdx.x, row = tid >> 4, part = tid & 15;
   pdl_wait();
   pdl_launch_dependents();
-  if (!work || w.per > mp.per) return;
   const float* buf = mp.scores + (long long)blockIdx.x * mp.per * MF_KT * mp.width;
-  do {
-    const int R = min(w.g.n * p.rep, MF_M), row = tid >> 4, part = tid & 15;
+  const MassPiece* pieces = mp.pieces + (long long)blockIdx.x * mp.most;
+  MassPiece g = pieces[0];
+  for (int n = 1; g.tiles > 0; ++n) {
+    const MassPiece next = pieces[n];
+    const int* table = p.table + (long long)g.request * p.table_ld;
+    const int keys = min(g.tiles * MF_KT, g.klen - g.key0), old = mp.add ? g.old : 0;
+    int k = (blockIdx.y * MF_KEYS_THREADS + tid) * 4;
+    // the page of all four (pages begin at multiples of 16); one outside the pool is written nothing
+    int page = k < keys ? table[(g.key0 + k) >> p.page_log2] : -1;
     float M = -INFINITY, L = 0.f;
-    if (row < R)
-      for (int i = part; i < w.count * MF_CONSUMERS; i += 16) {
-        const int block = i / MF_CONSUMERS;
-        const float2* at = w.count == 1 ? mp.row_ml + mass_whole_at(p, w.g, w.head, row)
-                                        : mp.part_ml + (((long long)(w.first + block) * 2 + (block == 0 ? 1 : 0)) * MF_M + row) * MF_CONSUMERS;
-        const float2 y = at[i % MF_CONSUMERS];
-        const float mn = fmaxf(M, y.x), mg = mn == -INFINITY ? 0.f : mn;
-        L = L * ex2_approx(M - mg) + y.y * ex2_approx(y.x - mg);
-        M = mn;
+    if (row < g.rows) {
+      if (g.count == 1) {
+        if (part < MF_CONSUMERS) {
+          const float2 y = mp.row_ml[(g.at + (long long)row) * MF_CONSUMERS + part];
+          M = y.x;
+          L = y.y;
+        }
+      } else {
+        for (int i = part; i < g.count * MF_CONSUMERS; i += 16) {
+          const int block = i / MF_CONSUMERS;
+          const float2 y = mp.part_ml[((((long long)g.first + block) * 2 + (block == 0 ? 1 : 0)) * MF_M + row) * MF_CONSUMERS + i % MF_CONSUMERS];
+          const float mn = fmaxf(M, y.x), mg = mn == -INFINITY ? 0.f : mn;
+          L = L * ex2_approx(M - mg) + y.y * ex2_approx(y.x - mg);
+          M = mn;
+        }
       }
+    }
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) {
       const float m2 = __shfl_xor_sync(0xffffffffu, M, o), l2 = __shfl_xor_sync(0xffffffffu, L, o);
@@ -508,48 +540,50 @@ __global__ void __launch_bounds__(MF_KEYS_THREADS) mass_few_keys_kernel(const __
       L = L * ex2_approx(M - mg) + l2 * ex2_approx(m2 - mg);
       M = mn;
     }
-    if (part == 0) ml[row] = mass_row(M, L);
-    __syncthreads();
-    const int key_first = w.kt0 * MF_KT, end = min(w.kt1 * MF_KT, w.g.klen), old = w.g.klen - w.g.n;
-    for (int k = (blockIdx.y * MF_KEYS_THREADS + tid) * 4; key_first + k < end; k += MF_SPREAD * MF_KEYS_THREADS * 4) {
-      const int key = key_first + k;
-      const int page = paged_page(p, w.g, key >> p.page_log2);  // of all four: pages begin at multiples of 16
-      float* to = mp.mass.ptr + page * mp.mass.page + w.head * mp.mass.head + (key & ((1 << p.page_log2) - 1));
+    if (part == 0) ml[n & 1][row] = mass_row(M, L);
+    __syncthreads();  // and the other buffer's readers have passed the one before
+    while (k < keys) {
+      const float* z = buf + (size_t)(k / MF_KT) * MF_KT * mp.width + k % MF_KT;
+      const int key = g.key0 + k;
+      float* to = nullptr;
       float was[4] = {0.f, 0.f, 0.f, 0.f};
-      const bool four = wide && key + 4 <= end;
-      if (page >= 0 && mp.add) {
+      const bool four = wide && k + 4 <= keys;
+      if (page >= 0 && page < p.pages) {
+        to = mp.mass.ptr + page * mp.mass.page + g.head * mp.mass.head + (key & ((1 << p.page_log2) - 1));
         if (four && key + 4 <= old) {
           const float4 y = *reinterpret_cast<const float4*>(to);
           was[0] = y.x, was[1] = y.y, was[2] = y.z, was[3] = y.w;
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (key + e < min(old, end)) was[e] = to[e];
+            if (key + e < old && k + e < keys) was[e] = to[e];
         }
       }
-      const float* z = buf + (size_t)(k / MF_KT) * MF_KT * mp.width + k % MF_KT;
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-      for (int r = 0; r < R; ++r) {
+      for (int r = 0; r < g.rows; ++r) {
         const float4 y = *reinterpret_cast<const float4*>(z + r * MF_KT);
-        const float2 s = ml[r];
+        const float2 s = ml[n & 1][r];
         sum[0] += ex2_approx(y.x - s.x) * s.y;
         sum[1] += ex2_approx(y.y - s.x) * s.y;
         sum[2] += ex2_approx(y.z - s.x) * s.y;
         sum[3] += ex2_approx(y.w - s.x) * s.y;
       }
-      if (page < 0) continue;
-      if (four) {
-        *reinterpret_cast<float4*>(to) = make_float4(was[0] + sum[0], was[1] + sum[1], was[2] + sum[2], was[3] + sum[3]);
-      } else {
+      if (to) {
+        if (four) {
+          *reinterpret_cast<float4*>(to) = make_float4(was[0] + sum[0], was[1] + sum[1], was[2] + sum[2], was[3] + sum[3]);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (key + e < end) to[e] = was[e] + sum[e];
+          for (int e = 0; e < 4; ++e)
+            if (k + e < keys) to[e] = was[e] + sum[e];
+        }
       }
+      k += MF_SPREAD * MF_KEYS_THREADS * 4;
+      if (k < keys) page = table[(g.key0 + k) >> p.page_log2];
     }
-    __syncthreads();
-    buf += (size_t)((end - key_first + MF_KT - 1) / MF_KT) * MF_KT * mp.width;
-  } while (w.next(p, mp.kinds));
+    buf += (size_t)g.tiles * MF_KT * mp.width;
+    g = next;
+  }
 }
 
 // ---- many rows (bf16 pages, more than 16 a KV head: windows and prompts)
