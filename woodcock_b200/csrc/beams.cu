@@ -10,18 +10,24 @@ using namespace wc;
 namespace {
 
 struct SelectLayout {
-  int pieces;
-  size_t stat, cand, bytes;
+  int pieces, rounds;
+  size_t stat, cand, counts, bytes;
 };
 
-SelectLayout select_layout(const wc_beam_select_args& a) {
+SelectLayout select_layout(const wc_ctx* ctx, const wc_beam_select_args& a) {
   SelectLayout l;
   std::memset(&l, 0, sizeof(l));
-  l.pieces = (a.vocab + BS_PIECE - 1) / BS_PIECE;
   const size_t rows = size_t(a.requests) * a.beams;
+  // A piece's first round costs as much as four later ones, and a piece of many leaves blocks idle at the end: as many
+  // rounds as leave three pieces for each place on the device.
+  const long long in_row = (a.vocab + BS_ROUND - 1) / BS_ROUND, places = ctx->num_sms * 4ll;
+  l.rounds = int(std::min(in_row, std::max(1ll, (long long)rows * in_row / (3 * places))));
+  l.pieces = int((in_row + l.rounds - 1) / l.rounds);
+  l.rounds = int((in_row + l.pieces - 1) / l.pieces);
   size_t at = 0;
   l.stat = take(at, rows * l.pieces * sizeof(double2));
-  l.cand = take(at, rows * l.pieces * a.n * sizeof(unsigned long long));
+  l.cand = take(at, rows * l.pieces * 2 * a.n * sizeof(unsigned long long));
+  l.counts = take(at, rows * l.pieces * sizeof(int));
   l.bytes = at;
   return l;
 }
@@ -43,7 +49,7 @@ extern "C" wc_status wc_beam_select_workspace(wc_ctx* ctx, const wc_beam_select_
   if (!ctx || !a || !bytes) return WC_ERR_INVALID;
   return guard(ctx, [&] {
     check_select(*a);
-    *bytes = select_layout(*a).bytes;
+    *bytes = select_layout(ctx, *a).bytes;
   });
 }
 
@@ -55,7 +61,7 @@ extern "C" wc_status wc_beam_select(wc_ctx* ctx, void* stream, const wc_beam_sel
     need(a->logits && reinterpret_cast<uintptr_t>(a->logits) % e == 0, "beam_select: null or misaligned logits");
     need(a->request_stride >= 0 && a->beam_stride >= 0, "beam_select: negative stride");
     need(a->scores && a->out_scores && a->out_parents && a->out_tokens, "beam_select: null argument");
-    const SelectLayout l = select_layout(*a);
+    const SelectLayout l = select_layout(ctx, *a);
     if (!a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 256 || a->workspace_bytes < l.bytes)
       fail(WC_ERR_CAPACITY, "beam_select: workspace missing, misaligned or too small");
     const long long rows = (long long)a->requests * a->beams, places = (long long)a->requests * a->n;
@@ -82,9 +88,11 @@ extern "C" wc_status wc_beam_select(wc_ctx* ctx, void* stream, const wc_beam_sel
     p.V = a->vocab;
     p.n = a->n;
     p.pieces = l.pieces;
+    p.rounds = l.rounds;
     p.pad = a->pad;
     p.stat = reinterpret_cast<double2*>(ws + l.stat);
     p.cand = reinterpret_cast<unsigned long long*>(ws + l.cand);
+    p.counts = reinterpret_cast<int*>(ws + l.counts);
     p.out_scores = a->out_scores;
     p.out_parents = a->out_parents;
     p.out_tokens = a->out_tokens;

@@ -11,19 +11,20 @@ namespace wc {
 // score(w, v) = s_w + (z_wv - lse_w), lse_w = log sum_v exp z_wv, the n best of a request's W x V, ties to
 // the lower beam, then to the lower token.
 //
-// Every logit is read once. A block takes a piece of one beam's row into registers (32 values a thread),
-// leaves the piece's maximum and sum of exponentials, and its n best: n of the threads' maxima are at
-// least some T, so at least n values are, and few more; those are collected and ranked among one
-// another. The second kernel, one block a request, has each beam's lse and does the same with the
-// candidates' scores.
+// Every logit is read once. A block has a piece of one beam's row, a few rounds of 32 values a thread; four
+// blocks an SM, so that some load while others work. The first round gives a bound: the n-th of the threads'
+// maxima, which n values at least reach; what reaches it, then and later, is collected, and the piece leaves
+// at least its n best and its sum of exponentials. The second kernel, one block a request, has each beam's lse
+// and does the same with the candidates' scores.
 //
-// Ranks are decided in 64 bits. Two beams' scores may lie closer than a 32-bit sum resolves: a score near -20
-// has steps of 2^-19, and with 64 x 16 neighbours in rank a step apart now and then. The exponentials
-// are of 32 bits, but with arguments corrected to 2^-30, and their sum's error averages over the row.
+// Ranks are decided in 64 bits: two beams' scores may lie closer than a 32-bit sum resolves, as a score near -20
+// has steps of 2^-19. The exponentials are of 32 bits, 2^(z log2(e) - R) with an integer R, so that sums with
+// other R are joined without a rounding and only the exponent's own counts: 2^-20 of a term that is e^-11 or
+// less, less nearer to the maximum; over a row's terms it averages to 2^-25 or so in lse.
 constexpr int BS_THREADS = 256;
-constexpr int BS_PER = 32;                       // values a thread
-constexpr int BS_PIECE = BS_THREADS * BS_PER;    // values a block
-constexpr int BS_LIST = BS_THREADS * 4;          // a piece of fewer values fits whole
+constexpr int BS_PER = 32;                       // values a thread and round
+constexpr int BS_ROUND = BS_THREADS * BS_PER;
+constexpr int BS_LIST = 1024;
 constexpr int BS_MAX_N = 64;
 constexpr int BS_MAX_W = 64;
 constexpr int BJ_THREADS = 512;
@@ -34,27 +35,15 @@ struct BeamSelectParams {
   long long request, beam;  // strides in elements
   const float* scores;      // [B][W]
   const uint8_t* finished;  // [B][W] or null
-  int B, W, V, n, pieces, pad;
+  int B, W, V, n, pieces, rounds, pad;
   // workspace
-  double2* stat;            // [B W][pieces]: maximum, sum of exponentials (NaN: a logit that is not a number or +inf)
-  unsigned long long* cand; // [B W][pieces][n]: argmax_key of value and token, best first; 0: none
+  double2* stat;            // [B W][pieces]: R and the sum of 2^(z log2(e) - R); sum 0: no token, not finite: no numbers
+  unsigned long long* cand; // [B W][pieces][2 n]: argmax_key of value and token, in any order
+  int* counts;              // [B W][pieces]
   float* out_scores;        // [B][n]
   int *out_parents, *out_tokens;
   int* err;
 };
-
-// e^(z - m), z <= m: what z - m and log2(e) lose to rounding is added back, so that the exponent is right to
-// 2^-30 of its size. Below e^-100 nothing is left beside the maximum's 1.
-__device__ __forceinline__ float exp_diff(float z, float m) {
-  const float d = z - m, v = d - z;  // d + e = z - m exactly
-  const float e = (z - (d - v)) - (m + v);
-  constexpr float kHi = 1.44269502162933349609375f, kLo = 1.925963033500966e-08f;  // log2(e), 24 bits and the rest
-  const float t = d * kHi;
-  const float r = fmaf(d, kHi, -t) + fmaf(d, kLo, e * kHi);
-  // 2^(t + r), r below 2^-18: 2^r = 1 + r ln 2
-  const float x = ex2_approx(t);
-  return d > -100.f ? fmaf(x, r * 0.69314718f, x) : 0.f;
-}
 
 // What a beam proposes: 0 nothing (it is dead, or its score is no number), 1 its tokens, 2 itself (it has ended).
 __device__ __forceinline__ int beam_kind(const BeamSelectParams& p, long long row) {
@@ -62,157 +51,234 @@ __device__ __forceinline__ int beam_kind(const BeamSelectParams& p, long long ro
   return !(score > -INFINITY && score < INFINITY) ? 0 : p.finished && p.finished[row] ? 2 : 1;
 }
 
-// The j-th largest of a warp's keys (0: there is none).
-__device__ __forceinline__ uint32_t warp_jth(uint32_t key, int j, int lane) {
-  uint32_t top = 0;
-  for (int i = 0; i < j; ++i) {
-    top = __reduce_max_sync(0xffffffffu, key);
-    const uint32_t who = __ballot_sync(0xffffffffu, key == top);
-    if (lane == __ffs(who) - 1) key = 0;
+// A bound that the keys of n threads of a block reach, and of few more; 1 where fewer threads have a key (0: none).
+// Halves the span between the lowest key and the highest.
+template <int kThreads>
+__device__ __forceinline__ uint32_t reached_by(uint32_t key, int n, uint32_t* s_low, uint32_t* s_high) {
+  const uint32_t wl = __reduce_min_sync(0xffffffffu, key ? key : 0xffffffffu), wh = __reduce_max_sync(0xffffffffu, key);
+  if (threadIdx.x % 32 == 0) {
+    s_low[threadIdx.x / 32] = wl;
+    s_high[threadIdx.x / 32] = wh;
   }
-  return top;
+  if (__syncthreads_count(key != 0) < n) return 1;
+  uint32_t low = s_low[0], high = s_high[0];
+#pragma unroll
+  for (int i = 1; i < kThreads / 32; ++i) {
+    low = min(low, s_low[i]);
+    high = max(high, s_high[i]);
+  }
+#pragma unroll 1
+  while (high - low > 64) {  // keys 64 apart are as good as one: the bound stays at or below the n-th
+    const uint32_t mid = low + (high - low) / 2 + 1;
+    const int c = __syncthreads_count(key >= mid);
+    if (c >= n) low = mid;
+    else high = mid - 1;
+    if (c >= n && c <= n + n / 4) break;
+  }
+  return low;
 }
 
-// N values from i on; -inf behind the row's end. A row that does not begin on a 16-byte boundary is read value by
-// value, so that its sum has the order of any other's: beams that are alike stay tied.
+// 16 bytes of a row, four fp32 or eight bf16 values.
 template <typename T>
-__device__ __forceinline__ void load_logits(const T* row, bool whole, int i, int V, float (&x)[16 / sizeof(T)]) {
-  constexpr int N = 16 / sizeof(T);
-  if (whole && i + N <= V) {
-    if constexpr (N == 4) {
-      const float4 a = ldg_stream_f4(reinterpret_cast<const float4*>(row + i));
-      x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
+struct Logits {
+  static constexpr int N = 16 / sizeof(T);
+  uint4 w;
+  __device__ __forceinline__ float at(int k) const {
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+    if constexpr (N == 4) return __uint_as_float(x[k]);
+    else return __uint_as_float(k & 1 ? x[k / 2] & 0xffff0000u : x[k / 2] << 16);
+  }
+  __device__ __forceinline__ void load(const T* row, int i) { w = ldg_stream(reinterpret_cast<const uint4*>(row + i)); }
+  // Values from i on; -inf behind the row's end. A row that does not begin on a 16-byte boundary is read value by
+  // value, so that its sum has the order of any other's: beams that are alike stay tied.
+  __device__ __forceinline__ void load_edge(const T* row, bool whole, int i, int V) {
+    if (whole && i + N <= V) {
+      load(row, i);
     } else {
-      const uint4 a = ldg_stream(reinterpret_cast<const uint4*>(row + i));
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+      uint32_t x[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        x[2 * k] = __uint_as_float(w[k] << 16);
-        x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+        if constexpr (N == 4) {
+          x[k] = i + k < V ? __float_as_uint(row[i + k]) : 0xff800000u;
+        } else {
+          const uint32_t lo = i + 2 * k < V ? row[i + 2 * k] : 0xff80u, hi = i + 2 * k + 1 < V ? row[i + 2 * k + 1] : 0xff80u;
+          x[k] = lo | (hi << 16);
+        }
       }
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      x[k] = -INFINITY;
-      if (i + k < V) {
-        if constexpr (N == 4) x[k] = row[i + k];
-        else x[k] = bf16_bits_to_f32(row[i + k]);
-      }
+      w = make_uint4(x[0], x[1], x[2], x[3]);
     }
   }
+};
+
+// Too many values at the bound (equal ones, or values in few threads): the n best of a row's [first, end), the n-th
+// found bit by bit. Reads the values again, so that the way that is always taken does not keep them.
+template <typename T>
+__device__ __noinline__ void beam_pieces_again(const T* z, int first, int end, float bound, int n, unsigned long long* list,
+                                               uint32_t* s_sum, int* s_count) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  auto key = [&](int i) -> unsigned long long {
+    float x;
+    if constexpr (sizeof(T) == 4) x = z[i];
+    else x = bf16_bits_to_f32(z[i]);
+    return x >= bound ? argmax_key(x + 0.f, uint32_t(i)) : 0;
+  };
+  unsigned long long nth = 0;
+#pragma unroll 1
+  for (int bit = 63; bit >= 0; --bit) {
+    const unsigned long long probe = nth | (1ull << bit);
+    int c = 0;
+    for (int i = first + tid; i < end; i += BS_THREADS) c += key(i) >= probe;
+    c = __reduce_add_sync(0xffffffffu, c);
+    __syncthreads();
+    if (lane == 0) s_sum[warp] = c;
+    __syncthreads();
+    c = 0;
+    for (int i = 0; i < BS_THREADS / 32; ++i) c += s_sum[i];
+    if (c >= n) nth = probe;
+  }
+  __syncthreads();
+  if (tid == 0) *s_count = 0;
+  __syncthreads();
+  for (int i = first + tid; i < end; i += BS_THREADS) {
+    const unsigned long long k = key(i);
+    if (k >= nth) list[atomicAdd(s_count, 1)] = k;  // n of them: keys differ
+  }
+  __syncthreads();
+}
+
+// A piece whose maximum's product with log2(e) is no number, or so low that all else counts as nothing (a type's
+// lowest value in every place): its sum relative to the maximum itself, for thread 0.
+template <typename T>
+__device__ __noinline__ double beam_piece_extreme(const T* z, int first, int end, float m, double* s_sum) {
+  double sum = 0;
+  for (int i = first + int(threadIdx.x); i < end; i += BS_THREADS) {
+    float x;
+    if constexpr (sizeof(T) == 4) x = z[i];
+    else x = bf16_bits_to_f32(z[i]);
+    sum += ex2_approx((x - m) * kLog2e);
+  }
+  sum = warp_sum_d(sum);
+  __syncthreads();
+  if (threadIdx.x % 32 == 0) s_sum[threadIdx.x / 32] = sum;
+  __syncthreads();
+  sum = 0;
+  for (int i = 0; i < BS_THREADS / 32; ++i) sum += s_sum[i];
+  return sum;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(BS_THREADS) beam_pieces_kernel(const __grid_constant__ BeamSelectParams p) {
+__global__ void __launch_bounds__(BS_THREADS, 4) beam_pieces_kernel(const __grid_constant__ BeamSelectParams p) {
   constexpr int N = 16 / sizeof(T), NV = BS_PER / N, WARPS = BS_THREADS / 32;
   __shared__ unsigned long long list[BS_LIST];
-  __shared__ float s_max[WARPS];
+  __shared__ float s_max[WARPS], s_ref[WARPS];
   __shared__ double s_sum[WARPS];
-  __shared__ uint32_t s_key[WARPS];
-  __shared__ int s_count, s_bad;
+  __shared__ uint32_t s_key[2 * WARPS];
+  __shared__ int s_count;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int row = blockIdx.x / p.pieces, piece = blockIdx.x - row * p.pieces;
   const int b = row / p.W;
   const T* z = static_cast<const T*>(p.logits) + b * p.request + (row - b * p.W) * p.beam;
-  if (tid == 0) s_count = s_bad = 0;
+  if (tid == 0) s_count = 0;
   pdl_wait();
   pdl_launch_dependents();
   if (beam_kind(p, row) != 1) return;  // its logits do not matter
   const bool whole = (reinterpret_cast<unsigned long long>(z) & 15) == 0;
-  const int first = piece * BS_PIECE;
-  float x[NV][N];
+  const int first = piece * p.rounds * BS_ROUND, end = min(first + p.rounds * BS_ROUND, p.V);
+  float best = -INFINITY, ref = -2e30f, sum[4] = {0.f, 0.f, 0.f, 0.f}, bound = 0.f;
+#pragma unroll 1
+  for (int at = first; at < end; at += BS_ROUND) {
+    Logits<T> x[NV];
+    if (whole && at + BS_ROUND <= p.V) {
 #pragma unroll
-  for (int v = 0; v < NV; ++v) load_logits<T>(z, whole, first + (v * BS_THREADS + tid) * N, p.V, x[v]);
-  float top = -INFINITY;
-  bool bad = false;
+      for (int v = 0; v < NV; ++v) x[v].load(z, at + (v * BS_THREADS + tid) * N);
+    } else {
 #pragma unroll
-  for (int v = 0; v < NV; ++v)
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      bad |= !(x[v][k] < INFINITY);
-      x[v][k] += 0.f;  // -0 ranks with +0
-      top = fmaxf(top, x[v][k]);
+      for (int v = 0; v < NV; ++v) x[v].load_edge(z, whole, at + (v * BS_THREADS + tid) * N, p.V);
     }
-  const uint32_t mine = uint32_t(argmax_key(top, 0) >> 32);
-  const uint32_t jth = warp_jth(mine, (p.n + WARPS - 1) / WARPS, lane);
-  const float wtop = warp_max(top);
-  if (lane == 0) {
-    s_max[warp] = wtop;
-    s_key[warp] = jth;
-  }
-  __syncthreads();
-  if (bad) s_bad = 1;
-  float m = s_max[0];
-  uint32_t least = s_key[0];
+    float vtop[NV], top = -INFINITY;
 #pragma unroll
-  for (int i = 1; i < WARPS; ++i) {
-    m = fmaxf(m, s_max[i]);
-    least = min(least, s_key[i]);
-  }
-  const float bound = argmax_key_value((unsigned long long)(max(least, 0x00800000u)) << 32);  // above -inf
-  float sum = 0.f;
-  const float mg = m == -INFINITY ? 0.f : m;
+    for (int v = 0; v < NV; ++v) {
+      vtop[v] = fmaxf(x[v].at(0), x[v].at(1));
 #pragma unroll
-  for (int v = 0; v < NV; ++v)
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      if (x[v][k] > -INFINITY) sum += exp_diff(x[v][k], mg);
-      if (x[v][k] >= bound) {
-        const int at = atomicAdd(&s_count, 1);
-        if (at < BS_LIST) list[at] = argmax_key(x[v][k], uint32_t(first + (v * BS_THREADS + tid) * N + k));
-      }
+      for (int k = 2; k < N; ++k) vtop[v] = fmaxf(vtop[v], x[v].at(k));
+      top = fmaxf(top, vtop[v]);
     }
-  const double ws = warp_sum_d(double(sum));
-  if (lane == 0) s_sum[warp] = ws;
-  __syncthreads();
-  unsigned long long* out = p.cand + (long long)blockIdx.x * p.n;
-  if (tid == 0) {
-    double s = 0;
-    for (int i = 0; i < WARPS; ++i) s += s_sum[i];
-    if (s_bad) raise_error(p.err, kErrLogits);
-    p.stat[blockIdx.x] = make_double2(m, s_bad ? NAN : s);
-  }
-  int count = s_count;
-  if (count > BS_LIST) {
-    // Too many values at the bound (equal ones, or values in few threads): the n-th best key, bit by bit.
-    unsigned long long nth = 0;
-    for (int bit = 63; bit >= 0; --bit) {
-      const unsigned long long probe = nth | (1ull << bit);
-      int c = 0;
+    best = fmaxf(best, top);
+    const float r = fmaxf(ref, ceilf(top * kLog2e));
+    if (r > ref) {
+      const float less = ex2_approx(ref - r);  // of integers: exact
 #pragma unroll
-      for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int k = 0; k < N; ++k)
-          c += x[v][k] >= bound && argmax_key(x[v][k], uint32_t(first + (v * BS_THREADS + tid) * N + k)) >= probe;
-      c = __reduce_add_sync(0xffffffffu, c);
-      __syncthreads();
-      if (lane == 0) s_key[warp] = c;
-      __syncthreads();
-      c = 0;
-      for (int i = 0; i < WARPS; ++i) c += s_key[i];
-      if (c >= p.n) nth = probe;
+      for (int k = 0; k < 4; ++k) sum[k] *= less;
+      ref = r;
     }
-    __syncthreads();
-    if (tid == 0) s_count = 0;
-    __syncthreads();
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const unsigned long long key = argmax_key(x[v][k], uint32_t(first + (v * BS_THREADS + tid) * N + k));
-        if (x[v][k] >= bound && key >= nth) list[atomicAdd(&s_count, 1)] = key;  // n of them: keys differ
+      for (int k = 0; k < N; ++k) sum[k & 3] += ex2_approx(fmaf(x[v].at(k), kLog2e, -ref));
+    if (at == first)  // n threads' maxima are at the bound or above; -inf is not
+      bound = argmax_key_value((unsigned long long)(max(reached_by<BS_THREADS>(uint32_t(argmax_key(top + 0.f, 0) >> 32), p.n,
+                                                                               s_key, s_key + WARPS), 0x00800000u)) << 32);
+    if (top >= bound) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        if (vtop[v] >= bound) {
+#pragma unroll
+          for (int k = 0; k < N; ++k)
+            if (x[v].at(k) >= bound) {
+              const int to = atomicAdd(&s_count, 1);
+              // -0 ranks with +0
+              if (to < BS_LIST) list[to] = argmax_key(x[v].at(k) + 0.f, uint32_t(at + (v * BS_THREADS + tid) * N + k));
+            }
+        }
       }
-    __syncthreads();
+    }  }
+  {
+    const float wref = warp_max(ref), wbest = warp_max(best);
+    const double s = warp_sum_d(double((sum[0] + sum[1]) + (sum[2] + sum[3])) * double(ex2_approx(ref - wref)));
+    if (lane == 0) {
+      s_sum[warp] = s;
+      s_ref[warp] = wref;
+      s_max[warp] = wbest;
+    }
+  }
+  __syncthreads();
+  unsigned long long* out = p.cand + (long long)blockIdx.x * 2 * p.n;
+  float m = s_max[0], R = s_ref[0];
+#pragma unroll
+  for (int i = 1; i < WARPS; ++i) {
+    m = fmaxf(m, s_max[i]);
+    R = fmaxf(R, s_ref[i]);
+  }
+  double total = 0, reference = R;
+  if (fabsf(m) > 1e30f && fabsf(m) < INFINITY) {
+    total = beam_piece_extreme(z, first, end, m, s_sum);
+    reference = double(m) * 1.4426950408889634;
+  } else if (tid == 0) {
+    for (int i = 0; i < WARPS; ++i) total += s_sum[i] * double(ex2_approx(s_ref[i] - R));
+  }
+  if (tid == 0) {
+    if (!(total < INFINITY)) raise_error(p.err, kErrLogits);
+    p.stat[blockIdx.x] = make_double2(reference, total);
+  }
+  int count = s_count;
+  if (count > BS_LIST) {
+    beam_pieces_again(z, first, end, bound, p.n, list, s_key, &s_count);
     count = s_count;
   }
-  for (int i = tid; i < count; i += BS_THREADS) {
-    const unsigned long long key = list[i];
-    int rank = 0;
-    for (int k = 0; k < count; ++k) rank += list[k] > key;
-    if (rank < p.n) out[rank] = key;
+  if (tid == 0) p.counts[blockIdx.x] = count <= 2 * p.n ? count : p.n;
+  if (count <= 2 * p.n) {  // as they are
+    if (tid < count) out[tid] = list[tid];
+    return;
   }
-  for (int i = count + tid; i < p.n; i += BS_THREADS) out[i] = 0;
+  for (int i0 = 0; i0 < count; i0 += BS_THREADS / 4) {  // the n best, four lanes a candidate
+    const int i = i0 + tid / 4;
+    const unsigned long long key = i < count ? list[i] : ~0ull;
+    int rank = 0;
+    for (int k = tid % 4; k < count; k += 4) rank += list[k] > key;
+    rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+    rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+    if (i < count && rank < p.n && tid % 4 == 0) out[rank] = key;
+  }
 }
 
 // A double's order as an unsigned number.
@@ -231,7 +297,7 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const __grid_cons
   __shared__ uint32_t place[BJ_LIST];       // beam * V + token
   __shared__ double s_score[BS_MAX_W], s_lse[BS_MAX_W];
   __shared__ int s_kind[BS_MAX_W];
-  __shared__ uint32_t s_key[WARPS];
+  __shared__ int s_sum[WARPS];
   __shared__ int s_count;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, b = blockIdx.x;
   if (tid == 0) s_count = 0;
@@ -241,85 +307,83 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const __grid_cons
     const double2* st = p.stat + row * p.pieces;
     const int kind = beam_kind(p, row);
     double m = -INFINITY, s = 0;
-    for (int i = lane; kind == 1 && i < p.pieces; i += 32) {
-      const double2 y = st[i];
-      const double mn = fmax(m, y.x);
-      if (!(y.x == -INFINITY && y.y == 0)) s = s * exp(m - mn) + y.y * exp(y.x - mn);
-      m = mn;
-    }
+    if (kind == 1) {
+      for (int i = lane; i < p.pieces; i += 32)
+        if (st[i].y != 0) m = fmax(m, st[i].x);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const double m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-      const double mn = fmax(m, m2);
-      if (mn > -INFINITY) s = s * exp(m - mn) + s2 * exp(m2 - mn);
-      m = mn;
+      for (int o = 16; o > 0; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
+      for (int i = lane; i < p.pieces; i += 32) {
+        const double2 y = st[i];
+        if (y.y != 0) s += y.y * exp2(y.x - m);
+      }
+      s = warp_sum_d(s);
     }
     if (lane == 0) {
       const float score = p.scores[row];
       if (!(score < INFINITY)) raise_error(p.err, kErrLogits);
       s_score[w] = score;
-      s_lse[w] = m + log(s);
-      s_kind[w] = kind != 1 || (m > -INFINITY && s > 0) ? kind : 0;  // not without a token, nor where s is no number
+      s_lse[w] = m * 0.69314718055994530942 + log(s);
+      s_kind[w] = kind != 1 || (s > 0 && s < INFINITY) ? kind : 0;  // not without a token, nor where s is no number
     }
   }
   __syncthreads();
-  const int per = p.pieces * p.n, total = p.W * per;
-  const unsigned long long* cand = p.cand + (long long)b * total;
-  // candidate i: its score's order (0: none) and its place
-  auto look = [&](int i, uint32_t& at) -> unsigned long long {
-    const int w = i / per, kind = s_kind[w];
-    if (kind == 1) {
-      const unsigned long long c = cand[i];
-      if (!c) return 0;
-      at = uint32_t(w) * uint32_t(p.V) + argmax_key_index(c);
-      return order_of(s_score[w] + (double(argmax_key_value(c)) - s_lse[w]));
+  // A warp goes through lists, a lane through their places: f(score's order, place) for every candidate.
+  const int slots = 2 * p.n, lists = p.W * p.pieces;
+  const unsigned long long* cand = p.cand + (long long)b * lists * slots;
+  const int* counts = p.counts + (long long)b * lists;
+  auto each = [&](auto f) {
+    for (int l0 = warp; l0 < lists; l0 += 2 * WARPS) {
+      unsigned long long c[2][4];
+      int m[2], w[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int l = l0 + u * WARPS;
+        w[u] = l < lists ? l / p.pieces : 0;
+        m[u] = l < lists && s_kind[w[u]] == 1 ? counts[l] : 0;
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (lane + 32 * k < m[u]) c[u][k] = cand[(long long)(l0 + u * WARPS) * slots + lane + 32 * k];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (lane + 32 * k < m[u])
+            f(order_of(s_score[w[u]] + (double(argmax_key_value(c[u][k])) - s_lse[w[u]])),
+              uint32_t(w[u]) * uint32_t(p.V) + argmax_key_index(c[u][k]));
     }
-    if (kind == 2 && i == w * per) {
-      at = uint32_t(w) * uint32_t(p.V) + uint32_t(p.pad);
-      return order_of(s_score[w]);
-    }
-    return 0;
+    for (int w = tid; w < p.W; w += BJ_THREADS)
+      if (s_kind[w] == 2) f(order_of(s_score[w]), uint32_t(w) * uint32_t(p.V) + uint32_t(p.pad));
   };
   uint32_t top = 0;
-  for (int i = tid; i < total; i += BJ_THREADS) {
-    uint32_t at;
-    top = max(top, uint32_t(look(i, at) >> 32));
-  }
-  const uint32_t jth = warp_jth(top, (p.n + WARPS - 1) / WARPS, lane);
-  if (lane == 0) s_key[warp] = jth;
-  __syncthreads();
-  uint32_t least = s_key[0];
-#pragma unroll
-  for (int i = 1; i < WARPS; ++i) least = min(least, s_key[i]);
-  least = max(least, 1u);
-  for (int i = tid; i < total; i += BJ_THREADS) {
-    uint32_t at;
-    const unsigned long long k = look(i, at);
-    if (uint32_t(k >> 32) >= least) {
-      const int to = atomicAdd(&s_count, 1);
-      if (to < BJ_LIST) {
-        key[to] = k;
-        place[to] = at;
+  each([&](unsigned long long k, uint32_t) { top = max(top, uint32_t(k >> 32)); });
+  __shared__ uint32_t s_low[WARPS], s_high[WARPS];
+  const uint32_t least = reached_by<BJ_THREADS>(top, p.n, s_low, s_high);
+  if (__any_sync(0xffffffffu, top >= least))
+    each([&](unsigned long long k, uint32_t at) {
+      if (uint32_t(k >> 32) >= least) {
+        const int to = atomicAdd(&s_count, 1);
+        if (to < BJ_LIST) {
+          key[to] = k;
+          place[to] = at;
+        }
       }
-    }
-  }
+    });
   __syncthreads();
   int count = s_count;
   if (count > BJ_LIST) {
     // Scores that are all but equal: the n-th best of (score, place), bit by bit.
     auto counted = [&](auto test) {
       int c = 0;
-      for (int i = tid; i < total; i += BJ_THREADS) {
-        uint32_t at = 0;
-        const unsigned long long k = look(i, at);
-        c += k != 0 && test(k, at);
-      }
+      each([&](unsigned long long k, uint32_t at) { c += test(k, at); });
       c = __reduce_add_sync(0xffffffffu, c);
       __syncthreads();
-      if (lane == 0) s_key[warp] = c;
+      if (lane == 0) s_sum[warp] = c;
       __syncthreads();
       c = 0;
-      for (int i = 0; i < WARPS; ++i) c += s_key[i];
+      for (int i = 0; i < WARPS; ++i) c += s_sum[i];
       return c;
     };
     unsigned long long nth = 0;
@@ -336,25 +400,30 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const __grid_cons
     __syncthreads();
     if (tid == 0) s_count = 0;
     __syncthreads();
-    for (int i = tid; i < total; i += BJ_THREADS) {
-      uint32_t at = 0;
-      const unsigned long long k = look(i, at);
-      if (k > nth || (k != 0 && k == nth && at <= last)) {
+    each([&](unsigned long long k, uint32_t at) {
+      if (k > nth || (k == nth && at <= last)) {
         const int to = atomicAdd(&s_count, 1);
         key[to] = k;
         place[to] = at;
       }
-    }
+    });
     __syncthreads();
     count = s_count;
   }
   const long long out = (long long)b * p.n;
-  for (int i = tid; i < count; i += BJ_THREADS) {
-    const unsigned long long k = key[i];
-    const uint32_t at = place[i];
+  // four lanes a candidate
+  for (int i0 = 0; i0 < count; i0 += BJ_THREADS / 4) {
+    const int i = i0 + tid / 4;
+    const unsigned long long k = i < count ? key[i] : ~0ull;
+    const uint32_t at = i < count ? place[i] : 0;
     int rank = 0;
-    for (int j = 0; j < count; ++j) rank += key[j] > k || (key[j] == k && place[j] < at);
-    if (rank < p.n) {
+    for (int j = tid % 4; j < count; j += 4) {
+      const unsigned long long y = key[j];
+      rank += y > k || (y == k && place[j] < at);
+    }
+    rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+    rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+    if (i < count && rank < p.n && tid % 4 == 0) {
       p.out_scores[out + rank] = float(value_of(k));
       p.out_parents[out + rank] = int(at / uint32_t(p.V));
       p.out_tokens[out + rank] = int(at % uint32_t(p.V));

@@ -345,14 +345,12 @@ __global__ void __launch_bounds__(MF_THREADS, 1)
   uint64_t* full = reinterpret_cast<uint64_t*>(tail + 8 * kWalkShared + 16);
   uint64_t* empty = full + NST;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (tid == 0) {
-    for (int s = 0; s < NST; ++s) {
-      mbar_init(full + s, 32);
-      mbar_init(empty + s, MF_CONSUMERS / 2);
-    }
+  if (tid < NST) {
+    mbar_init(full + tid, 32);
+    mbar_init(empty + tid, MF_CONSUMERS / 2);
     mbar_fence_init();
-    *dead = 0;
   }
+  if (tid == 0) *dead = 0;
   pdl_wait();
   pdl_launch_dependents();
   __syncthreads();
