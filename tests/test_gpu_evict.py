@@ -291,6 +291,10 @@ def check_evict(c, budgets, sinks, recent, arg=None):
     ([300, 1000, 77], 2, 3, 128, 256, BF, 65, 1, 7),
     ([20000, 16400], 1, 2, 64, 64, BF, 3001, 4, 100),      # more sums than shared memory holds
     ([1025], 2, 2, 128, 16, BF, 1024, 0, 0),
+    # lists enough that one kernel selects and moves
+    ([300, 1, 700, 333, 65], 8, 4, 128, 32, BF, 64, 2, 9),
+    ([17000, 16384, 900], 10, 5, 64, 16, BF, 900, 3, 50),
+    ([129] * 40, 1, 4, 64, 128, F32, 128, 0, 1),
 ])
 def test_eviction(lens, L, Hk, D, page, dtype, budget, sinks, recent):
     check_evict(Pool(8, lens, L, Hk, D, page, dtype), [budget] * len(lens), sinks, recent)

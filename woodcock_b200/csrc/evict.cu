@@ -240,6 +240,7 @@ void check_evict_args(const wc_paged_evict_args& a) {
   need(a.sinks >= 0 && a.recent >= 0 && a.sinks < (1 << 30) && a.recent < (1 << 30), "paged_evict: negative sinks or recent");
   need(a.budgets || a.budget >= a.sinks + a.recent, "paged_evict: budget below sinks + recent");
   need((long long)a.pages.layers * a.requests * a.pages.kv_heads < (1ll << 31), "paged_evict: batch too large");
+  if ((long long)a.pages.pages * a.pages.page_size >= (1ll << 31)) fail(WC_ERR_UNSUPPORTED, "paged_evict: a pool of 2^31 keys");
 }
 
 int evict_most(const wc_paged_evict_args& a) {
@@ -309,12 +310,13 @@ extern "C" wc_status wc_paged_evict(wc_ctx* ctx, void* stream, const wc_paged_ev
     p.list = static_cast<int*>(a->workspace);
     p.most = most;
     p.cache = std::min(a->table_cols * g.page_size, EV_CACHE);
-    p.splits = 1;
+    // One kernel from a block for every SM on; below, rows by 64-byte parts at the least.
+    p.splits = lists >= ctx->num_sms ? 0 : std::min(p.row_chunks / 4, 4);
     p.err = ctx->d_err;
     const cudaStream_t st = stream_of(ctx, stream);
-    opt_in(ctx, evict_select_kernel, EV_CACHE * sizeof(float));
-    launch_on(ctx, st, "evict_select", evict_select_kernel, dim3(unsigned(lists)), dim3(EV_THREADS), p.cache * sizeof(float),
-              true, 1, p);
-    launch_on(ctx, st, "evict_move", evict_move_kernel, dim3(unsigned(lists), 2 * p.splits), dim3(EM_THREADS), 0, true, 1, p);
+    opt_in(ctx, evict_kernel, EV_CACHE * sizeof(float));
+    launch_on(ctx, st, "evict", evict_kernel, dim3(unsigned(lists)), dim3(EV_THREADS), p.cache * sizeof(float), true, 1, p);
+    if (p.splits)
+      launch_on(ctx, st, "evict_move", evict_move_kernel, dim3(unsigned(lists), 2 * p.splits), dim3(EV_THREADS), 0, true, 1, p);
   });
 }

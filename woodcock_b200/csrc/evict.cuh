@@ -1119,11 +1119,13 @@ __global__ void __launch_bounds__(MK_KEYS) mass_fold_kernel(const __grid_constan
 
 // ---------------------------------------------------------------------------- eviction
 // Of n keys the first `sinks` and the last `recent` stay, and of those between the ones of the largest mass,
-// ties to the lower key, until m are left; they move together in order. The selection writes the list of
-// kept keys and moves their sums; a second kernel moves the rows.
+// ties to the lower key, until m are left; they move together in order. A block selects for one list (layer,
+// request, head), writes down where the kept rows lie and moves their sums. Where there are lists enough it
+// moves the rows as well: its selection, bound by latency, runs beside other blocks' copies, bound by HBM.
+// Where there are few, a second kernel moves them, several blocks a list.
 constexpr int EV_THREADS = 512;
 constexpr int EV_CACHE = 16384;  // sums held in shared memory; those behind are read again in every pass
-constexpr int EM_THREADS = 256;
+constexpr int EM_ROWS = 4;       // rows a thread has on their way, twice
 
 struct EvictParams {
   PagePool K, V;
@@ -1136,10 +1138,10 @@ struct EvictParams {
   const int* budgets;  // [B] or null: `budget`
   int budget, sinks, recent;
   int* lens_out;
-  int* list;           // [layers][B][Hk][1 + most]: how many rows stay in place, then the kept keys
+  int* list;           // [layers][B][Hk][1 + most]: how many rows stay in place, then the kept keys' rows in the pool
   int most;
   int cache;           // sums in shared memory
-  int splits;          // blocks of a list and pool: each moves a part of every row
+  int splits;          // of the second kernel: blocks of a list and pool, each with a part of every row; 0: no second kernel
   int* err;
 };
 
@@ -1161,7 +1163,55 @@ __device__ __forceinline__ uint32_t mass_key(float x) {
   return x != x ? 0u : uint32_t(argmax_key(x + 0.f, 0) >> 32);
 }
 
-__global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const __grid_constant__ EvictParams p) {
+// Moves the kept rows of one list together, in one pool, or a part of every row's columns: kept row i comes from
+// key s_i >= i, so a step's rows are read before any is written, and no later step reads a row that an earlier
+// one wrote: the next step's may be on their way before this one's are stored. Block-collective.
+__device__ __forceinline__ void evict_rows(const EvictParams& p, const PagePool& pool, long long layer_stride, int layer, int b,
+                                           int h, int m, const int* list, int split, int splits) {
+  const int mask = (1 << p.page_log2) - 1, chunks = p.row_chunks / splits, step = EV_THREADS / chunks;
+  const int* row = p.table + (long long)b * p.table_ld;
+  char* base = static_cast<char*>(pool.ptr) + ((layer_stride * layer + h * pool.head) << p.esize_log2) +
+               (split * chunks + int(threadIdx.x) % chunks) * 16;
+  auto at = [&](int page, int r) {
+    return reinterpret_cast<uint4*>(base + ((page * pool.page + r * pool.row) << p.esize_log2));
+  };
+  uint4 x[EM_ROWS], y[EM_ROWS];
+  auto read = [&](uint4(&to)[EM_ROWS], int i0) {
+    int from[EM_ROWS];
+#pragma unroll
+    for (int u = 0; u < EM_ROWS; ++u) from[u] = i0 + u * step < m ? list[i0 + u * step] : -1;
+#pragma unroll
+    for (int u = 0; u < EM_ROWS; ++u)
+      if (from[u] >= 0) to[u] = *at(from[u] >> p.page_log2, from[u] & mask);
+  };
+  auto write = [&](const uint4(&from)[EM_ROWS], int i0) {
+#pragma unroll
+    for (int u = 0; u < EM_ROWS; ++u) {
+      const int i = i0 + u * step;
+      if (i < m) *at(row[i >> p.page_log2], i & mask) = from[u];
+    }
+  };
+  const int tile = EM_ROWS * step;
+  int i = list[-1], mine = i + int(threadIdx.x) / chunks;
+  if (i >= m) return;
+  read(x, mine);
+  for (;;) {
+    if (i + tile < m) read(y, mine + tile);
+    __syncthreads();  // this step's rows are read
+    write(x, mine);
+    i += tile;
+    mine += tile;
+    if (i >= m) break;
+    if (i + tile < m) read(x, mine + tile);
+    __syncthreads();
+    write(y, mine);
+    i += tile;
+    mine += tile;
+    if (i >= m) break;
+  }
+}
+
+__global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_constant__ EvictParams p) {
   constexpr int BINS = 2048, WARPS = EV_THREADS / 32;
   extern __shared__ float ev_cache[];
   __shared__ int hist[BINS];
@@ -1192,8 +1242,17 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const __grid_c
   auto at = [&](int j) { return base + row[j >> p.page_log2] * p.mass.page + (j & mask); };
   const int lo = p.sinks, hi = n - p.recent;
   int left = m - p.sinks - p.recent;  // to be taken of [lo, hi), fewer than there are
-  for (int j = lo + tid; j < hi && j - lo < p.cache; j += EV_THREADS) ev_cache[j - lo] = *at(j);
-  auto value = [&](int j) { return j - lo < p.cache ? ev_cache[j - lo] : *at(j); };
+  const bool held = n <= p.cache;     // all sums in shared memory
+  for (int j0 = tid; j0 < min(n, p.cache); j0 += 8 * EV_THREADS) {
+    float x[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (j0 + u * EV_THREADS < min(n, p.cache)) x[u] = *at(j0 + u * EV_THREADS);
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (j0 + u * EV_THREADS < min(n, p.cache)) ev_cache[j0 + u * EV_THREADS] = x[u];
+  }
+  auto value = [&](int j) { return j < p.cache ? ev_cache[j] : *at(j); };
   // The key of the last one taken, from its upper bits down: 11, 11, 10
   uint32_t prefix = 0;
   int shift = 32;
@@ -1243,63 +1302,104 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const __grid_c
   const bool any = m > p.sinks + p.recent;
   int* list = p.list + (long long)blockIdx.x * (p.most + 1);
   int kept = 0, equal = 0, still = 0;
-  for (int j0 = 0; j0 < n; j0 += EV_THREADS) {
-    const int j = j0 + tid;
-    float x = 0.f;
-    bool in = false, tie = false;
-    if (j < n) {
-      x = *at(j);
+  auto keep = [&](int j, int to, float x) {
+    list[1 + to] = (row[j >> p.page_log2] << p.page_log2) + (j & mask);
+    if (to != j) *at(to) = x;
+    else ++still;  // keys before the first gap
+  };
+  if (held) {
+    // a warp has a run of keys: counts first, then places; sums are written to where no block reads them any more
+    const int run = ((n + WARPS - 1) / WARPS + 31) & ~31, j0 = warp * run, j1 = min(j0 + run, n);
+    auto look = [&](int j, bool& in, bool& tie) {
+      in = tie = false;
+      if (j >= j1) return;
       if (j < lo || j >= hi) {
         in = true;
       } else if (any) {
-        const uint32_t k = mass_key(x);
+        const uint32_t k = mass_key(ev_cache[j]);
         in = k > prefix;
         tie = k == prefix;
       }
+    };
+    int ties = 0, ins = 0;
+    for (int j = j0 + lane; j - lane < j1; j += 32) {
+      bool in, tie;
+      look(j, in, tie);
+      ins += __popc(__ballot_sync(0xffffffffu, in));
+      ties += __popc(__ballot_sync(0xffffffffu, tie));
     }
-    const uint32_t ties = __ballot_sync(0xffffffffu, tie);
-    const uint32_t ins = __ballot_sync(0xffffffffu, in);
     if (lane == 0) {
-      s_warp[0][warp] = __popc(ties);
-      s_warp[1][warp] = __popc(ins);
+      s_warp[0][warp] = ties;
+      s_warp[1][warp] = ins;
     }
-    __syncthreads();  // all of this step's sums are read, and none of a later one's is written to
-    int te = equal, ki = kept, tie_all = 0, in_all = 0;
-    for (int i = 0; i < WARPS; ++i) {
-      if (i < warp) {
-        te += s_warp[0][i];
-        ki += s_warp[1][i];
-      }
-      tie_all += s_warp[0][i];
-      in_all += s_warp[1][i];
-    }
-    const uint32_t below = (1u << lane) - 1;
-    te += __popc(ties & below);                        // equal ones before
-    ki += __popc(ins & below) + min(te, left) - min(equal, left);
-    // of the ties before this one, those of earlier steps are in `kept` already
-    if (in || (tie && te < left)) {
-      list[1 + ki] = j;
-      if (ki != j) *at(ki) = x;
-      else ++still;  // keys before the first gap
-    }
-    kept += in_all + min(equal + tie_all, left) - min(equal, left);
-    equal += tie_all;
     __syncthreads();
+    for (int i = 0; i < warp; ++i) {
+      equal += s_warp[0][i];
+      kept += s_warp[1][i];
+    }
+    for (int j = j0 + lane; j - lane < j1; j += 32) {
+      bool in, tie;
+      look(j, in, tie);
+      const uint32_t bi = __ballot_sync(0xffffffffu, in), bt = __ballot_sync(0xffffffffu, tie), below = (1u << lane) - 1;
+      const int te = equal + __popc(bt & below);
+      if (in || (tie && te < left)) keep(j, kept + __popc(bi & below) + min(te, left), ev_cache[j]);
+      kept += __popc(bi);
+      equal += __popc(bt);
+    }
+  } else {
+    for (int j0 = 0; j0 < n; j0 += EV_THREADS) {
+      const int j = j0 + tid;
+      float x = 0.f;
+      bool in = false, tie = false;
+      if (j < n) {
+        x = *at(j);
+        if (j < lo || j >= hi) {
+          in = true;
+        } else if (any) {
+          const uint32_t k = mass_key(x);
+          in = k > prefix;
+          tie = k == prefix;
+        }
+      }
+      const uint32_t ties = __ballot_sync(0xffffffffu, tie);
+      const uint32_t ins = __ballot_sync(0xffffffffu, in);
+      if (lane == 0) {
+        s_warp[0][warp] = __popc(ties);
+        s_warp[1][warp] = __popc(ins);
+      }
+      __syncthreads();  // all of this step's sums are read, and none of a later one's is written to
+      int te = equal, ki = kept, tie_all = 0, in_all = 0;
+      for (int i = 0; i < WARPS; ++i) {
+        if (i < warp) {
+          te += s_warp[0][i];
+          ki += s_warp[1][i];
+        }
+        tie_all += s_warp[0][i];
+        in_all += s_warp[1][i];
+      }
+      const uint32_t below = (1u << lane) - 1;
+      te += __popc(ties & below);                        // equal ones before
+      ki += __popc(ins & below) + min(te, left) - min(equal, left);
+      // of the ties before this one, those of earlier steps are in `kept` already
+      if (in || (tie && te < left)) keep(j, ki, x);
+      kept += in_all + min(equal + tie_all, left) - min(equal, left);
+      equal += tie_all;
+      __syncthreads();
+    }
   }
   still = __reduce_add_sync(0xffffffffu, still);
   if (lane == 0) atomicAdd(&s_still, still);
   __syncthreads();
   if (tid == 0) list[0] = s_still;
+  if (p.splits) return;
+  __syncthreads();
+  evict_rows(p, p.K, p.k_layer, layer, b, h, m, list + 1, 0, 1);
+  evict_rows(p, p.V, p.v_layer, layer, b, h, m, list + 1, 0, 1);
 }
 
-// Moves the kept rows of one list together, K or V, or a part of every row's columns: kept row i comes from
-// row list[i] >= i, so a step's rows are read before any is written, and no later step reads a row that
-// an earlier one wrote.
-__global__ void __launch_bounds__(EM_THREADS) evict_move_kernel(const __grid_constant__ EvictParams p) {
-  constexpr int U = 8;
+__global__ void __launch_bounds__(EV_THREADS, 2) evict_move_kernel(const __grid_constant__ EvictParams p) {
   const int tid = threadIdx.x;
   const int h = blockIdx.x % p.Hk, lb = blockIdx.x / p.Hk, b = lb % p.B, layer = lb / p.B;
-  const int isv = blockIdx.y & 1, split = blockIdx.y >> 1;
   pdl_wait();
   pdl_launch_dependents();
   int bad = 0;
@@ -1307,32 +1407,11 @@ __global__ void __launch_bounds__(EM_THREADS) evict_move_kernel(const __grid_con
   if (bad || job.n <= job.m) return;
   const int mask = (1 << p.page_log2) - 1;
   const int* row = p.table + (long long)b * p.table_ld;
-  for (int c = tid; c < (job.n + mask) >> p.page_log2; c += EM_THREADS) bad |= row[c] < 0 || row[c] >= p.pages;
+  for (int c = tid; c < (job.n + mask) >> p.page_log2; c += EV_THREADS) bad |= row[c] < 0 || row[c] >= p.pages;
   if (__syncthreads_or(bad)) return;
-  const int* list = p.list + (long long)blockIdx.x * (p.most + 1) + 1;
-  const PagePool& pool = isv ? p.V : p.K;
-  const int chunks = p.row_chunks / p.splits, rows_step = EM_THREADS / chunks;
-  char* base = static_cast<char*>(pool.ptr) +
-               (((isv ? p.v_layer : p.k_layer) * layer + h * pool.head) << p.esize_log2) +
-               (split * chunks + tid % chunks) * 16;
-  auto at = [&](int j) {
-    return reinterpret_cast<uint4*>(base + ((row[j >> p.page_log2] * pool.page + (j & mask) * pool.row) << p.esize_log2));
-  };
-  const int first = list[-1];
-  for (int i0 = first; i0 < job.m; i0 += U * rows_step) {
-    uint4 x[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * rows_step + tid / chunks;
-      if (i < job.m) x[u] = *at(list[i]);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * rows_step + tid / chunks;
-      if (i < job.m) *at(i) = x[u];
-    }
-  }
+  const bool isv = blockIdx.y & 1;
+  evict_rows(p, isv ? p.V : p.K, isv ? p.v_layer : p.k_layer, layer, b, h, job.m, p.list + (long long)blockIdx.x * (p.most + 1) + 1,
+             blockIdx.y >> 1, p.splits);
 }
 
 }  // namespace wc
