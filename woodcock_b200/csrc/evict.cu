@@ -39,7 +39,8 @@ struct MassLayout {
   bool few, many;        // requests of at most 16 rows a KV head, of more
   int blocks, few_blocks, per, width, most;
   MassModes rows, keys;
-  size_t row_ml, part_ml, rec, tiles, few_ml, few_part, scores, pieces, part_sum, keys_rec, bytes;
+  size_t row_ml, part_ml, rec, tiles, few_ml, few_part, scores, pieces, part_sum, keys_rec, rows_q, rows_l, bytes;
+  int ids;
 };
 
 MassLayout mass_layout(const wc_ctx* ctx, const wc_paged_mass_args& a) {
@@ -63,12 +64,15 @@ MassLayout mass_layout(const wc_ctx* ctx, const wc_paged_mass_args& a) {
     l.few_part = take(at, size_t(l.few_blocks) * 2 * MF_M * MF_CONSUMERS * sizeof(float2));
     l.scores = take(at, size_t(l.few_blocks) * l.per * MF_KT * l.width * sizeof(float));
   }
-  l.row_ml = take(at, size_t(b.rows) * b.heads * sizeof(float2));
+  if (g.dtype != WC_BF16) l.row_ml = take(at, size_t(b.rows) * b.heads * sizeof(float2));
   if (l.many && g.dtype == WC_BF16) {
     const long long mean = (rep * b.rows + b.requests - 1) / b.requests;
     l.blocks = ctx->num_sms;
     l.rows = mean <= 128 ? kRows128 : kRows256;
     l.keys = mean <= 256 ? kKeysWindow : kKeysPrompt;
+    l.ids = int(rep * b.rows / 128) + b.requests + 1;
+    l.rows_q = take(at, size_t(g.kv_heads) * l.ids * 128 * g.head_dim * 2);
+    l.rows_l = take(at, size_t(g.kv_heads) * l.ids * 128 * sizeof(float));
     l.part_sum = take(at, size_t(l.blocks) * 2 * MK_KEYS * sizeof(float));
     l.keys_rec = take(at, l.blocks * sizeof(MassRec));
   } else {
@@ -129,6 +133,9 @@ void launch_many(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, const MassPara
 template <int D>
 void gather_many(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, MassParams p, const MassLayout& l, char* ws) {
   p.part_sum = reinterpret_cast<float*>(ws + l.part_sum);
+  p.rows_q = reinterpret_cast<unsigned char*>(ws + l.rows_q);
+  p.rows_l = reinterpret_cast<float*>(ws + l.rows_l);
+  p.ids = l.ids;
   p.keys_rec = reinterpret_cast<MassRec*>(ws + l.keys_rec);
   if (l.rows == kRows128) launch_many<D, kRows128>(ctx, st, g, p);
   else launch_many<D, kRows256>(ctx, st, g, p);

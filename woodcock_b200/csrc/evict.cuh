@@ -47,6 +47,9 @@ struct MassParams {
   int per, width;        // key tiles of a block at most, rows of a tile at most
   MassPiece* pieces;     // [blocks][most]
   int most;
+  unsigned char* rows_q; // many rows: [Hk][ids] tiles of 128 query rows as shared memory has them
+  float* rows_l;         // [Hk][ids][128]: -(M + log2(sum)) of their rows; -inf: a row that weighs nothing
+  int ids;
   float* part_sum;       // many rows: [blocks][2][256], of divided key tiles
   MassRec* keys_rec;     // [blocks]: the divided key tile that begins in the block
   int key_blocks;
@@ -55,6 +58,12 @@ struct MassParams {
 // What a weight is before the sums are joined: rows that see nothing keep 0.
 __device__ __forceinline__ float2 mass_row(float m, float l) {
   return make_float2(m == -INFINITY ? 0.f : m, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l));
+}
+
+// The same as one number: 2^(s - M) / sum = 2^(s + it).
+__device__ __forceinline__ float mass_minus_l(float m, float l) {
+  const float2 y = mass_row(m, l);
+  return log2f(y.y) - y.x;
 }
 
 // The first kernel's scores, one row tile against one key tile: 16 rows x 64 keys, a key and four rows a
@@ -162,6 +171,11 @@ __global__ void __launch_bounds__(MS_THREADS) mass_rows_kernel(const __grid_cons
   } while (w.next(p, mp.kinds));
 }
 
+// A row tile's number among those of its head: distinct, below T rep / 128 + requests + 1.
+__device__ __forceinline__ int mass_tile(const PagedAttnParams& p, int tok0, int request, int qt) {
+  return tok0 * p.rep / 128 + request + qt;  // rows x heads is below 2^30
+}
+
 // Key tiles of requests that share no pages, at most.
 __host__ __device__ __forceinline__ long long mass_most_tiles(int pages, int page_log2, int B, int Hk, int KT) {
   return (((long long)pages << page_log2) / KT + B) * Hk;
@@ -228,7 +242,11 @@ __global__ void __launch_bounds__(256) mass_join_kernel(const __grid_constant__ 
     l = l * exp2f(m - mg) + l2 * exp2f(m2 - mg);
     m = mn;
   }
-  if (rho < rec.rows && tid % LANES == 0) {
+  if constexpr (M > MS_M) {
+    if (tid % LANES == 0 && rho / 128 * 128 < rec.rows)
+      mp.rows_l[(size_t)(rec.head * mp.ids + mass_tile(p, rec.tok0, rec.idx, rho / 128)) * 128 + rho % 128] =
+          rho < rec.rows ? mass_minus_l(m, l) : -INFINITY;
+  } else if (rho < rec.rows && tid % LANES == 0) {
     const int i = rho / p.rep;
     mp.row_ml[(long long)(rec.tok0 + i) * p.H + rec.head * p.rep + rho - i * p.rep] = mass_row(m, l);
   }
@@ -590,20 +608,23 @@ __global__ void __launch_bounds__(MF_KEYS_THREADS, 4) mass_few_keys_kernel(const
 // are 128 rows, and the key's weights are added up where they are, without an exchange between threads.
 // Weights are 2^(s - L), L = M + log2(sum).
 //
-// Both kernels are one code: a lane operand A that stays for an item, a column operand B that streams, two
-// groups of four warps that read the products from tensor memory, two buffers each. kMode: rows of at most
-// 128 a request (the groups take alternate B tiles); rows of more (a group each half of 256 lanes); keys
-// (the same, 256 keys), with rings for prompts (Q streams) or for windows (K streams).
-// Bound by the exponential unit: 16 a clock, 1024 clocks for a product of 512.
+// Both kernels are one code: a lane operand A that stays for an item, a column operand B that streams, four
+// groups of four warps that read the products from tensor memory, a buffer each. kMode: rows of at most
+// 128 a request (the groups take the B tiles in turn); rows of more (two groups for each half of 256 lanes);
+// keys (the same, 256 keys), with rings for prompts (Q streams) or for windows (K streams). The first kernel
+// leaves the query tiles as it had them in shared memory, so that the second has each of them by one copy:
+// gathered row by row again, they took 3600 clocks a tile.
+// Bound by the exponential unit: 16 a clock, 1024 clocks for a product of 512. With two groups of two
+// buffers the unit was 48 to 60% busy, two warps a scheduler being too few to cover the loads' latency.
 enum MassModes : int { kRows128 = 0, kRows256 = 1, kKeysPrompt = 2, kKeysWindow = 3 };
-constexpr int MM_THREADS = 384;  // K copies, products, 2 warps of Q copies; 2 x 4 warps of sums
+constexpr int MM_THREADS = 672;  // 2 warps of K copies, products, 2 warps of Q copies; 4 x 4 warps of sums
 constexpr int MM_OVER = 2, MK_OVER = 2, MK_KEYS = 256;
 
 template <int D, int kMode>
 struct MmLayout {
   static constexpr int KS = kMode == kKeysPrompt ? 2 : 4, QS = 6 - KS;  // tiles of 128 rows
   static constexpr int kTile = 128 * D * 2;
-  static constexpr int kTail = 8 * kWalkShared + 256 + QS * 128 * 4 + 2 * 128 * 8;
+  static constexpr int kTail = 8 * kWalkShared + 256 + QS * 128 * 4 + 2 * 3 * 128 * 8;
   static constexpr size_t bytes() { return 1024 + size_t(KS + QS) * kTile + kTail; }
 };
 
@@ -741,28 +762,28 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
   uint64_t* k_empty = bars + 4;   // [4]
   uint64_t* q_full = bars + 8;    // [4]
   uint64_t* q_empty = bars + 12;  // [4]
-  uint64_t* s_full = bars + 16;   // [4]: group * 2 + buffer
-  uint64_t* s_empty = bars + 20;  // [4]
-  uint64_t* x_full = bars + 24;   // [2]: the second group's states are in shared memory
+  uint64_t* s_full = bars + 16;   // [4]: a group's product is complete
+  uint64_t* s_empty = bars + 20;  // [4]: and read
+  uint64_t* x_full = bars + 24;   // [2]: the other groups' states are in shared memory
   uint64_t* x_empty = bars + 26;  // [2]: and read
   uint64_t* drain = bars + 28;
   volatile int* dead = reinterpret_cast<volatile int*>(bars + 29);
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + 30);
   float* nl = reinterpret_cast<float*>(tail + 8 * kWalkShared + 256);  // [QS][128]: -L of the tile's rows
-  float2* xml = reinterpret_cast<float2*>(nl + QS * 128);              // [item & 1][row]
+  float2* xml = reinterpret_cast<float2*>(nl + QS * 128);              // [item & 1][group - 1][lane]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < 4; ++i) {
       mbar_init(k_full + i, 1);
       mbar_init(k_empty + i, 1);
-      mbar_init(q_full + i, 2);
-      mbar_init(q_empty + i, kKeys ? 9 : 1);
+      mbar_init(q_full + i, kKeys ? 1 : 2);
+      mbar_init(q_empty + i, kKeys ? 17 : 1);
       mbar_init(s_full + i, 1);
       mbar_init(s_empty + i, 4);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(x_full + i, 4);
-      mbar_init(x_empty + i, 4);
+      mbar_init(x_full + i, kTwo ? 8 : 12);
+      mbar_init(x_empty + i, kTwo ? 8 : 4);
     }
     mbar_init(drain, 1);
     mbar_fence_init();
@@ -790,8 +811,8 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
 
   // An item: its A tiles (one or two in use), its B tiles, the K tiles' first key
   struct Item {
-    int nb, key0, rho0;
-    bool two;
+    int nb, key0, rho0, tile;  // tile: the first row tile's number
+    bool two, first;           // first: this block has the item's first key tile
   };
   auto item_of = [&](const Walk& x) {
     Item it;
@@ -800,61 +821,76 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
       it.key0 = x.kt * MK_KEYS;
       it.rho0 = x.qt0 * 128;
       it.two = x.g.klen - it.key0 > 128;
+      it.tile = mass_tile(p, x.g.tok0, x.g.idx, x.qt0);
+      it.first = false;
     } else {
       it.nb = x.kt1 - x.kt0;
       it.key0 = x.kt0 * 128;
       it.rho0 = x.qt * M;
       it.two = kTwo && x.g.n * p.rep - it.rho0 > 128;
+      it.tile = mass_tile(p, x.g.tok0, x.g.idx, x.qt * (M / 128));
+      it.first = x.kt0 == 0;
     }
     return it;
   };
 
-  if (warp == 0) {  // ---- K tiles
+  if (warp < 2) {  // ---- K tiles: two warps in turn
     const int psize = 1 << p.page_log2, box = min(psize, 128), parts = 128 / box;
     const int part = lane / HALVES, half = lane % HALVES, at = half * (128 * 128) + part * box * 128;
-    int pos = 0;
+    int pos = 0, last = -1;
     do {
       const Item it = item_of(w);
       const int nt = kKeys ? 2 : it.nb;
-      PageWindow win;
-      win.start(p, w.g, it.key0 >> p.page_log2, lane);
-      for (int t = 0; t < nt; ++t, ++pos) {
-        const int s = pos % KS, first = (it.key0 + t * 128) >> p.page_log2;
-        win.seek(p, first, lane);
-        const int page = __shfl_sync(0xffffffffu, win.cur, (first - win.base + part) & 31);
-        if (lane == 0) {
-          if (pos >= KS) paged_wait(k_empty + s, ((pos / KS) - 1) & 1, dead, p.err);
-          if (!*dead) mbar_arrive_expect_tx(k_full + s, L::kTile);
-        }
+      const int* row = p.table + (long long)w.g.idx * p.table_ld;
+      const int npages = min((w.g.klen + psize - 1) >> p.page_log2, p.table_cols);
+      auto fetch = [&](int t) {  // the page of this lane's copy of tile t; one outside the pool reads as zeros
+        const int i = ((it.key0 + t * 128) >> p.page_log2) + part;
+        if (part >= parts || t >= nt || i >= npages) return p.pages;
+        const int page = row[i];
+        if (page >= 0 && page < p.pages) return page;
+        raise_error(p.err, kErrPage);
+        return p.pages;
+      };
+      int t = (warp ^ pos) & 1;
+      int page = fetch(t);
+      for (; t < nt; t += 2) {
+        const int q = pos + t, s = q % KS, next = fetch(t + 2);
+        if (q >= KS) paged_wait(k_empty + s, ((q / KS) - 1) & 1, dead, p.err);
+        if (__any_sync(0xffffffffu, *dead)) break;
+        if (lane == 0) mbar_arrive_expect_tx(k_full + s, L::kTile);
         __syncwarp();
-        if (*dead) break;
         if (part < parts)
           tma_load_5d(ks + size_t(s) * L::kTile + at, &tk, 0, (it.key0 + t * 128) & (psize - 1), half, w.head, page, k_full + s);
-        __syncwarp();
+        page = next;
+        last = q;
       }
+      pos += nt;
     } while (!*dead && w.next(p, mp.kinds));
-    // shared memory must outlive the copies
+    // shared memory must outlive the copies: the last one of this warp's, and those before it where nobody waited
     if (lane == 0)
-      for (int q = max(0, pos - KS); q < pos; ++q)
+      for (int q = max(warp, last - KS + 2); q <= last; q += 2)
         if (!mbar_wait(k_full + q % KS, (q / KS) & 1)) raise_error(p.err, kErrTimeout);
-  } else if (warp == 1) {  // ---- products: the warp walks together, one lane issues
+  } else if (warp == 2) {  // ---- products: the warp walks together, one lane issues
     constexpr uint32_t id = umma_idesc_bf16_m128(128, 0);
     const bool issuer = elect_one();
     const uint32_t k_lo = umma_lo(smem_addr(ks), 1), q_lo = umma_lo(smem_addr(qs), 1);
     int kpos = 0, qpos = 0;
-    int ns0 = 0, ns1 = 0;  // products of each group
+    uint32_t used = 0, phase = 0;  // by group, as bits
     auto product = [&](int group, int kslot, int qslot) {
-      const int i = group ? ns1++ : ns0++, buf = group * 2 + (i & 1);
-      if (i >= 2) paged_wait(s_empty + buf, ((i >> 1) - 1) & 1, dead, p.err);
+      if ((used >> group) & 1) {
+        paged_wait(s_empty + group, (phase >> group) & 1, dead, p.err);
+        phase ^= 1u << group;
+      }
+      used |= 1u << group;
       tc_fence_after();
       if (issuer) {
         const uint32_t kt = k_lo + kslot * (L::kTile / 16), qt = q_lo + qslot * (L::kTile / 16);
         const uint32_t a = kKeys ? kt : qt, b = kKeys ? qt : kt;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          umma_ss(tmem + buf * 128, a + (kk / 4) * (128 * 128 / 16) + (kk % 4) * 2, b + (kk / 4) * (128 * 128 / 16) + (kk % 4) * 2,
+          umma_ss(tmem + group * 128, a + (kk / 4) * (128 * 128 / 16) + (kk % 4) * 2, b + (kk / 4) * (128 * 128 / 16) + (kk % 4) * 2,
                   id, kk != 0);
-        umma_commit(s_full + buf);
+        umma_commit(s_full + group);
       }
     };
     auto done = [&](uint64_t* bar) {
@@ -873,18 +909,19 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
           const int s = qpos % QS;
           paged_wait(q_full + s, (qpos / QS) & 1, dead, p.err);
           ++qpos;
-          product(0, ka % KS, s);
-          if (it.two) product(1, (ka + 1) % KS, s);
+          const int turn = (qpos - 1) & 1;
+          product(turn, ka % KS, s);
+          if (it.two) product(2 + turn, (ka + 1) % KS, s);
           done(q_empty + s);
         } else {
           const int s = kpos % KS;
           paged_wait(k_full + s, (kpos / KS) & 1, dead, p.err);
           ++kpos;
           if constexpr (kTwo) {
-            product(0, s, qa % QS);
-            if (it.two) product(1, s, (qa + 1) % QS);
-          } else {
             product(t & 1, s, qa % QS);
+            if (it.two) product(2 + (t & 1), s, (qa + 1) % QS);
+          } else {
+            product(t & 3, s, qa % QS);
           }
           done(k_empty + s);
         }
@@ -898,30 +935,45 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
     done(drain);  // tensor memory is given back only when nothing writes it any more
     if (!mbar_wait(drain, 0)) raise_error(p.err, kErrTimeout);
     __syncwarp();
-  } else if (warp < 4) {  // ---- Q tiles: two warps, 64 rows each, 16 or 8 lanes a row
+  } else if (kKeys && warp < 5) {  // ---- Q tiles with their rows' L, as the first kernel left them
+    if (warp == 3 && lane == 0) {
+      int pos = 0;
+      do {
+        const Item it = item_of(w);
+        const int tile = w.head * mp.ids + it.tile;
+        for (int t = 0; t < it.nb; ++t, ++pos) {
+          const int s = pos % QS;
+          if (pos >= QS) paged_wait(q_empty + s, ((pos / QS) - 1) & 1, dead, p.err);
+          if (*dead) break;
+          mbar_arrive_expect_tx(q_full + s, L::kTile + 512);
+          bulk_g2s(qs + size_t(s) * L::kTile, mp.rows_q + (size_t)(tile + t) * L::kTile, L::kTile, q_full + s);
+          bulk_g2s(nl + s * 128, mp.rows_l + (size_t)(tile + t) * 128, 512, q_full + s);
+        }
+      } while (!*dead && w.next(p, mp.kinds));
+      for (int q = max(0, pos - QS); q < pos; ++q)
+        if (!mbar_wait(q_full + q % QS, (q / QS) & 1)) raise_error(p.err, kErrTimeout);
+    }
+  } else if (warp < 5) {  // ---- Q tiles: two warps, 64 rows each, 16 or 8 lanes a row
     constexpr int CH = D / 8, RPI = 32 / CH;
-    const int r0 = (warp - 2) * 64, c = lane % CH;
+    const int r0 = (warp - 3) * 64, c = lane % CH;
     int pos = 0;
     do {
       const Item it = item_of(w);
-      const int nt = kKeys ? it.nb : kTwo ? 2 : 1;
+      const int nt = kTwo ? 2 : 1;
       for (int t = 0; t < nt && !*dead; ++t, ++pos) {
         const int s = pos % QS;
         long long from[2];
-        float minus_l[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const PagedRow r = paged_row(p, w.g, w.head, it.rho0 + t * 128 + r0 + e * 32 + lane);
           from[e] = r.valid ? r.tok * p.q_row + r.h * p.q_head : -1;
-          if constexpr (kKeys) {
-            // 2^(s - M) / sum = 2^(s - (M - log2(1 / sum))); a row that sees nothing weighs nothing
-            const float2 ml = r.valid ? mp.row_ml[(long long)r.tok * p.H + r.h] : make_float2(0.f, 0.f);
-            minus_l[e] = log2f(ml.y) - ml.x;
-          }
         }
         if (pos >= QS) paged_wait(q_empty + s, ((pos / QS) - 1) & 1, dead, p.err);
         if (*dead) break;
-        unsigned char* dst = qs + size_t(s) * L::kTile + (c / 8) * (128 * 128) + r0 * 128;
+        if (lane == 0) bulk_wait_read();  // the slot's tile has left it
+        __syncwarp();
+        unsigned char* slot = qs + size_t(s) * L::kTile + r0 * 128;
+        unsigned char* dst = slot + (c / 8) * (128 * 128);
 #pragma unroll
         for (int e = 0; e < 2; ++e)
 #pragma unroll 4
@@ -932,42 +984,65 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
                        static_cast<const uint16_t*>(p.q) + (at < 0 ? 0 : at) + c * 8, at < 0 ? 0 : 16);
           }
         cp_async_commit();
-        if constexpr (kKeys) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) nl[s * 128 + r0 + e * 32 + lane] = minus_l[e];
-        }
         cp_async_wait<0>();
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(q_full + s);
+        if (lane == 0) {
+          mbar_arrive(q_full + s);
+          if (it.first && (t == 0 || it.two)) {
+            unsigned char* to = mp.rows_q + (size_t)(w.head * mp.ids + it.tile + t) * L::kTile + r0 * 128;
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h) bulk_s2g(to + h * (128 * 128), slot + h * (128 * 128), 64 * 128);
+            bulk_commit();
+          }
+        }
       }
     } while (!*dead && w.next(p, mp.kinds));
+    if (lane == 0) bulk_wait();
   } else {  // ---- sums: a thread has a lane of its group's products
-    const int group = (warp - 4) >> 2, qd = warp & 3, r128 = qd * 32 + lane;
-    const uint32_t ts = tmem + (uint32_t(qd * 32) << 16) + group * 256;
+    const int group = (warp - 5) >> 2, qd = warp & 3, r128 = qd * 32 + lane;
+    const int half = kTwo ? group >> 1 : 0;                    // of the item's lanes
+    const int t0 = kTwo ? group & 1 : group, dt = kTwo ? 2 : 4;  // the B tiles
+    const uint32_t ts = tmem + (uint32_t(qd * 32) << 16) + group * 128;
     const float sl2 = p.scale_log2;
     int ns = 0, qpos = 0, nitem = 0;
-    auto scores = [&]() {  // waits for the group's next product; its columns
-      const int buf = ns & 1;
-      paged_wait(s_full + group * 2 + buf, (ns >> 1) & 1, dead, p.err);
+    auto scores = [&]() {  // waits for the group's next product
+      paged_wait(s_full + group, ns & 1, dead, p.err);
+      ++ns;
       tc_fence_after();
-      return ts + buf * 128;
     };
     auto scores_read = [&]() {
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(s_empty + group * 2 + (ns & 1));
-      ++ns;
+      if (lane == 0) mbar_arrive(s_empty + group);
+    };
+    // the states of the groups with the same lanes meet in the first of them: f(another's), in order
+    auto meet = [&](float2 mine, auto f) {
+      const int xb = nitem & 1, xn = nitem >> 1;
+      ++nitem;
+      if (t0 > 0) {
+        if (xn > 0) paged_wait(x_empty + xb, (xn - 1) & 1, dead, p.err);
+        xml[(xb * 3 + group - 1) * 128 + r128] = mine;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(x_full + xb);
+      } else {
+        paged_wait(x_full + xb, xn & 1, dead, p.err);
+#pragma unroll
+        for (int i = 1; i < (kTwo ? 2 : 4); ++i) f(xml[(xb * 3 + group + i - 1) * 128 + r128]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(x_empty + xb);
+      }
     };
     if constexpr (kKeys) {
       do {
         const Item it = item_of(w);
-        const bool active = group == 0 || it.two;
-        const int key = it.key0 + group * 128 + r128;
-        const bool mine = key < w.g.klen;
+        const bool active = half == 0 || it.two;
+        const int key = it.key0 + half * 128 + r128;
         float* to = nullptr;
         float was = 0.f;
-        if (mine && w.count == 1) {
+        // one tile: its group has the item alone, and the other goes on to the next; several: the first group adds up
+        const bool mine = it.nb > 1 ? t0 == 0 : (qpos & 1) == t0;
+        if (mine && key < w.g.klen && w.count == 1) {
           const int page = paged_page(p, w.g, key >> p.page_log2);
           if (page >= 0) {
             to = mp.mass.ptr + page * mp.mass.page + w.head * mp.mass.head + (key & ((1 << p.page_log2) - 1));
@@ -980,15 +1055,15 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
         for (int t = 0; t < it.nb; ++t, ++qpos) {
           const int s = qpos % QS;
           paged_wait(q_full + s, (qpos / QS) & 1, dead, p.err);
-          if (active && !__any_sync(0xffffffffu, *dead)) {  // tensor memory is read by whole warps
-            const uint32_t cols = scores();
+          if (active && (qpos & 1) == t0 && !__any_sync(0xffffffffu, *dead)) {  // tensor memory is read by whole warps
+            scores();
             const float* row = nl + s * 128;
             const int hide = int(min(see - (it.rho0 + t * 128), 128ll));  // columns before this one do not see the key
             if (__any_sync(0xffffffffu, hide > 0)) {
 #pragma unroll 1
               for (int c = 0; c < 128; c += 32) {
                 uint32_t v[32];
-                tmem_ld32(cols + c, v);
+                tmem_ld32(ts + c, v);
 #pragma unroll
                 for (int i = 0; i < 32; i += 4) {
                   const float4 l4 = *reinterpret_cast<const float4*>(row + c + i);
@@ -1004,7 +1079,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
 #pragma unroll 1
               for (int c = 0; c < 128; c += 32) {
                 uint32_t v[32];
-                tmem_ld32(cols + c, v);
+                tmem_ld32(ts + c, v);
 #pragma unroll
                 for (int i = 0; i < 32; i += 4) {
                   const float4 l4 = *reinterpret_cast<const float4*>(row + c + i);
@@ -1021,38 +1096,43 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
           if (lane == 0) mbar_arrive(q_empty + s);
         }
         if (*dead) break;
-        const float total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        if (w.count == 1) {
-          if (to) *to = was + total;
-        } else {
-          mp.part_sum[((long long)blockIdx.x * 2 + w.slot()) * MK_KEYS + group * 128 + r128] = total;
-          if (warp == 4 && lane == 0 && w.slot() == 1) mp.keys_rec[blockIdx.x] = MassRec{w.seg, w.head, w.kt, w.count};
+        float total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (it.nb > 1) meet(make_float2(total, 0.f), [&](float2 y) { total += y.x; });
+        if (mine) {
+          if (w.count == 1) {
+            if (to) *to = was + total;
+          } else {
+            mp.part_sum[((long long)blockIdx.x * 2 + w.slot()) * MK_KEYS + half * 128 + r128] = total;
+            if (half == 0 && qd == 0 && lane == 0 && w.slot() == 1)
+              mp.keys_rec[blockIdx.x] = MassRec{w.seg, w.head, w.kt, w.count};
+          }
         }
       } while (w.next(p, mp.kinds));
     } else {
       do {
         const Item it = item_of(w);
-        const PagedRow r = paged_row(p, w.g, w.head, it.rho0 + (kTwo ? group * 128 : 0) + r128);
+        const PagedRow r = paged_row(p, w.g, w.head, it.rho0 + half * 128 + r128);
         const int lim = r.valid ? r.lim : 0x7fffffff;  // rows that pad the tile see everything, for nobody
         float m = -INFINITY, l = 0.f;
-        if (!kTwo || group == 0 || it.two) {
-          for (int t = kTwo ? 0 : group; t < it.nb; t += kTwo ? 1 : 2) {
-            const uint32_t cols = scores();
+        if (half == 0 || it.two) {
+          for (int t = t0; t < it.nb; t += dt) {
+            scores();
             if (__any_sync(0xffffffffu, *dead)) break;
             const int key0 = it.key0 + t * 128;
             const bool masked = __any_sync(0xffffffffu, key0 + 128 > lim);
 #pragma unroll 1
             for (int c = 0; c < 128; c += 32) {
               uint32_t v[32];
-              tmem_ld32(cols + c, v);
+              tmem_ld32(ts + c, v);
               if (masked) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
                   if (key0 + c + i >= lim) v[i] = 0xff800000u;
               }
-              float mx = fmaxf(__uint_as_float(v[0]), __uint_as_float(v[1]));
+              float mx = max3(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]));
 #pragma unroll
-              for (int i = 2; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(v[i]));
+              for (int i = 3; i < 31; i += 2) mx = max3(mx, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+              mx = fmaxf(mx, __uint_as_float(v[31]));
               const float mn = fmaxf(m, mx * sl2), mg = mn == -INFINITY ? 0.f : mn;
               float sum[4] = {l * ex2_approx(m - mg), 0.f, 0.f, 0.f};
 #pragma unroll
@@ -1064,28 +1144,15 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
           }
         }
         if (*dead) break;
-        if (!kTwo) {  // the groups' states
-          const int xb = nitem & 1, xn = nitem >> 1;
-          if (group == 1) {
-            if (xn > 0) paged_wait(x_empty + xb, (xn - 1) & 1, dead, p.err);
-            xml[xb * 128 + r128] = make_float2(m, l);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(x_full + xb);
-          } else {
-            paged_wait(x_full + xb, xn & 1, dead, p.err);
-            const float2 y = xml[xb * 128 + r128];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(x_empty + xb);
-            const float mn = fmaxf(m, y.x), mg = mn == -INFINITY ? 0.f : mn;
-            l = l * ex2_approx(m - mg) + y.y * ex2_approx(y.x - mg);
-            m = mn;
-          }
-          ++nitem;
-        }
-        if (warp == 4 && lane == 0) w.report(p);
-        if (r.valid && (kTwo || group == 0)) {
-          if (w.count == 1) mp.row_ml[(long long)r.tok * p.H + r.h] = mass_row(m, l);
-          else mp.part_ml[((long long)blockIdx.x * 2 + w.slot()) * M + (kTwo ? group * 128 : 0) + r128] = make_float2(m, l);
+        meet(make_float2(m, l), [&](float2 y) {
+          const float mn = fmaxf(m, y.x), mg = mn == -INFINITY ? 0.f : mn;
+          l = l * ex2_approx(m - mg) + y.y * ex2_approx(y.x - mg);
+          m = mn;
+        });
+        if (group == 0 && qd == 0 && lane == 0) w.report(p);
+        if (t0 == 0 && (half == 0 || it.two)) {
+          if (w.count == 1) mp.rows_l[(size_t)(w.head * mp.ids + it.tile + half) * 128 + r128] = r.valid ? mass_minus_l(m, l) : -INFINITY;
+          else mp.part_ml[((long long)blockIdx.x * 2 + w.slot()) * M + half * 128 + r128] = make_float2(m, l);
         }
       } while (w.next(p, mp.kinds));
     }

@@ -853,12 +853,6 @@ struct PmLayout {
   static constexpr size_t bytes() { return 1024 + size_t(kQ) + size_t(kStages) * kTile + kTail; }
 };
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-
 // Bits of the 32 keys from k0 on that a row sees.
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u); }
 __device__ __forceinline__ uint32_t seen_bits(const PagedRow& r, int k0) {

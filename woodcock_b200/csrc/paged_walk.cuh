@@ -59,7 +59,7 @@ enum PagedKinds : int {
 
 // A divided item as the joining kernel needs it; count 0: none.
 struct PagedRec {
-  int tok0, rows, qt, head, count, pad[3];  // rows: the segment's, times rep
+  int tok0, rows, qt, head, count, idx, pad[2];  // rows: the segment's, times rep
 };
 
 struct PagedAttnParams {
@@ -283,7 +283,7 @@ struct PagedWalk {
   __device__ void report(const PagedAttnParams& p) const {
     if (kt0 > 0) return;
     if (p.G > 0) p.desc[g.prefix][item(p) * p.Hk + head] = make_int2(first, count);
-    else if (count > 1) p.rec[blockIdx.x] = PagedRec{g.tok0, g.n * p.rep, qt, head, count, {}};
+    else if (count > 1) p.rec[blockIdx.x] = PagedRec{g.tok0, g.n * p.rep, qt, head, count, g.idx, {}};
   }
 };
 // Before the first report of a block.
@@ -344,6 +344,12 @@ __device__ __forceinline__ int paged_page(const PagedAttnParams& p, const PagedS
     return -1;
   }
   return page;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 __device__ __forceinline__ void store4(float* p, const float (&x)[4]) {
