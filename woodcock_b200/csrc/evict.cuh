@@ -617,7 +617,7 @@ __global__ void __launch_bounds__(MF_KEYS_THREADS, 4) mass_few_keys_kernel(const
 // Bound by the exponential unit: 16 a clock, 1024 clocks for a product of 512. With two groups of two
 // buffers the unit was 48 to 60% busy, two warps a scheduler being too few to cover the loads' latency.
 enum MassModes : int { kRows128 = 0, kRows256 = 1, kKeysPrompt = 2, kKeysWindow = 3 };
-constexpr int MM_THREADS = 672;  // 2 warps of K copies, products, 2 warps of Q copies; 4 x 4 warps of sums
+constexpr int MM_THREADS = 640;  // 3 warps of copies (K and Q), products; 4 x 4 warps of sums
 constexpr int MM_OVER = 2, MK_OVER = 2, MK_KEYS = 256;
 
 template <int D, int kMode>
@@ -749,6 +749,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
   constexpr bool kKeys = kMode >= kKeysPrompt, kTwo = kMode != kRows128;
   using L = MmLayout<D, kMode>;
   using Walk = std::conditional_t<kKeys, MassWalk, PagedWalk<kTwo ? 256 : 128, 128, MM_OVER>>;
+  constexpr int KW = kMode == kRows256 ? 1 : 2, QW = 3 - KW;  // warps that copy K and Q; the third has the products
   constexpr int M = kTwo ? 256 : 128, KS = L::KS, QS = L::QS, HALVES = D / 64;
   const PagedAttnParams& p = mp.a;
   extern __shared__ unsigned char mm_raw[];
@@ -776,7 +777,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
     for (int i = 0; i < 4; ++i) {
       mbar_init(k_full + i, 1);
       mbar_init(k_empty + i, 1);
-      mbar_init(q_full + i, kKeys ? 1 : 2);
+      mbar_init(q_full + i, kKeys ? 1 : QW);
       mbar_init(q_empty + i, kKeys ? 17 : 1);
       mbar_init(s_full + i, 1);
       mbar_init(s_empty + i, 4);
@@ -834,7 +835,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
     return it;
   };
 
-  if (warp < 2) {  // ---- K tiles: two warps in turn
+  if (warp < KW) {  // ---- K tiles, in turn
     const int psize = 1 << p.page_log2, box = min(psize, 128), parts = 128 / box;
     const int part = lane / HALVES, half = lane % HALVES, at = half * (128 * 128) + part * box * 128;
     int pos = 0, last = -1;
@@ -851,10 +852,10 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
         raise_error(p.err, kErrPage);
         return p.pages;
       };
-      int t = (warp ^ pos) & 1;
+      int t = (warp + pos) % KW;
       int page = fetch(t);
-      for (; t < nt; t += 2) {
-        const int q = pos + t, s = q % KS, next = fetch(t + 2);
+      for (; t < nt; t += KW) {
+        const int q = pos + t, s = q % KS, next = fetch(t + KW);
         if (q >= KS) paged_wait(k_empty + s, ((q / KS) - 1) & 1, dead, p.err);
         if (__any_sync(0xffffffffu, *dead)) break;
         if (lane == 0) mbar_arrive_expect_tx(k_full + s, L::kTile);
@@ -868,9 +869,9 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
     } while (!*dead && w.next(p, mp.kinds));
     // shared memory must outlive the copies: the last one of this warp's, and those before it where nobody waited
     if (lane == 0)
-      for (int q = max(warp, last - KS + 2); q <= last; q += 2)
+      for (int q = max(warp, last - KS + KW); q <= last; q += KW)
         if (!mbar_wait(k_full + q % KS, (q / KS) & 1)) raise_error(p.err, kErrTimeout);
-  } else if (warp == 2) {  // ---- products: the warp walks together, one lane issues
+  } else if (warp == 3) {  // ---- products: the warp walks together, one lane issues
     constexpr uint32_t id = umma_idesc_bf16_m128(128, 0);
     const bool issuer = elect_one();
     const uint32_t k_lo = umma_lo(smem_addr(ks), 1), q_lo = umma_lo(smem_addr(qs), 1);
@@ -935,8 +936,8 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
     done(drain);  // tensor memory is given back only when nothing writes it any more
     if (!mbar_wait(drain, 0)) raise_error(p.err, kErrTimeout);
     __syncwarp();
-  } else if (kKeys && warp < 5) {  // ---- Q tiles with their rows' L, as the first kernel left them
-    if (warp == 3 && lane == 0) {
+  } else if (kKeys && warp < 3) {  // ---- Q tiles with their rows' L, as the first kernel left them
+    if (lane == 0) {
       int pos = 0;
       do {
         const Item it = item_of(w);
@@ -953,18 +954,18 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
       for (int q = max(0, pos - QS); q < pos; ++q)
         if (!mbar_wait(q_full + q % QS, (q / QS) & 1)) raise_error(p.err, kErrTimeout);
     }
-  } else if (warp < 5) {  // ---- Q tiles: two warps, 64 rows each, 16 or 8 lanes a row
-    constexpr int CH = D / 8, RPI = 32 / CH;
-    const int r0 = (warp - 3) * 64, c = lane % CH;
+  } else if (warp < 3) {  // ---- Q tiles: 64 or 128 rows a warp, 16 or 8 lanes a row
+    constexpr int CH = D / 8, RPI = 32 / CH, QR = 128 / QW;
+    const int r0 = (warp - KW) * QR, c = lane % CH;
     int pos = 0;
     do {
       const Item it = item_of(w);
       const int nt = kTwo ? 2 : 1;
       for (int t = 0; t < nt && !*dead; ++t, ++pos) {
         const int s = pos % QS;
-        long long from[2];
+        long long from[QR / 32];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
+        for (int e = 0; e < QR / 32; ++e) {
           const PagedRow r = paged_row(p, w.g, w.head, it.rho0 + t * 128 + r0 + e * 32 + lane);
           from[e] = r.valid ? r.tok * p.q_row + r.h * p.q_head : -1;
         }
@@ -975,7 +976,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
         unsigned char* slot = qs + size_t(s) * L::kTile + r0 * 128;
         unsigned char* dst = slot + (c / 8) * (128 * 128);
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
+        for (int e = 0; e < QR / 32; ++e)
 #pragma unroll 4
           for (int k = 0; k < 32; k += RPI) {
             const int row = k + lane / CH;
@@ -992,7 +993,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
           if (it.first && (t == 0 || it.two)) {
             unsigned char* to = mp.rows_q + (size_t)(w.head * mp.ids + it.tile + t) * L::kTile + r0 * 128;
 #pragma unroll
-            for (int h = 0; h < HALVES; ++h) bulk_s2g(to + h * (128 * 128), slot + h * (128 * 128), 64 * 128);
+            for (int h = 0; h < HALVES; ++h) bulk_s2g(to + h * (128 * 128), slot + h * (128 * 128), QR * 128);
             bulk_commit();
           }
         }
@@ -1000,7 +1001,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
     } while (!*dead && w.next(p, mp.kinds));
     if (lane == 0) bulk_wait();
   } else {  // ---- sums: a thread has a lane of its group's products
-    const int group = (warp - 5) >> 2, qd = warp & 3, r128 = qd * 32 + lane;
+    const int group = (warp - 4) >> 2, qd = warp & 3, r128 = qd * 32 + lane;
     const int half = kTwo ? group >> 1 : 0;                    // of the item's lanes
     const int t0 = kTwo ? group & 1 : group, dt = kTwo ? 2 : 4;  // the B tiles
     const uint32_t ts = tmem + (uint32_t(qd * 32) << 16) + group * 128;
