@@ -622,7 +622,8 @@ constexpr int MM_OVER = 2, MK_OVER = 2, MK_KEYS = 256;
 
 template <int D, int kMode>
 struct MmLayout {
-  static constexpr int KS = kMode == kKeysPrompt ? 2 : 4, QS = 6 - KS;  // tiles of 128 rows
+  // tiles of 128 rows: the operand that streams has the deeper ring (windows: K from memory, at 44 GB/s an SM)
+  static constexpr int KS = kMode == kRows128 ? 5 : kMode == kRows256 ? 3 : kMode == kKeysPrompt ? 2 : 4, QS = 6 - KS;
   static constexpr int kTile = 128 * D * 2;
   static constexpr int kTail = 8 * kWalkShared + 256 + QS * 128 * 4 + 2 * 3 * 128 * 8;
   static constexpr size_t bytes() { return 1024 + size_t(KS + QS) * kTile + kTail; }
@@ -718,8 +719,8 @@ struct MassWalk {
     const long long at = pos + MK_OVER;
     qt0 = qf + int(max(0ll, lo - at));
     qt1 = int(min((long long)QT, qf + hi - at));
-    first = int(at / per);
-    count = int((at + QT - qf - 1) / per) - first + 1;
+    first = int(paged_div(at, per));
+    count = int(paged_div(at + QT - qf - 1, per)) - first + 1;
     return qt1 > qt0;
   }
   __device__ bool next(const PagedAttnParams& p, int kinds) {
@@ -749,8 +750,10 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
   constexpr bool kKeys = kMode >= kKeysPrompt, kTwo = kMode != kRows128;
   using L = MmLayout<D, kMode>;
   using Walk = std::conditional_t<kKeys, MassWalk, PagedWalk<kTwo ? 256 : 128, 128, MM_OVER>>;
-  constexpr int KW = kMode == kRows256 ? 1 : 2, QW = 3 - KW;  // warps that copy K and Q; the third has the products
+  // Warps that copy K and Q. Where two take K's tiles in turn the ring is even: a stage stays with one of them.
+  constexpr int KW = kKeys ? 2 : 1, QW = 3 - KW;
   constexpr int M = kTwo ? 256 : 128, KS = L::KS, QS = L::QS, HALVES = D / 64;
+  static_assert(KS % KW == 0, "stages");
   const PagedAttnParams& p = mp.a;
   extern __shared__ unsigned char mm_raw[];
   unsigned char* sm = mm_raw + ((1024u - (smem_addr(mm_raw) & 1023u)) & 1023u);
@@ -759,26 +762,31 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
   unsigned char* tail = qs + size_t(QS) * L::kTile;
   long long* sh = reinterpret_cast<long long*>(tail);
   uint64_t* bars = reinterpret_cast<uint64_t*>(tail + 8 * kWalkShared);
-  uint64_t* k_full = bars;        // [4]
-  uint64_t* k_empty = bars + 4;   // [4]
-  uint64_t* q_full = bars + 8;    // [4]
-  uint64_t* q_empty = bars + 12;  // [4]
-  uint64_t* s_full = bars + 16;   // [4]: a group's product is complete
-  uint64_t* s_empty = bars + 20;  // [4]: and read
-  uint64_t* x_full = bars + 24;   // [2]: the other groups' states are in shared memory
-  uint64_t* x_empty = bars + 26;  // [2]: and read
-  uint64_t* drain = bars + 28;
-  volatile int* dead = reinterpret_cast<volatile int*>(bars + 29);
-  uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + 30);
+  uint64_t* k_full = bars;        // [KS]
+  uint64_t* k_empty = bars + 5;   // [KS]
+  uint64_t* q_full = bars + 10;   // [QS]
+  uint64_t* q_empty = bars + 14;  // [QS]
+  uint64_t* s_full = bars + 18;   // [4]: a group's product is complete
+  uint64_t* s_empty = bars + 22;  // [4]: and read
+  uint64_t* x_full = bars + 26;   // [2]: the other groups' states are in shared memory
+  uint64_t* x_empty = bars + 28;  // [2]: and read
+  uint64_t* drain = bars + 30;
+  volatile int* dead = reinterpret_cast<volatile int*>(bars + 31);
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + 31) + 1;
+  static_assert(KS <= 5 && QS <= 4, "barriers");
   float* nl = reinterpret_cast<float*>(tail + 8 * kWalkShared + 256);  // [QS][128]: -L of the tile's rows
   float2* xml = reinterpret_cast<float2*>(nl + QS * 128);              // [item & 1][group - 1][lane]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < KS; ++i) {
       mbar_init(k_full + i, 1);
       mbar_init(k_empty + i, 1);
+    }
+    for (int i = 0; i < QS; ++i) {
       mbar_init(q_full + i, kKeys ? 1 : QW);
       mbar_init(q_empty + i, kKeys ? 17 : 1);
+    }
+    for (int i = 0; i < 4; ++i) {
       mbar_init(s_full + i, 1);
       mbar_init(s_empty + i, 4);
     }
@@ -903,8 +911,9 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
       if constexpr (kKeys) {
         for (int a = 0; a < 2; ++a, ++kpos) paged_wait(k_full + kpos % KS, (kpos / KS) & 1, dead, p.err);
       } else {
-        for (int a = 0; a < (kTwo ? 2 : 1); ++a, ++qpos) paged_wait(q_full + qpos % QS, (qpos / QS) & 1, dead, p.err);
+        qpos += kTwo ? 2 : 1;
       }
+      auto query = [&](int a) { paged_wait(q_full + (qa + a) % QS, ((qa + a) / QS) & 1, dead, p.err); };
       for (int t = 0; t < it.nb && !*dead; ++t) {
         if constexpr (kKeys) {
           const int s = qpos % QS;
@@ -918,8 +927,10 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
           const int s = kpos % KS;
           paged_wait(k_full + s, (kpos / KS) & 1, dead, p.err);
           ++kpos;
+          if (t == 0) query(0);
           if constexpr (kTwo) {
             product(t & 1, s, qa % QS);
+            if (t == 0) query(1);
             if (it.two) product(2 + (t & 1), s, (qa + 1) % QS);
           } else {
             product(t & 3, s, qa % QS);
@@ -1039,17 +1050,18 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
         const Item it = item_of(w);
         const bool active = half == 0 || it.two;
         const int key = it.key0 + half * 128 + r128;
+        // one tile: its group has the item alone, and the other goes on to the next; several: the first group adds up
+        const bool mine = (it.nb > 1 ? t0 == 0 : (qpos & 1) == t0) && key < w.g.klen && w.count == 1;
+        int page = -1;
         float* to = nullptr;
         float was = 0.f;
-        // one tile: its group has the item alone, and the other goes on to the next; several: the first group adds up
-        const bool mine = it.nb > 1 ? t0 == 0 : (qpos & 1) == t0;
-        if (mine && key < w.g.klen && w.count == 1) {
-          const int page = paged_page(p, w.g, key >> p.page_log2);
-          if (page >= 0) {
-            to = mp.mass.ptr + page * mp.mass.page + w.head * mp.mass.head + (key & ((1 << p.page_log2) - 1));
-            if (mp.add && key < w.g.klen - w.g.n) was = *to;
-          }
-        }
+        if (mine) page = paged_page(p, w.g, key >> p.page_log2);
+        auto sum_before = [&]() {  // once the page's number is here, on its way beside the sums
+          if (page < 0) return;
+          to = mp.mass.ptr + page * mp.mass.page + w.head * mp.mass.head + (key & ((1 << p.page_log2) - 1));
+          if (mp.add && key < w.g.klen - w.g.n) was = *to;
+          page = -1;
+        };
         // rows from this one on see the key
         const long long see = (long long)max(0, key - (w.g.klen - w.g.n)) * p.rep;
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -1081,6 +1093,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
               for (int c = 0; c < 128; c += 32) {
                 uint32_t v[32];
                 tmem_ld32(ts + c, v);
+                if (c == 32) sum_before();
 #pragma unroll
                 for (int i = 0; i < 32; i += 4) {
                   const float4 l4 = *reinterpret_cast<const float4*>(row + c + i);
@@ -1099,14 +1112,13 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
         if (*dead) break;
         float total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
         if (it.nb > 1) meet(make_float2(total, 0.f), [&](float2 y) { total += y.x; });
-        if (mine) {
-          if (w.count == 1) {
-            if (to) *to = was + total;
-          } else {
-            mp.part_sum[((long long)blockIdx.x * 2 + w.slot()) * MK_KEYS + half * 128 + r128] = total;
-            if (half == 0 && qd == 0 && lane == 0 && w.slot() == 1)
-              mp.keys_rec[blockIdx.x] = MassRec{w.seg, w.head, w.kt, w.count};
-          }
+        if (w.count == 1) {
+          sum_before();
+          if (to) *to = was + total;
+        } else if (it.nb > 1 ? t0 == 0 : ((qpos - 1) & 1) == t0) {
+          mp.part_sum[((long long)blockIdx.x * 2 + w.slot()) * MK_KEYS + half * 128 + r128] = total;
+          if (half == 0 && qd == 0 && lane == 0 && w.slot() == 1)
+            mp.keys_rec[blockIdx.x] = MassRec{w.seg, w.head, w.kt, w.count};
         }
       } while (w.next(p, mp.kinds));
     } else {

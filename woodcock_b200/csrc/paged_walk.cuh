@@ -361,7 +361,7 @@ __device__ __forceinline__ void store4(uint16_t* p, const float (&x)[4]) {
 
 // Waits give up after a bound; then `dead` lets the block's other waits pass, so that it ends.
 __device__ __forceinline__ void paged_wait(uint64_t* bar, uint32_t parity, volatile int* dead, int* err) {
-  if (*dead) return;
+  if (mbar_wait(bar, parity, 1) || *dead) return;
   if (!mbar_wait(bar, parity)) {
     *dead = 1;
     raise_error(err, kErrTimeout);
