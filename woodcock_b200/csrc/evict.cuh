@@ -640,7 +640,8 @@ struct MassWalk {
   long long pos, lo, hi;
 
   __device__ __forceinline__ int first_row_tile(const PagedAttnParams& p, int k) const {
-    return int((long long)max(0, k * MK_KEYS - (g.klen - g.n)) * p.rep / 128);
+    const int i = k * MK_KEYS - (g.klen - g.n);  // the first row that sees the tile's first key
+    return i <= 0 ? 0 : int((long long)i * p.rep / 128);
   }
   __device__ __forceinline__ void enter(const PagedAttnParams& p) {  // a segment
     nkt = (g.klen + MK_KEYS - 1) / MK_KEYS;
@@ -717,6 +718,13 @@ struct MassWalk {
   }
   __device__ bool place() {
     const long long at = pos + MK_OVER;
+    if (at >= lo && at + QT - qf <= hi) {  // whole, without a division
+      qt0 = qf;
+      qt1 = QT;
+      first = blockIdx.x;
+      count = 1;
+      return true;
+    }
     qt0 = qf + int(max(0ll, lo - at));
     qt1 = int(min((long long)QT, qf + hi - at));
     first = int(paged_div(at, per));
@@ -784,7 +792,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
     }
     for (int i = 0; i < QS; ++i) {
       mbar_init(q_full + i, kKeys ? 1 : QW);
-      mbar_init(q_empty + i, kKeys ? 17 : 1);
+      mbar_init(q_empty + i, kKeys ? 9 : 1);  // two groups read a tile's L
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(s_full + i, 1);
@@ -1051,7 +1059,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
         const bool active = half == 0 || it.two;
         const int key = it.key0 + half * 128 + r128;
         // one tile: its group has the item alone, and the other goes on to the next; several: the first group adds up
-        const bool mine = (it.nb > 1 ? t0 == 0 : (qpos & 1) == t0) && key < w.g.klen && w.count == 1;
+        const bool adds = it.nb > 1 ? t0 == 0 : (qpos & 1) == t0, mine = adds && key < w.g.klen && w.count == 1;
         int page = -1;
         float* to = nullptr;
         float was = 0.f;
@@ -1065,10 +1073,10 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
         // rows from this one on see the key
         const long long see = (long long)max(0, key - (w.g.klen - w.g.n)) * p.rep;
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int t = 0; t < it.nb; ++t, ++qpos) {
-          const int s = qpos % QS;
-          paged_wait(q_full + s, (qpos / QS) & 1, dead, p.err);
-          if (active && (qpos & 1) == t0 && !__any_sync(0xffffffffu, *dead)) {  // tensor memory is read by whole warps
+        for (int t = (t0 ^ qpos) & 1; t < it.nb; t += 2) {
+          const int q = qpos + t, s = q % QS;
+          paged_wait(q_full + s, (q / QS) & 1, dead, p.err);
+          if (active && !__any_sync(0xffffffffu, *dead)) {  // tensor memory is read by whole warps
             scores();
             const float* row = nl + s * 128;
             const int hide = int(min(see - (it.rho0 + t * 128), 128ll));  // columns before this one do not see the key
@@ -1109,13 +1117,15 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(q_empty + s);
         }
+        qpos += it.nb;
         if (*dead) break;
+        if (it.nb == 1 && !adds) continue;
         float total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
         if (it.nb > 1) meet(make_float2(total, 0.f), [&](float2 y) { total += y.x; });
         if (w.count == 1) {
           sum_before();
           if (to) *to = was + total;
-        } else if (it.nb > 1 ? t0 == 0 : ((qpos - 1) & 1) == t0) {
+        } else if (adds) {
           mp.part_sum[((long long)blockIdx.x * 2 + w.slot()) * MK_KEYS + half * 128 + r128] = total;
           if (half == 0 && qd == 0 && lane == 0 && w.slot() == 1)
             mp.keys_rec[blockIdx.x] = MassRec{w.seg, w.head, w.kt, w.count};
