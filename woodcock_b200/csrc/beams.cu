@@ -146,7 +146,7 @@ extern "C" wc_status wc_beam_reorder(wc_ctx* ctx, void* stream, const wc_beam_re
     p.table_out = a->table_out;
     p.out_ld = int(a->out_stride);
     p.W = a->beams;
-    p.parts = 4;
+    p.parts = BR_PARTS;
     p.err = ctx->d_err;
     launch_on(ctx, stream_of(ctx, stream), "beam_reorder", beam_reorder_kernel, dim3(a->requests, g.layers, p.parts),
               dim3(BR_THREADS), 0, true, 1, p);
