@@ -302,24 +302,25 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const __grid_cons
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, b = blockIdx.x;
   if (tid == 0) s_count = 0;
   pdl_wait();
-  for (int w = warp; w < p.W; w += WARPS) {
-    const long long row = (long long)b * p.W + w;
+  // Each beam's log of the sum of exponentials, 16 lanes a beam.
+  for (int w0 = 0; w0 < p.W; w0 += BJ_THREADS / 16) {
+    const int w = w0 + tid / 16, part = tid % 16;
+    const long long row = (long long)b * p.W + min(w, p.W - 1);
     const double2* st = p.stat + row * p.pieces;
-    const int kind = beam_kind(p, row);
+    const float score = p.scores[row];
+    const int kind = beam_kind(p, row), n = kind == 1 ? p.pieces : 0;
     double m = -INFINITY, s = 0;
-    if (kind == 1) {
-      for (int i = lane; i < p.pieces; i += 32)
-        if (st[i].y != 0) m = fmax(m, st[i].x);
+    for (int i = part; i < n; i += 16)
+      if (st[i].y != 0) m = fmax(m, st[i].x);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
-      for (int i = lane; i < p.pieces; i += 32) {
-        const double2 y = st[i];
-        if (y.y != 0) s += y.y * exp2(y.x - m);
-      }
-      s = warp_sum_d(s);
+    for (int o = 8; o > 0; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int i = part; i < n; i += 16) {
+      const double2 y = st[i];
+      if (y.y != 0) s += y.y * exp2(y.x - m);
     }
-    if (lane == 0) {
-      const float score = p.scores[row];
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (part == 0 && w < p.W) {
       if (!(score < INFINITY)) raise_error(p.err, kErrLogits);
       s_score[w] = score;
       s_lse[w] = m * 0.69314718055994530942 + log(s);
@@ -327,47 +328,67 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const __grid_cons
     }
   }
   __syncthreads();
-  // A warp goes through lists, a lane through their places: f(score's order, place) for every candidate.
+  // Candidates, eight of a thread at a time: score's order (0: none) and place. A list's places lie over 8, 16 or 32
+  // threads, of longer lists 2 or 4 in a thread. A ninth is the beam itself where it has ended.
+  constexpr int U = 8;
   const int slots = 2 * p.n, lists = p.W * p.pieces;
+  const int wide = slots <= 8 ? 3 : slots <= 16 ? 4 : 5, more = slots <= 32 ? 0 : slots <= 64 ? 1 : 2;  // log2
+  const int step = BJ_THREADS >> wide, units = ((lists + step - 1) / step) << more;
   const unsigned long long* cand = p.cand + (long long)b * lists * slots;
   const int* counts = p.counts + (long long)b * lists;
-  auto each = [&](auto f) {
-    for (int l0 = warp; l0 < lists; l0 += 2 * WARPS) {
-      unsigned long long c[2][4];
-      int m[2], w[2];
+  unsigned long long k[U + 1];
+  uint32_t at[U + 1];
+  k[U] = at[U] = 0;
+  if (tid < p.W && s_kind[tid] == 2) {
+    k[U] = order_of(s_score[tid]);
+    at[U] = uint32_t(tid) * uint32_t(p.V) + uint32_t(p.pad);
+  }
+  // list / pieces: the half keeps a quotient's border further away than rounding goes (beams x pieces < 2^18 + 64)
+  const float each_piece = 1.f / float(p.pieces);
+  auto fill = [&](int u0) {
+    int w[U], held[U];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int l = l0 + u * WARPS;
-        w[u] = l < lists ? l / p.pieces : 0;
-        m[u] = l < lists && s_kind[w[u]] == 1 ? counts[l] : 0;
-      }
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (lane + 32 * k < m[u]) c[u][k] = cand[(long long)(l0 + u * WARPS) * slots + lane + 32 * k];
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (lane + 32 * k < m[u])
-            f(order_of(s_score[w[u]] + (double(argmax_key_value(c[u][k])) - s_lse[w[u]])),
-              uint32_t(w[u]) * uint32_t(p.V) + argmax_key_index(c[u][k]));
+    for (int u = 0; u < U; ++u) {
+      const int list = ((u0 + u) >> more) * step + (tid >> wide);
+      w[u] = min(int((float(list) + 0.5f) * each_piece), p.W - 1);
+      held[u] = list < lists ? counts[list] : 0;
     }
-    for (int w = tid; w < p.W; w += BJ_THREADS)
-      if (s_kind[w] == 2) f(order_of(s_score[w]), uint32_t(w) * uint32_t(p.V) + uint32_t(p.pad));
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int list = ((u0 + u) >> more) * step + (tid >> wide);
+      const int j = (tid & ((1 << wide) - 1)) + (((u0 + u) & ((1 << more) - 1)) << wide);
+      k[u] = s_kind[w[u]] == 1 && j < held[u] ? cand[(long long)list * slots + j] : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (k[u]) {
+        at[u] = uint32_t(w[u]) * uint32_t(p.V) + argmax_key_index(k[u]);
+        k[u] = order_of(s_score[w[u]] + (double(argmax_key_value(k[u])) - s_lse[w[u]]));
+      }
+  };
+  // f for every candidate; what fits in one fill is not fetched again
+  bool filled = false;
+  auto each = [&](auto f) {
+    for (int u0 = 0; u0 < units; u0 += U) {
+      if (!filled) fill(u0);
+      filled = units <= U;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (k[u]) f(k[u], at[u]);
+    }
+    if (k[U]) f(k[U], at[U]);
   };
   uint32_t top = 0;
-  each([&](unsigned long long k, uint32_t) { top = max(top, uint32_t(k >> 32)); });
+  each([&](unsigned long long x, uint32_t) { top = max(top, uint32_t(x >> 32)); });
   __shared__ uint32_t s_low[WARPS], s_high[WARPS];
   const uint32_t least = reached_by<BJ_THREADS>(top, p.n, s_low, s_high);
   if (__any_sync(0xffffffffu, top >= least))
-    each([&](unsigned long long k, uint32_t at) {
-      if (uint32_t(k >> 32) >= least) {
+    each([&](unsigned long long x, uint32_t where) {
+      if (uint32_t(x >> 32) >= least) {
         const int to = atomicAdd(&s_count, 1);
         if (to < BJ_LIST) {
-          key[to] = k;
-          place[to] = at;
+          key[to] = x;
+          place[to] = where;
         }
       }
     });
@@ -377,7 +398,7 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const __grid_cons
     // Scores that are all but equal: the n-th best of (score, place), bit by bit.
     auto counted = [&](auto test) {
       int c = 0;
-      each([&](unsigned long long k, uint32_t at) { c += test(k, at); });
+      each([&](unsigned long long x, uint32_t where) { c += test(x, where); });
       c = __reduce_add_sync(0xffffffffu, c);
       __syncthreads();
       if (lane == 0) s_sum[warp] = c;
@@ -387,24 +408,26 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const __grid_cons
       return c;
     };
     unsigned long long nth = 0;
+#pragma unroll 1
     for (int bit = 63; bit >= 0; --bit) {
       const unsigned long long probe = nth | (1ull << bit);
-      if (counted([&](unsigned long long k, uint32_t) { return k >= probe; }) >= p.n) nth = probe;
+      if (counted([&](unsigned long long x, uint32_t) { return x >= probe; }) >= p.n) nth = probe;
     }
-    const int more = p.n - counted([&](unsigned long long k, uint32_t) { return k > nth; });
-    uint32_t last = 0xffffffffu;  // the lowest place up to which `more` of the equal ones lie
+    const int left = p.n - counted([&](unsigned long long x, uint32_t) { return x > nth; });
+    uint32_t last = 0xffffffffu;  // the lowest place up to which `left` of the equal ones lie
+#pragma unroll 1
     for (int bit = 31; bit >= 0; --bit) {
       const uint32_t probe = last & ~(1u << bit);
-      if (counted([&](unsigned long long k, uint32_t at) { return k == nth && at <= probe; }) >= more) last = probe;
+      if (counted([&](unsigned long long x, uint32_t where) { return x == nth && where <= probe; }) >= left) last = probe;
     }
     __syncthreads();
     if (tid == 0) s_count = 0;
     __syncthreads();
-    each([&](unsigned long long k, uint32_t at) {
-      if (k > nth || (k == nth && at <= last)) {
+    each([&](unsigned long long x, uint32_t where) {
+      if (x > nth || (x == nth && where <= last)) {
         const int to = atomicAdd(&s_count, 1);
-        key[to] = k;
-        place[to] = at;
+        key[to] = x;
+        place[to] = where;
       }
     });
     __syncthreads();
@@ -414,19 +437,19 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const __grid_cons
   // four lanes a candidate
   for (int i0 = 0; i0 < count; i0 += BJ_THREADS / 4) {
     const int i = i0 + tid / 4;
-    const unsigned long long k = i < count ? key[i] : ~0ull;
-    const uint32_t at = i < count ? place[i] : 0;
+    const unsigned long long mine = i < count ? key[i] : ~0ull;
+    const uint32_t where = i < count ? place[i] : 0;
     int rank = 0;
     for (int j = tid % 4; j < count; j += 4) {
       const unsigned long long y = key[j];
-      rank += y > k || (y == k && place[j] < at);
+      rank += y > mine || (y == mine && place[j] < where);
     }
     rank += __shfl_xor_sync(0xffffffffu, rank, 1);
     rank += __shfl_xor_sync(0xffffffffu, rank, 2);
     if (i < count && rank < p.n && tid % 4 == 0) {
-      p.out_scores[out + rank] = float(value_of(k));
-      p.out_parents[out + rank] = int(at / uint32_t(p.V));
-      p.out_tokens[out + rank] = int(at % uint32_t(p.V));
+      p.out_scores[out + rank] = float(value_of(mine));
+      p.out_parents[out + rank] = int(where / uint32_t(p.V));
+      p.out_tokens[out + rank] = int(where % uint32_t(p.V));
     }
   }
   for (int i = count + tid; i < p.n; i += BJ_THREADS) {
