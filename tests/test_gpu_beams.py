@@ -308,6 +308,20 @@ def test_strided_pages_and_an_output_that_is_given():
     assert torch.equal(out, new) and torch.equal(kk, k) and torch.equal(vv, v)
 
 
+def test_pages_far_into_a_large_pool():
+    """Offsets beyond 2^31 elements."""
+    from woodcock_b200 import ops
+
+    c = Beams(36, [23, 30], 3, 1, 8, 128, 16, BF)
+    total, n = 140_000, c.k.shape[1]  # 16384 elements a page
+    k, v = (torch.empty((total, 8, 16, 128), dtype=BF, device="cuda") for _ in range(2))
+    k[total - n:], v[total - n:] = c.k[0], c.v[0]
+    want = c.expect([[2, 2, 2], [1, 0, 0]])
+    got = ops.beam_reorder(k, v, c.table + (total - n), c.kv, i32([[2, 2, 2], [1, 0, 0]]))
+    assert torch.equal(got - (total - n), want[2])
+    assert torch.equal(k[total - n:], want[0][0]) and torch.equal(v[total - n:], want[1][0])
+
+
 def test_requests_that_are_left_as_they_are():
     from woodcock_b200 import ops
     from woodcock_b200._lib import WcError

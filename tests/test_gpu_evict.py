@@ -428,6 +428,33 @@ def test_other_streams_and_two_at_once():
             check(c, m, g)
 
 
+@pytest.mark.parametrize("rows", [1, 40])
+def test_pages_far_into_a_large_pool(rows):
+    """Offsets beyond 2^31 elements: K, V and their sums."""
+    from woodcock_b200 import ops
+
+    total, cols = 140_000, 10  # 16384 elements a page
+    c = Case(17, [150], [rows], 16, 8, 128, 16, BF, spare=0)
+    far = torch.randperm(cols, generator=c.g, device="cuda") + total - cols
+    k, v = (torch.empty((total, 8, 16, 128), dtype=BF, device="cuda") for _ in range(2))
+    mass = torch.empty((total, 8, 16), device="cuda")
+    near = mass_of(c)
+    order = c.table[0].long()
+    k[far], v[far], mass[far] = c.k[order], c.v[order], near[order]
+    table = far.to(torch.int32)[None].contiguous()
+    ops.paged_mass(c.q, k, mass, table, c.kv)
+    after = near.clone()
+    after[order] = mass[far]
+    check(c, near, after)
+    p = Pool.__new__(Pool)
+    p.k, p.v, p.mass, p.lens, p.page, p.L, p.Hk, p.table = k[far][None].clone(), v[far][None].clone(), mass[far][None].clone(), [150], 16, \
+        1, 8, torch.arange(cols, device="cuda", dtype=torch.int32)[None]
+    want = evicted(p, [70], 3, 9)
+    assert ops.paged_evict(k, v, mass, table, c.kv, 70, sinks=3, recent=9).tolist() == [70]
+    for x, y in ((k, want[0]), (v, want[1]), (mass, want[2])):
+        assert torch.equal(bits(x[far]), bits(y[0]))
+
+
 # ---------------------------------------------------------------------------- together
 
 

@@ -55,8 +55,10 @@ MassLayout mass_layout(const wc_ctx* ctx, const wc_paged_mass_args& a) {
   if (l.few) {
     l.few_blocks = ctx->num_sms;
     l.width = int(std::min(16ll, each));
-    const long long units = mass_most_tiles(g.pages, log2i(g.page_size), b.requests, g.kv_heads, MF_KT) +
-                            (long long)b.requests * g.kv_heads * MF_OVER;
+    // what the pool holds, or the tables, and each item's units beside its tiles
+    const long long in_table = ((long long)b.table_cols * g.page_size + MF_KT - 1) / MF_KT + 1, heads = (long long)b.requests * g.kv_heads;
+    const long long units = std::min(mass_most_tiles(g.pages, log2i(g.page_size), b.requests, g.kv_heads, MF_KT), heads * in_table) +
+                            heads * MF_OVER;
     l.per = int((units + l.few_blocks - 1) / l.few_blocks);
     l.most = l.per / (1 + MF_OVER) + 4;  // an item's units but at both ends, and the list's end
     l.pieces = take(at, size_t(l.few_blocks) * l.most * sizeof(MassPiece));
@@ -154,11 +156,11 @@ void gather_mass(wc_ctx* ctx, cudaStream_t st, const wc_pages& g, MassParams p, 
     if (l.many) gather_many<D>(ctx, st, g, p, l, ws);
   } else {
     p.kinds = kOwnRows;
-    opt_in(ctx, mass_rows_kernel<S, D>, mass_simt_smem<D>());
-    opt_in(ctx, mass_keys_kernel<S, D>, mass_simt_smem<D>());
-    launch_on(ctx, st, "mass_rows", mass_rows_kernel<S, D>, dim3(p.blocks), dim3(MS_THREADS), mass_simt_smem<D>(), true, 1, p);
+    opt_in(ctx, mass_rows_kernel<D>, mass_simt_smem<D>());
+    opt_in(ctx, mass_keys_kernel<D>, mass_simt_smem<D>());
+    launch_on(ctx, st, "mass_rows", mass_rows_kernel<D>, dim3(p.blocks), dim3(MS_THREADS), mass_simt_smem<D>(), true, 1, p);
     launch_on(ctx, st, "mass_join", mass_join_kernel<MS_M, MS_KT>, dim3(p.blocks + 1), dim3(256), 0, true, 1, p);
-    launch_on(ctx, st, "mass_keys", mass_keys_kernel<S, D>, dim3(ctx->num_sms * 2), dim3(MS_THREADS), mass_simt_smem<D>(),
+    launch_on(ctx, st, "mass_keys", mass_keys_kernel<D>, dim3(ctx->num_sms * 2), dim3(MS_THREADS), mass_simt_smem<D>(),
               true, 1, p);
   }
 }

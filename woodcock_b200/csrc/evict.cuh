@@ -83,24 +83,24 @@ __device__ __forceinline__ void mass_scores(const float* qs, const float* ks, in
 
 constexpr int MS_THREADS = 256, MS_M = 16, MS_KT = 64;
 
-template <typename S, int D>
+template <int D>
 __device__ __forceinline__ void mass_load_q(const PagedAttnParams& p, const PagedSeg& g, int head, int rho0, float* qs) {
   for (int c = threadIdx.x; c < MS_M * (D / 8); c += MS_THREADS) {
     const int m = c / (D / 8), col = (c % (D / 8)) * 8;
     const PagedRow r = paged_row(p, g, head, rho0 + m);
     float x[8] = {};
-    if (r.valid) load8(static_cast<const S*>(p.q) + r.tok * p.q_row + r.h * p.q_head + col, x);
+    if (r.valid) load8(static_cast<const float*>(p.q) + r.tok * p.q_row + r.h * p.q_head + col, x);
     store8(qs + m * D + col, x);
   }
 }
-template <typename S, int D>
+template <int D>
 __device__ __forceinline__ void mass_load_k(const PagedAttnParams& p, const PagedSeg& g, int head, int kt, float* ks) {
   for (int c = threadIdx.x; c < MS_KT * (D / 8); c += MS_THREADS) {
     const int kr = c / (D / 8), cc = (c % (D / 8)) * 8, key = kt * MS_KT + kr;
     float x[8] = {};
     const int page = key < g.klen ? paged_page(p, g, key >> p.page_log2) : -1;
     if (page >= 0)
-      load8(static_cast<const S*>(p.K.ptr) + page * p.K.page + head * p.K.head +
+      load8(static_cast<const float*>(p.K.ptr) + page * p.K.page + head * p.K.head +
                 (key & ((1 << p.page_log2) - 1)) * p.K.row + cc, x);
     store8(ks + kr * (D + 4) + cc, x);
   }
@@ -111,8 +111,8 @@ constexpr size_t mass_simt_smem() {
   return sizeof(float) * (size_t(MS_KT) * (D + 4) + MS_M * D + MS_M * (MS_KT + 4)) + 8 * kWalkShared;
 }
 
-// Every row's maximum and sum, on the CUDA cores. Items as in paged attention; a divided one leaves its parts.
-template <typename S, int D>
+// Every row's maximum and sum, for fp32 pages on the CUDA cores. Items as in paged attention; a divided one leaves its parts.
+template <int D>
 __global__ void __launch_bounds__(MS_THREADS) mass_rows_kernel(const __grid_constant__ MassParams mp) {
   const PagedAttnParams& p = mp.a;
   constexpr int M = MS_M, KT = MS_KT, LS = KT + 4;
@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(MS_THREADS) mass_rows_kernel(const __grid_cons
   if (!w.begin(p, mp.kinds, 1, sh)) return;
   do {
     __syncthreads();
-    mass_load_q<S, D>(p, w.g, w.head, w.qt * M, qs);
+    mass_load_q<D>(p, w.g, w.head, w.qt * M, qs);
     const int sk = tid & 63, sr = (tid >> 6) * 4;
     PagedRow rows[2];
 #pragma unroll
@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(MS_THREADS) mass_rows_kernel(const __grid_cons
     float m2[2] = {-INFINITY, -INFINITY}, l2[2] = {0.f, 0.f};
     for (int kt = w.kt0; kt < w.kt1; ++kt) {
       __syncthreads();
-      mass_load_k<S, D>(p, w.g, w.head, kt, ks);
+      mass_load_k<D>(p, w.g, w.head, kt, ks);
       __syncthreads();
       float s[4] = {};
       mass_scores<D>(qs, ks, sk, sr, s);
@@ -267,7 +267,7 @@ __device__ __forceinline__ int mass_request(const long long* tiles, int B, long 
 }
 
 // Sums over the rows, a key tile and head at a time: every row tile that sees the keys, in order.
-template <typename S, int D>
+template <int D>
 __global__ void __launch_bounds__(MS_THREADS) mass_keys_kernel(const __grid_constant__ MassParams mp) {
   const PagedAttnParams& p = mp.a;
   constexpr int M = MS_M, KT = MS_KT;
@@ -288,14 +288,14 @@ __global__ void __launch_bounds__(MS_THREADS) mass_keys_kernel(const __grid_cons
     const int nt = (g.klen + KT - 1) / KT;
     const int head = int((at - mp.tiles[b]) / nt), kt = int((at - mp.tiles[b]) - (long long)head * nt);
     __syncthreads();
-    mass_load_k<S, D>(p, g, head, kt, ks);
+    mass_load_k<D>(p, g, head, kt, ks);
     const int key = kt * KT + sk, rows = g.n * p.rep;
     // the first row that sees the tile's first key
     const int first = max(0, kt * KT - (g.klen - g.n)) * p.rep / M * M;
     float sum = 0.f;
     for (int rho0 = first; rho0 < rows; rho0 += M) {
       __syncthreads();
-      mass_load_q<S, D>(p, g, head, rho0, qs);
+      mass_load_q<D>(p, g, head, rho0, qs);
       if (tid < M) {
         const PagedRow r = paged_row(p, g, head, rho0 + tid);
         ml[tid] = r.valid ? mp.row_ml[(long long)r.tok * p.H + r.h] : make_float2(0.f, 0.f);
@@ -331,7 +331,8 @@ __global__ void __launch_bounds__(MS_THREADS) mass_keys_kernel(const __grid_cons
 // warp; each warp keeps its own maximum and sum. A product sums over head_dim in any order, so a lane's
 // 16 consecutive bytes of a key serve as the places that the operand's layout gives it, if the query's are
 // taken alike: no operand is rearranged.
-constexpr int MF_CONSUMERS = 8, MF_PRODUCERS = 4, MF_THREADS = 32 * (MF_CONSUMERS + MF_PRODUCERS), MF_M = 16, MF_KT = 64, MF_OVER = 2;
+constexpr int MF_CONSUMERS = 8, MF_PRODUCERS = 4, MF_THREADS = 32 * (MF_CONSUMERS + MF_PRODUCERS), MF_M = 16, MF_KT = 64;
+constexpr int MF_OVER = 4;  // 64 ragged steps: 0, 1 and 2 185 to 187 us, 4 182
 constexpr int MF_SPREAD = 4, MF_KEYS_THREADS = 256;  // blocks of the second kernel for one of the first
 
 template <int D>

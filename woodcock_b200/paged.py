@@ -30,6 +30,7 @@ from __future__ import annotations
 import ctypes as C
 import struct
 from functools import lru_cache
+from numbers import Integral
 
 import torch
 
@@ -323,8 +324,8 @@ def paged_mass(q: torch.Tensor, k_pages: torch.Tensor, mass_pages: torch.Tensor,
     be all that were appended: after a verification the accepted ones, behind a prompt its last ones. A row that
     sees nothing adds nothing. Statistics and sums are fp32, in the same order every time.
 
-    Requests must not share pages: with a common prompt each needs keys of its own. Where their keys are far
-    more than the pool holds, nothing is written and the device error word is raised."""
+    Requests must not share pages, since two would write a sum: with a common prompt each needs keys of its own. A
+    call whose keys outgrow the pool because they do raises the device error word and may leave sums as they were."""
     dev = k_pages.device
     pages = _pages(k_pages, k_pages)
     D, kind = pages[14], k_pages.dtype
@@ -364,7 +365,8 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, mass_pages: torch.
     B, cols = table.shape
     lens = _ints(kv_lens, dev, B, "kv_lens")
     most, budgets = cols * pages[12], None
-    if isinstance(budget, int):
+    if isinstance(budget, Integral):
+        budget = int(budget)
         if budget < sinks + recent:
             _fail("budget must not be below sinks + recent")
         budget = min(budget, 0x7FFFFFFF)
