@@ -66,8 +66,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int | None = None
         ls = logits.stride()
     scores = scores.contiguous()
     finished = None if finished is None else finished.contiguous()
-    out = scores.new_empty((B, n)) if n > 0 else _fail("n must be positive")
-    parents, tokens = (torch.empty((B, n), dtype=torch.int32, device=dev) for _ in range(2))
+    if n <= 0:
+        _fail("n must be positive")
+    out, parents, tokens = scores.new_empty((B, n)), *scores.new_empty((2, B, n), dtype=torch.int32).unbind()
     if B == 0:
         return out, parents, tokens
     ctx = _context(dev)
