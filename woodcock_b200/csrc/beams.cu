@@ -18,8 +18,9 @@ SelectLayout select_layout(const wc_ctx* ctx, const wc_beam_select_args& a) {
   SelectLayout l;
   std::memset(&l, 0, sizeof(l));
   const size_t rows = size_t(a.requests) * a.beams;
-  // A piece's first round costs as much as four later ones, and a piece of many leaves blocks idle at the end: as many
-  // rounds as leave three pieces for each place on the device.
+  // A piece's first round costs more than later ones, and a piece of many leaves blocks idle at the end: as many rounds
+  // as leave three pieces for each place on the device (64 x 8 beams over 151,936 tokens: 68 us, one piece 74,
+  // two 71, four 69, eight 75).
   const long long in_row = (a.vocab + BS_ROUND - 1) / BS_ROUND, places = ctx->num_sms * 4ll;
   l.rounds = int(std::min(in_row, std::max(1ll, (long long)rows * in_row / (3 * places))));
   l.pieces = int((in_row + l.rounds - 1) / l.rounds);

@@ -22,7 +22,7 @@ namespace wc {
 // other R are joined without a rounding and only the exponent's own counts: 2^-20 of a term that is e^-11 or
 // less, less nearer to the maximum; over a row's terms it averages to 2^-25 or so in lse.
 //
-// 64 x 8 beams over 151,936 fp32 logits: 68 us (one round a piece 78, five 73), 4.7 TB/s in the first kernel.
+// 64 x 8 beams over 151,936 fp32 logits: 68 us (two rounds a piece 75, five 68, seven 71, ten 74), 4.7 TB/s in the first kernel.
 constexpr int BS_THREADS = 256;
 constexpr int BS_PER = 32;                       // values a thread and round
 constexpr int BS_ROUND = BS_THREADS * BS_PER;
