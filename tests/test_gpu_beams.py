@@ -150,6 +150,65 @@ def test_the_types_lowest_value_is_a_logit():
         check(z, s, 2)
 
 
+# of the kind that a constrained vocabulary is masked with, where -inf is not wanted
+FILLS = [-1e4, -1e6, -1e9, -1e10, -1e12, -1e16, -1e20, -1e30]
+
+
+@pytest.mark.parametrize("fill", FILLS)
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("V, shift", [(3000, 0), (20000, 0), (20001, 3)])
+def test_a_vocabulary_masked_by_a_finite_value(fill, dtype, V, shift):
+    """A handful of tokens is allowed, in pieces with none, a few and many of them; the rest is as good as absent."""
+    from woodcock_b200.context import Context
+
+    n = 6
+    place = torch.arange(V, device="cuda")
+    for allowed in (place % 1111 == 17, (place > 900) & (place < 900 + n), place < 300, place % 7 == 0, place == V - 5):
+        want = n if allowed.sum() > 1 else 3
+        for seed in range(20):
+            z, s = spaced(seed, 2, 3, V, dtype)
+            z = torch.where(allowed, z, fill).to(dtype)
+            if selected(z, s, want)[3]:
+                break
+        wide = torch.full((2, 3, V + 8), math.nan, dtype=dtype, device="cuda")
+        row = wide[:, :, shift: shift + V]
+        row.copy_(z)
+        got = check(row, s, want)
+        assert allowed[got[2].long()].all()
+    Context.get(0).synchronize()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_masked_values_in_several_rounds_of_a_piece(dtype):
+    from woodcock_b200.context import Context
+
+    place = torch.arange(65536, device="cuda")  # two rounds a piece
+    allowed = torch.where(place % 16384 < 8192, place % 4096 == 5, place % 3 == 0)  # few in a round, many in the next
+    for seed in range(8):
+        z, s = spaced(seed, 64, 8, 65536, dtype)
+        if selected(torch.where(allowed, z, -math.inf), s, 8)[3]:
+            break
+    for fill in (-1e10, -1e20):
+        got = check(torch.where(allowed, z, fill).to(dtype), s, 8)
+        assert allowed[got[2].long()].all()
+    Context.get(0).synchronize()
+
+
+@pytest.mark.parametrize("level", [1e10, -1e10, 1e16, -1e16, 1e20, -1e20, 1e30, -1e30, 2e38, -2e38])
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_rows_at_large_values_offer_their_tokens(level, dtype):
+    """Whole rows, and single tokens above the others."""
+    from woodcock_b200 import ops
+    from woodcock_b200.context import Context
+
+    z, s = spaced(43, 1, 2, 9000, dtype)
+    assert (ops.beam_select(torch.full_like(z, level), s, 4)[0] > -math.inf).all()
+    z[:, :, 4000] = level
+    got = ops.beam_select(z, s, 1)
+    assert (got[0] > -math.inf).all() and (got[2] == 4000).all() == (level > 0)
+    Context.get(0).synchronize()
+
+
 def test_dead_and_finished_beams():
     z, s = try_seeds(3, 6, 700, 12)
     first = torch.full_like(s, -math.inf)

@@ -31,6 +31,10 @@ constexpr int BS_MAX_N = 64;
 constexpr int BS_MAX_W = 64;
 constexpr int BJ_THREADS = 512;
 constexpr int BJ_LIST = 2048;
+// Exponents are taken against integers: a logit times log2(e), rounded to 32 bits, then up. Up to 2^20 that leaves less
+// than 1.1 above the exact product; from 2^31 on the rounding alone would make a sum infinite or 0. Logits
+// below -2^21 / log2(e) are no maximum of a piece that is summed this way, and add 0 to it.
+constexpr float BS_FLOOR = -0x1p21f, BS_FAR = 0x1p20f;
 
 struct BeamSelectParams {
   const void* logits;
@@ -148,8 +152,8 @@ __device__ __noinline__ void beam_pieces_again(const T* z, int first, int end, f
   __syncthreads();
 }
 
-// A piece whose maximum's product with log2(e) is no number, or so low that all else counts as nothing (a type's
-// lowest value in every place): its sum relative to the maximum itself, for thread 0.
+// A piece whose maximum lies far from 0 (a mask's value in every place, a type's lowest): its sum relative to the maximum
+// itself, for thread 0.
 template <typename T>
 __device__ __noinline__ double beam_piece_extreme(const T* z, int first, int end, float m, double* s_sum) {
   double sum = 0;
@@ -186,7 +190,7 @@ __global__ void __launch_bounds__(BS_THREADS, 4) beam_pieces_kernel(const __grid
   if (beam_kind(p, row) != 1) return;  // its logits do not matter
   const bool whole = (reinterpret_cast<unsigned long long>(z) & 15) == 0;
   const int first = piece * p.rounds * BS_ROUND, end = min(first + p.rounds * BS_ROUND, p.V);
-  float best = -INFINITY, ref = -2e30f, sum[4] = {0.f, 0.f, 0.f, 0.f}, bound = 0.f;
+  float best = -INFINITY, ref = BS_FLOOR, sum[4] = {0.f, 0.f, 0.f, 0.f}, bound = 0.f;
 #pragma unroll 1
   for (int at = first; at < end; at += BS_ROUND) {
     Logits<T> x[NV];
@@ -252,7 +256,7 @@ __global__ void __launch_bounds__(BS_THREADS, 4) beam_pieces_kernel(const __grid
     R = fmaxf(R, s_ref[i]);
   }
   double total = 0, reference = R;
-  if (fabsf(m) > 1e30f && fabsf(m) < INFINITY) {
+  if (fabsf(m) > BS_FAR && fabsf(m) < INFINITY) {
     total = beam_piece_extreme(z, first, end, m, s_sum);
     reference = double(m) * 1.4426950408889634;
   } else if (tid == 0) {
