@@ -535,7 +535,8 @@ typedef struct {
 } wc_beam_select_args;
 /* The n best continuations of each request over its beams and the vocabulary, by
  * scores[w] + log_softmax(logits[w])[token], ties to the lower beam, then to the lower token; ranked in 64 bits,
- * given in 32. A beam that has ended offers itself alone, with its score and token `pad`; a token at -inf,
+ * given in 32, with a beam's log-sum-exp (exponentials of 32 bits) within 2^-18 of the formula's wherever its logits
+ * lie, for calls of up to 70 million logits (beyond, at worst in proportion). A beam that has ended offers itself alone, with its score and token `pad`; a token at -inf,
  * a dead beam and a beam of which nothing is left offer nothing. Places for which no candidate is left hold
  * score -inf, parent 0, token 0. A beam with a logit (where they are looked at) or score that is NaN or +inf
  * offers nothing and raises the device error word. n and beams at most 64, beams x vocab below 2^31. */

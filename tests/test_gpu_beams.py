@@ -209,6 +209,33 @@ def test_rows_at_large_values_offer_their_tokens(level, dtype):
     Context.get(0).synchronize()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("levels", [(0, 20, -20), (0, 300, -300), (0, 1000, -1000), (1e4, 0, -1e5), (1e6, -1e6, 3e6), (-1e9, 1e9, 0),
+                                    (1e12, -1e16, 2e38)])
+def test_a_row_may_be_shifted(levels, dtype):
+    """Beams at levels of their own, against the formula of what the type makes of them, with the bound that holds at 0.
+    At the last levels a row is of one value and 64 bits hold lse in steps of 2^-13 and more, for both alike."""
+    for V, n in ((700, 6), (20001, 9)):
+        for seed in range(20):
+            z, s = spaced(60 + seed, 2, 3, V)
+            z = (z + torch.tensor(levels, device="cuda")[None, :, None]).to(dtype)
+            if selected(z, s, n)[3]:
+                break
+        check(z, s, n, apart=False)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("fill", [-1e4, -1e6, -1e9, -1e10, -1e16, -1e20, -1e30, 1e9, 1e16, 2e38])
+def test_rows_of_one_value(fill, dtype):
+    """Every token has log-probability -log V, wherever the row lies (64 bits: log V in steps of 2^-53 of the level)."""
+    s = torch.tensor([[-1.0, -2.0], [-7.0, -3.0]], device="cuda")
+    for V in (50, 40000):
+        z = torch.full((2, 2, V), fill, dtype=dtype, device="cuda")
+        check(z, s, 7, apart=False)
+        z[1, 0, V - 3] = 0.0 if fill < 0 else 3e38  # one token beside which the others are nothing
+        check(z, s, 1, apart=False)
+
+
 def test_dead_and_finished_beams():
     z, s = try_seeds(3, 6, 700, 12)
     first = torch.full_like(s, -math.inf)

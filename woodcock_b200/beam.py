@@ -41,8 +41,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int | None = None
     logits [requests][beams][vocab] fp32 or bf16, any strides with contiguous tokens; scores fp32
     [requests][beams], the beams' log probabilities so far (-inf: a dead beam, as all but the first are at the
     start). A continuation's score is scores[w] + log_softmax(logits[w])[token]; ties go to the lower beam, then
-    to the lower token. Ranks are decided in 64 bits, the scores given are rounded to 32. n: default the number of
-    beams, at most 64 (twice the beams leaves enough where some end); at most 64 beams.
+    to the lower token. Ranks are decided in 64 bits, the scores given are rounded to 32; the exponentials behind a
+    beam's log_softmax are of 32 bits, which leaves its scores within 2^-18 of the formula's wherever the row lies (calls of
+    up to 70 million logits; beyond, at worst in proportion). n: default the number of beams, at most 64
+    (twice the beams leaves enough where some end); at most 64 beams.
 
     ``finished`` (bool [requests][beams]): a beam that has ended offers itself alone, with its score and token
     ``pad``; its logits are not looked at, nor a dead beam's. A token at -inf is never chosen; places for which no

@@ -18,9 +18,11 @@ namespace wc {
 // and does the same with the candidates' scores.
 //
 // Ranks are decided in 64 bits: two beams' scores may lie closer than a 32-bit sum resolves, as a score near -20
-// has steps of 2^-19. The exponentials are of 32 bits, 2^(z log2(e) - R) with an integer R, so that sums with
-// other R are joined without a rounding and only the exponent's own counts: 2^-20 of a term that is e^-11 or
-// less, less nearer to the maximum; over a row's terms it averages to 2^-25 or so in lse.
+// has steps of 2^-19. The exponentials are of 32 bits, 2^(z c - R) with c, log2(e) in 32 bits, and an integer R, so that
+// sums with other R are joined without a rounding. c is 1.34e-8 of itself too small, so lse = R / c + log sum, which
+// shifts with the row and has that share of z's distance from R alone. With d, the mean distance of a row's terms
+// from its maximum (at most log V), lse is off by less than 2^-24 (d + 1) for the exponents' rounding, 2^-26 d for c, 2^-22
+// for ex2 and, at worst, 2^-21 a round for the additions: under 2^-18 up to five rounds a piece and V below 2^18.
 //
 // 64 x 8 beams over 151,936 fp32 logits: 68 us (two rounds a piece 75, five 68, seven 71, ten 74), 4.7 TB/s in the first kernel.
 constexpr int BS_THREADS = 256;
@@ -34,6 +36,7 @@ constexpr int BJ_LIST = 2048;
 // Exponents are taken against integers: a logit times log2(e), rounded to 32 bits, then up. Up to 2^20 that leaves less
 // than 1.1 above the exact product; from 2^31 on the rounding alone would make a sum infinite or 0. Logits
 // below -2^21 / log2(e) are no maximum of a piece that is summed this way, and add 0 to it.
+constexpr double kLog2eUsed = kLog2e;  // as the exponents have it
 constexpr float BS_FLOOR = -0x1p21f, BS_FAR = 0x1p20f;
 
 struct BeamSelectParams {
@@ -43,7 +46,7 @@ struct BeamSelectParams {
   const uint8_t* finished;  // [B][W] or null
   int B, W, V, n, pieces, rounds, pad;
   // workspace
-  double2* stat;            // [B W][pieces]: R and the sum of 2^(z log2(e) - R); sum 0: no token, not finite: no numbers
+  double2* stat;            // [B W][pieces]: R and the sum of 2^(z c - R); sum 0: no token, not finite: no numbers
   unsigned long long* cand; // [B W][pieces][2 n]: argmax_key of value and token, in any order
   int* counts;              // [B W][pieces]
   float* out_scores;        // [B][n]
@@ -258,7 +261,7 @@ __global__ void __launch_bounds__(BS_THREADS, 4) beam_pieces_kernel(const __grid
   double total = 0, reference = R;
   if (fabsf(m) > BS_FAR && fabsf(m) < INFINITY) {
     total = beam_piece_extreme(z, first, end, m, s_sum);
-    reference = double(m) * 1.4426950408889634;
+    reference = double(m) * kLog2eUsed;  // exact, and so is the quotient
   } else if (tid == 0) {
     for (int i = 0; i < WARPS; ++i) total += s_sum[i] * double(ex2_approx(s_ref[i] - R));
   }
@@ -329,7 +332,7 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const __grid_cons
     if (part == 0 && w < p.W) {
       if (!(score < INFINITY)) raise_error(p.err, kErrLogits);
       s_score[w] = score;
-      s_lse[w] = m * 0.69314718055994530942 + log(s);
+      s_lse[w] = m / kLog2eUsed + log(s);
       s_kind[w] = kind != 1 || (s > 0 && s < INFINITY) ? kind : 0;  // not without a token, nor where s is no number
     }
   }
