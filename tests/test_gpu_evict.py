@@ -156,6 +156,68 @@ def test_a_row_beside_what_is_not_finite(rows):
     assert torch.isfinite(got[:, [0, 1, 2, 4, 5, 6, 7]]).all() and torch.isfinite(at_keys(mass, c, 1, 200)).all()
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows, lens", [
+    ([0, 1, 0, 2, 0], [700, 90, 0, 33, 64]),                # idle requests among steps
+    ([40, 0, 1, 0], [200, 333, 70, 5]),                     # beside a window
+    ([0] * 3, [257, 0, 1]),                                 # nobody has a row, offsets say so
+    ([0, 3] * 200, [(i * 37) % 90 for i in range(400)]),    # more requests than blocks
+])
+def test_requests_without_rows_start_anew_too(dtype, rows, lens):
+    """add=False: every key's sum is that of this call's weights, 0 where no row looks; with add nothing changes."""
+    from woodcock_b200 import ops
+    from woodcock_b200.context import Context
+
+    c = Case(21, lens, rows, 8, 2, 64, 16, dtype)
+    before = mass_of(c)
+    for b, n in enumerate(lens):  # what lies there does not count
+        at = torch.arange(n, device="cuda")
+        before[c.table[b].long()[at // 16], :, at % 16] = math.nan
+    mass = before.clone()
+    ops.paged_mass(c.q, c.k, mass, c.table, c.kv, q_offsets=c.off, add=False)
+    Context.get(0).synchronize()
+    idle = before.clone()
+    for b, (n, r) in enumerate(zip(lens, rows)):
+        if r == 0:
+            assert (at_keys(mass, c, b, n) == 0).all(), f"request {b}"
+            at = torch.arange(n, device="cuda")
+            idle[c.table[b].long()[at // 16], :, at % 16] = 0.0
+    check(c, idle, mass, add=False)
+    before = mass_of(c)
+    mass = before.clone()
+    ops.paged_mass(c.q, c.k, mass, c.table, c.kv, q_offsets=c.off)
+    check(c, before, mass)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_a_call_without_rows_or_offsets(dtype):
+    from woodcock_b200 import ops
+    from woodcock_b200._lib import WcError
+    from woodcock_b200.context import Context
+
+    c = Case(22, [100, 17], [0, 0], 4, 2, 64, 32, dtype, layout="rows")
+    before = mass_of(c)
+    mass = before.clone()
+    assert ops.paged_mass(c.q, c.k, mass, c.table, c.kv) is mass
+    assert torch.equal(mass.nan_to_num(-1), before.nan_to_num(-1))
+    assert ops.paged_mass(c.q, c.k, mass, c.table, c.kv, add=False) is mass
+    want = before.clone()
+    for b, n in enumerate(c.lens):
+        at = torch.arange(n, device="cuda")
+        want[c.table[b].long()[at // 32], :, at % 32] = 0.0
+    assert torch.equal(mass.nan_to_num(-1), want.nan_to_num(-1))
+    Context.get(0).synchronize()
+    for kw, what in (({"mass_pages": mass.double()}, "fp32"), ({"scale": -1.0}, "scale"),
+                     ({"mass_pages": mass[:1].expand(mass.shape)}, "overlap")):
+        with pytest.raises(ValueError, match=what):  # refused as with rows
+            ops.paged_mass(**{"q": c.q, "k_pages": c.k, "mass_pages": mass, "page_table": c.table, "kv_lens": c.kv, "add": False, **kw})
+    table = c.table.clone()
+    table[0, 1] = -1
+    ops.paged_mass(c.q, c.k, mass, table, c.kv, add=False)
+    with pytest.raises(WcError):
+        Context.get(0).synchronize()
+
+
 @pytest.mark.parametrize("rows, dtype", [(1, BF), (20, BF), (3, F32)])
 def test_bad_tables_raise_the_error_word(rows, dtype):
     from woodcock_b200 import ops

@@ -184,29 +184,15 @@ extern "C" wc_status wc_paged_mass(wc_ctx* ctx, void* stream, const wc_paged_mas
     const wc_pages g = keys_only(a->pages);
     const wc_paged_batch& b = a->batch;
     check_mass(g, a->mass);
-    if (b.rows == 0) return;
-    check_rows(a->q, a->q_stride, g.dtype, "paged_mass: q must be 16-byte aligned, rows contiguous");
-    const MassLayout l = mass_layout(ctx, *a);
-    if (!a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 256 || a->workspace_bytes < l.bytes)
-      fail(WC_ERR_CAPACITY, "paged_mass: workspace missing, misaligned or too small");
-    const Run scratch{a->workspace, (long long)l.bytes},
-        q = rows_run(a->q, a->q_stride, g.dtype, b.rows, b.heads, g.head_dim),
-        table = table_run(b.page_table, b.table_stride, b.table_cols, b.requests), lens = ints_run(b.kv_lens, b.requests),
-        offsets = ints_run(b.q_offsets, b.requests + 1ll);
-    check_apart(scratch, {q, table, lens, offsets}, "paged_mass: the workspace must not overlap an input");
+    const Run table = table_run(b.page_table, b.table_stride, b.table_cols, b.requests), lens = ints_run(b.kv_lens, b.requests),
+              offsets = ints_run(b.q_offsets, b.requests + 1ll);
     const Strided K = places(g, g.k, g.k_stride, a->layer), mass = mass_places(g, a->mass, a->layer);
     need(mass.nested, "paged: mass pages must not overlap");
     need(!meets(K, mass), "paged_mass: mass must not overlap the pages");
-    need(!meets_run(K, scratch.p, scratch.bytes), "paged_mass: the workspace must not overlap the pages");
-    for (const Run& x : {scratch, q, table, lens, offsets})
+    for (const Run& x : {table, lens, offsets})
       need(!meets_run(mass, x.p, x.bytes), "paged_mass: mass must not overlap the workspace or an input");
-    DeviceScope scope(ctx->device);
-    char* ws = static_cast<char*>(a->workspace);
     MassParams p;
     std::memset(&p, 0, sizeof(p));
-    p.a.q = a->q;
-    p.a.q_row = a->q_stride[0];
-    p.a.q_head = a->q_stride[1];
     p.a.K = pool(g, g.k, g.k_stride, a->layer);
     p.a.pages = g.pages;
     p.a.page_log2 = log2i(g.page_size);
@@ -221,15 +207,38 @@ extern "C" wc_status wc_paged_mass(wc_ctx* ctx, void* stream, const wc_paged_mas
     p.a.Hk = g.kv_heads;
     p.a.rep = b.heads / g.kv_heads;
     p.a.scale_log2 = a->scale * kLog2e;
-    p.a.rec = reinterpret_cast<PagedRec*>(ws + l.rec);
     p.a.err = ctx->d_err;
     p.mass = {a->mass.p + a->mass.stride[0] * a->layer, a->mass.stride[0], a->mass.stride[1], a->mass.stride[2]};
     p.add = a->add;
+    const cudaStream_t st = stream_of(ctx, stream);
+    if (b.rows == 0) {
+      DeviceScope scope(ctx->device);
+      const long long heads = (long long)b.requests * g.kv_heads;
+      if (!a->add)
+        launch_on(ctx, st, "mass_clear", mass_clear_kernel, dim3(unsigned(std::min(heads, ctx->num_sms * 8ll))), dim3(256), 0, true, 1,
+                  p);
+      return;
+    }
+    check_rows(a->q, a->q_stride, g.dtype, "paged_mass: q must be 16-byte aligned, rows contiguous");
+    const MassLayout l = mass_layout(ctx, *a);
+    if (!a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 256 || a->workspace_bytes < l.bytes)
+      fail(WC_ERR_CAPACITY, "paged_mass: workspace missing, misaligned or too small");
+    const Run scratch{a->workspace, (long long)l.bytes},
+        q = rows_run(a->q, a->q_stride, g.dtype, b.rows, b.heads, g.head_dim);
+    check_apart(scratch, {q, table, lens, offsets}, "paged_mass: the workspace must not overlap an input");
+    need(!meets_run(K, scratch.p, scratch.bytes), "paged_mass: the workspace must not overlap the pages");
+    for (const Run& x : {scratch, q})
+      need(!meets_run(mass, x.p, x.bytes), "paged_mass: mass must not overlap the workspace or an input");
+    DeviceScope scope(ctx->device);
+    char* ws = static_cast<char*>(a->workspace);
+    p.a.q = a->q;
+    p.a.q_row = a->q_stride[0];
+    p.a.q_head = a->q_stride[1];
+    p.a.rec = reinterpret_cast<PagedRec*>(ws + l.rec);
     p.row_ml = reinterpret_cast<float2*>(ws + l.row_ml);
     p.part_ml = reinterpret_cast<float2*>(ws + l.part_ml);
     p.tiles = reinterpret_cast<long long*>(ws + l.tiles);
     p.blocks = l.blocks;
-    const cudaStream_t st = stream_of(ctx, stream);
     if (g.dtype == WC_BF16) {
       if (g.head_dim == 64) gather_mass<uint16_t, 64>(ctx, st, g, p, l, ws);
       else gather_mass<uint16_t, 128>(ctx, st, g, p, l, ws);

@@ -66,6 +66,27 @@ __device__ __forceinline__ float mass_minus_l(float m, float l) {
   return log2f(y.y) - y.x;
 }
 
+// A call that starts the sums anew does so for requests without rows too. Each block takes its share of their heads.
+__device__ __forceinline__ void mass_clear(const MassParams& mp, int block, int blocks) {
+  const PagedAttnParams& p = mp.a;
+  for (long long at = block; at < (long long)p.B * p.Hk; at += blocks) {
+    const int b = int(at / p.Hk), head = int(at - (long long)b * p.Hk);
+    const PagedSeg g = paged_seg(p, kOwnRows, b);
+    if (g.n > 0) continue;
+    for (int key = threadIdx.x; key < g.klen; key += blockDim.x) {
+      const int page = paged_page(p, g, key >> p.page_log2);
+      if (page >= 0) mp.mass.ptr[page * mp.mass.page + head * mp.mass.head + (key & ((1 << p.page_log2) - 1))] = 0.f;
+    }
+  }
+}
+
+// A call in which no request has a row.
+__global__ void __launch_bounds__(256) mass_clear_kernel(const __grid_constant__ MassParams mp) {
+  pdl_wait();
+  pdl_launch_dependents();
+  mass_clear(mp, blockIdx.x, gridDim.x);
+}
+
 // The first kernel's scores, one row tile against one key tile: 16 rows x 64 keys, a key and four rows a
 // thread. qs [16][D], ks [64][D + 4].
 template <int D>
@@ -320,6 +341,7 @@ __global__ void __launch_bounds__(MS_THREADS) mass_keys_kernel(const __grid_cons
     }
     __syncthreads();
   }
+  if (!mp.add && p.offsets) mass_clear(mp, blockIdx.x, gridDim.x);
 }
 
 // ---- few rows (bf16 pages, at most 16 a KV head: steps and accepted chains)
@@ -603,6 +625,7 @@ __global__ void __launch_bounds__(MF_KEYS_THREADS, 4) mass_few_keys_kernel(const
     buf += (size_t)g.tiles * MF_KT * mp.width;
     g = next;
   }
+  if (!mp.add && p.offsets) mass_clear(mp, blockIdx.y * gridDim.x + blockIdx.x, gridDim.x * gridDim.y);
 }
 
 // ---- many rows (bf16 pages, more than 16 a KV head: windows and prompts)

@@ -320,9 +320,10 @@ def paged_mass(q: torch.Tensor, k_pages: torch.Tensor, mass_pages: torch.Tensor,
     mass[b][kv head][key] = was + the sum over request b's new rows and the kv head's query heads of
     softmax(scale q K^T)[key], the weights that paged_attention gives without a tree_mask. q as there
     ([rows][heads][head_dim] of the pages' dtype). ``was`` is what the key gathered before: 0 for the keys that
-    are new in this call (a page may hold anything before), and with ``add=False`` for all of them. Rows need not
-    be all that were appended: after a verification the accepted ones, behind a prompt its last ones. A row that
-    sees nothing adds nothing. Statistics and sums are fp32, in the same order every time.
+    are new in this call (a page may hold anything before), and with ``add=False`` for all of them, so that the
+    keys of a request without rows have 0 then. Rows need not be all that were appended: after a verification the
+    accepted ones, behind a prompt its last ones. A row that sees nothing adds nothing. Statistics and sums are
+    fp32, in the same order every time.
 
     Requests must not share pages, since two would write a sum: with a common prompt each needs keys of its own. A
     call whose keys outgrow the pool because they do raises the device error word and may leave sums as they were."""
@@ -333,12 +334,12 @@ def paged_mass(q: torch.Tensor, k_pages: torch.Tensor, mass_pages: torch.Tensor,
     q, qs, shape = _rows(q, kind, dev, None, D, None, "q")
     T, H, _ = shape
     batch, B, keep = _batch(T, H, page_table, kv_lens, q_offsets, dev)
-    if T == 0 or B == 0:
+    if B == 0:
         return mass_pages
     ctx = _context(dev)
     device = ctx.device.index
     n = _mass_workspace(device, pages[10], pages[11], pages[12], pages[13], D, batch[2], B,
-                        q_offsets is not None, T, H)
+                        q_offsets is not None, T, H) if T else 0
     ws = q.new_empty(n + 256, dtype=torch.uint8)
     ctx.check(lib().wc_paged_mass(ctx.h, _stream(device), _MASS.pack(
         *pages, *batch, q.data_ptr(), qs[0], qs[1], *mass, -(-ws.data_ptr() // 256) * 256, n,
