@@ -218,6 +218,29 @@ def test_a_call_without_rows_or_offsets(dtype):
         Context.get(0).synchronize()
 
 
+@pytest.mark.parametrize("rows, H, dtype", [(5, 8, BF), (2, 32, BF), (5, 8, F32), (40, 8, BF), (200, 8, BF)])
+@pytest.mark.parametrize("first", [0, 1])
+def test_a_row_that_is_not_finite_weighs_what_it_sees(rows, H, dtype, first):
+    """A NaN in a row's query makes the keys NaN that the row sees; those behind them keep the other rows' weight."""
+    from woodcock_b200 import ops
+
+    c = Case(23, [100, 300], [rows, rows], H, 4, 64, 16, dtype)
+    rep, clean = H // 4, c.q.clone()
+    c.q[first, 2 * rep] = math.nan  # of the first request, third key head
+    before = mass_of(c, 0.5)
+    mass = before.clone()
+    ops.paged_mass(c.q, c.k, mass, c.table, c.kv)
+    seen = max(0, 100 - rows + first + 1)
+    got = at_keys(mass, c, 0, 100)
+    assert got[:seen, 2].isnan().all()
+    c.q = clean
+    c.q[first] = 0  # the formula without the row's weight: at the keys it does not see it has none
+    want, rel = gathered(c, 0, 0)
+    late = got[seen:, 2].double()
+    assert ((late - want[seen:, 2]).abs() <= want[seen:, 2] * (rel + 2.0 ** -23)).all()
+    assert torch.isfinite(got[:, [0, 1, 3]]).all() and torch.isfinite(at_keys(mass, c, 1, 300)).all()
+
+
 @pytest.mark.parametrize("rows, dtype", [(1, BF), (20, BF), (3, F32)])
 def test_bad_tables_raise_the_error_word(rows, dtype):
     from woodcock_b200 import ops

@@ -610,6 +610,17 @@ __global__ void __launch_bounds__(MF_KEYS_THREADS, 4) mass_few_keys_kernel(const
         sum[2] += ex2_approx(y.z - s.x) * s.y;
         sum[3] += ex2_approx(y.w - s.x) * s.y;
       }
+      // The score that a row has for a new key it does not see, -inf, gives a weight of 0 unless the row's sum is no
+      // number: then without such rows.
+      if (key + 3 > g.old && !(fabsf((sum[0] + sum[1]) + (sum[2] + sum[3])) < INFINITY)) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          sum[e] = 0.f;
+#pragma unroll 1
+          for (int r = max(0, key + e - g.old) * p.rep; r < g.rows; ++r)
+            sum[e] += ex2_approx(z[r * MF_KT + e] - ml[n & 1][r].x) * ml[n & 1][r].y;
+        }
+      }
       if (to) {
         if (four) {
           *reinterpret_cast<float4*>(to) = make_float4(was[0] + sum[0], was[1] + sum[1], was[2] + sum[2], was[3] + sum[3]);
