@@ -332,7 +332,8 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const __grid_cons
     if (part == 0 && w < p.W) {
       if (!(score < INFINITY)) raise_error(p.err, kErrLogits);
       s_score[w] = score;
-      s_lse[w] = m / kLog2eUsed + log(s);
+      // far from 0 the quotient has to be exact
+      s_lse[w] = (fabs(m) > 2 * BS_FAR ? m / kLog2eUsed : m * (1 / kLog2eUsed)) + log(s);
       s_kind[w] = kind != 1 || (s > 0 && s < INFINITY) ? kind : 0;  // not without a token, nor where s is no number
     }
   }
