@@ -241,6 +241,31 @@ def test_a_row_that_is_not_finite_weighs_what_it_sees(rows, H, dtype, first):
     assert torch.isfinite(got[:, [0, 1, 3]]).all() and torch.isfinite(at_keys(mass, c, 1, 300)).all()
 
 
+@pytest.mark.parametrize("rows, dtype", [(1, BF), (5, BF), (5, F32), (20, BF), (40, BF), (150, BF)])
+def test_a_key_that_no_row_can_want(rows, dtype):
+    """A key that is -inf where every query is positive has the score -inf: no weight, and none lost by the others."""
+    from woodcock_b200 import ops
+
+    c = Case(24, [200, 333], [rows, rows], 8, 4, 64, 16, dtype)
+    c.q[:, :, 5] = c.q[:, :, 5].abs() + 0.5
+    want, rel = [], []
+    for b in range(2):  # the formula with a key far away, whose weight is 0 in 64 bits
+        c.k[c.table[b, 2].long(), 1, 3] = 0.0
+        c.k[c.table[b, 2].long(), 1, 3, 5] = -3e4
+        w, _ = gathered(c, b, b * rows)
+        assert w[35, 1] == 0
+        want.append(w)
+        c.k[c.table[b, 2].long(), 1, 3, 5] = 0.0
+        rel.append(gathered(c, b, b * rows)[1])  # the bound is of the other keys' scores
+        c.k[c.table[b, 2].long(), 1, 3, 5] = -math.inf
+    mass = mass_of(c, math.nan)
+    ops.paged_mass(c.q, c.k, mass, c.table, c.kv, add=False)
+    for b in range(2):
+        got = at_keys(mass, c, b, c.lens[b]).double()
+        assert torch.isfinite(got).all()
+        assert ((got - want[b]).abs() <= want[b] * (rel[b] + 2.0 ** -23)).all()
+
+
 @pytest.mark.parametrize("rows, dtype", [(1, BF), (20, BF), (3, F32)])
 def test_bad_tables_raise_the_error_word(rows, dtype):
     from woodcock_b200 import ops

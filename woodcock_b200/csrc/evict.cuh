@@ -1024,7 +1024,10 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
         long long from[QR / 32];
 #pragma unroll
         for (int e = 0; e < QR / 32; ++e) {
-          const PagedRow r = paged_row(p, w.g, w.head, it.rho0 + t * 128 + r0 + e * 32 + lane);
+          // A tile is filled up with the request's last row, for nobody: it sees every key, so that where its product is
+          // no number nor is the key's sum, as 0 times an infinite key would make it. Tiles of no rows are zeros.
+          const int rho = it.rho0 + t * 128 + r0 + e * 32 + lane;
+          const PagedRow r = paged_row(p, w.g, w.head, t == 0 || it.two ? min(rho, w.g.n * p.rep - 1) : rho);
           from[e] = r.valid ? r.tok * p.q_row + r.h * p.q_head : -1;
         }
         if (pos >= QS) paged_wait(q_empty + s, ((pos / QS) - 1) & 1, dead, p.err);
@@ -1174,7 +1177,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
       do {
         const Item it = item_of(w);
         const PagedRow r = paged_row(p, w.g, w.head, it.rho0 + half * 128 + r128);
-        const int lim = r.valid ? r.lim : 0x7fffffff;  // rows that pad the tile see everything, for nobody
+        const int lim = r.valid ? r.lim : 0x7fffffff;  // rows that fill the tile up see everything, for nobody
         float m = -INFINITY, l = 0.f;
         if (half == 0 || it.two) {
           for (int t = t0; t < it.nb; t += dt) {
