@@ -487,9 +487,9 @@ typedef struct {
  * it sees its weight, one that sees nothing none. `was` is what the key gathered before; 0 for the keys
  * that are new in this call (the request's last ones, one for each of its rows), and for all of them where
  * `add` is 0, those of requests without rows among them. Statistics and sums are fp32, added in the same
- * order every time. Requests must not share
- * pages (two would write a sum); a call whose keys outgrow the pool because they do raises the device error
- * word and may leave sums as they were. The pages themselves are only read. */
+ * order every time. Requests must not share pages (two would write a sum); a call whose requests have more
+ * pages than the pool because they do raises the device error word, and the pages' sums are not to be used.
+ * The pages themselves are only read. */
 WC_API wc_status wc_paged_mass(wc_ctx* ctx, void* stream, const wc_paged_mass_args* args);
 /* Bytes of workspace that wc_paged_mass needs for these arguments (buffers are not looked at, but for
  * whether there are q_offsets). */

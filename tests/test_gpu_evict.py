@@ -307,6 +307,33 @@ def test_requests_that_share_pages_leave_the_mass_as_it_was():
     assert torch.equal(mass.nan_to_num(-1), before.nan_to_num(-1))
 
 
+@pytest.mark.parametrize("rows, dtype", [([1, 1], BF), ([5, 5], BF), ([20, 20], BF), ([200, 200], BF), ([3, 3], F32), ([1, 20], BF),
+                                         ([40, 0], BF), ([0, 3], F32)])
+def test_more_pages_than_the_pool_has_raise_the_error_word(rows, dtype):
+    """Two requests on the same 20 pages of 21, whichever kernels their rows take; a pool that is full to its last page will do."""
+    from woodcock_b200 import ops
+    from woodcock_b200._lib import WcError
+    from woodcock_b200.context import Context
+
+    ctx = Context.get(0)
+    ctx.synchronize()
+    c = Case(25, [320], [sum(rows)], 8, 4, 64, 16, dtype)
+    ops.paged_mass(c.q, c.k, mass_of(c, 0.0), c.table.expand(2, -1).contiguous(), i32([320, 320]), q_offsets=offsets(rows),
+                   add=False)
+    with pytest.raises(WcError):
+        ctx.synchronize()
+    c = Case(25, [320, 161], rows, 8, 4, 64, 16, dtype, spare=0)
+    for b in range(2):  # every page of the pool
+        c.lens[b] = 320
+    c.kv = i32(c.lens)
+    c.k.nan_to_num_(0.25)
+    before = mass_of(c)
+    mass = before.clone()
+    ops.paged_mass(c.q, c.k, mass, c.table, c.kv, q_offsets=c.off)
+    ctx.synchronize()
+    check(c, before, mass)
+
+
 def test_arguments_of_mass_that_are_refused():
     from woodcock_b200 import ops
 

@@ -66,6 +66,26 @@ __device__ __forceinline__ float mass_minus_l(float m, float l) {
   return log2f(y.y) - y.x;
 }
 
+// Pages of a request whose sums the call writes.
+__device__ __forceinline__ int mass_pages(const MassParams& mp, const PagedSeg& g) {
+  return g.n > 0 || !mp.add ? (g.klen + (1 << mp.a.page_log2) - 1) >> mp.a.page_log2 : 0;
+}
+
+// Requests that share no pages have no more of them than the pool: raises the error bit where the call's have, whose
+// sums several blocks write. For kThreads threads of one block, t their numbers, while they would wait for their
+// first tiles anyway (in a kernel's last block, or before its search, it costs 1 us); `pages` is 0 before.
+template <int kThreads>
+__device__ __forceinline__ void mass_check_pool(const MassParams& mp, int t, unsigned long long* pages) {
+  const PagedAttnParams& p = mp.a;
+  unsigned long long mine = 0;
+  for (int b = t; b < p.B; b += kThreads) mine += mass_pages(mp, paged_seg(p, kOwnRows, b));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if (t % 32 == 0 && mine) atomicAdd(pages, mine);
+  named_sync(1, kThreads);
+  if (t == 0 && *pages > (unsigned long long)p.pages) raise_error(p.err, kErrPage);
+}
+
 // A call that starts the sums anew does so for requests without rows too. Each block takes its share of their heads.
 __device__ __forceinline__ void mass_clear(const MassParams& mp, int block, int blocks) {
   const PagedAttnParams& p = mp.a;
@@ -198,12 +218,12 @@ __device__ __forceinline__ int mass_tile(const PagedAttnParams& p, int tok0, int
 }
 
 // Key tiles of requests that share no pages, at most.
-__host__ __device__ __forceinline__ long long mass_most_tiles(int pages, int page_log2, int B, int Hk, int KT) {
+inline long long mass_most_tiles(int pages, int page_log2, int B, int Hk, int KT) {
   return (((long long)pages << page_log2) / KT + B) * Hk;
 }
 
 // Joins the parts of divided items, one block an item; where `tiles` is asked for, a last block counts the key
-// tiles before each request.
+// tiles before each request, and the pages of all.
 template <int M, int KT>
 __global__ void __launch_bounds__(256) mass_join_kernel(const __grid_constant__ MassParams mp) {
   constexpr int LANES = 256 / M;  // lanes a row
@@ -213,13 +233,14 @@ __global__ void __launch_bounds__(256) mass_join_kernel(const __grid_constant__ 
   pdl_launch_dependents();
   if (int(blockIdx.x) == mp.blocks) {
     __shared__ long long sums[8];
-    long long base = 0;
+    long long base = 0, pages = 0;
     for (int b0 = 0; b0 < p.B; b0 += 256) {
       const int b = b0 + tid;
       long long w = 0;
       if (b < p.B) {
         const PagedSeg g = paged_seg(p, mp.kinds, b);
         if (g.n > 0) w = (long long)((g.klen + KT - 1) / KT) * p.Hk;
+        pages += mass_pages(mp, g);
       }
       long long x = w;
 #pragma unroll
@@ -237,9 +258,13 @@ __global__ void __launch_bounds__(256) mass_join_kernel(const __grid_constant__ 
       if (b < p.B) mp.tiles[b] = before + x - w;
       __syncthreads();
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) pages += __shfl_xor_sync(0xffffffffu, pages, o);
+    if (lane == 0) sums[warp] = pages;
+    __syncthreads();
     if (tid == 0) {
-      // more than the pool holds: requests share pages, whose sums two blocks would write
-      const bool shared = base > mass_most_tiles(p.pages, p.page_log2, p.B, p.Hk, KT);
+      for (int i = 1; i < 8; ++i) pages += sums[i];
+      const bool shared = pages > p.pages;  // requests share pages, whose sums two blocks would write
       if (shared) raise_error(p.err, kErrPage);
       mp.tiles[p.B] = shared ? 0 : base;
     }
@@ -392,7 +417,10 @@ __global__ void __launch_bounds__(MF_THREADS, 1)
     mbar_init(empty + tid, MF_CONSUMERS / 2);
     mbar_fence_init();
   }
-  if (tid == 0) *dead = 0;
+  if (tid == 0) {
+    *dead = 0;
+    sh[35] = 0;
+  }
   pdl_wait();
   pdl_launch_dependents();
   __syncthreads();
@@ -448,6 +476,8 @@ __global__ void __launch_bounds__(MF_THREADS, 1)
   const int g8 = lane >> 2, t4 = lane & 3, kr = (g8 >> 1) | ((g8 & 1) << 2);
   const int set = warp >> 2, slice = (warp & 3) * 16;
   float* buf = mp.scores + (long long)blockIdx.x * mp.per * MF_KT * mp.width;
+  if (blockIdx.x == MF_OVER / w.per)  // it has the line's first tile
+    mass_check_pool<32 * MF_CONSUMERS>(mp, tid, reinterpret_cast<unsigned long long*>(sh + 35));
   do {
     const int R = min(w.g.n * p.rep, 8 * NT);
     uint4 q[NT][NV];
@@ -844,6 +874,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
     mbar_init(drain, 1);
     mbar_fence_init();
     *dead = 0;
+    sh[35] = 0;
   }
   pdl_wait();
   pdl_launch_dependents();
@@ -1174,6 +1205,8 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
         }
       } while (w.next(p, mp.kinds));
     } else {
+      if (blockIdx.x == MM_OVER / w.per)  // it has the line's first tile
+        mass_check_pool<512>(mp, tid - 128, reinterpret_cast<unsigned long long*>(sh + 35));
       do {
         const Item it = item_of(w);
         const PagedRow r = paged_row(p, w.g, w.head, it.rho0 + half * 128 + r128);

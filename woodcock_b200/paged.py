@@ -326,7 +326,8 @@ def paged_mass(q: torch.Tensor, k_pages: torch.Tensor, mass_pages: torch.Tensor,
     fp32, in the same order every time.
 
     Requests must not share pages, since two would write a sum: with a common prompt each needs keys of its own. A
-    call whose keys outgrow the pool because they do raises the device error word and may leave sums as they were."""
+    call whose requests have more pages than the pool because they do raises the device error word, and the pages'
+    sums are not to be used; sharing of fewer pages goes unnoticed."""
     dev = k_pages.device
     pages = _pages(k_pages, k_pages)
     D, kind = pages[14], k_pages.dtype
