@@ -119,8 +119,10 @@ struct Logits {
   }
 };
 
-// Too many values at the bound (equal ones, or values in few threads): the n best of a row's [first, end), the n-th
-// found bit by bit. Reads the values again, so that the way that is always taken does not keep them.
+// Too many values at the bound (equal ones, values in few threads, values that rise behind the first round): the n best
+// of a row's [first, end), the n-th found bit by bit. Reads the values again, 65 times, so that the way that is always
+// taken does not keep them. 64 x 8 beams over 151,936 tokens where every piece comes here (all logits alike or rising; a
+// hundred tokens in a run and the rest at a finite mask, while -inf is below every bound: 56 us): 2.7 ms, else 68 us.
 template <typename T>
 __device__ __noinline__ void beam_pieces_again(const T* z, int first, int end, float bound, int n, unsigned long long* list,
                                                uint32_t* s_sum, int* s_count) {

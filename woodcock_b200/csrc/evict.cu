@@ -71,7 +71,9 @@ MassLayout mass_layout(const wc_ctx* ctx, const wc_paged_mass_args& a) {
     const long long mean = (rep * b.rows + b.requests - 1) / b.requests;
     l.blocks = ctx->num_sms;
     // 8 requests of 8192 keys, 32 query and 8 KV heads: 68 rows a head 82 us in the windows' modes and 88 in the
-    // prompts', 128 rows 83 and 89, 192 rows 129 and 124, 256 rows 129 and 124; 2 prompts of 1000 rows 193 and 174
+    // prompts', 128 rows 83 and 89, 192 rows 129 and 124, 256 rows 129 and 124; 2 prompts of 1000 rows 193 and 174.
+    // Which requests have how many rows is device data: the mean counts those that these kernels do not see, so
+    // that a prompt beside many steps may get the windows' modes.
     l.rows = mean <= 128 ? kRows128 : kRows256;
     l.keys = mean <= 128 ? kKeysWindow : kKeysPrompt;
     l.ids = int(rep * b.rows / 128) + b.requests + 1;

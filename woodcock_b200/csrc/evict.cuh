@@ -60,7 +60,8 @@ __device__ __forceinline__ float2 mass_row(float m, float l) {
   return make_float2(m == -INFINITY ? 0.f : m, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l));
 }
 
-// The same as one number: 2^(s - M) / sum = 2^(s + it).
+// The same as one number: 2^(s - M) / sum = 2^(s + it). Its rounding, 2^-24 of M + log2(sum), is the weights' own;
+// with M and 1 / sum apart an exponential would take an instruction more, and they are what bounds the many rows.
 __device__ __forceinline__ float mass_minus_l(float m, float l) {
   const float2 y = mass_row(m, l);
   return log2f(y.y) - y.x;
@@ -1288,7 +1289,8 @@ __global__ void __launch_bounds__(MK_KEYS) mass_fold_kernel(const __grid_constan
 // request, head), writes down where the kept rows lie and moves their sums. Where there are lists enough it
 // moves the rows as well: its selection, bound by latency, runs beside other blocks' copies, bound by HBM.
 // Where there are few, a second kernel moves them, several blocks a list. 32 requests, 4 layers, 1024 lists: 305 us
-// (5.3 TB/s; in two kernels 331); one request, 28 layers, 224 lists: 33 us (in two kernels 40).
+// (5.3 TB/s; in two kernels 331); one request, 28 layers, 224 lists: 33 us (in two kernels 40). Lists beyond EV_CACHE
+// read their sums from memory in four passes.
 constexpr int EV_THREADS = 512;
 constexpr int EV_CACHE = 16384;  // sums held in shared memory; those behind are read again in every pass
 constexpr int EM_ROWS = 4;       // rows a thread has on their way, twice

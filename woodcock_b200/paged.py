@@ -323,7 +323,9 @@ def paged_mass(q: torch.Tensor, k_pages: torch.Tensor, mass_pages: torch.Tensor,
     are new in this call (a page may hold anything before), and with ``add=False`` for all of them, so that the
     keys of a request without rows have 0 then. Rows need not be all that were appended: after a verification the
     accepted ones, behind a prompt its last ones. A row that sees nothing adds nothing. Statistics and sums are
-    fp32, in the same order every time.
+    fp32, in the same order every time. Beside what the additions of its score and of the sums round, a weight is
+    within 2^-20 + 2^-22 |s| of itself, s the row's score of largest magnitude times log2(e): with bf16 pages and more
+    than 16 rows a head the row's maximum and the logarithm of its sum are held as one fp32 number.
 
     Requests must not share pages, since two would write a sum: with a common prompt each needs keys of its own. A
     call whose requests have more pages than the pool because they do raises the device error word, and the pages'
@@ -359,7 +361,8 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, mass_pages: torch.
 
     Pages [layers][pages][kv_heads][page_size][head_dim] with mass [layers][pages][kv_heads][page_size], or one
     layer's. A request whose budget is below sinks + recent keeps everything and raises the device error word.
-    Requests must not share pages."""
+    Requests must not share pages. Scratch is 4 bytes for each layer, request, kv head and key of the budget; with
+    budgets on the device, of the table's width in keys, so that tables no wider than needed save memory."""
     dev = k_pages.device
     pages = _pages(k_pages, v_pages, layers=k_pages.dim() == 5)
     mass = _mass(mass_pages, k_pages)
