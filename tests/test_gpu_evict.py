@@ -334,6 +334,33 @@ def test_more_pages_than_the_pool_has_raise_the_error_word(rows, dtype):
     check(c, before, mass)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_requests_that_fall_idle_between_replays(dtype):
+    """Offsets are device data: a captured call that starts the sums anew meets requests without rows at a replay."""
+    from woodcock_b200 import ops
+    from woodcock_b200.context import Context
+
+    c = Case(26, [300, 90, 41], [2, 30, 4], 8, 2, 64, 16, dtype)
+    mass = mass_of(c, math.nan)
+    ops.paged_mass(c.q, c.k, mass, c.table, c.kv, q_offsets=c.off, add=False)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.paged_mass(c.q, c.k, mass, c.table, c.kv, q_offsets=c.off, add=False)
+    for rows in ([0, 30, 6], [36, 0, 0], [0, 0, 0], [2, 30, 4]):
+        c.rows = rows
+        c.off.copy_(offsets(rows))
+        mass.fill_(math.nan)
+        graph.replay()
+        before = torch.full_like(mass, math.nan)
+        for b, (n, r) in enumerate(zip(c.lens, rows)):
+            if r == 0:
+                assert (at_keys(mass, c, b, n) == 0).all()
+                at = torch.arange(n, device="cuda")
+                before[c.table[b].long()[at // 16], :, at % 16] = 0.0
+        check(c, before, mass, add=False)
+    Context.get(0).synchronize()
+
+
 def test_arguments_of_mass_that_are_refused():
     from woodcock_b200 import ops
 
